@@ -11,6 +11,7 @@
 #include <mutex>
 
 #include "../../include/flash_attn_gfx950_bench.h"
+#include "fa_check.h"
 #include "fa_params.h"
 
 // ---- fa_fwd_block_noalloc: the block activity maps live in this file-scope device array instead of caller scratch.
@@ -24,12 +25,8 @@ std::atomic<int> g_launch_policy{0};
 }
 namespace fa {
 int launch_policy() { return g_launch_policy.load(std::memory_order_relaxed); }
-}  // namespace fa
 
-namespace {
-
-thread_local char g_err[512] = "";
-
+static thread_local char g_err[512] = "";
 int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -37,23 +34,15 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+}  // namespace fa
 
-#define FA_REQUIRE(cond, ...) \
-  do {                        \
-    if (!(cond)) return fail(FA_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
-  } while (0)
+namespace {
 
-#define FA_LAUNCH(expr)                                                                              \
-  do {                                                                                               \
-    hipError_t e_ = (expr);                                                                          \
-    if (e_ != hipSuccess) return fail(FA_ERR_LAUNCH, "%s failed: %s", #expr, hipGetErrorString(e_)); \
-  } while (0)
+using fa::fail;
 
-inline size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// strides are in elements: multiples of 8 (16-byte vectors), non-negative, and below 2^24 so that the kernels' 32-bit
-// per-lane byte offsets inside a tile (up to 63 rows) cannot overflow
-inline bool stride_ok(int64_t s) { return s % 8 == 0 && s >= 0 && s < ((int64_t)1 << 24); }
+using fa::align16;
+using fa::aligned16;
+using fa::stride_ok;
 // tensors that are written: rows and heads must not overlap (a zero or short stride would make several workgroups write
 // the same bytes)
 inline bool out_stride_ok(int64_t s, int head_dim) { return stride_ok(s) && s >= head_dim; }
@@ -818,7 +807,7 @@ int fa_set_launch_policy(int policy) {
   return FA_OK;
 }
 
-const char* fa_last_error(void) { return g_err; }
+const char* fa_last_error(void) { return fa::g_err; }
 int fa_abi_version(void) { return FA_ABI_VERSION; }
 
 }  // extern "C"

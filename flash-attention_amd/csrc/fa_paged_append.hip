@@ -1,0 +1,180 @@
+// fa_paged_append: the new tokens' k and v go into their sequences' pages, k (and q, into q_out) normalised and turned on the way (fa_norm.h).
+// HBM-bound for prompts (each vector read once, written once); for a decode step's few rows bound by latency: the row's sequence, its
+// length, its page and the store depend on each other, so the rows are loaded before any of them is asked for, and a wave finds a row's sequence
+// with one load and a ballot for 64 sequences.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "fa_norm.h"
+#include "fa_paged.h"
+
+namespace fa {
+
+namespace {
+
+struct AppendParams {
+  PagedCache c;
+  const void *q, *k, *v;
+  void* q_out;
+  const void *qw, *kw;
+  const void *cos, *sin;
+  const int32_t* given_positions;
+  int64_t q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, qo_rs, qo_hs;  // elements
+  int w_fp32, table_rows;
+  float eps;
+  int q_heads;  // 0 without q
+  int per_row, pieces;
+};
+
+// The sequence that row `row` of the packed batch belongs to (B: none); row is wave-uniform.  cu is non-decreasing: the number of sequences
+// that end at or before the row.
+FA_DEVICE int sequence_of(const int32_t* cu, int B, int row) {
+  const int lane = threadIdx.x & 63;
+  int b = 0;
+  for (int at = 0; at < B; at += 64) {
+    const int i = at + lane;
+    const int n = __popcll(__ballot(i < B && cu[i + 1 < B ? i + 1 : B] <= row));
+    b += n;
+    if (n < 64) break;
+  }
+  return b;
+}
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
+  constexpr int CH = D / 8;
+  using vec8 = typename Elem<T>::vec8;
+  const int group = blockIdx.x / p.pieces, piece = blockIdx.x - group * p.pieces;
+  const int j = piece * (int)blockDim.x + threadIdx.x;
+  const int head = j / CH, ch = j % CH;
+  const bool on = j < p.per_row;
+  // heads of q, then of k, then of v
+  const int part = head < p.q_heads ? 0 : (head < p.q_heads + p.c.HK ? 1 : 2);
+  const int h = part == 0 ? head : (part == 1 ? head - p.q_heads : head - p.q_heads - p.c.HK);
+  const T* const src = reinterpret_cast<const T*>(part == 0 ? p.q : (part == 1 ? p.k : p.v)) +
+                       (int64_t)h * (part == 0 ? p.q_hs : (part == 1 ? p.k_hs : p.v_hs)) + ch * 8;
+  const int64_t rs = part == 0 ? p.q_rs : (part == 1 ? p.k_rs : p.v_rs);
+  const int row0 = group * ROWS;
+  vec8 x8[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; i++)
+    if (on && row0 + i < p.c.total_q) x8[i] = bitcast<vec8>(ld_global16(src + (int64_t)(row0 + i) * rs));
+  const bool norm = p.kw != nullptr && part < 2, rot = p.cos != nullptr && part < 2;
+  float w[8];
+  if (on && norm) load_weights<T>(part == 0 ? p.qw : p.kw, p.w_fp32 != 0, ch, w);
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    const int row = row0 + i;
+    if (row >= p.c.total_q) break;
+    const int b = __builtin_amdgcn_readfirstlane(sequence_of(p.c.cu_q, p.c.B, row));
+    if (b >= p.c.B) break;  // (rows behind the last sequence)
+    const int begin = ld_scalar(p.c.cu_q, b), end = ld_scalar(p.c.cu_q, b + 1);
+    const int len = ld_scalar(p.c.seqlens, b);
+    const int slot = append_slot(len, begin, end, row, p.c.max_sq, p.c.max_keys);
+    if (slot < 0) continue;
+    const int page = ld_scalar(p.c.table + (int64_t)b * p.c.table_rs, slot >> p.c.page_log2);
+    const int pos = p.given_positions ? ld_scalar(p.given_positions, row) : slot;
+    if (!page_is_one(page, p.c.n_pages)) continue;  // (everything up to here is wave-uniform)
+    if (on) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = (float)x8[i][e];
+      if (norm) {
+        const float r = inverse_rms<CH>(x, p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = x[e] * r * w[e];
+      }
+      if (rot) {
+        const int t = table_row(pos, p.table_rows);
+        const int64_t at = (int64_t)t * (D / 2) + ch * 4;
+        turn(x, *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.cos) + at),
+             *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.sin) + at));
+      }
+      vec8 y;
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = (T)x[e];
+      const int at = slot & ((1 << p.c.page_log2) - 1);
+      char* dst;
+      if (part == 0) dst = reinterpret_cast<char*>(reinterpret_cast<T*>(p.q_out) + (int64_t)row * p.qo_rs + (int64_t)h * p.qo_hs);
+      else if (part == 1) dst = p.c.k + page * p.c.k_ps + at * p.c.k_ss + h * p.c.k_hs;
+      else dst = p.c.v + page * p.c.v_ps + at * p.c.v_ss + h * p.c.v_hs;
+      st_global16(dst + ch * 16, bitcast<u32x4>(y));
+      if (part == 1 && ch == 0) {
+        const int64_t m = ((int64_t)page * p.c.HK + h) << p.c.page_log2;
+        if (p.c.weights) p.c.weights[m + at] = 0.f;
+        if (p.c.positions) p.c.positions[m + at] = pos;
+      }
+    }
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_append_d(const AppendParams& p, hipStream_t stream) {
+  // A decode step's few rows: one a workgroup, so that as many as there are run side by side; prompts: eight a thread in flight.
+  const bool few = (int64_t)p.c.total_q * p.pieces <= 2048;
+  const int rows = few ? 1 : 8;
+  const dim3 grid((unsigned)((p.c.total_q + rows - 1) / rows * p.pieces));
+  if (few) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((paged_append_kernel<T, D, 8>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_append(const AppendParams& p, int D, hipStream_t stream) {
+  switch (D) {
+    case 16: return launch_append_d<T, 16>(p, stream);
+    case 32: return launch_append_d<T, 32>(p, stream);
+    case 64: return launch_append_d<T, 64>(p, stream);
+    case 128: return launch_append_d<T, 128>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" int fa_paged_append(const fa_paged_append_args* a) {
+  const char* const name = "fa_paged_append";
+  FA_REQUIRE(a && a->struct_bytes == sizeof(fa_paged_append_args), "%s: struct size mismatch", name);
+  FA_REQUIRE(a->dtype == FA_FP16 || a->dtype == FA_BF16, "%s: dtype must be fp16 or bf16", name);
+  const int rc = fa::check_paged_cache(&a->cache, true, true, true, name);
+  if (rc) return rc;
+  const fa_paged_cache& c = a->cache;
+  FA_REQUIRE(c.k_slot_stride >= c.head_dim && c.v_slot_stride >= c.head_dim && (c.nheads_k == 1 || (c.k_head_stride >= c.head_dim && c.v_head_stride >= c.head_dim)) &&
+                 (c.n_pages == 1 || (c.k_page_stride >= c.head_dim && c.v_page_stride >= c.head_dim)),
+             "%s: the cache's slots, heads and pages must not overlap", name);
+  if (c.total_q == 0) return FA_OK;
+  FA_REQUIRE(a->k && a->v && fa::aligned16(a->k) && fa::aligned16(a->v) && fa::stride_ok(a->k_row_stride) && fa::stride_ok(a->k_head_stride) &&
+                 fa::stride_ok(a->v_row_stride) && fa::stride_ok(a->v_head_stride),
+             "%s: k and v must be 16-byte aligned, their strides multiples of 8 elements in [0, 2^24)", name);
+  FA_REQUIRE((a->q == nullptr) == (a->q_out == nullptr), "%s: q and q_out come together", name);
+  if (a->q)
+    FA_REQUIRE(fa::aligned16(a->q) && fa::aligned16(a->q_out) && fa::stride_ok(a->q_row_stride) && fa::stride_ok(a->q_head_stride) &&
+                   fa::stride_ok(a->q_out_row_stride) && fa::stride_ok(a->q_out_head_stride) && a->q_out_row_stride >= c.head_dim &&
+                   (c.nheads_q == 1 || a->q_out_head_stride >= c.head_dim),
+               "%s: q and q_out must be 16-byte aligned, their strides multiples of 8 elements in [0, 2^24), written rows and heads apart", name);
+  FA_REQUIRE(!a->q || (a->q_weight == nullptr) == (a->k_weight == nullptr), "%s: q_weight and k_weight come together", name);
+  FA_REQUIRE(!a->k_weight || a->weight_dtype == a->dtype || a->weight_dtype == FA_FP32, "%s: weights must be of the tensors' dtype or fp32", name);
+  FA_REQUIRE(a->eps >= 0.f, "%s: eps must not be negative", name);
+  FA_REQUIRE((a->cos_table == nullptr) == (a->sin_table == nullptr) && (!a->cos_table || a->table_rows >= 1), "%s: cos_table and sin_table come together, with rows", name);
+  FA_REQUIRE(((reinterpret_cast<uintptr_t>(a->cos_table) | reinterpret_cast<uintptr_t>(a->sin_table)) & 7) == 0, "%s: tables must be 8-byte aligned", name);
+  fa::AppendParams p{};
+  p.c = fa::paged_cache(&c);
+  p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out;
+  p.qw = a->q_weight; p.kw = a->k_weight;
+  p.cos = a->cos_table; p.sin = a->sin_table;
+  p.given_positions = a->positions;
+  p.q_rs = a->q_row_stride; p.q_hs = a->q_head_stride; p.k_rs = a->k_row_stride; p.k_hs = a->k_head_stride;
+  p.v_rs = a->v_row_stride; p.v_hs = a->v_head_stride; p.qo_rs = a->q_out_row_stride; p.qo_hs = a->q_out_head_stride;
+  p.w_fp32 = a->weight_dtype == FA_FP32;
+  p.table_rows = a->table_rows;
+  p.eps = a->eps;
+  p.q_heads = a->q ? c.nheads_q : 0;
+  p.per_row = (p.q_heads + 2 * c.nheads_k) * (c.head_dim / 8);
+  p.pieces = (p.per_row + 255) / 256;
+  FA_REQUIRE((int64_t)c.total_q * p.pieces < ((int64_t)1 << 31), "%s: too many rows", name);
+  const hipStream_t stream = reinterpret_cast<hipStream_t>(a->stream);
+  FA_LAUNCH(a->dtype == FA_FP16 ? fa::launch_append<_Float16>(p, c.head_dim, stream) : fa::launch_append<__bf16>(p, c.head_dim, stream));
+  return FA_OK;
+}

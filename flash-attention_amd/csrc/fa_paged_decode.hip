@@ -1,0 +1,407 @@
+// Attention of a few rows a key head (decoding: one new token of each sequence, or a handful, times the heads of a group) over a paged cache:
+// every key and value is read once and used for at most 32 rows, a stream of K and V that HBM bounds.
+//
+// A wave owns 32-key tiles: it stages them into a double buffer of its own by direct-to-LDS loads, counts its outstanding loads instead of meeting the
+// other waves, and multiplies in the orientation S^T = K Q^T, O^T = V^T P^T (a lane is a row); the workgroup's waves join their partial results in
+// LDS at the end of a pair.  Lengths differ and are known on the device only, so the launch does not cut sequences into equal numbers of pieces: all
+// units of kDecodeUnit keys of all pairs are laid out in one line, and each of the resident workgroups takes an equal share of it - the end of one
+// pair, some whole pairs, the beginning of another.  Pairs that more than one workgroup has touched are joined by a second kernel.
+#include "fa_paged_fwd.h"
+
+namespace fa {
+
+namespace {
+
+template <int D>
+struct Cfg {
+  static constexpr int NW = kDecodeWaves(D);
+  static constexpr int BN = 32;
+  static constexpr int DV = D < 32 ? 32 : D;
+  static constexpr int kTile = BN * D * 2;
+  static constexpr int kWave = 2 * 2 * kTile;     // two stages of (K tile, V tile)
+  static constexpr int kSlack = D < 32 ? 64 : 0;  // the 32-wide transposed reads run past a 16-wide V row
+  static constexpr int XS = DV + 4;               // merge: floats per (wave, row)
+  static constexpr int kMerge = NW * 32 * XS * 4 + 3 * NW * 32 * 4;
+  static constexpr int kTiles = NW * kWave + kSlack;
+  static constexpr int kLds = kTiles > kMerge ? kTiles : kMerge;
+};
+
+template <int N>
+FA_DEVICE void wait_vmcnt() {  // at most N of this wave's global loads (direct-to-LDS ones included) are still outstanding
+  static_assert(N < 64, "vmcnt has six bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
+}
+
+// The line of units.  Sequence b has HK pairs of units(b) each; a sequence without new tokens has none.
+FA_DEVICE int units_of(const PagedCache& c, int b) {
+  const int keys = keys_in_reach(c.seqlens[b], c.max_keys);
+  const int s = c.cu_q[b], e = c.cu_q[b + 1];
+  if (s < 0 || e <= s || e > c.total_q) return 0;
+  return keys <= kDecodeUnit ? 1 : (keys + kDecodeUnit - 1) / kDecodeUnit;
+}
+// Units of 64 sequences from `first` on as inclusive sums over the lanes; the same in every wave
+FA_DEVICE int unit_sums(const PagedCache& c, int first) {
+  const int b = first + (threadIdx.x & 63);
+  return wave_prefix_sum(b < c.B ? units_of(c, b) : 0);
+}
+FA_DEVICE int64_t all_units(const PagedCache& c) {
+  int64_t n = 0;
+  for (int first = 0; first < c.B; first += 64) n += __builtin_amdgcn_readlane(unit_sums(c, first), 63);
+  return n * c.HK;
+}
+struct Spot {  // a unit of the line
+  int b, h, unit, units;  // units: of each pair of sequence b
+};
+FA_DEVICE Spot spot_of(const PagedCache& c, int64_t u) {
+  int64_t before = 0;
+  for (int first = 0; first < c.B; first += 64) {
+    const int sums = unit_sums(c, first);
+    const int all = __builtin_amdgcn_readlane(sums, 63);
+    if (u < before + (int64_t)all * c.HK) {
+      const int64_t rest = u - before;
+      const int lane = __popcll(__ballot((int64_t)sums * c.HK <= rest));  // sequences that end before the unit
+      const int upto = lane > 0 ? __builtin_amdgcn_readlane(sums, lane > 0 ? lane - 1 : 0) : 0;
+      const int units = __builtin_amdgcn_readlane(sums, lane) - upto;
+      const int in_seq = (int)(rest - (int64_t)upto * c.HK);
+      return Spot{first + lane, in_seq / units, in_seq % units, units};
+    }
+    before += (int64_t)all * c.HK;
+  }
+  return Spot{c.B, 0, 0, 1};
+}
+// Workgroups that share the line, and the first unit of workgroup w
+FA_DEVICE int sharers(const PagedFwdParams& p, int64_t units) {
+  const int64_t most = (units + p.least - 1) / p.least;
+  return (int)(most < p.groups ? (most > 0 ? most : 1) : p.groups);
+}
+FA_DEVICE int64_t share_begin(int64_t units, int w, int sharers) { return units * w / sharers; }
+FA_DEVICE int share_of(int64_t units, int64_t u, int sharers) {  // the workgroup whose share holds unit u
+  int w = (int)((u * sharers) / units);
+  while (w + 1 < sharers && share_begin(units, w + 1, sharers) <= u) w++;
+  while (w > 0 && share_begin(units, w, sharers) > u) w--;
+  return w;
+}
+
+}  // namespace
+
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * Cfg<D>::NW) fa_paged_decode_kernel(const PagedFwdParams p) {
+  using C = Cfg<D>;
+  using E = Elem<T>;
+  using vec8 = typename E::vec8;
+  constexpr int NW = C::NW, BN = C::BN, DV = C::DV;
+  using KStager = GroupStager<D, kSwzRow>;
+  using VStager = GroupStager<D, kSwzTr>;
+  constexpr int NI = 2 * KStager::NI;  // loads of a tile's K, and of its V
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[C::kLds];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hf = lane >> 5;
+  const float cs = p.scale_log2;
+
+  KStager ks_;
+  VStager vs_;
+  ks_.init(lane, p.c.k_ss);
+  vs_.init(lane, p.c.v_ss);
+  unsigned char* const lds_wave = lds_raw + wave * C::kWave;
+  int koff[D / 16], voff[DV / 32];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ks++) koff[ks] = frag_off<D, kSwzRow>(c, ks * 2 + hf);
+#pragma unroll
+  for (int db = 0; db < DV / 32; db++) voff[db] = tr_off<D, kSwzTr>(0, db * 4, lane);
+
+  // ---- this workgroup's share of the line: [u, u_end), from `at` on
+  int64_t u, u_end;
+  Spot at;
+  if (p.least > 0) {
+    const int64_t units = all_units(p.c);
+    const int n = sharers(p, units);
+    if ((int)blockIdx.x >= n || units == 0) return;
+    u = share_begin(units, blockIdx.x, n);
+    u_end = share_begin(units, blockIdx.x + 1, n);
+    at = spot_of(p.c, u);
+  } else {  // one pair
+    const int b = blockIdx.x / p.c.HK;
+    at = Spot{b, (int)blockIdx.x - b * p.c.HK, 0, units_of(p.c, b)};
+    if (at.units == 0) return;
+    u = 0;
+    u_end = at.units;
+  }
+
+  bool first = true;
+  while (u < u_end) {
+    const int b = __builtin_amdgcn_readfirstlane(at.b), h = __builtin_amdgcn_readfirstlane(at.h);
+    const int unit0 = __builtin_amdgcn_readfirstlane(at.unit), pair_units = __builtin_amdgcn_readfirstlane(at.units);
+    const int unit1 = u_end - u < pair_units - unit0 ? unit0 + (int)(u_end - u) : pair_units;
+    int q_begin = 0, Lq = 0;
+    if (!paged_rows(p.c, b, &q_begin, &Lq)) return;  // (never: such a sequence has no units)
+    const int Lk = paged_len(p.c, b), G = p.c.G, rows = Lq * G;
+    const int k_lo = unit0 * kDecodeUnit;
+    const int k_hi = Lk < unit1 * kDecodeUnit ? Lk : unit1 * kDecodeUnit;
+    const int ntiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
+    const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
+    const char* const kb = p.c.k + h * p.c.k_hs;
+    const char* const vb = p.c.v + h * p.c.v_hs;
+    const int last_group = (Lk - 1) >> 4;
+
+    // a tile's two groups of 16 keys: their pages are asked for a step before they are needed
+    int page[2];
+    auto ask = [&](int t) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int g = (k_lo >> 4) + 2 * t + j;
+        page[j] = page_of_group(p.c, table, g < last_group ? g : last_group);
+      }
+    };
+    auto issue = [&](int t, int stage) {
+      unsigned char* const dst = lds_wave + stage * 2 * C::kTile;
+      int slot[2], last[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int g0 = (k_lo >> 4) + 2 * t + j, g = g0 < last_group ? g0 : last_group;
+        slot[j] = slot_of_group(p.c, g);
+        last[j] = g < last_group ? 15 : (Lk - 1) & 15;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; j++) ks_.issue(kb + page[j] * p.c.k_ps + slot[j] * p.c.k_ss, p.c.k_ss, last[j], dst + j * KStager::kBytes);
+#pragma unroll
+      for (int j = 0; j < 2; j++) vs_.issue(vb + page[j] * p.c.v_ps + slot[j] * p.c.v_ss, p.c.v_ss, last[j], dst + C::kTile + j * VStager::kBytes);
+    };
+
+    int t = wave, stage = 0;
+    if (t < ntiles) {
+      ask(t);
+      issue(t, 0);
+    }
+    if (t + NW < ntiles) {
+      ask(t + NW);
+      issue(t + NW, 1);
+    }
+    const int row = c < rows ? c : rows - 1;  // (columns past the last row repeat it and are dropped at the end)
+    const int tok = row / G;
+    vec8 qreg[D / 16];
+    {
+      const T* qp = reinterpret_cast<const T*>(p.q) + (int64_t)(q_begin + tok) * p.q_rs + (int64_t)(h * G + (row - tok * G)) * p.q_hs + hf * 8;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ks++) qreg[ks] = bitcast<vec8>(ld_global16(qp + ks * 16));
+      // waited for here (with the first two tiles): the main loop counts this wave's outstanding loads, these are not to be among them
+      wait_vmcnt<0>();
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ks++) asm volatile("" : "+v"(qreg[ks]));
+    }
+    const int limit = p.causal ? Lk - Lq + tok + 1 : Lk;
+    const int least_limit = p.causal ? Lk - Lq + 1 : Lk;  // of row 0
+
+    f32x16 o_acc[DV / 32];
+#pragma unroll
+    for (int i = 0; i < DV / 32; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) o_acc[i][r] = 0.f;
+    float m_i = -INFINITY, l_i = 0.f, u_i = 0.f;  // l_i, u_i: this lane's share, the other half's in lane ^ 32
+
+    for (; t < ntiles; t += NW) {
+      const bool next = t + NW < ntiles;  // its 2 * NI loads were issued after this tile's
+      if (next) wait_vmcnt<3 * NI>();
+      else wait_vmcnt<NI>();
+      if (t + 2 * NW < ntiles) ask(t + 2 * NW);
+      const T* const Ks = reinterpret_cast<const T*>(lds_wave + stage * 2 * C::kTile);
+      const T* const Vs = Ks + BN * D;
+      f32x16 s;
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ks++) s = E::mfma32(*reinterpret_cast<const vec8*>(Ks + koff[ks]), qreg[ks], s);
+      const int n0 = k_lo + t * BN;
+      if (n0 + BN > least_limit) {
+        const int dead = limit - n0 - 4 * hf;
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (8 * (r >> 2) + (r & 3) >= dead) s[r] = -INFINITY;
+      }
+      float mt = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
+      mt = half_max(mt);
+      if (__any(mt > m_i)) {
+        const float m_new = fmaxf(m_i, mt);
+        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2((m_i - m_new) * cs);
+        m_i = m_new;
+        l_i *= alpha;
+        u_i *= alpha;
+#pragma unroll
+        for (int i = 0; i < DV / 32; i++) o_acc[i] = o_acc[i] * alpha;
+      }
+      const float mc = (m_i == -INFINITY ? 0.f : m_i) * cs;
+      vec8 pb[2];
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++) {
+        f32x8 pf;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          pf[i] = fast_exp2(__builtin_fmaf(s[8 * tt + i], cs, -mc));
+          u_i += pf[i];
+        }
+        pb[tt] = cvt8<T>(pf);
+        l_i = sum8_acc(pb[tt], l_i);
+      }
+      if (next) wait_vmcnt<2 * NI>();
+      else wait_vmcnt<0>();
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+        for (int db = 0; db < DV / 32; db++) {
+          const T* vp = Vs + 16 * tt * D + voff[db];
+          const u32x2 lo = lds_read_tr16(vp), hi = lds_read_tr16(vp + 8 * D);
+          o_acc[db] = E::mfma32(bitcast<vec8>(u32x4{lo[0], lo[1], hi[0], hi[1]}), pb[tt], o_acc[db]);
+        }
+      if (t + 2 * NW < ntiles) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage has been read before it is refilled
+        issue(t + 2 * NW, stage);
+      }
+      stage ^= 1;
+    }
+
+    // ---- the waves' partial results joined: row r of wave w at X[(w * 32 + r) * XS], m, l and u behind all rows
+    __syncthreads();
+    float* const X = reinterpret_cast<float*>(lds_raw);
+    float* const Xm = X + NW * 32 * C::XS;
+    float* const Xl = Xm + NW * 32;
+    float* const Xu = Xl + NW * 32;
+    l_i = half_sum(l_i);
+    u_i = half_sum(u_i);
+    if (c < rows) {
+      if (hf == 0) {
+        Xm[wave * 32 + c] = m_i;
+        Xl[wave * 32 + c] = l_i;
+        Xu[wave * 32 + c] = u_i;
+      }
+#pragma unroll
+      for (int db = 0; db < DV / 32; db++)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; g4++) {
+          f32x4 x;
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[i] = o_acc[db][g4 * 4 + i];
+          *reinterpret_cast<f32x4*>(X + (wave * 32 + c) * C::XS + db * 32 + g4 * 8 + hf * 4) = x;
+        }
+    }
+    __syncthreads();
+    const bool whole = unit0 == 0 && unit1 == pair_units;
+    float* const part_o = whole ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * (kPartRows * (D + 3));
+    for (int idx = tid; idx < rows * (D / 4); idx += 64 * NW) {
+      const int r = idx / (D / 4), d0 = idx % (D / 4) * 4;
+      float m = Xm[r];
+#pragma unroll
+      for (int w = 1; w < NW; w++) m = fmaxf(m, Xm[w * 32 + r]);
+      const float mu = m == -INFINITY ? 0.f : m;
+      float l = 0.f, us = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        const float f = fast_exp2((Xm[w * 32 + r] - mu) * cs);  // 0 for a wave without keys
+        l = __builtin_fmaf(Xl[w * 32 + r], f, l);
+        us = __builtin_fmaf(Xu[w * 32 + r], f, us);
+        o = o + *reinterpret_cast<const f32x4*>(X + (w * 32 + r) * C::XS + d0) * f;
+      }
+      if (whole) {
+        store_row_piece<T>(p, q_begin, h, r, d0, o * (l > 0.f ? fast_rcp(l) : 1.f));
+        if (d0 == 0) store_lse(p, b, h, r, lse_of(m, us, cs));
+      } else {
+        *reinterpret_cast<f32x4*>(part_o + r * D + d0) = o;
+        if (d0 == 0) {
+          float* const ml = part_o + kPartRows * D + r;
+          ml[0] = m;
+          ml[kPartRows] = l;
+          ml[2 * kPartRows] = us;
+        }
+      }
+    }
+    first = false;
+    u += unit1 - unit0;
+    if (u >= u_end) return;
+    // the next pair
+    at.unit = 0;
+    if (h + 1 < p.c.HK) {
+      at.h = h + 1;
+    } else {
+      at.h = 0;
+      do at.b++; while (at.b < p.c.B && units_of(p.c, at.b) == 0);
+      if (at.b >= p.c.B) return;  // (never: the line does not end here)
+      at.units = units_of(p.c, at.b);
+    }
+    __syncthreads();  // the joined results have been read before the tiles come in over them
+  }
+}
+
+namespace {
+
+// The pairs that several workgroups' shares have cut: a workgroup per pair, 128 threads.
+template <typename T>
+__global__ void __launch_bounds__(128) paged_decode_join_kernel(const PagedFwdParams p, int D) {
+  const int b = blockIdx.x / p.c.HK, h = (int)blockIdx.x - b * p.c.HK;
+  const int own = units_of(p.c, b);
+  if (own == 0) return;
+  int64_t units = 0, begin = 0;  // of the line; of this pair
+  for (int first = 0; first < p.c.B; first += 64) {
+    const int sums = unit_sums(p.c, first);
+    if (b >= first && b < first + 64) {
+      const int upto = __builtin_amdgcn_readlane(sums, b - first) - own;
+      begin = (units + upto) * p.c.HK + (int64_t)h * own;
+    }
+    units += __builtin_amdgcn_readlane(sums, 63);
+  }
+  units *= p.c.HK;
+  const int n = sharers(p, units);
+  const int w0 = share_of(units, begin, n), w1 = share_of(units, begin + own - 1, n);
+  if (w0 == w1) return;
+  int q_begin = 0, Lq = 0;
+  if (!paged_rows(p.c, b, &q_begin, &Lq)) return;
+  const float cs = p.scale_log2;
+  const int per_row = D / 4, each = kPartRows * (D + 3);
+  // the pair is the last of workgroup w0's share, and its first, too, if the share begins with it; it is the first of the others'
+  const int first_slot = share_begin(units, w0, n) == begin ? 0 : 1;
+  for (int idx = threadIdx.x; idx < Lq * p.c.G * per_row; idx += 128) {
+    const int r = idx / per_row, d0 = idx % per_row * 4;
+    float m = -INFINITY;
+    for (int w = w0; w <= w1; w++) m = fmaxf(m, p.part[((int64_t)w * 2 + (w == w0 ? first_slot : 0)) * each + kPartRows * D + r]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f, us = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int w = w0; w <= w1; w++) {
+      const float* const s = p.part + ((int64_t)w * 2 + (w == w0 ? first_slot : 0)) * each;
+      const float* const ml = s + kPartRows * D + r;
+      const float f = fast_exp2((ml[0] - mu) * cs);
+      l = __builtin_fmaf(ml[kPartRows], f, l);
+      us = __builtin_fmaf(ml[2 * kPartRows], f, us);
+      o = o + *reinterpret_cast<const f32x4*>(s + r * D + d0) * f;
+    }
+    store_row_piece<T>(p, q_begin, h, r, d0, o * (l > 0.f ? fast_rcp(l) : 1.f));
+    if (d0 == 0) store_lse(p, b, h, r, lse_of(m, us, cs));
+  }
+}
+
+template <typename T>
+hipError_t launch_t(const PagedFwdParams& p, int head_dim, hipStream_t stream) {
+  const unsigned pairs = (unsigned)(p.c.B * p.c.HK);
+  const dim3 grid(p.least > 0 ? (unsigned)p.groups : pairs);
+  switch (head_dim) {
+    case 16: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 16>), grid, dim3(64 * Cfg<16>::NW), 0, stream, p); break;
+    case 32: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 32>), grid, dim3(64 * Cfg<32>::NW), 0, stream, p); break;
+    case 64: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 64>), grid, dim3(64 * Cfg<64>::NW), 0, stream, p); break;
+    case 128: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 128>), grid, dim3(64 * Cfg<128>::NW), 0, stream, p); break;
+    default: return hipErrorInvalidValue;
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.least == 0) return e;
+  hipLaunchKernelGGL(paged_decode_join_kernel<T>, dim3(pairs), dim3(128), 0, stream, p, head_dim);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_decode(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream) {
+  return dtype == 0 ? launch_t<_Float16>(p, head_dim, stream) : launch_t<__bf16>(p, head_dim, stream);
+}
+
+}  // namespace fa

@@ -1,0 +1,259 @@
+// fa_paged_evict: every key head of a sequence keeps `budget` keys, the newest and the heaviest; the kept ones that lie behind slot `budget` move into
+// the holes that the others leave before it.  Nothing else moves: the order of a cache's keys does not matter to attention, and a decode step that is
+// one key over its budget moves one key.
+//
+// A workgroup per (sequence, key head) finds the weight of the budget-th key by a radix selection over the weights' bits, mapped to integers of
+// the same order (three digits of 11, 11 and 10 bits, counted in LDS), where the newest keys come above every weight; keys of just that weight stay
+// from the lowest slot on.  Holes and moving keys are numbered by prefix sums in slot order, so the n-th hole takes the n-th key, and left in the
+// workspace; a second kernel copies them, a launch of many workgroups, since sources and destinations are different slots.
+// Bound by one read of weights and positions (8 bytes a slot) and two passes over each moved vector.
+#include <algorithm>
+
+#include "fa_paged.h"
+
+namespace fa {
+
+namespace {
+
+struct EvictParams {
+  PagedCache c;
+  const int32_t* next;
+  int32_t* new_len;
+  int budget, recent, cap;  // cap: most moves of a head
+  int32_t* counts;          // [B * HK]
+  int32_t* moves;           // [B * HK][2][cap]: holes, keys that come
+  int row_bytes;
+};
+
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+constexpr uint32_t kNewest = 0xffffffffu;
+
+// A weight as an unsigned integer of the same order; NaN as -inf, -0 as 0
+FA_DEVICE uint32_t ordered(float w) {
+  const uint32_t u = __float_as_uint(w != w ? -INFINITY : w + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// kCap: keys whose mapped weights are kept in LDS (0: read again in every pass)
+template <int kCap>
+__global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictParams p) {
+  __shared__ uint32_t keys[kCap > 0 ? kCap : 1];
+  __shared__ int hist[2048];
+  __shared__ int sums[2][kEvictWaves];
+  __shared__ uint32_t found[2];  // digit, keys above it
+  const int b = blockIdx.x / p.c.HK, h = (int)blockIdx.x - b * p.c.HK;
+  const int L = paged_len(p.c, b);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (h == 0 && tid == 0) p.new_len[b] = L < p.budget ? L : p.budget;
+  if (L <= p.budget) {
+    if (tid == 0) p.counts[blockIdx.x] = 0;
+    return;
+  }
+  const int64_t newest = (int64_t)p.next[b] - p.recent;
+  const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
+  const int mask = (1 << p.c.page_log2) - 1;
+  auto read_key = [&](int j) {
+    const int page = page_in_pool(table[j >> p.c.page_log2], p.c.n_pages);
+    const int64_t at = (((int64_t)page * p.c.HK + h) << p.c.page_log2) + (j & mask);
+    const uint32_t k = ordered(p.c.weights[at]);
+    return p.c.positions[at] >= newest ? kNewest : k;
+  };
+  auto key_of = [&](int j) { return kCap > 0 ? keys[j] : read_key(j); };
+
+  // ---- the budget-th largest key
+  uint32_t prefix = 0;
+  int want = p.budget;  // of the keys that begin with `prefix`
+  for (int pass = 0; pass < 3; pass++) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
+    __syncthreads();
+    for (int j = tid; j < L; j += kEvictThreads) {
+      uint32_t k;
+      if (kCap > 0 && pass == 0) {
+        k = read_key(j);
+        keys[j] = k;
+      } else {
+        k = key_of(j);
+      }
+      if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // thread t holds the digits 2047 - 2 t and 2046 - 2 t: prefix sums count from the largest digit down
+    const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
+    const int incl = wave_prefix_sum(hi + lo);
+    if (lane == 63) sums[0][wave] = incl;
+    __syncthreads();
+    int above = incl - hi - lo;
+    for (int w = 0; w < wave; w++) above += sums[0][w];
+    if (above < want && want <= above + hi) {
+      found[0] = 2047 - 2 * tid;
+      found[1] = above;
+    } else if (above + hi < want && want <= above + hi + lo) {
+      found[0] = 2046 - 2 * tid;
+      found[1] = above + hi;
+    }
+    __syncthreads();
+    prefix = (prefix << bits) | found[0];
+    want -= (int)found[1];
+    __syncthreads();  // (found and hist are written again)
+  }
+  const uint32_t edge = prefix;  // keys above it stay, and the first `want` that equal it
+
+  // ---- slots in order: a wave takes a run of whole 64s
+  const int run = (L + kEvictThreads - 1) / kEvictThreads * 64;
+  const int j0 = wave * run, j1 = j0 + run < L ? j0 + run : L;
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  int ties = 0;
+  for (int j = j0 + lane; j - lane < j1; j += 64) ties += __popcll(__ballot(j < j1 && key_of(j) == edge));
+  if (lane == 0) sums[0][wave] = ties;
+  __syncthreads();
+  int tie0 = 0;
+  for (int w = 0; w < wave; w++) tie0 += sums[0][w];
+  int hole0 = 0, come0 = 0;
+  int32_t* const holes = p.moves + (int64_t)blockIdx.x * 2 * p.cap;
+  for (int round = 0; round < 2; round++) {  // counted, then written
+    int tie = tie0, hole = hole0, come = come0;
+    for (int j = j0 + lane; j - lane < j1; j += 64) {
+      const bool in = j < j1;
+      const uint32_t k = in ? key_of(j) : 0;
+      const uint64_t tied = __ballot(in && k == edge);
+      const bool stays = in && (k > edge || (k == edge && tie + __popcll(tied & below) < want));
+      tie += __popcll(tied);
+      const bool is_hole = in && !stays && j < p.budget, comes = stays && j >= p.budget;
+      const uint64_t hb = __ballot(is_hole), cb = __ballot(comes);
+      if (round == 1) {
+        const int nh = hole + __popcll(hb & below), nc = come + __popcll(cb & below);
+        if (is_hole && nh < p.cap) holes[nh] = j;
+        if (comes && nc < p.cap) holes[p.cap + nc] = j;
+      }
+      hole += __popcll(hb);
+      come += __popcll(cb);
+    }
+    if (round == 0) {
+      __syncthreads();  // (the ties have been read)
+      if (lane == 0) {
+        sums[0][wave] = hole;
+        sums[1][wave] = come;
+      }
+      __syncthreads();
+      int n = 0;
+      for (int w = 0; w < kEvictWaves; w++) {
+        if (w < wave) {
+          hole0 += sums[0][w];
+          come0 += sums[1][w];
+        }
+        n += sums[0][w];
+      }
+      if (tid == 0) p.counts[blockIdx.x] = n < p.cap ? n : p.cap;
+    }
+  }
+}
+
+constexpr int kMovesPerGroup = 64;
+
+// A workgroup copies 64 of a head's moves: a thread 16 bytes at a time of a key or a value.
+__global__ void __launch_bounds__(256) paged_move_kernel(const EvictParams p) {
+  const int pair = blockIdx.y, n = p.counts[pair];
+  const int first = blockIdx.x * kMovesPerGroup;
+  if (first >= n) return;
+  const int b = pair / p.c.HK, h = pair - b * p.c.HK;
+  const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
+  const int32_t* const holes = p.moves + (int64_t)pair * 2 * p.cap;
+  const int mask = (1 << p.c.page_log2) - 1, cpr = p.row_bytes / 16;
+  const int moves = n - first < kMovesPerGroup ? n - first : kMovesPerGroup;
+  for (int i = threadIdx.x; i < moves * 2 * cpr; i += 256) {
+    const int m = i / (2 * cpr), rest = i - m * 2 * cpr;
+    const bool value = rest >= cpr;
+    const int ch = value ? rest - cpr : rest;
+    const int to = holes[first + m], from = holes[p.cap + first + m];
+    const int to_page = table[to >> p.c.page_log2];
+    const int from_page = page_in_pool(table[from >> p.c.page_log2], p.c.n_pages);
+    if (!page_is_one(to_page, p.c.n_pages)) continue;
+    char* const base = value ? p.c.v : p.c.k;
+    const int64_t ps = value ? p.c.v_ps : p.c.k_ps, ss = value ? p.c.v_ss : p.c.k_ss, hs = value ? p.c.v_hs : p.c.k_hs;
+    const char* const src = base + from_page * ps + (from & mask) * ss + h * hs + ch * 16;
+    char* const dst = base + to_page * ps + (to & mask) * ss + h * hs + ch * 16;
+    st_global16(dst, ld_global16(src));
+    if (rest == 0) {
+      const int64_t d = (((int64_t)to_page * p.c.HK + h) << p.c.page_log2) + (to & mask);
+      const int64_t s = (((int64_t)from_page * p.c.HK + h) << p.c.page_log2) + (from & mask);
+      p.c.weights[d] = p.c.weights[s];
+      p.c.positions[d] = p.c.positions[s];
+    }
+  }
+}
+
+struct EvictPlan {
+  int cap;
+  size_t bytes;
+};
+EvictPlan evict_plan(const fa_paged_evict_args* a) {
+  const int max_keys = (int)std::min<int64_t>(a->cache.max_seqlen_k, (int64_t)a->cache.table_cols * a->cache.page_size);
+  EvictPlan pl;
+  pl.cap = std::max(0, std::min(a->budget, max_keys - a->budget));
+  pl.bytes = (size_t)a->cache.batch * a->cache.nheads_k * ((size_t)2 * pl.cap + 1) * 4;
+  return pl;
+}
+
+hipError_t launch_evict(const EvictParams& p, hipStream_t stream) {
+  const dim3 pairs((unsigned)(p.c.B * p.c.HK));
+  // (LDS decides how many heads a compute unit selects for at once: nine, two, one)
+  if (p.c.max_keys <= 4096) hipLaunchKernelGGL(paged_evict_kernel<4096>, pairs, dim3(kEvictThreads), 0, stream, p);
+  else if (p.c.max_keys <= 16384) hipLaunchKernelGGL(paged_evict_kernel<16384>, pairs, dim3(kEvictThreads), 0, stream, p);
+  else if (p.c.max_keys <= 32768) hipLaunchKernelGGL(paged_evict_kernel<32768>, pairs, dim3(kEvictThreads), 0, stream, p);
+  else hipLaunchKernelGGL(paged_evict_kernel<0>, pairs, dim3(kEvictThreads), 0, stream, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.cap == 0) return e;
+  const unsigned gx = (unsigned)((p.cap + kMovesPerGroup - 1) / kMovesPerGroup);
+  hipLaunchKernelGGL(paged_move_kernel, dim3(gx, pairs.x), dim3(256), 0, stream, p);  // (at most 65535 heads: see check_sizes)
+  return hipGetLastError();
+}
+
+int check_sizes(const fa_paged_evict_args* a, const char* name) {
+  FA_REQUIRE(a && a->struct_bytes == sizeof(fa_paged_evict_args), "%s: struct size mismatch", name);
+  const int rc = check_paged_cache(&a->cache, false, false, false, name);
+  if (rc) return rc;
+  FA_REQUIRE(a->budget > 0 && a->recent >= 0, "%s: budget must be positive, recent not negative", name);
+  FA_REQUIRE((int64_t)a->cache.batch * a->cache.nheads_k <= 65535, "%s: more than 65535 key heads of sequences", name);
+  return FA_OK;
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" {
+
+size_t fa_paged_evict_workspace_bytes(const fa_paged_evict_args* a) {
+  return fa::check_sizes(a, "fa_paged_evict") == FA_OK ? fa::evict_plan(a).bytes : 0;
+}
+
+int fa_paged_evict(const fa_paged_evict_args* a) {
+  const char* const name = "fa_paged_evict";
+  int rc = fa::check_sizes(a, name);
+  if (rc == FA_OK) rc = fa::check_paged_cache(&a->cache, true, true, false, name);
+  if (rc) return rc;
+  const fa_paged_cache& c = a->cache;
+  FA_REQUIRE(c.k_slot_stride >= c.head_dim && c.v_slot_stride >= c.head_dim && (c.nheads_k == 1 || (c.k_head_stride >= c.head_dim && c.v_head_stride >= c.head_dim)) &&
+                 (c.n_pages == 1 || (c.k_page_stride >= c.head_dim && c.v_page_stride >= c.head_dim)),
+             "%s: the cache's slots, heads and pages must not overlap", name);
+  FA_REQUIRE(c.key_weights && c.key_positions && a->next_positions && a->new_seqlens_k, "%s: key_weights, key_positions, next_positions and new_seqlens_k are needed", name);
+  FA_REQUIRE(a->new_seqlens_k != c.seqlens_k, "%s: new_seqlens_k may not be seqlens_k", name);
+  FA_REQUIRE(((reinterpret_cast<uintptr_t>(a->next_positions) | reinterpret_cast<uintptr_t>(a->new_seqlens_k)) & 3) == 0, "%s: integers must be 4-byte aligned", name);
+  const fa::EvictPlan pl = fa::evict_plan(a);
+  if (!a->workspace || a->workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(a->workspace) & 3))
+    return fa::fail(FA_ERR_WORKSPACE, "%s: needs %zu bytes of 4-byte aligned workspace", name, pl.bytes);
+  fa::EvictParams p{};
+  p.c = fa::paged_cache(&c);
+  p.next = a->next_positions;
+  p.new_len = a->new_seqlens_k;
+  p.budget = a->budget;
+  p.recent = a->recent;
+  p.cap = pl.cap;
+  p.counts = reinterpret_cast<int32_t*>(a->workspace);
+  p.moves = p.counts + (size_t)c.batch * c.nheads_k;
+  p.row_bytes = c.head_dim * 2;
+  FA_LAUNCH(fa::launch_evict(p, reinterpret_cast<hipStream_t>(a->stream)));
+  return FA_OK;
+}
+
+}  // extern "C"

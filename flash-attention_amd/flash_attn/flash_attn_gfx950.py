@@ -22,7 +22,7 @@ LIB_NAME = "libflash_attn_gfx950.so"
 LIB_PATH = os.path.join(_HERE, LIB_NAME)
 HOST_PATH = os.path.join(_HERE, "fa_host.so")
 
-FA_FP16, FA_BF16 = 0, 1
+FA_FP16, FA_BF16, FA_FP32 = 0, 1, 2  # (fp32: weights of norms only)
 FA_ABI_VERSION = 5
 
 _c_i32p = ctypes.c_void_p
@@ -119,12 +119,63 @@ class RotaryArgs(ctypes.Structure):
     ]
 
 
+class QkNormArgs(ctypes.Structure):
+    """struct fa_qk_norm_args, field for field."""
+    _fields_ = (
+        [("struct_bytes", ctypes.c_uint32), ("dtype", ctypes.c_int32)] +
+        [(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "cos_table", "sin_table", "positions", "dq_out", "dk_out",
+                                        "dq", "dk", "dq_weight", "dk_weight")] +
+        [(n + s, ctypes.c_int64) for n in ("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk") for s in ("_row_stride", "_head_stride")] +
+        [("n_rows", ctypes.c_int64), ("nheads_q", ctypes.c_int32), ("nheads_k", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+         ("weight_dtype", ctypes.c_int32), ("seqlen", ctypes.c_int32), ("table_rows", ctypes.c_int32), ("eps", ctypes.c_float),
+         ("reserved0", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p)])
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """struct fa_paged_cache, field for field."""
+    _fields_ = (
+        [("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p)] +
+        [(n + s, ctypes.c_int64) for n in ("k", "v") for s in ("_page_stride", "_slot_stride", "_head_stride")] +
+        [("page_table", ctypes.c_void_p), ("table_row_stride", ctypes.c_int64), ("seqlens_k", ctypes.c_void_p), ("cu_seqlens_q", ctypes.c_void_p)] +
+        [(n, ctypes.c_int32) for n in ("n_pages", "page_size", "table_cols", "batch", "nheads_q", "nheads_k", "head_dim", "total_q", "max_seqlen_q",
+                                       "max_seqlen_k")] +
+        [("key_weights", ctypes.c_void_p), ("key_positions", ctypes.c_void_p)])
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """struct fa_paged_append_args, field for field."""
+    _fields_ = (
+        [("struct_bytes", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("cache", PagedCacheArgs)] +
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "q_weight", "k_weight", "cos_table", "sin_table", "positions")] +
+        [(n + s, ctypes.c_int64) for n in ("q", "k", "v", "q_out") for s in ("_row_stride", "_head_stride")] +
+        [("weight_dtype", ctypes.c_int32), ("table_rows", ctypes.c_int32), ("eps", ctypes.c_float), ("reserved0", ctypes.c_int32),
+         ("stream", ctypes.c_void_p)])
+
+
+class PagedFwdArgs(ctypes.Structure):
+    """struct fa_paged_fwd_args, field for field."""
+    _fields_ = (
+        [("struct_bytes", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("cache", PagedCacheArgs)] +
+        [(n, ctypes.c_void_p) for n in ("q", "o", "softmax_lse")] +
+        [(n + s, ctypes.c_int64) for n in ("q", "o") for s in ("_row_stride", "_head_stride")] +
+        [("softmax_scale", ctypes.c_float), ("is_causal", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+         ("stream", ctypes.c_void_p)])
+
+
+class PagedEvictArgs(ctypes.Structure):
+    """struct fa_paged_evict_args, field for field."""
+    _fields_ = [("struct_bytes", ctypes.c_uint32), ("budget", ctypes.c_int32), ("recent", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+                ("cache", PagedCacheArgs), ("next_positions", ctypes.c_void_p), ("new_seqlens_k", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p)]
+
+
 EXPORTED_SYMBOLS = (
     "fa_fwd", "fa_bwd", "fa_fwd_block", "fa_bwd_block", "fa_fwd_block_noalloc", "fa_fwd_workspace_bytes", "fa_bwd_workspace_bytes",
     "fa_round_seqlens", "fa_philox_offset_increment", "fa_last_error", "fa_abi_version",
     "fa_gather_rows", "fa_scatter_rows", "fa_scatter_rows_workspace_bytes", "fa_rotary", "fa_set_launch_policy",
     "fa_keep_words_bytes", "fa_blocksparse_row_order", "fa_bias_grad_reduce", "fa_bias_grad_reduce_ragged", "fa_pad_bias_rows", "fa_padding_rows", "fa_fwd_padded",
-    "fa_token_positions",
+    "fa_token_positions", "fa_qk_norm_rotary", "fa_qk_norm_rotary_bwd", "fa_qk_norm_rotary_bwd_workspace_bytes", "fa_paged_append", "fa_paged_fwd",
+    "fa_paged_fwd_workspace_bytes", "fa_paged_key_weights", "fa_paged_evict", "fa_paged_evict_workspace_bytes",
 )
 # declared in include/flash_attn_gfx950_bench.h: instrumentation for bench.py, not part of the drop-in boundary
 BENCH_SYMBOLS = ("fa_bwd_profiled",)
@@ -224,6 +275,13 @@ def load_library():
         lib.fa_token_positions.restype = ctypes.c_int
         lib.fa_blocksparse_row_order.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
         lib.fa_blocksparse_row_order.restype = ctypes.c_int
+        for name, args in (("fa_qk_norm_rotary", QkNormArgs), ("fa_qk_norm_rotary_bwd", QkNormArgs), ("fa_paged_append", PagedAppendArgs),
+                           ("fa_paged_fwd", PagedFwdArgs), ("fa_paged_key_weights", PagedFwdArgs), ("fa_paged_evict", PagedEvictArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(args)]
+            getattr(lib, name).restype = ctypes.c_int
+        for name, args in (("fa_qk_norm_rotary_bwd", QkNormArgs), ("fa_paged_fwd", PagedFwdArgs), ("fa_paged_evict", PagedEvictArgs)):
+            getattr(lib, name + "_workspace_bytes").argtypes = [ctypes.POINTER(args)]
+            getattr(lib, name + "_workspace_bytes").restype = ctypes.c_size_t
         lib.fa_set_launch_policy.argtypes = [ctypes.c_int]
         lib.fa_set_launch_policy.restype = ctypes.c_int
         _host = _passes = _load_host(lib)
@@ -971,3 +1029,269 @@ def rotary(src, dst, cos, sin, n_rotated, conjugate=False, positions=None):
     if rc != 0:
         _raise(rc, lib)
     return dst
+
+
+# ---- norm and rotation of queries and keys; the paged cache
+
+def _check_heads(name, t, like, rows, head_dim):
+    """A (rows, heads, head_dim) tensor beside `like`."""
+    _check(t.is_cuda and t.device == like.device and t.dtype == like.dtype, "%s must be a GPU tensor of the others' device and dtype" % name)
+    _check(t.dim() == 3 and t.shape[0] == rows and t.shape[2] == head_dim, "%s has shape %s, expected (%d, heads, %d)" % (name, tuple(t.shape), rows, head_dim))
+    _check(t.stride(2) == 1, "%s must have a contiguous last dimension" % name)
+
+
+def _check_norm(q_weight, k_weight, like, head_dim):
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _check(w.device == like.device and w.dtype in (like.dtype, torch.float32) and tuple(w.shape) == (head_dim,) and w.is_contiguous(),
+               "%s must be a contiguous (%d,) tensor of the tensors' dtype or fp32 on their device" % (name, head_dim))
+    _check(q_weight.dtype == k_weight.dtype, "q_weight and k_weight must have one dtype")
+    return FA_FP32 if q_weight.dtype == torch.float32 else _dtype_code(like)
+
+
+def _check_tables(cos, sin, like, head_dim):
+    _check((cos is None) == (sin is None), "cos and sin come together")
+    if cos is not None:
+        _check(cos.shape == sin.shape and cos.ndim == 2 and cos.shape[0] > 0 and cos.shape[1] == head_dim // 2 and cos.dtype == sin.dtype == like.dtype and
+               cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == like.device,
+               "cos / sin must be contiguous (rows, headdim / 2) tables in the tensors' dtype on their device")
+
+
+def _check_positions(positions, like, rows):
+    if positions is not None:
+        _check(positions.dtype == torch.int32 and positions.numel() == rows and positions.is_contiguous() and positions.device == like.device,
+               "positions must be a contiguous int32 tensor with one entry per row")
+
+
+def _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps):
+    _check(q.is_cuda and q.dim() == 3, "q must be a (rows, heads, head_dim) GPU tensor")
+    rows, _, D = q.shape
+    a = QkNormArgs()
+    a.struct_bytes = ctypes.sizeof(a)
+    a.dtype = _dtype_code(q)
+    _check_heads("q", q, q, rows, D)
+    _check_heads("k", k, q, rows, D)
+    a.weight_dtype = _check_norm(q_weight, k_weight, q, D)
+    _check_tables(cos, sin, q, D)
+    _check_positions(positions, q, rows)
+    if cos is not None and positions is None:
+        _check(0 < seqlen <= cos.shape[0], "the tables have fewer rows than the sequence has positions")
+    a.q, a.k, a.q_weight, a.k_weight = q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr()
+    a.q_row_stride, a.q_head_stride, a.k_row_stride, a.k_head_stride = q.stride(0), q.stride(1), k.stride(0), k.stride(1)
+    if cos is not None:
+        a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    a.positions = positions.data_ptr() if positions is not None else None
+    a.n_rows, a.nheads_q, a.nheads_k, a.head_dim = rows, q.shape[1], k.shape[1], D
+    a.seqlen, a.eps = seqlen, eps
+    a.stream = _stream_handle(q.device)
+    return a
+
+
+def qk_norm_rotary(q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions=None, seqlen=0, eps=1e-6):
+    """Every head's vector of q and k (rows, heads, head_dim) normalised by its root mean square, times q_weight / k_weight, turned by its position (cos and
+    sin None: not turned), into q_out and k_out (which may be q and k) in one pass of fa_qk_norm_rotary.  positions: int32 table rows, or None: row %
+    seqlen."""
+    a = _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps)
+    for name, t, like in (("q_out", q_out, q), ("k_out", k_out, k)):
+        _check_heads(name, t, q, q.shape[0], q.shape[2])
+        _check(t.shape == like.shape, "%s must have the shape of what it is made of" % name)
+    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
+    a.q_out_row_stride, a.q_out_head_stride, a.k_out_row_stride, a.k_out_head_stride = q_out.stride(0), q_out.stride(1), k_out.stride(0), k_out.stride(1)
+    lib = load_library()
+    with _OnDevice(q.device):
+        rc = lib.fa_qk_norm_rotary(ctypes.byref(a))
+    if rc != 0:
+        _raise(rc, lib)
+    return q_out, k_out
+
+
+def qk_norm_rotary_bwd(dq_out, dk_out, q, k, dq, dk, q_weight, k_weight, cos, sin, positions=None, seqlen=0, eps=1e-6):
+    """Gradients through qk_norm_rotary(): q and k as it read them, dq_out and dk_out those of its results; fills dq and dk (which may be dq_out and
+    dk_out) and returns (dq_weight, dk_weight)."""
+    a = _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps)
+    for name, t, like in (("dq_out", dq_out, q), ("dk_out", dk_out, k), ("dq", dq, q), ("dk", dk, k)):
+        _check_heads(name, t, q, q.shape[0], q.shape[2])
+        _check(t.shape == like.shape, "%s must have the shape of the tensor it belongs to" % name)
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_row_stride", t.stride(0))
+        setattr(a, name + "_head_stride", t.stride(1))
+    lib = load_library()
+    with _OnDevice(q.device):
+        dw = torch.empty((2, q.shape[2]), dtype=q_weight.dtype, device=q.device)
+        a.dq_weight, a.dk_weight = dw.data_ptr(), dw.data_ptr() + dw.stride(0) * dw.element_size()
+        if q.shape[0] == 0:
+            return tuple(dw.zero_())
+        ws_bytes = lib.fa_qk_norm_rotary_bwd_workspace_bytes(ctypes.byref(a))
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws_bytes
+        rc = lib.fa_qk_norm_rotary_bwd(ctypes.byref(a))
+    if rc != 0:
+        _raise(rc, lib)
+    return dw[0], dw[1]
+
+
+def _check_seqlens(name, t, batch, device):
+    _check(t.device == device and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == batch and t.is_contiguous(),
+           "%s must be a contiguous int32 tensor with one entry per sequence on the cache's device" % name)
+
+
+def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_weights=None, key_positions=None):
+    """Fills a PagedCacheArgs from a cache's tensors; v_cache may be None where it is not read."""
+    _check(k_cache.is_cuda and k_cache.dim() == 4, "k_cache must be a (pages, page size, heads, head_dim) GPU tensor")
+    n_pages, page_size, heads, D = k_cache.shape
+    _dtype_code(k_cache)
+    for name, t in (("k", k_cache), ("v", v_cache)):
+        if t is None:
+            continue
+        _check(t.device == k_cache.device and t.dtype == k_cache.dtype and t.shape == k_cache.shape and t.stride(3) == 1,
+               "k_cache and v_cache must be (pages, page size, heads, head_dim) tensors of one shape, dtype and device, contiguous in the last dimension")
+        setattr(a, name + "_cache", t.data_ptr())
+        setattr(a, name + "_page_stride", t.stride(0))
+        setattr(a, name + "_slot_stride", t.stride(1))
+        setattr(a, name + "_head_stride", t.stride(2))
+    _check(page_table.device == k_cache.device and page_table.dtype == torch.int32 and page_table.dim() == 2 and
+           (page_table.stride(1) == 1 or page_table.shape[1] == 1), "page_table must be a (batch, pages) int32 tensor with contiguous rows on the cache's device")
+    batch, cols = page_table.shape
+    _check(batch > 0 and cols > 0, "page_table must have a row for each sequence and a page in each")
+    _check_seqlens("seqlens_k", seqlens_k, batch, k_cache.device)
+    a.page_table, a.table_row_stride, a.table_cols = page_table.data_ptr(), (page_table.stride(0) if batch > 1 else cols), cols
+    a.seqlens_k = seqlens_k.data_ptr()
+    a.n_pages, a.page_size, a.batch, a.nheads_k, a.head_dim, a.max_seqlen_k = n_pages, page_size, batch, heads, D, int(max_seqlen_k)
+    for name, t, dtype in (("key_weights", key_weights, torch.float32), ("key_positions", key_positions, torch.int32)):
+        if t is not None:
+            _check(t.device == k_cache.device and t.dtype == dtype and tuple(t.shape) == (n_pages, heads, page_size) and t.is_contiguous(),
+                   "%s must be a contiguous (pages, heads, page size) tensor of %s on the cache's device" % (name, dtype))
+            setattr(a, name, t.data_ptr())
+
+
+def _paged_queries(a, q, k_cache, cu_seqlens_q, max_seqlen_q):
+    _check(q.is_cuda and q.device == k_cache.device and q.dtype == k_cache.dtype and q.dim() == 3 and q.shape[2] == k_cache.shape[3] and q.stride(2) == 1,
+           "q must be a (total, heads, head_dim) tensor of the cache's dtype and device, contiguous in the last dimension")
+    _check(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "the query heads must be a multiple of the key heads")
+    _check_cu("cu_seqlens_q", cu_seqlens_q, a.batch)
+    _check(cu_seqlens_q.device == k_cache.device, "cu_seqlens_q must be on the cache's device")
+    a.cu_seqlens_q, a.nheads_q, a.total_q, a.max_seqlen_q = cu_seqlens_q.data_ptr(), q.shape[1], q.shape[0], int(max_seqlen_q)
+
+
+def paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, q_out=None, q_weight=None, k_weight=None, cos=None, sin=None,
+                 positions=None, eps=1e-6, key_weights=None, key_positions=None):
+    """Stores the new tokens' k and v (total, heads, head_dim) into the pages of their sequences and returns q_out: fa_paged_append.  q may be None."""
+    lib = load_library()
+    a = PagedAppendArgs()
+    a.struct_bytes = ctypes.sizeof(a)
+    c = a.cache
+    _check(k_cache.dim() == 4, "k_cache must be a (pages, page size, heads, head_dim) GPU tensor")
+    total, D = k.shape[0], k_cache.shape[3]
+    _paged_cache(c, k_cache, v_cache, page_table, seqlens_k, page_table.shape[-1] * k_cache.shape[1], key_weights, key_positions)
+    a.dtype = _dtype_code(k_cache)
+    for name, t in (("k", k), ("v", v)):
+        _check_heads(name, t, k_cache, total, D)
+        _check(t.shape[1] == k_cache.shape[2], "%s must have the cache's heads" % name)
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_row_stride", t.stride(0))
+        setattr(a, name + "_head_stride", t.stride(1))
+    _check_cu("cu_seqlens_q", cu_seqlens_q, c.batch)
+    _check(cu_seqlens_q.device == k_cache.device, "cu_seqlens_q must be on the cache's device")
+    c.cu_seqlens_q, c.nheads_q, c.total_q, c.max_seqlen_q = cu_seqlens_q.data_ptr(), c.nheads_k, total, max(total, 1)
+    _check((q_weight is None) == (k_weight is None), "q_weight and k_weight come together")
+    if k_weight is not None:
+        a.weight_dtype = _check_norm(q_weight, k_weight, k_cache, D)
+        a.q_weight, a.k_weight = q_weight.data_ptr(), k_weight.data_ptr()
+    _check_tables(cos, sin, k_cache, D)
+    if cos is not None:
+        a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    _check_positions(positions, k_cache, total)
+    a.positions = positions.data_ptr() if positions is not None else None
+    a.eps = eps
+    with _OnDevice(k_cache.device):
+        if q is not None:
+            _check_heads("q", q, k_cache, total, D)
+            _check(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "the query heads must be a multiple of the key heads")
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            _check_heads("q_out", q_out, k_cache, total, D)
+            _check(q_out.shape == q.shape, "q_out must have q's shape")
+            c.nheads_q, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
+            a.q_row_stride, a.q_head_stride, a.q_out_row_stride, a.q_out_head_stride = q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
+        a.stream = _stream_handle(k_cache.device)
+        rc = lib.fa_paged_append(ctypes.byref(a))
+    if rc != 0:
+        _raise(rc, lib)
+    return q_out
+
+
+def paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, return_lse=False, out=None):
+    """Attention of the new tokens' q (total, heads, head_dim) over a paged cache: [o] or [o, softmax_lse] (fa_paged_fwd)."""
+    lib = load_library()
+    a = PagedFwdArgs()
+    a.struct_bytes = ctypes.sizeof(a)
+    _paged_cache(a.cache, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k)
+    _paged_queries(a.cache, q, k_cache, cu_seqlens_q, max_seqlen_q)
+    a.dtype = _dtype_code(q)
+    dev = q.device
+    with _OnDevice(dev):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        _check_heads("out", out, q, q.shape[0], q.shape[2])
+        _check(out.shape == q.shape, "out must have q's shape")
+        lse = None
+        if return_lse:
+            lse = torch.empty((a.cache.batch, q.shape[1], (int(max_seqlen_q) + 15) // 16 * 16), dtype=torch.float32, device=dev)
+            a.softmax_lse = lse.data_ptr()
+        a.q, a.o = q.data_ptr(), out.data_ptr()
+        a.q_row_stride, a.q_head_stride, a.o_row_stride, a.o_head_stride = q.stride(0), q.stride(1), out.stride(0), out.stride(1)
+        a.softmax_scale, a.is_causal = float(softmax_scale), int(bool(is_causal))
+        a.workspace_bytes = lib.fa_paged_fwd_workspace_bytes(ctypes.byref(a))
+        ws = torch.empty((a.workspace_bytes,), dtype=torch.uint8, device=dev) if a.workspace_bytes else None
+        a.workspace = ws.data_ptr() if ws is not None else None
+        a.stream = _stream_handle(dev)
+        rc = lib.fa_paged_fwd(ctypes.byref(a))
+    if rc != 0:
+        _raise(rc, lib)
+    return [out, lse] if return_lse else [out]
+
+
+def paged_key_weights(q, softmax_lse, k_cache, key_weights, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal):
+    """Adds what every cached key receives of the new tokens' attention to key_weights (fa_paged_key_weights); q and softmax_lse: those of paged_fwd."""
+    lib = load_library()
+    a = PagedFwdArgs()
+    a.struct_bytes = ctypes.sizeof(a)
+    _check(key_weights is not None, "key_weights is required")
+    _paged_cache(a.cache, k_cache, None, page_table, seqlens_k, max_seqlen_k, key_weights)
+    _paged_queries(a.cache, q, k_cache, cu_seqlens_q, max_seqlen_q)
+    _check(softmax_lse.device == q.device and softmax_lse.dtype == torch.float32 and softmax_lse.is_contiguous() and
+           tuple(softmax_lse.shape) == (a.cache.batch, q.shape[1], (int(max_seqlen_q) + 15) // 16 * 16),
+           "softmax_lse must be the contiguous fp32 (batch, heads, max_seqlen_q rounded up to 16) tensor of the forward")
+    a.dtype = _dtype_code(q)
+    a.q, a.softmax_lse = q.data_ptr(), softmax_lse.data_ptr()
+    a.q_row_stride, a.q_head_stride = q.stride(0), q.stride(1)
+    a.softmax_scale, a.is_causal = float(softmax_scale), int(bool(is_causal))
+    a.stream = _stream_handle(q.device)
+    with _OnDevice(q.device):
+        rc = lib.fa_paged_key_weights(ctypes.byref(a))
+    if rc != 0:
+        _raise(rc, lib)
+    return key_weights
+
+
+def paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k):
+    """Cuts the caches to `budget` keys a head, in place; returns the new lengths (fa_paged_evict)."""
+    lib = load_library()
+    a = PagedEvictArgs()
+    a.struct_bytes = ctypes.sizeof(a)
+    _check(key_weights is not None and key_positions is not None, "key_weights and key_positions are required")
+    _check(k_cache.dim() == 4 and v_cache is not None, "k_cache and v_cache must be (pages, page size, heads, head_dim) GPU tensors")
+    _paged_cache(a.cache, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_weights, key_positions)
+    _check_seqlens("next_positions", next_positions, a.cache.batch, k_cache.device)
+    a.budget, a.recent = int(budget), int(recent)
+    dev = k_cache.device
+    with _OnDevice(dev):
+        new_seqlens = torch.empty_like(seqlens_k)
+        a.next_positions, a.new_seqlens_k = next_positions.data_ptr(), new_seqlens.data_ptr()
+        a.workspace_bytes = lib.fa_paged_evict_workspace_bytes(ctypes.byref(a))
+        ws = torch.empty((max(a.workspace_bytes, 4),), dtype=torch.uint8, device=dev)
+        a.workspace = ws.data_ptr()
+        a.stream = _stream_handle(dev)
+        rc = lib.fa_paged_evict(ctypes.byref(a))
+    if rc != 0:
+        _raise(rc, lib)
+    return new_seqlens

@@ -56,6 +56,57 @@ def apply_rotary_emb_qkv_(qkv, cos_half, sin_half):
     return _ApplyRotaryQKV.apply(qkv, cos_half, sin_half)
 
 
+class _QkNormRotary(torch.autograd.Function):
+    """q and k normalised, weighted and turned; the backward forms the norms again from q and k, so nothing but the inputs is kept."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos_half, sin_half, positions, seqlen, eps):
+        from . import flash_attn_gfx950 as backend
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        backend.qk_norm_rotary(q, k, q_out, k_out, q_weight, k_weight, cos_half, sin_half, positions, seqlen, eps)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos_half, sin_half, positions)
+        ctx.seqlen, ctx.eps = seqlen, eps
+        return q_out, k_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        from . import flash_attn_gfx950 as backend
+        q, k, q_weight, k_weight, cos_half, sin_half, positions = ctx.saved_tensors
+        dq_out, dk_out = _kernel_rows(dq_out), _kernel_rows(dk_out)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dqw, dkw = backend.qk_norm_rotary_bwd(dq_out, dk_out, q, k, dq, dk, q_weight, k_weight, cos_half, sin_half, positions, ctx.seqlen, ctx.eps)
+        return dq, dk, dqw, dkw, None, None, None, None, None
+
+
+def _kernel_rows(t):
+    """t as the kernels read a (rows, heads, headdim) tensor: itself, or a contiguous copy where its strides or its address are not theirs."""
+    ok = t.stride(2) == 1 and all(0 <= s < 1 << 24 and s % 8 == 0 for s in t.stride()[:2]) and t.data_ptr() % 16 == 0
+    return t if ok else t.contiguous()
+
+
+def apply_qk_norm_rotary(q, k, q_weight, k_weight, cos_half=None, sin_half=None, positions=None, eps=1e-6):
+    """Queries and keys as attention wants them: every head's vector divided by its root mean square, times the headdim weights, then turned by its
+    position (cos_half, sin_half: RotaryEmbedding.half_tables; None: not turned), in one pass, products in fp32, rounded once.
+    q: (total, nheads, headdim) or (batch, seqlen, nheads, headdim), k the same with its own number of heads, fp16 or bf16, headdim 16, 32, 64 or 128;
+    q_weight, k_weight: (headdim,) in the tensors' dtype or fp32.  positions: int32, one table row for each row of q (entries outside the tables are
+    clamped to them); None: the place in the sequence, for tensors with a seqlen dimension or a single packed sequence.
+    Returns (q', k'), new tensors; differentiable in q, k and the weights."""
+    if q.dim() == 4:
+        b, s = q.shape[:2]
+        if k.dim() != 4 or tuple(k.shape[:2]) != (b, s):
+            raise RuntimeError("q and k must both be (batch, seqlen, heads, headdim)")
+        flat = None if positions is None else positions.reshape(-1)
+        q2, k2 = _QkNormRotary.apply(_kernel_rows(q.reshape(b * s, *q.shape[2:])), _kernel_rows(k.reshape(b * s, *k.shape[2:])), q_weight, k_weight, cos_half,
+                                     sin_half, flat, s, eps)
+        return q2.reshape(q.shape), k2.reshape(k.shape)
+    if q.dim() != 3 or k.dim() != 3:
+        raise RuntimeError("q and k must be (total, heads, headdim) or (batch, seqlen, heads, headdim)")
+    return _QkNormRotary.apply(_kernel_rows(q), _kernel_rows(k), q_weight, k_weight, cos_half, sin_half, positions, q.shape[0], eps)
+
+
 class RotaryEmbedding(torch.nn.Module):
     """Rotary embedding of RoFormer (Su et al., arXiv:2104.09864) for queries and keys."""
 

@@ -321,6 +321,132 @@ int fa_rotary(const fa_rotary_args* args);
  * total rows, b the sequence row i lies in (rows behind the last sequence count on from its end).  cu_seqlens: batch + 1 int32. */
 int fa_token_positions(const int32_t* cu_seqlens, int32_t batch, int32_t total, int32_t* positions, void* stream);
 
+/* ---- Serving with a paged key / value cache, and the norm of queries and keys in front of it (no counterparts in the reference) ----
+ *
+ * fa_qk_norm_rotary: every head's vector x of q and k becomes R_t (w * x / sqrt(mean(x^2) + eps)), w the head_dim weights of q or of k (shared
+ * by the heads) and R_t the rotation of fa_rotary by table row t.  fp32 between one read and one rounding.  q, k, q_out, k_out: [n_rows,
+ * nheads_q or nheads_k, head_dim], strides in elements, innermost 1, multiples of 8; 16-byte aligned; q_out / k_out may be q / k with the same
+ * strides.  weight_dtype: enum fa_dtype, or FA_FP32.  Tables as in fa_rotary, or both NULL (no rotation); t = positions[row], clamped to
+ * the table, or row % seqlen.  The backward takes q, k (as the forward read them) and dq_out, dk_out, and writes dq, dk (which may be dq_out,
+ * dk_out with the same strides) and dq_weight, dk_weight ([head_dim], weight_dtype; summed in fp32 in a fixed order).  workspace: of
+ * fa_qk_norm_rotary_bwd_workspace_bytes() bytes, 16-byte aligned; the forward needs none. */
+#define FA_FP32 2 /* weights only */
+typedef struct fa_qk_norm_args {
+  uint32_t struct_bytes;
+  int32_t dtype;
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void *q_weight, *k_weight;
+  const void *cos_table, *sin_table;
+  const int32_t* positions;
+  const void *dq_out, *dk_out;
+  void *dq, *dk;
+  void *dq_weight, *dk_weight;
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
+  int64_t q_out_row_stride, q_out_head_stride, k_out_row_stride, k_out_head_stride;
+  int64_t dq_out_row_stride, dq_out_head_stride, dk_out_row_stride, dk_out_head_stride;
+  int64_t dq_row_stride, dq_head_stride, dk_row_stride, dk_head_stride;
+  int64_t n_rows;
+  int32_t nheads_q, nheads_k, head_dim, weight_dtype;
+  int32_t seqlen, table_rows;
+  float eps;
+  int32_t reserved0; /* 0 */
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+} fa_qk_norm_args;
+int fa_qk_norm_rotary(const fa_qk_norm_args* args);
+int fa_qk_norm_rotary_bwd(const fa_qk_norm_args* args);
+size_t fa_qk_norm_rotary_bwd_workspace_bytes(const fa_qk_norm_args* args);
+
+/* A paged cache.  Key (and value) j of sequence b and key head h is k_cache + page * page_stride + (j % page_size) * slot_stride + h *
+ * head_stride (elements; multiples of 8, innermost 1; 16-byte aligned), page = page_table[b * table_row_stride + j / page_size].  page_size is a
+ * power of two from 16 to 1024.  seqlens_k: batch int32, keys per sequence, the new tokens' among them; row i of the seqlen_q = cu_seqlens_q[b + 1] -
+ * cu_seqlens_q[b] new tokens of sequence b is its token number seqlens_k[b] - seqlen_q + i.  Query head h attends with key head h / (nheads_q /
+ * nheads_k).  Nothing that lies in device memory is trusted with an address: a length counts at most max_seqlen_k and table_cols * page_size
+ * keys, an entry of page_table outside [0, n_pages) stands for page 0 or n_pages - 1 when it is read and drops what would be stored there.  Pages
+ * that several sequences list may be read, not written. */
+typedef struct fa_paged_cache {
+  void* k_cache;
+  void* v_cache;
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  const int32_t* page_table;
+  int64_t table_row_stride;
+  const int32_t* seqlens_k;
+  const int32_t* cu_seqlens_q; /* batch + 1 */
+  int32_t n_pages, page_size, table_cols;
+  int32_t batch, nheads_q, nheads_k, head_dim;
+  int32_t total_q, max_seqlen_q, max_seqlen_k;
+  float* key_weights;     /* [n_pages, nheads_k, page_size] contiguous: attention weight a key has received */
+  int32_t* key_positions; /* the same shape: the key's position in its sequence, as counted when it was stored */
+} fa_paged_cache;
+
+/* Stores the new tokens' k and v ([total_q, nheads_k, head_dim]) into the cache; k through the map of fa_qk_norm_rotary if k_weight or cos_table is
+ * given, and q, if it is, through the same into q_out.  A token's table row is positions[row] or its number in the sequence.  key_weights
+ * and key_positions, where given, become 0 and that position.  Rows behind the last sequence and tokens whose slot is none are not stored (and
+ * their q_out rows are left as they were). */
+typedef struct fa_paged_append_args {
+  uint32_t struct_bytes;
+  int32_t dtype;
+  fa_paged_cache cache;
+  const void *q, *k, *v;
+  void* q_out;
+  const void *q_weight, *k_weight; /* both or neither */
+  const void *cos_table, *sin_table;
+  const int32_t* positions;
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride, q_out_row_stride, q_out_head_stride;
+  int32_t weight_dtype, table_rows;
+  float eps;
+  int32_t reserved0; /* 0 */
+  void* stream;
+} fa_paged_append_args;
+int fa_paged_append(const fa_paged_append_args* args);
+
+/* Attention of the new tokens over their sequences' pages.  is_causal: row i sees keys 0 .. seqlens_k[b] - seqlen_q + i (the mask is
+ * aligned at the end, unlike fa_fwd's, whose queries and keys begin together); else every key.  A row that sees none gives zeros and -inf.
+ * softmax_lse: NULL, or [batch, nheads_q, max_seqlen_q rounded up to 16] fp32.  workspace: fa_paged_fwd_workspace_bytes() bytes, 16-byte aligned,
+ * its contents on entry do not matter; the size depends on the struct's integers alone, not on the lengths in device memory. */
+typedef struct fa_paged_fwd_args {
+  uint32_t struct_bytes;
+  int32_t dtype;
+  fa_paged_cache cache;
+  const void* q;
+  void* o;
+  float* softmax_lse;
+  int64_t q_row_stride, q_head_stride, o_row_stride, o_head_stride;
+  float softmax_scale;
+  int32_t is_causal;
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+} fa_paged_fwd_args;
+int fa_paged_fwd(const fa_paged_fwd_args* args);
+size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_args* args);
+
+/* key_weights of every key += the sum over the new tokens and the query heads of its group of exp(softmax_scale * q.k - softmax_lse), q and
+ * softmax_lse being those of fa_paged_fwd over the same cache (o and workspace are not read).  One owner per key: reproducible bit for bit. */
+int fa_paged_key_weights(const fa_paged_fwd_args* args);
+
+/* Cuts the sequences' caches to `budget` keys per head (nothing happens to shorter ones): the keys whose position is at least next_positions[b] -
+ * recent stay, then the ones with the largest key_weights (NaN counts as -inf; ties: the lower slot; should more than `budget` be recent, those in
+ * the lowest slots).  The n-th slot below `budget` whose key goes takes the n-th key from behind it that stays, with its value, weight and position;
+ * slots from `budget` on are left as they were.  Each key head chooses for itself.  new_seqlens_k: batch int32, min(seqlens_k, budget); may
+ * not be seqlens_k.  cu_seqlens_q, nheads_q, total_q and max_seqlen_q are not read.  workspace: fa_paged_evict_workspace_bytes() bytes. */
+typedef struct fa_paged_evict_args {
+  uint32_t struct_bytes;
+  int32_t budget, recent;
+  int32_t reserved0; /* 0 */
+  fa_paged_cache cache;
+  const int32_t* next_positions;
+  int32_t* new_seqlens_k;
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+} fa_paged_evict_args;
+int fa_paged_evict(const fa_paged_evict_args* args);
+size_t fa_paged_evict_workspace_bytes(const fa_paged_evict_args* args);
+
 /* Host-side helper of the block-sparse entry points (no GPU work, no counterpart in the reference): an order of the 16-row
  * blocks for fa_fwd_args.row_order / fa_bwd_args.row_order that puts row blocks with similar key-block lists into the same
  * workgroup (eight consecutive entries) and wave (two).  layout: HOST array [n_row_blocks][n_col_blocks] of bytes, non-zero
