@@ -45,6 +45,7 @@ struct NormParams {
   int n_rows, seqlen, table_rows;
   float eps;
   int w_fp32;
+  int rows;        // in flight
   float* partial;  // backward: [blocks of both parts][D] sums of the weights' gradients
 };
 
@@ -73,8 +74,9 @@ FA_DEVICE typename Elem<T>::vec8 to_elem(const float (&x)[8]) {
   return v;
 }
 
-// Rows a thread has in flight.
+// Rows a thread of the forward has in flight: one where there are few, whose time is a chain of latencies.
 constexpr int kNormRows = 4;
+inline int norm_rows(int64_t n_rows, int heads, int D) { return n_rows * heads * (D / 8) <= 256 * 1024 ? 1 : kNormRows; }
 
 struct Place {  // of a thread in its part
   int row0, step, head, ch;
@@ -95,7 +97,7 @@ FA_DEVICE Place place_of(const NormPart& q, int block) {
   return pl;
 }
 
-template <typename T, int D, bool kTurn>
+template <typename T, int D, bool kTurn, int kRows>
 __global__ void __launch_bounds__(512) qk_norm_rotary_kernel(const NormParams p) {
   constexpr int CH = D / 8;
   const bool second = (int)blockIdx.x >= p.part[1].first_block;
@@ -106,27 +108,29 @@ __global__ void __launch_bounds__(512) qk_norm_rotary_kernel(const NormParams p)
   load_weights<T>(q.w, p.w_fp32 != 0, pl.ch, w);
   const T* const src = reinterpret_cast<const T*>(q.x) + (int64_t)pl.head * q.x_hs + pl.ch * 8;
   T* const dst = reinterpret_cast<T*>(q.out) + (int64_t)pl.head * q.out_hs + pl.ch * 8;
-  typename Elem<T>::vec8 v[kNormRows];
-  Turned<T> t[kNormRows];
+  for (int64_t row0 = pl.row0; row0 < p.n_rows; row0 += (int64_t)kRows * pl.step) {
+    typename Elem<T>::vec8 v[kRows];
+    Turned<T> t[kRows];
 #pragma unroll
-  for (int i = 0; i < kNormRows; i++) {
-    const int64_t row = (int64_t)pl.row0 + (int64_t)i * pl.step;
-    if (row < p.n_rows) {
-      v[i] = bitcast<typename Elem<T>::vec8>(ld_global16(src + row * q.x_rs));
-      if (kTurn) t[i].load(p, (int)row, pl.ch, D / 2);
+    for (int i = 0; i < kRows; i++) {
+      const int64_t row = row0 + (int64_t)i * pl.step;
+      if (row < p.n_rows) {
+        v[i] = bitcast<typename Elem<T>::vec8>(ld_global16(src + row * q.x_rs));
+        if (kTurn) t[i].load(p, (int)row, pl.ch, D / 2);
+      }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < kNormRows; i++) {
-    const int64_t row = (int64_t)pl.row0 + (int64_t)i * pl.step;
-    if (row < p.n_rows) {
-      float x[8];
-      to_float(v[i], x);
-      const float r = inverse_rms<CH>(x, p.eps);
+    for (int i = 0; i < kRows; i++) {
+      const int64_t row = row0 + (int64_t)i * pl.step;
+      if (row < p.n_rows) {
+        float x[8];
+        to_float(v[i], x);
+        const float r = inverse_rms<CH>(x, p.eps);
 #pragma unroll
-      for (int k = 0; k < 8; k++) x[k] = x[k] * r * w[k];
-      if (kTurn) turn(x, t[i].c, t[i].s);
-      st_global16(dst + row * q.out_rs, bitcast<u32x4>(to_elem<T>(x)));
+        for (int k = 0; k < 8; k++) x[k] = x[k] * r * w[k];
+        if (kTurn) turn(x, t[i].c, t[i].s);
+        st_global16(dst + row * q.out_rs, bitcast<u32x4>(to_elem<T>(x)));
+      }
     }
   }
 }
@@ -196,27 +200,33 @@ __global__ void __launch_bounds__(512) qk_norm_rotary_bwd_kernel(const NormParam
   }
 }
 
-// The workgroups' sums added up: a workgroup for 16 weights of one part, 16 rows of 16 lanes, joined in LDS.  A fixed order.
+// The workgroups' sums added up: a workgroup for 16 weights of one part, 64 rows of 16 lanes, joined in LDS.  A fixed order.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_weights_kernel(const NormParams p, int D) {
-  __shared__ float sums[256];
+__global__ void __launch_bounds__(1024) norm_weights_kernel(const NormParams p, int D) {
+  __shared__ float sums[1024];
   const int cols = D / 16;
   const NormPart& q = p.part[(int)blockIdx.x / cols];
   const int col = (int)blockIdx.x % cols * 16 + (threadIdx.x & 15);
+  const float* const from = p.partial + (int64_t)q.first_block * D + col;
   float s = 0.f;
-  for (int b = threadIdx.x >> 4; b < q.blocks; b += 16) s += p.partial[(int64_t)(q.first_block + b) * D + col];
+#pragma unroll 4
+  for (int b = threadIdx.x >> 4; b < q.blocks; b += 64) s += from[(int64_t)b * D];
   sums[threadIdx.x] = s;
   __syncthreads();
+  for (int half = 512; half >= 16; half >>= 1) {
+    if ((int)threadIdx.x < half) sums[threadIdx.x] += sums[threadIdx.x + half];
+    __syncthreads();
+  }
   if (threadIdx.x < 16) {
-    for (int i = 1; i < 16; i++) s += sums[i * 16 + threadIdx.x];
+    s = sums[threadIdx.x];
     if (p.w_fp32) reinterpret_cast<float*>(q.dw)[col] = s;
     else reinterpret_cast<T*>(q.dw)[col] = (T)s;
   }
 }
 
-// How the launches are cut: rows_in_flight rows per thread of the forward; the backward's workgroups stay and walk on (each leaves a row of
-// sums): at most kNormBwdBlocks for both parts, shared by their sizes.
-constexpr int kNormBwdBlocks = 1024;
+// How the launches are cut.  At most kNormBlocks workgroups for both parts, shared by their sizes, which walk on over the rows: the forward of 32768 rows
+// of 20 heads, d = 128 71 us (4.7 TB/s), with 2048 of them 78, a workgroup for every four rows 85; and the backward's each leave a row of sums.
+constexpr int kNormBlocks = 1024;
 
 void cut(NormPart* part, int heads, int D, int n_rows, int rows_in_flight, int most_blocks, int first_block) {
   part->heads = heads;
@@ -247,10 +257,12 @@ int block_threads(const NormParams& p) {
 int cut_parts(NormParams* p, const fa_qk_norm_args* a, bool bwd) {
   const int n = (int)a->n_rows, D = a->head_dim, all = std::max(1, a->nheads_q + a->nheads_k);
   // (pieces of a row are 256 threads wide: parts that share a launch with a wider one keep to rows of their own)
-  const int64_t q_share = bwd ? std::max<int64_t>(1, (int64_t)kNormBwdBlocks * a->nheads_q / all) : 0;
-  const int64_t k_share = bwd ? std::max<int64_t>(1, (int64_t)kNormBwdBlocks * a->nheads_k / all) : 0;
-  cut(&p->part[0], a->nheads_q, D, n, bwd ? kNormBwdRows : kNormRows, (int)q_share, 0);
-  cut(&p->part[1], a->nheads_k, D, n, bwd ? kNormBwdRows : kNormRows, (int)k_share, p->part[0].blocks);
+  const int64_t most = kNormBlocks;
+  const int64_t q_share = std::max<int64_t>(1, most * a->nheads_q / all), k_share = std::max<int64_t>(1, most * a->nheads_k / all);
+  const int rows = bwd ? kNormBwdRows : norm_rows(n, all, D);
+  cut(&p->part[0], a->nheads_q, D, n, rows, (int)q_share, 0);
+  cut(&p->part[1], a->nheads_k, D, n, rows, (int)k_share, p->part[0].blocks);
+  p->rows = rows;
   return p->part[0].blocks + p->part[1].blocks;
 }
 
@@ -324,19 +336,20 @@ NormParams params(const fa_qk_norm_args* a, bool bwd) {
   return p;
 }
 
-#define FA_NORM_LAUNCH(KERNEL, T, D)                                                                              \
-  do {                                                                                                            \
-    if (p.cos) hipLaunchKernelGGL((KERNEL<T, D, true>), dim3(blocks), dim3(threads), 0, stream, p);               \
-    else hipLaunchKernelGGL((KERNEL<T, D, false>), dim3(blocks), dim3(threads), 0, stream, p);                    \
-  } while (0)
+template <typename T, int D, bool kTurn>
+void launch_norm_d(const NormParams& p, int blocks, int threads, bool bwd, hipStream_t stream) {
+  if (bwd) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, D, kTurn>), dim3(blocks), dim3(threads), 0, stream, p);
+  else if (p.rows == 1) hipLaunchKernelGGL((qk_norm_rotary_kernel<T, D, kTurn, 1>), dim3(blocks), dim3(threads), 0, stream, p);
+  else hipLaunchKernelGGL((qk_norm_rotary_kernel<T, D, kTurn, kNormRows>), dim3(blocks), dim3(threads), 0, stream, p);
+}
 
 template <typename T>
 hipError_t launch_norm(const NormParams& p, int D, int blocks, bool bwd, hipStream_t stream) {
   const int threads = block_threads(p);
-#define FA_NORM_D(D_)                                               \
-  case D_:                                                          \
-    if (bwd) FA_NORM_LAUNCH(qk_norm_rotary_bwd_kernel, T, D_);      \
-    else FA_NORM_LAUNCH(qk_norm_rotary_kernel, T, D_);              \
+#define FA_NORM_D(D_)                                                           \
+  case D_:                                                                      \
+    if (p.cos) launch_norm_d<T, D_, true>(p, blocks, threads, bwd, stream);     \
+    else launch_norm_d<T, D_, false>(p, blocks, threads, bwd, stream);          \
     break;
   switch (D) {
     FA_NORM_D(16)
@@ -349,7 +362,7 @@ hipError_t launch_norm(const NormParams& p, int D, int blocks, bool bwd, hipStre
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !bwd) return e;
   const int parts = p.part[1].heads > 0 ? 2 : 1;
-  hipLaunchKernelGGL(norm_weights_kernel<T>, dim3((unsigned)(parts * (D / 16))), dim3(256), 0, stream, p, D);
+  hipLaunchKernelGGL(norm_weights_kernel<T>, dim3((unsigned)(parts * (D / 16))), dim3(1024), 0, stream, p, D);
   return hipGetLastError();
 }
 

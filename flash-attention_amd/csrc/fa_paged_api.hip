@@ -14,7 +14,9 @@ namespace {
 struct Plan {
   bool decode;
   int groups, least;       // decode (fa_paged_decode.hip)
+  bool wide;               // ... eight (d = 128: four) waves a workgroup
   int nq_tiles, n_splits;  // chunk (fa_paged_chunk.hip)
+  bool deal;
   size_t bytes;
 };
 
@@ -29,8 +31,9 @@ Plan plan_of(const fa_paged_cache& c) {
   pl.decode = rows <= fa::kDecodeMaxQ;
   if (pl.decode) {
     const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
+    pl.wide = pairs <= 256 && max_keys <= 128 * fa::kDecodeWide(c.head_dim);
     pl.least = 2;
-    if (units <= pl.least) pl.least = 0;  // a workgroup a pair
+    if (units <= pl.least || pl.wide) pl.least = 0;  // a workgroup a pair
     else {
       pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim), (pairs * units + pl.least - 1) / pl.least);
       pl.bytes = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
@@ -40,9 +43,12 @@ Plan plan_of(const fa_paged_cache& c) {
   pl.nq_tiles = (rows + fa::kChunkRows - 1) / fa::kChunkRows;
   const int64_t items = pairs * pl.nq_tiles;
   const int tiles = (max_keys + 63) / 64;
-  // fewer row tiles than would fill the compute units twice share their keys, at least four tiles of them each
-  int64_t n = items >= 384 ? 1 : (768 + items - 1) / items;
-  n = std::min<int64_t>({n, tiles / 4, 64});
+  pl.deal = pairs % 8 == 0 || pairs >= 48;  // (else one XCD would have a quarter more of them than another, or none)
+  // Row tiles that do not fill the compute units share their keys, at least 512 of them each, so that there are two workgroups a compute unit.  us with
+  // 512 workgroups and 512 keys / 768 and 256 (d = 128, 8 key heads of 32 heads): 64 tokens behind 16000 49.5 / 59.2, 512 behind 7700 101 / 99.5;
+  // d = 64: 3 x 100 tokens behind 6000, 12 heads 29.4 / 35.9, 2 x 200 behind 1800 28.6 / 31.3.
+  int64_t n = items >= 384 ? 1 : (512 + items - 1) / items;
+  n = std::min<int64_t>({n, tiles / 8, 64});
   pl.n_splits = n < 2 ? 1 : (int)n;
   if (pl.n_splits > 1) pl.bytes = (size_t)pl.n_splits * items * fa::kChunkRows * (c.head_dim + 3) * 4;
   return pl;
@@ -104,8 +110,10 @@ int fa_paged_fwd(const fa_paged_fwd_args* a) {
   fa::PagedFwdParams p = params(a);
   p.groups = pl.groups;
   p.least = pl.least;
+  p.wide = pl.wide;
   p.nq_tiles = pl.nq_tiles;
   p.n_splits = pl.n_splits;
+  p.deal = pl.deal;
   p.part = reinterpret_cast<float*>(a->workspace);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(a->stream);
   if (pl.decode) FA_LAUNCH(fa::launch_paged_decode(p, a->dtype, a->cache.head_dim, stream));

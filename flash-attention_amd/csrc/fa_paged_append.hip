@@ -25,25 +25,11 @@ struct AppendParams {
   int w_fp32, table_rows;
   float eps;
   int q_heads;  // 0 without q
-  int per_row, pieces;
+  int per_row, pieces, threads;
 };
 
-// The sequence that row `row` of the packed batch belongs to (B: none); row is wave-uniform.  cu is non-decreasing: the number of sequences
-// that end at or before the row.
-FA_DEVICE int sequence_of(const int32_t* cu, int B, int row) {
-  const int lane = threadIdx.x & 63;
-  int b = 0;
-  for (int at = 0; at < B; at += 64) {
-    const int i = at + lane;
-    const int n = __popcll(__ballot(i < B && cu[i + 1 < B ? i + 1 : B] <= row));
-    b += n;
-    if (n < 64) break;
-  }
-  return b;
-}
-
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p) {
   constexpr int CH = D / 8;
   using vec8 = typename Elem<T>::vec8;
   const int group = blockIdx.x / p.pieces, piece = blockIdx.x - group * p.pieces;
@@ -64,19 +50,45 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
   const bool norm = p.kw != nullptr && part < 2, rot = p.cos != nullptr && part < 2;
   float w[8];
   if (on && norm) load_weights<T>(part == 0 ? p.qw : p.kw, p.w_fp32 != 0, ch, w);
+  // Where the rows go, wave-uniform and for all of them at once: their sequences (cu is non-decreasing: as many as end at or before the row; a load
+  // and a ballot for 64 of them), then lengths, then pages.
+  int seq[ROWS], slot[ROWS], page[ROWS], pos[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) seq[i] = 0;
+  for (int at = 0; at < p.c.B; at += 64) {
+    const int s = at + (threadIdx.x & 63);
+    const int end = p.c.cu_q[s < p.c.B ? s + 1 : p.c.B];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) seq[i] += __popcll(__ballot(s < p.c.B && end <= row0 + i));
+  }
 #pragma unroll
   for (int i = 0; i < ROWS; i++) {
-    const int row = row0 + i;
-    if (row >= p.c.total_q) break;
-    const int b = __builtin_amdgcn_readfirstlane(sequence_of(p.c.cu_q, p.c.B, row));
-    if (b >= p.c.B) break;  // (rows behind the last sequence)
-    const int begin = ld_scalar(p.c.cu_q, b), end = ld_scalar(p.c.cu_q, b + 1);
-    const int len = ld_scalar(p.c.seqlens, b);
-    const int slot = append_slot(len, begin, end, row, p.c.max_sq, p.c.max_keys);
-    if (slot < 0) continue;
-    const int page = ld_scalar(p.c.table + (int64_t)b * p.c.table_rs, slot >> p.c.page_log2);
-    const int pos = p.given_positions ? ld_scalar(p.given_positions, row) : slot;
-    if (!page_is_one(page, p.c.n_pages)) continue;  // (everything up to here is wave-uniform)
+    const int b = __builtin_amdgcn_readfirstlane(seq[i]), row = row0 + i;
+    seq[i] = b < p.c.B ? b : p.c.B - 1;  // (no branches here and below: the rows' loads are on their way together)
+    slot[i] = append_slot(ld_scalar(p.c.seqlens, seq[i]), ld_scalar(p.c.cu_q, seq[i]), ld_scalar(p.c.cu_q, seq[i] + 1), row, p.c.max_sq, p.c.max_keys);
+    if (b >= p.c.B || row >= p.c.total_q) slot[i] = -1;  // (rows behind the last sequence)
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    const int row = row0 + i < p.c.total_q ? row0 + i : p.c.total_q - 1;
+    page[i] = ld_scalar(p.c.table + (int64_t)seq[i] * p.c.table_rs, (slot[i] < 0 ? 0 : slot[i]) >> p.c.page_log2);
+    pos[i] = p.given_positions ? ld_scalar(p.given_positions, row) : slot[i];
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; i++)
+    if (slot[i] < 0) page[i] = -1;
+  typename Elem<T>::vec4 c4[ROWS], s4[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    if (on && rot && page_is_one(page[i], p.c.n_pages)) {
+      const int64_t at = (int64_t)table_row(pos[i], p.table_rows) * (D / 2) + ch * 4;
+      c4[i] = *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.cos) + at);
+      s4[i] = *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.sin) + at);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    if (!page_is_one(page[i], p.c.n_pages)) continue;  // (wave-uniform)
     if (on) {
       float x[8];
 #pragma unroll
@@ -86,25 +98,20 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = x[e] * r * w[e];
       }
-      if (rot) {
-        const int t = table_row(pos, p.table_rows);
-        const int64_t at = (int64_t)t * (D / 2) + ch * 4;
-        turn(x, *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.cos) + at),
-             *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.sin) + at));
-      }
+      if (rot) turn(x, c4[i], s4[i]);
       vec8 y;
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = (T)x[e];
-      const int at = slot & ((1 << p.c.page_log2) - 1);
+      const int at = slot[i] & ((1 << p.c.page_log2) - 1);
       char* dst;
-      if (part == 0) dst = reinterpret_cast<char*>(reinterpret_cast<T*>(p.q_out) + (int64_t)row * p.qo_rs + (int64_t)h * p.qo_hs);
-      else if (part == 1) dst = p.c.k + page * p.c.k_ps + at * p.c.k_ss + h * p.c.k_hs;
-      else dst = p.c.v + page * p.c.v_ps + at * p.c.v_ss + h * p.c.v_hs;
+      if (part == 0) dst = reinterpret_cast<char*>(reinterpret_cast<T*>(p.q_out) + (int64_t)(row0 + i) * p.qo_rs + (int64_t)h * p.qo_hs);
+      else if (part == 1) dst = p.c.k + page[i] * p.c.k_ps + at * p.c.k_ss + h * p.c.k_hs;
+      else dst = p.c.v + page[i] * p.c.v_ps + at * p.c.v_ss + h * p.c.v_hs;
       st_global16(dst + ch * 16, bitcast<u32x4>(y));
       if (part == 1 && ch == 0) {
-        const int64_t m = ((int64_t)page * p.c.HK + h) << p.c.page_log2;
+        const int64_t m = ((int64_t)page[i] * p.c.HK + h) << p.c.page_log2;
         if (p.c.weights) p.c.weights[m + at] = 0.f;
-        if (p.c.positions) p.c.positions[m + at] = pos;
+        if (p.c.positions) p.c.positions[m + at] = pos[i];
       }
     }
   }
@@ -115,9 +122,9 @@ hipError_t launch_append_d(const AppendParams& p, hipStream_t stream) {
   // A decode step's few rows: one a workgroup, so that as many as there are run side by side; prompts: eight a thread in flight.
   const bool few = (int64_t)p.c.total_q * p.pieces <= 2048;
   const int rows = few ? 1 : 8;
-  const dim3 grid((unsigned)((p.c.total_q + rows - 1) / rows * p.pieces));
-  if (few) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((paged_append_kernel<T, D, 8>), grid, dim3(256), 0, stream, p);
+  const dim3 grid((unsigned)((p.c.total_q + rows - 1) / rows * p.pieces)), block((unsigned)p.threads);
+  if (few) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((paged_append_kernel<T, D, 8>), grid, block, 0, stream, p);
   return hipGetLastError();
 }
 template <typename T>
@@ -172,7 +179,9 @@ extern "C" int fa_paged_append(const fa_paged_append_args* a) {
   p.eps = a->eps;
   p.q_heads = a->q ? c.nheads_q : 0;
   p.per_row = (p.q_heads + 2 * c.nheads_k) * (c.head_dim / 8);
-  p.pieces = (p.per_row + 255) / 256;
+  // a row's vectors go to one workgroup of whole waves if at most 512 threads, else to workgroups of 256
+  p.threads = p.per_row <= 512 ? (p.per_row + 63) / 64 * 64 : 256;
+  p.pieces = (p.per_row + p.threads - 1) / p.threads;
   FA_REQUIRE((int64_t)c.total_q * p.pieces < ((int64_t)1 << 31), "%s: too many rows", name);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(a->stream);
   FA_LAUNCH(a->dtype == FA_FP16 ? fa::launch_append<_Float16>(p, c.head_dim, stream) : fa::launch_append<__bf16>(p, c.head_dim, stream));

@@ -22,21 +22,53 @@ struct ChunkCfg {
   static constexpr int OS = D + 8;  // stride of the output's way through LDS
   static constexpr int kOut = 128 * OS * 2;
   static constexpr int kLds = 2 * kBuf + kSlack > kOut ? 2 * kBuf + kSlack : kOut;
-  static constexpr int kWaves = D == 128 ? 3 : 4;  // per SIMD
+  // Waves per SIMD; with the second sum that lse wants one less, without registers in scratch (d = 64: 44 of them).  Without lse d = 128 keeps the third
+  // wave and eight registers in scratch: 16 x 1024 tokens of 32 heads behind 5120 keys 1427 us (1060 TFLOP/s), with two waves 1550.
+  static constexpr int kWaves = D == 128 ? 3 : 4;
 };
 
-// Workgroup ids are dealt to the eight XCDs in turn: each takes a contiguous piece of the (pair, tile) line, so that the tiles that read one pair's
-// keys mostly run on one of them.  Tiles of a pair from the last (longest walk under the mask) on.
-FA_DEVICE int64_t xcd_order(int64_t id, int64_t n) {
-  const int64_t each = (n + 7) / 8;
-  const int64_t at = (id & 7) * each + (id >> 3);
-  return at;
+// The sequence with the rank-th largest number of keys (ties: lower index first); more than 64: in their order.
+FA_DEVICE int longest_sequence(const PagedCache& c, int rank) {
+  if (c.B > 64 || c.B < 2) return rank;
+  const int lane = threadIdx.x & 63;
+  const int len = keys_in_reach(c.seqlens[lane < c.B ? lane : c.B - 1], c.max_keys);
+  int before = 0;
+  for (int j = 0; j < c.B; j++) {
+    const int lj = __builtin_amdgcn_readlane(len, j);
+    before += (lj > len || (lj == len && j < lane)) ? 1 : 0;
+  }
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < c.B && before == rank);
+  return __builtin_amdgcn_readfirstlane(hit != 0 ? (int)__builtin_ctzll(hit) : rank);
+}
+
+// Workgroup id -> (sequence, key head, row tile).  Ids go to the eight XCDs in turn; the tiles of a pair should run on one of them, side by side, since
+// they read the same keys, and the longest sequences should begin first.  With pairs enough (p.deal) those are dealt to the XCDs one by one, longest
+// sequences first: 4 sequences of 4096 .. 8192 keys, 8 key heads, 1024 new tokens each, d = 128 417 us, in contiguous pieces, which give an XCD
+// one sequence's heads, 516.  Few pairs: each XCD takes a contiguous piece of the line of all tiles.  Tiles of a pair from the last (longest walk under the mask) on.
+FA_DEVICE bool place(const PagedFwdParams& p, int id, int* b, int* h, int* tile) {
+  const int pairs = p.c.B * p.c.HK, x = id & 7, j = id >> 3;
+  int64_t at;
+  if (p.deal) {
+    const int64_t rank = x + 8 * (int64_t)(j / p.nq_tiles);
+    if (rank >= pairs) return false;
+    at = rank * p.nq_tiles + j % p.nq_tiles;
+  } else {
+    const int64_t items = (int64_t)pairs * p.nq_tiles, each = (items + 7) / 8;
+    at = x * each + j;
+    if (j >= each || at >= items) return false;
+  }
+  const int rank = (int)(at / p.nq_tiles);
+  *tile = p.nq_tiles - 1 - (int)(at - (int64_t)rank * p.nq_tiles);
+  const int s = rank / p.c.HK;
+  *h = rank - s * p.c.HK;
+  *b = longest_sequence(p.c, s);
+  return true;
 }
 
 }  // namespace
 
 template <typename T, int D, bool kLse>
-__global__ void __launch_bounds__(256, ChunkCfg<D>::kWaves) fa_paged_chunk_kernel(const PagedFwdParams p) {
+__global__ void __launch_bounds__(256, ChunkCfg<D>::kWaves - (kLse ? 1 : 0)) fa_paged_chunk_kernel(const PagedFwdParams p) {
   using C = ChunkCfg<D>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
@@ -44,12 +76,8 @@ __global__ void __launch_bounds__(256, ChunkCfg<D>::kWaves) fa_paged_chunk_kerne
   constexpr int GW = BN / 32;  // groups of 16 keys that a wave stages (waves 0 and 1: K, 2 and 3: V)
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[C::kLds];
 
-  const int64_t pairs = (int64_t)p.c.B * p.c.HK;
-  const int64_t items = pairs * p.nq_tiles;
-  const int64_t item = xcd_order(blockIdx.x, items);
-  if ((blockIdx.x >> 3) >= (items + 7) / 8 || item >= items) return;
-  const int pair = (int)(item / p.nq_tiles), qt = p.nq_tiles - 1 - (int)(item - (int64_t)pair * p.nq_tiles);
-  const int b = pair / p.c.HK, h = pair - b * p.c.HK;
+  int b, h, qt;
+  if (!place(p, blockIdx.x, &b, &h, &qt)) return;
   const int split = blockIdx.y;
   int q_begin = 0, Lq = 0;
   if (!paged_rows(p.c, b, &q_begin, &Lq)) return;
@@ -241,7 +269,7 @@ __global__ void __launch_bounds__(256, ChunkCfg<D>::kWaves) fa_paged_chunk_kerne
   const float u_tot = kLse ? half_sum(u_i) : 0.f;
   if (p.n_splits > 1) {  // partial result of this split, fp32: [split][pair][row of nq_tiles * 128][D], m, l and u behind all of them
     if (mw + c < rows) {
-      const int64_t all = pairs * p.nq_tiles * kChunkRows, at = (int64_t)pair * p.nq_tiles * kChunkRows + mw + c;
+      const int64_t all = (int64_t)p.c.B * p.c.HK * p.nq_tiles * kChunkRows, at = ((int64_t)b * p.c.HK + h) * p.nq_tiles * kChunkRows + mw + c;
       float* const op = p.part + (int64_t)split * all * (D + 3) + at * D;
       if (hf == 0) {
         float* const ml = p.part + (int64_t)split * all * (D + 3) + all * D + at * 3;
@@ -331,7 +359,8 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedFwdPar
 template <typename T, int D>
 hipError_t launch_d(const PagedFwdParams& p, hipStream_t stream) {
   const int64_t items = (int64_t)p.c.B * p.c.HK * p.nq_tiles;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8), (unsigned)p.n_splits);
+  const int64_t pairs = (int64_t)p.c.B * p.c.HK;
+  const dim3 grid((unsigned)(p.deal ? (pairs + 7) / 8 * 8 * p.nq_tiles : (items + 7) / 8 * 8), (unsigned)p.n_splits);
   if (p.lse) hipLaunchKernelGGL((fa_paged_chunk_kernel<T, D, true>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((fa_paged_chunk_kernel<T, D, false>), grid, dim3(256), 0, stream, p);
   const hipError_t e = hipGetLastError();

@@ -12,9 +12,9 @@ namespace fa {
 
 namespace {
 
-template <int D>
+template <int D, int NW_>
 struct Cfg {
-  static constexpr int NW = kDecodeWaves(D);
+  static constexpr int NW = NW_;
   static constexpr int BN = 32;
   static constexpr int DV = D < 32 ? 32 : D;
   static constexpr int kTile = BN * D * 2;
@@ -44,18 +44,19 @@ FA_DEVICE int unit_sums(const PagedCache& c, int first) {
   const int b = first + (threadIdx.x & 63);
   return wave_prefix_sum(b < c.B ? units_of(c, b) : 0);
 }
-FA_DEVICE int64_t all_units(const PagedCache& c) {
-  int64_t n = 0;
-  for (int first = 0; first < c.B; first += 64) n += __builtin_amdgcn_readlane(unit_sums(c, first), 63);
+// (sums0: the first 64 sequences' sums, made once)
+FA_DEVICE int64_t all_units(const PagedCache& c, int sums0) {
+  int64_t n = __builtin_amdgcn_readlane(sums0, 63);
+  for (int first = 64; first < c.B; first += 64) n += __builtin_amdgcn_readlane(unit_sums(c, first), 63);
   return n * c.HK;
 }
 struct Spot {  // a unit of the line
   int b, h, unit, units;  // units: of each pair of sequence b
 };
-FA_DEVICE Spot spot_of(const PagedCache& c, int64_t u) {
+FA_DEVICE Spot spot_of(const PagedCache& c, int64_t u, int sums0) {
   int64_t before = 0;
   for (int first = 0; first < c.B; first += 64) {
-    const int sums = unit_sums(c, first);
+    const int sums = first == 0 ? sums0 : unit_sums(c, first);
     const int all = __builtin_amdgcn_readlane(sums, 63);
     if (u < before + (int64_t)all * c.HK) {
       const int64_t rest = u - before;
@@ -84,9 +85,9 @@ FA_DEVICE int share_of(int64_t units, int64_t u, int sharers) {  // the workgrou
 
 }  // namespace
 
-template <typename T, int D>
-__global__ void __launch_bounds__(64 * Cfg<D>::NW) fa_paged_decode_kernel(const PagedFwdParams p) {
-  using C = Cfg<D>;
+template <typename T, int D, int NW_>
+__global__ void __launch_bounds__(64 * NW_) fa_paged_decode_kernel(const PagedFwdParams p) {
+  using C = Cfg<D, NW_>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
   constexpr int NW = C::NW, BN = C::BN, DV = C::DV;
@@ -115,16 +116,16 @@ __global__ void __launch_bounds__(64 * Cfg<D>::NW) fa_paged_decode_kernel(const 
   int64_t u, u_end;
   Spot at;
   if (p.least > 0) {
-    const int64_t units = all_units(p.c);
+    const int sums0 = unit_sums(p.c, 0);
+    const int64_t units = all_units(p.c, sums0);
     const int n = sharers(p, units);
     if ((int)blockIdx.x >= n || units == 0) return;
     u = share_begin(units, blockIdx.x, n);
     u_end = share_begin(units, blockIdx.x + 1, n);
-    at = spot_of(p.c, u);
+    at = spot_of(p.c, u, sums0);
   } else {  // one pair
-    const int b = blockIdx.x / p.c.HK;
-    at = Spot{b, (int)blockIdx.x - b * p.c.HK, 0, units_of(p.c, b)};
-    if (at.units == 0) return;
+    const int b = blockIdx.x / p.c.HK, keys = paged_len(p.c, b);
+    at = Spot{b, (int)blockIdx.x - b * p.c.HK, 0, keys <= kDecodeUnit ? 1 : (keys + kDecodeUnit - 1) / kDecodeUnit};
     u = 0;
     u_end = at.units;
   }
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(64 * Cfg<D>::NW) fa_paged_decode_kernel(const 
     const int unit0 = __builtin_amdgcn_readfirstlane(at.unit), pair_units = __builtin_amdgcn_readfirstlane(at.units);
     const int unit1 = u_end - u < pair_units - unit0 ? unit0 + (int)(u_end - u) : pair_units;
     int q_begin = 0, Lq = 0;
-    if (!paged_rows(p.c, b, &q_begin, &Lq)) return;  // (never: such a sequence has no units)
+    if (!paged_rows(p.c, b, &q_begin, &Lq)) return;  // (on the line such a sequence has no units)
     const int Lk = paged_len(p.c, b), G = p.c.G, rows = Lq * G;
     const int k_lo = unit0 * kDecodeUnit;
     const int k_hi = Lk < unit1 * kDecodeUnit ? Lk : unit1 * kDecodeUnit;
@@ -336,10 +337,14 @@ __global__ void __launch_bounds__(64 * Cfg<D>::NW) fa_paged_decode_kernel(const 
 
 namespace {
 
-// The pairs that several workgroups' shares have cut: a workgroup per pair, 128 threads.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_decode_join_kernel(const PagedFwdParams p, int D) {
-  const int b = blockIdx.x / p.c.HK, h = (int)blockIdx.x - b * p.c.HK;
+// The pairs that several workgroups' shares have cut: a workgroup joins one row of one, D / 4 threads over its elements times 1024 / D over the parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_decode_join_kernel(const PagedFwdParams p) {
+  constexpr int kCols = D / 4, kLanes = 256 / kCols;
+  __shared__ f32x4 os[256];
+  __shared__ PartRow ms[256];
+  const int pair = blockIdx.x, r = blockIdx.y;
+  const int b = pair / p.c.HK, h = pair - b * p.c.HK;
   const int own = units_of(p.c, b);
   if (own == 0) return;
   int64_t units = 0, begin = 0;  // of the line; of this pair
@@ -354,48 +359,60 @@ __global__ void __launch_bounds__(128) paged_decode_join_kernel(const PagedFwdPa
   units *= p.c.HK;
   const int n = sharers(p, units);
   const int w0 = share_of(units, begin, n), w1 = share_of(units, begin + own - 1, n);
-  if (w0 == w1) return;
   int q_begin = 0, Lq = 0;
-  if (!paged_rows(p.c, b, &q_begin, &Lq)) return;
+  if (w0 == w1 || !paged_rows(p.c, b, &q_begin, &Lq) || r >= Lq * p.c.G) return;
   const float cs = p.scale_log2;
-  const int per_row = D / 4, each = kPartRows * (D + 3);
+  constexpr int kEach = kPartRows * (D + 3);
   // the pair is the last of workgroup w0's share, and its first, too, if the share begins with it; it is the first of the others'
   const int first_slot = share_begin(units, w0, n) == begin ? 0 : 1;
-  for (int idx = threadIdx.x; idx < Lq * p.c.G * per_row; idx += 128) {
-    const int r = idx / per_row, d0 = idx % per_row * 4;
-    float m = -INFINITY;
-    for (int w = w0; w <= w1; w++) m = fmaxf(m, p.part[((int64_t)w * 2 + (w == w0 ? first_slot : 0)) * each + kPartRows * D + r]);
-    const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f, us = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int w = w0; w <= w1; w++) {
-      const float* const s = p.part + ((int64_t)w * 2 + (w == w0 ? first_slot : 0)) * each;
-      const float* const ml = s + kPartRows * D + r;
-      const float f = fast_exp2((ml[0] - mu) * cs);
-      l = __builtin_fmaf(ml[kPartRows], f, l);
-      us = __builtin_fmaf(ml[2 * kPartRows], f, us);
-      o = o + *reinterpret_cast<const f32x4*>(s + r * D + d0) * f;
-    }
-    store_row_piece<T>(p, q_begin, h, r, d0, o * (l > 0.f ? fast_rcp(l) : 1.f));
-    if (d0 == 0) store_lse(p, b, h, r, lse_of(m, us, cs));
+  const int col = threadIdx.x % kCols, lane = threadIdx.x / kCols;
+  PartRow a{-INFINITY, 0.f, 0.f};
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int w = w0 + lane; w <= w1; w += kLanes) {
+    const float* const s = p.part + ((int64_t)w * 2 + (w == w0 ? first_slot : 0)) * kEach;
+    const float* const ml = s + kPartRows * D + r;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(s + r * D + col * 4);
+    const float m = ml[0], l = ml[kPartRows], u = ml[2 * kPartRows];
+    const float top = fmaxf(a.m, m), ref = top == -INFINITY ? 0.f : top;
+    const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((m - ref) * cs);
+    a = PartRow{top, a.l * fa + l * fb, a.u * fa + u * fb};
+    o = o * fa + x * fb;
   }
+  os[threadIdx.x] = o;
+  ms[threadIdx.x] = a;
+  __syncthreads();
+  if (lane > 0) return;
+  for (int i = 1; i < kLanes && i <= w1 - w0; i++) {
+    const PartRow x = ms[i * kCols + col];
+    const float top = fmaxf(a.m, x.m), ref = top == -INFINITY ? 0.f : top;
+    const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((x.m - ref) * cs);
+    a = PartRow{top, a.l * fa + x.l * fb, a.u * fa + x.u * fb};
+    o = o * fa + os[i * kCols + col] * fb;
+  }
+  store_row_piece<T>(p, q_begin, h, r, col * 4, o * (a.l > 0.f ? fast_rcp(a.l) : 1.f));
+  if (col == 0) store_lse(p, b, h, r, lse_of(a.m, a.u, cs));
 }
 
-template <typename T>
-hipError_t launch_t(const PagedFwdParams& p, int head_dim, hipStream_t stream) {
+template <typename T, int D>
+hipError_t launch_d(const PagedFwdParams& p, hipStream_t stream) {
   const unsigned pairs = (unsigned)(p.c.B * p.c.HK);
   const dim3 grid(p.least > 0 ? (unsigned)p.groups : pairs);
-  switch (head_dim) {
-    case 16: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 16>), grid, dim3(64 * Cfg<16>::NW), 0, stream, p); break;
-    case 32: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 32>), grid, dim3(64 * Cfg<32>::NW), 0, stream, p); break;
-    case 64: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 64>), grid, dim3(64 * Cfg<64>::NW), 0, stream, p); break;
-    case 128: hipLaunchKernelGGL((fa_paged_decode_kernel<T, 128>), grid, dim3(64 * Cfg<128>::NW), 0, stream, p); break;
-    default: return hipErrorInvalidValue;
-  }
+  if (p.wide) hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWide(D)>), grid, dim3(64 * kDecodeWide(D)), 0, stream, p);
+  else hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWaves(D)>), grid, dim3(64 * kDecodeWaves(D)), 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.least == 0) return e;
-  hipLaunchKernelGGL(paged_decode_join_kernel<T>, dim3(pairs), dim3(128), 0, stream, p, head_dim);
+  hipLaunchKernelGGL((paged_decode_join_kernel<T, D>), dim3(pairs, (unsigned)(p.c.max_sq * p.c.G)), dim3(256), 0, stream, p);
   return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_t(const PagedFwdParams& p, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 16: return launch_d<T, 16>(p, stream);
+    case 32: return launch_d<T, 32>(p, stream);
+    case 64: return launch_d<T, 64>(p, stream);
+    case 128: return launch_d<T, 128>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 }  // namespace

@@ -22,11 +22,11 @@ struct EvictParams {
   int budget, recent, cap;  // cap: most moves of a head
   int32_t* counts;          // [B * HK]
   int32_t* moves;           // [B * HK][2][cap]: holes, keys that come
-  int row_bytes;
 };
 
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 constexpr uint32_t kNewest = 0xffffffffu;
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
 // A weight as an unsigned integer of the same order; NaN as -inf, -0 as 0
 FA_DEVICE uint32_t ordered(float w) {
@@ -34,10 +34,59 @@ FA_DEVICE uint32_t ordered(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// kCap: keys whose mapped weights are kept in LDS (0: read again in every pass)
-template <int kCap>
+// Copies `moves` (at most kMovesPerGroup) of a head's keys and values: first where each comes from and goes to, into LDS, then 16 bytes a thread at a time,
+// four of them in flight (8 x 8 heads cut from 4915 .. 16384 keys to 4096, d = 128, 149 MB: the whole operator 68 us, with two 70, with eight 103).
+constexpr int kMovesPerGroup = 64;
+struct MoveSpots {
+  int64_t at[kMovesPerGroup][4];  // k from, k to (negative: nowhere), v from, v to: bytes
+};
+template <int D, int kThreads>
+FA_DEVICE void move_keys(const EvictParams& p, int b, int h, const int32_t* holes, const int32_t* comes, int moves, MoveSpots& spots) {
+  constexpr int CH = D / 8, kEach = kMovesPerGroup * 2 * CH / kThreads, kFly = kEach < 1 ? 1 : (kEach < 4 ? kEach : 4);
+  const int mask = (1 << p.c.page_log2) - 1;
+  if ((int)threadIdx.x < moves) {
+    const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
+    const int to = holes[threadIdx.x], from = comes[threadIdx.x];
+    const int to_page = table[to >> p.c.page_log2], from_page = page_in_pool(table[from >> p.c.page_log2], p.c.n_pages);
+    int64_t* const at = spots.at[threadIdx.x];
+    at[0] = from_page * p.c.k_ps + (from & mask) * p.c.k_ss + h * p.c.k_hs;
+    at[2] = from_page * p.c.v_ps + (from & mask) * p.c.v_ss + h * p.c.v_hs;
+    if (page_is_one(to_page, p.c.n_pages)) {
+      at[1] = to_page * p.c.k_ps + (to & mask) * p.c.k_ss + h * p.c.k_hs;
+      at[3] = to_page * p.c.v_ps + (to & mask) * p.c.v_ss + h * p.c.v_hs;
+      const int64_t d = (((int64_t)to_page * p.c.HK + h) << p.c.page_log2) + (to & mask);
+      const int64_t s = (((int64_t)from_page * p.c.HK + h) << p.c.page_log2) + (from & mask);
+      p.c.weights[d] = p.c.weights[s];
+      p.c.positions[d] = p.c.positions[s];
+    } else {
+      at[1] = at[3] = -1;
+    }
+  }
+  __syncthreads();
+  const int n = moves * 2 * CH;
+  for (int i0 = threadIdx.x; i0 < n; i0 += kThreads * kFly) {
+    u32x4 x[kFly];
+#pragma unroll
+    for (int f = 0; f < kFly; f++) {
+      const int i = i0 + f * kThreads;
+      if (i < n) x[f] = ld_global16((i / CH & 1 ? p.c.v : p.c.k) + spots.at[i / (2 * CH)][i / CH & 1 ? 2 : 0] + i % CH * 16);
+    }
+#pragma unroll
+    for (int f = 0; f < kFly; f++) {
+      const int i = i0 + f * kThreads;
+      if (i < n) {
+        const int64_t to = spots.at[i / (2 * CH)][i / CH & 1 ? 3 : 1];
+        if (to >= 0) st_global16((i / CH & 1 ? p.c.v : p.c.k) + to + i % CH * 16, x[f]);
+      }
+    }
+  }
+}
+
+// kCap: keys whose mapped weights are kept in LDS (0: read again in every pass).  kMoveD: 0, or the head dimension where a head has at most
+// kMovesPerGroup moves: the workgroup then makes them itself, without another launch.
+template <int kCap, int kMoveD>
 __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictParams p) {
-  __shared__ uint32_t keys[kCap > 0 ? kCap : 1];
+  __shared__ __attribute__((aligned(16))) uint32_t keys[kCap > 0 ? kCap : 4];
   __shared__ int hist[2048];
   __shared__ int sums[2][kEvictWaves];
   __shared__ uint32_t found[2];  // digit, keys above it
@@ -46,7 +95,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (h == 0 && tid == 0) p.new_len[b] = L < p.budget ? L : p.budget;
   if (L <= p.budget) {
-    if (tid == 0) p.counts[blockIdx.x] = 0;
+    if (kMoveD == 0 && tid == 0) p.counts[blockIdx.x] = 0;
     return;
   }
   const int64_t newest = (int64_t)p.next[b] - p.recent;
@@ -67,15 +116,45 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
     for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
     __syncthreads();
-    for (int j = tid; j < L; j += kEvictThreads) {
-      uint32_t k;
-      if (kCap > 0 && pass == 0) {
-        k = read_key(j);
-        keys[j] = k;
-      } else {
-        k = key_of(j);
+    if (kCap > 0 && pass == 0) {
+      // four slots a thread (a page holds 16 at least), the pages of its next ones asked for before
+      constexpr int kAhead = kCap <= 4096 ? 1 : 4;
+      for (int q0 = tid * 4; q0 < L; q0 += kEvictThreads * 4 * kAhead) {
+        int64_t at[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+          const int q = q0 + i * kEvictThreads * 4;
+          const int page = page_in_pool(table[(q < L ? q : L - 1) >> p.c.page_log2], p.c.n_pages);
+          at[i] = (((int64_t)page * p.c.HK + h) << p.c.page_log2) + (q & mask);
+        }
+        f32x4 w[kAhead];
+        i32x4 pos[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+          if (q0 + i * kEvictThreads * 4 < L) {
+            w[i] = *reinterpret_cast<const f32x4*>(p.c.weights + at[i]);
+            pos[i] = *reinterpret_cast<const i32x4*>(p.c.positions + at[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+          const int q = q0 + i * kEvictThreads * 4;
+          if (q < L) {
+            u32x4 k;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              k[e] = pos[i][e] >= newest ? kNewest : ordered(w[i][e]);
+              if (q + e < L) atomicAdd(&hist[k[e] >> 21], 1);
+            }
+            *reinterpret_cast<u32x4*>(keys + q) = k;
+          }
+        }
       }
-      if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
+    } else {
+#pragma unroll 4
+      for (int j = tid; j < L; j += kEvictThreads) {
+        const uint32_t k = key_of(j);
+        if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
+      }
     }
     __syncthreads();
     // thread t holds the digits 2047 - 2 t and 2046 - 2 t: prefix sums count from the largest digit down
@@ -109,8 +188,10 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   __syncthreads();
   int tie0 = 0;
   for (int w = 0; w < wave; w++) tie0 += sums[0][w];
-  int hole0 = 0, come0 = 0;
-  int32_t* const holes = p.moves + (int64_t)blockIdx.x * 2 * p.cap;
+  int hole0 = 0, come0 = 0, moves = 0;
+  __shared__ int32_t own_moves[kMoveD > 0 ? 2 * kMovesPerGroup : 1];
+  int32_t* const holes = kMoveD > 0 ? own_moves : p.moves + (int64_t)blockIdx.x * 2 * p.cap;
+  const int cap = kMoveD > 0 ? kMovesPerGroup : p.cap;
   for (int round = 0; round < 2; round++) {  // counted, then written
     int tie = tie0, hole = hole0, come = come0;
     for (int j = j0 + lane; j - lane < j1; j += 64) {
@@ -123,8 +204,8 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
       const uint64_t hb = __ballot(is_hole), cb = __ballot(comes);
       if (round == 1) {
         const int nh = hole + __popcll(hb & below), nc = come + __popcll(cb & below);
-        if (is_hole && nh < p.cap) holes[nh] = j;
-        if (comes && nc < p.cap) holes[p.cap + nc] = j;
+        if (is_hole && nh < cap) holes[nh] = j;
+        if (comes && nc < cap) holes[cap + nc] = j;
       }
       hole += __popcll(hb);
       come += __popcll(cb);
@@ -136,51 +217,34 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
         sums[1][wave] = come;
       }
       __syncthreads();
-      int n = 0;
       for (int w = 0; w < kEvictWaves; w++) {
         if (w < wave) {
           hole0 += sums[0][w];
           come0 += sums[1][w];
         }
-        n += sums[0][w];
+        moves += sums[0][w];
       }
-      if (tid == 0) p.counts[blockIdx.x] = n < p.cap ? n : p.cap;
+      moves = moves < cap ? moves : cap;  // (as many as the cap, by its definition)
+      if (kMoveD == 0 && tid == 0) p.counts[blockIdx.x] = moves;
     }
+  }
+  if constexpr (kMoveD > 0) {
+    __shared__ MoveSpots spots;
+    __syncthreads();
+    move_keys<kMoveD, kEvictThreads>(p, b, h, holes, holes + cap, moves, spots);
   }
 }
 
-constexpr int kMovesPerGroup = 64;
-
-// A workgroup copies 64 of a head's moves: a thread 16 bytes at a time of a key or a value.
+// A workgroup copies 64 of a head's moves.
+template <int D>
 __global__ void __launch_bounds__(256) paged_move_kernel(const EvictParams p) {
+  __shared__ MoveSpots spots;
   const int pair = blockIdx.y, n = p.counts[pair];
   const int first = blockIdx.x * kMovesPerGroup;
   if (first >= n) return;
-  const int b = pair / p.c.HK, h = pair - b * p.c.HK;
-  const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
   const int32_t* const holes = p.moves + (int64_t)pair * 2 * p.cap;
-  const int mask = (1 << p.c.page_log2) - 1, cpr = p.row_bytes / 16;
-  const int moves = n - first < kMovesPerGroup ? n - first : kMovesPerGroup;
-  for (int i = threadIdx.x; i < moves * 2 * cpr; i += 256) {
-    const int m = i / (2 * cpr), rest = i - m * 2 * cpr;
-    const bool value = rest >= cpr;
-    const int ch = value ? rest - cpr : rest;
-    const int to = holes[first + m], from = holes[p.cap + first + m];
-    const int to_page = table[to >> p.c.page_log2];
-    const int from_page = page_in_pool(table[from >> p.c.page_log2], p.c.n_pages);
-    if (!page_is_one(to_page, p.c.n_pages)) continue;
-    char* const base = value ? p.c.v : p.c.k;
-    const int64_t ps = value ? p.c.v_ps : p.c.k_ps, ss = value ? p.c.v_ss : p.c.k_ss, hs = value ? p.c.v_hs : p.c.k_hs;
-    const char* const src = base + from_page * ps + (from & mask) * ss + h * hs + ch * 16;
-    char* const dst = base + to_page * ps + (to & mask) * ss + h * hs + ch * 16;
-    st_global16(dst, ld_global16(src));
-    if (rest == 0) {
-      const int64_t d = (((int64_t)to_page * p.c.HK + h) << p.c.page_log2) + (to & mask);
-      const int64_t s = (((int64_t)from_page * p.c.HK + h) << p.c.page_log2) + (from & mask);
-      p.c.weights[d] = p.c.weights[s];
-      p.c.positions[d] = p.c.positions[s];
-    }
-  }
+  const int b = pair / p.c.HK;
+  move_keys<D, 256>(p, b, pair - b * p.c.HK, holes + first, holes + p.cap + first, n - first < kMovesPerGroup ? n - first : kMovesPerGroup, spots);
 }
 
 struct EvictPlan {
@@ -195,18 +259,35 @@ EvictPlan evict_plan(const fa_paged_evict_args* a) {
   return pl;
 }
 
-hipError_t launch_evict(const EvictParams& p, hipStream_t stream) {
+template <int D>
+hipError_t launch_evict_d(const EvictParams& p, hipStream_t stream) {
   const dim3 pairs((unsigned)(p.c.B * p.c.HK));
-  // (LDS decides how many heads a compute unit selects for at once: nine, two, one)
-  if (p.c.max_keys <= 4096) hipLaunchKernelGGL(paged_evict_kernel<4096>, pairs, dim3(kEvictThreads), 0, stream, p);
-  else if (p.c.max_keys <= 16384) hipLaunchKernelGGL(paged_evict_kernel<16384>, pairs, dim3(kEvictThreads), 0, stream, p);
-  else if (p.c.max_keys <= 32768) hipLaunchKernelGGL(paged_evict_kernel<32768>, pairs, dim3(kEvictThreads), 0, stream, p);
-  else hipLaunchKernelGGL(paged_evict_kernel<0>, pairs, dim3(kEvictThreads), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.cap == 0) return e;
+  const bool few = p.cap <= kMovesPerGroup;  // (decoding: a step or a few of them over the budget)
+  // (LDS decides how many heads a compute unit selects for at once: two of 16 waves, at more than 16384 keys one)
+#define FA_EVICT(CAP)                                                                                                         \
+  do {                                                                                                                        \
+    if (few) hipLaunchKernelGGL((paged_evict_kernel<CAP, D>), pairs, dim3(kEvictThreads), 0, stream, p);                      \
+    else hipLaunchKernelGGL((paged_evict_kernel<CAP, 0>), pairs, dim3(kEvictThreads), 0, stream, p);                          \
+  } while (0)
+  if (p.c.max_keys <= 4096) FA_EVICT(4096);
+  else if (p.c.max_keys <= 16384) FA_EVICT(16384);
+  else if (p.c.max_keys <= 32768) FA_EVICT(32768);
+  else FA_EVICT(0);
+#undef FA_EVICT
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || few) return e;
   const unsigned gx = (unsigned)((p.cap + kMovesPerGroup - 1) / kMovesPerGroup);
-  hipLaunchKernelGGL(paged_move_kernel, dim3(gx, pairs.x), dim3(256), 0, stream, p);  // (at most 65535 heads: see check_sizes)
+  hipLaunchKernelGGL(paged_move_kernel<D>, dim3(gx, pairs.x), dim3(256), 0, stream, p);  // (at most 65535 heads: see check_sizes)
   return hipGetLastError();
+}
+hipError_t launch_evict(const EvictParams& p, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 16: return launch_evict_d<16>(p, stream);
+    case 32: return launch_evict_d<32>(p, stream);
+    case 64: return launch_evict_d<64>(p, stream);
+    case 128: return launch_evict_d<128>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 int check_sizes(const fa_paged_evict_args* a, const char* name) {
@@ -237,6 +318,7 @@ int fa_paged_evict(const fa_paged_evict_args* a) {
                  (c.n_pages == 1 || (c.k_page_stride >= c.head_dim && c.v_page_stride >= c.head_dim)),
              "%s: the cache's slots, heads and pages must not overlap", name);
   FA_REQUIRE(c.key_weights && c.key_positions && a->next_positions && a->new_seqlens_k, "%s: key_weights, key_positions, next_positions and new_seqlens_k are needed", name);
+  FA_REQUIRE(fa::aligned16(c.key_weights) && fa::aligned16(c.key_positions), "%s: key_weights and key_positions must be 16-byte aligned", name);
   FA_REQUIRE(a->new_seqlens_k != c.seqlens_k, "%s: new_seqlens_k may not be seqlens_k", name);
   FA_REQUIRE(((reinterpret_cast<uintptr_t>(a->next_positions) | reinterpret_cast<uintptr_t>(a->new_seqlens_k)) & 3) == 0, "%s: integers must be 4-byte aligned", name);
   const fa::EvictPlan pl = fa::evict_plan(a);
@@ -251,8 +333,7 @@ int fa_paged_evict(const fa_paged_evict_args* a) {
   p.cap = pl.cap;
   p.counts = reinterpret_cast<int32_t*>(a->workspace);
   p.moves = p.counts + (size_t)c.batch * c.nheads_k;
-  p.row_bytes = c.head_dim * 2;
-  FA_LAUNCH(fa::launch_evict(p, reinterpret_cast<hipStream_t>(a->stream)));
+  FA_LAUNCH(fa::launch_evict(p, c.head_dim, reinterpret_cast<hipStream_t>(a->stream)));
   return FA_OK;
 }
 

@@ -198,6 +198,9 @@ def _load_host(lib):
     host.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
         "fa_fwd", "fa_fwd_block", "fa_bwd", "fa_bwd_block", "fa_fwd_workspace_bytes", "fa_bwd_workspace_bytes", "fa_round_seqlens",
         "fa_last_error", "fa_pad_bias_rows", "fa_bias_grad_reduce_ragged", "fa_rotary", "fa_token_positions")))
+    host.bind_paged(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+        "fa_qk_norm_rotary", "fa_qk_norm_rotary_bwd", "fa_qk_norm_rotary_bwd_workspace_bytes", "fa_paged_append", "fa_paged_fwd", "fa_paged_fwd_workspace_bytes",
+        "fa_paged_key_weights", "fa_paged_evict", "fa_paged_evict_workspace_bytes")))
     return host
 
 
@@ -287,6 +290,13 @@ def load_library():
         _host = _passes = _load_host(lib)
         _lib = lib
     return _lib
+
+
+def passes():
+    """The native calls (host/fa_host.cpp) around and beside fwd and bwd: each returns None for what is to be run by way of this module."""
+    if _passes is None:
+        load_library()
+    return _passes
 
 
 def set_launch_policy(policy):

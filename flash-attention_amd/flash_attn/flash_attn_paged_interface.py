@@ -33,6 +33,10 @@ def paged_append_func(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens
     key_weights, key_positions (pages, nheads_k, page size): set to 0 and the position for the new tokens (for paged_key_weights_func and
     paged_evict_func).  Rows behind the last sequence, and tokens for which the page table has no room, are not stored; their rows of the returned q
     hold nothing."""
+    done = _backend.passes().paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, q_weight, k_weight, cos_half, sin_half, positions, eps,
+                                          key_weights, key_positions)
+    if done is not None:
+        return None if q is None else done
     _inference(q, k, v, q_weight, k_weight)
     return _backend.paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, None, q_weight, k_weight, cos_half, sin_half, positions, eps,
                                  key_weights, key_positions)
@@ -45,6 +49,10 @@ def flash_attn_paged_func(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens
     own keys are in the cache); a token that sees no key gives zeros.  max_seqlen_q, max_seqlen_k: at least the longest of each.
     Returns out (total, nheads, headdim), or (out, softmax_lse), softmax_lse (batch, nheads, max_seqlen_q rounded up to 16) fp32, -inf for a token
     that sees no key.  Rows of out behind the last sequence hold nothing."""
+    done = _backend.passes().paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
+                                       return_softmax_lse)
+    if done is not None:
+        return done
     _inference(q, k_cache, v_cache)
     scale = q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale
     r = _backend.paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, return_softmax_lse)
@@ -56,6 +64,9 @@ def paged_key_weights_func(q, softmax_lse, k_cache, key_weights, page_table, cu_
     """Adds to key_weights (pages, nheads_k, page size) fp32 what every key has received of the new tokens' attention: the sum of its probabilities
     over the tokens and over the query heads of its group.  q and softmax_lse: those of flash_attn_paged_func over the same cache.  In place; returns
     key_weights."""
+    if _backend.passes().paged_key_weights(q, softmax_lse, k_cache, key_weights, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale,
+                                           causal):
+        return key_weights
     _inference(q, k_cache)
     scale = q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale
     return _backend.paged_key_weights(q, softmax_lse, k_cache, key_weights, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal)
@@ -66,5 +77,8 @@ def paged_evict_func(k_cache, v_cache, key_weights, key_positions, page_table, s
     the keys whose position is at least next_positions[b] - recent, and then those with the largest key_weights (NaN counts as -inf; ties: the lower
     slot).  Each key head chooses for itself; a kept key from behind the budget takes the place, and the weight and position, of one that goes.  Slots
     from `budget` on are left as they were.  next_positions: (batch,) int32, the position that each sequence's next token would have."""
+    done = _backend.passes().paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k)
+    if done is not None:
+        return done
     _inference(k_cache, v_cache)
     return _backend.paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k)

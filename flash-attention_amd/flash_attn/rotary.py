@@ -93,7 +93,11 @@ def apply_qk_norm_rotary(q, k, q_weight, k_weight, cos_half=None, sin_half=None,
     q: (total, nheads, headdim) or (batch, seqlen, nheads, headdim), k the same with its own number of heads, fp16 or bf16, headdim 16, 32, 64 or 128;
     q_weight, k_weight: (headdim,) in the tensors' dtype or fp32.  positions: int32, one table row for each row of q (entries outside the tables are
     clamped to them); None: the place in the sequence, for tensors with a seqlen dimension or a single packed sequence.
-    Returns (q', k'), new tensors; differentiable in q, k and the weights."""
+    Returns (q', k'), new tensors; differentiable in q, k and the weights (once)."""
+    from . import flash_attn_gfx950 as backend
+    done = backend.passes().qk_norm_rotary(q, k, q_weight, k_weight, cos_half, sin_half, positions, eps)
+    if done is not None:
+        return done
     if q.dim() == 4:
         b, s = q.shape[:2]
         if k.dim() != 4 or tuple(k.shape[:2]) != (b, s):

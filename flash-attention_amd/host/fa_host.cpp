@@ -16,7 +16,10 @@
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <pybind11/gil.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
 
 #include "../../include/flash_attn_gfx950.h"
 
@@ -420,6 +423,12 @@ PyObject* reduce_bias_grad(PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
+}  // namespace
+
+#include "fa_host_paged.h"
+
+namespace {
+
 // C++ exceptions (an allocation that fails, memory that may not be touched under tracing) do not leave the module: the call is handed back and
 // the binding meets the same condition
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
@@ -439,6 +448,12 @@ PyMethodDef methods[] = {
     {"rotated_keys", (PyCFunction)(void (*)(void))guarded<rotated_keys>, METH_FASTCALL, nullptr},
     {"pad_bias", (PyCFunction)(void (*)(void))guarded<pad_bias>, METH_FASTCALL, nullptr},
     {"reduce_bias_grad", (PyCFunction)(void (*)(void))guarded<reduce_bias_grad>, METH_FASTCALL, nullptr},
+    {"bind_paged", (PyCFunction)(void (*)(void))py_bind_paged, METH_FASTCALL, nullptr},
+    {"qk_norm_rotary", (PyCFunction)(void (*)(void))guarded<qk_norm_rotary>, METH_FASTCALL, nullptr},
+    {"paged_append", (PyCFunction)(void (*)(void))guarded<paged_append>, METH_FASTCALL, nullptr},
+    {"paged_fwd", (PyCFunction)(void (*)(void))guarded<paged_fwd>, METH_FASTCALL, nullptr},
+    {"paged_key_weights", (PyCFunction)(void (*)(void))guarded<paged_key_weights>, METH_FASTCALL, nullptr},
+    {"paged_evict", (PyCFunction)(void (*)(void))guarded<paged_evict>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fa_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -432,7 +432,8 @@ int fa_paged_key_weights(const fa_paged_fwd_args* args);
  * recent stay, then the ones with the largest key_weights (NaN counts as -inf; ties: the lower slot; should more than `budget` be recent, those in
  * the lowest slots).  The n-th slot below `budget` whose key goes takes the n-th key from behind it that stays, with its value, weight and position;
  * slots from `budget` on are left as they were.  Each key head chooses for itself.  new_seqlens_k: batch int32, min(seqlens_k, budget); may
- * not be seqlens_k.  cu_seqlens_q, nheads_q, total_q and max_seqlen_q are not read.  workspace: fa_paged_evict_workspace_bytes() bytes. */
+ * not be seqlens_k.  cu_seqlens_q, nheads_q, total_q and max_seqlen_q are not read; key_weights
+ * and key_positions are 16-byte aligned.  workspace: fa_paged_evict_workspace_bytes() bytes. */
 typedef struct fa_paged_evict_args {
   uint32_t struct_bytes;
   int32_t budget, recent;

@@ -212,7 +212,7 @@ ENTRY = {"norm": "fa_qk_norm_rotary", "append": "fa_paged_append", "fwd": "fa_pa
     ("fwd", {"cache.total_q": 1}, "q must be"), ("fwd", {"cache.total_q": 1, "q": 1 << 20}, "o must be"),
     ("weights", {"cache.total_q": 1, "q": 1 << 20}, "softmax_lse"),
     ("evict", {"budget": 0}, "budget"), ("evict", {"recent": -1}, "recent"), ("evict", {"new_seqlens_k": 1 << 20, "cache.seqlens_k": 1 << 20}, "may not be"),
-    ("evict", {"cache.key_weights": None}, "needed"), ("evict", {"next_positions": None}, "needed"), ("evict", {"cache.batch": 40000}, "65535"), ("evict", {}, "workspace"),
+    ("evict", {"cache.key_weights": None}, "needed"), ("evict", {"next_positions": None}, "needed"), ("evict", {"cache.key_weights": (1 << 20) + 4}, "16-byte"), ("evict", {"cache.batch": 40000}, "65535"), ("evict", {}, "workspace"),
     ("norm", {"head_dim": 24}, "head_dim"), ("norm", {"weight_dtype": 1}, "weights must be"), ("norm", {"n_rows": -1}, "n_rows"), ("norm", {"n_rows": 1 << 30}, "n_rows"),
     ("norm", {"nheads_q": -1}, "heads"), ("norm", {"eps": -1.0}, "eps"), ("norm", {"eps": math.nan}, "eps"),
     ("norm", {"n_rows": 1, "cos_table": 1 << 20}, "come together"), ("norm", {"n_rows": 1, "cos_table": 1 << 20, "sin_table": 1 << 20}, "empty table"),
