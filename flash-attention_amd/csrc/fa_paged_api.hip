@@ -68,8 +68,8 @@ int check(const fa_paged_fwd_args* a, bool weights, const char* name) {
              "%s: q must be 16-byte aligned, its strides multiples of 8 elements in [0, 2^24)", name);
   if (weights) {
     FA_REQUIRE(a->softmax_lse && c.key_weights, "%s: softmax_lse and key_weights are needed", name);
-    // (a tile's 32 rows are addressed from its first one's token with 32-bit offsets in bytes)
-    FA_REQUIRE((c.nheads_q / c.nheads_k) * a->q_head_stride + 33 * a->q_row_stride < ((int64_t)1 << 30), "%s: q's heads of a group lie too far apart", name);
+    // (a tile's 64 or 128 rows are addressed from its first one's token with 32-bit offsets in bytes)
+    FA_REQUIRE((c.nheads_q / c.nheads_k) * a->q_head_stride + 129 * a->q_row_stride < ((int64_t)1 << 30), "%s: q's heads of a group lie too far apart", name);
   } else {
     FA_REQUIRE(a->o && fa::aligned16(a->o) && fa::stride_ok(a->o_row_stride) && fa::stride_ok(a->o_head_stride) && a->o_row_stride >= c.head_dim &&
                    (c.nheads_q == 1 || a->o_head_stride >= c.head_dim),

@@ -24,7 +24,7 @@ struct EvictParams {
   int32_t* moves;           // [B * HK][2][cap]: holes, keys that come
 };
 
-constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+constexpr int kEvictThreads = 1024;  // (32 x 8 heads of 2049 keys 10.4 us; 512 threads 12.5, 256 15.1)
 constexpr uint32_t kNewest = 0xffffffffu;
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
@@ -82,13 +82,23 @@ FA_DEVICE void move_keys(const EvictParams& p, int b, int h, const int32_t* hole
   }
 }
 
+// Sum of the values that the waves before this one left in x (one a wave); *all: of all of them
+template <int kWaves>
+FA_DEVICE int before_wave(const int* x, int wave, int* all) {
+  const int lane = threadIdx.x & 63;
+  const int pre = wave_prefix_sum(lane < kWaves ? x[lane] : 0);
+  *all = __builtin_amdgcn_readlane(pre, kWaves - 1);
+  return wave > 0 ? __builtin_amdgcn_readlane(pre, wave > 0 ? wave - 1 : 0) : 0;
+}
+
 // kCap: keys whose mapped weights are kept in LDS (0: read again in every pass).  kMoveD: 0, or the head dimension where a head has at most
 // kMovesPerGroup moves: the workgroup then makes them itself, without another launch.
 template <int kCap, int kMoveD>
 __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictParams p) {
+  constexpr int kThreads = kEvictThreads, kWaves = kThreads / 64;
   __shared__ __attribute__((aligned(16))) uint32_t keys[kCap > 0 ? kCap : 4];
   __shared__ int hist[2048];
-  __shared__ int sums[2][kEvictWaves];
+  __shared__ int sums[2][kWaves];
   __shared__ uint32_t found[2];  // digit, keys above it
   const int b = blockIdx.x / p.c.HK, h = (int)blockIdx.x - b * p.c.HK;
   const int L = paged_len(p.c, b);
@@ -114,16 +124,16 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   int want = p.budget;  // of the keys that begin with `prefix`
   for (int pass = 0; pass < 3; pass++) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
+    for (int i = tid; i < 2048; i += kThreads) hist[i] = 0;
     __syncthreads();
     if (kCap > 0 && pass == 0) {
       // four slots a thread (a page holds 16 at least), the pages of its next ones asked for before
-      constexpr int kAhead = kCap <= 4096 ? 1 : 4;
-      for (int q0 = tid * 4; q0 < L; q0 += kEvictThreads * 4 * kAhead) {
+      constexpr int kAhead = 4;
+      for (int q0 = tid * 4; q0 < L; q0 += kThreads * 4 * kAhead) {
         int64_t at[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-          const int q = q0 + i * kEvictThreads * 4;
+          const int q = q0 + i * kThreads * 4;
           const int page = page_in_pool(table[(q < L ? q : L - 1) >> p.c.page_log2], p.c.n_pages);
           at[i] = (((int64_t)page * p.c.HK + h) << p.c.page_log2) + (q & mask);
         }
@@ -131,13 +141,13 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
         i32x4 pos[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; i++)
-          if (q0 + i * kEvictThreads * 4 < L) {
+          if (q0 + i * kThreads * 4 < L) {
             w[i] = *reinterpret_cast<const f32x4*>(p.c.weights + at[i]);
             pos[i] = *reinterpret_cast<const i32x4*>(p.c.positions + at[i]);
           }
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-          const int q = q0 + i * kEvictThreads * 4;
+          const int q = q0 + i * kThreads * 4;
           if (q < L) {
             u32x4 k;
 #pragma unroll
@@ -151,25 +161,32 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
       }
     } else {
 #pragma unroll 4
-      for (int j = tid; j < L; j += kEvictThreads) {
+      for (int j = tid; j < L; j += kThreads) {
         const uint32_t k = key_of(j);
         if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
       }
     }
     __syncthreads();
-    // thread t holds the digits 2047 - 2 t and 2046 - 2 t: prefix sums count from the largest digit down
-    const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
-    const int incl = wave_prefix_sum(hi + lo);
+    // thread t holds kBins digits from 2047 - kBins t down: prefix sums count from the largest digit on
+    constexpr int kBins = 2048 / kThreads;
+    int bin[kBins], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kBins; i++) {
+      bin[i] = hist[2047 - kBins * tid - i];
+      mine += bin[i];
+    }
+    const int incl = wave_prefix_sum(mine);
     if (lane == 63) sums[0][wave] = incl;
     __syncthreads();
-    int above = incl - hi - lo;
-    for (int w = 0; w < wave; w++) above += sums[0][w];
-    if (above < want && want <= above + hi) {
-      found[0] = 2047 - 2 * tid;
-      found[1] = above;
-    } else if (above + hi < want && want <= above + hi + lo) {
-      found[0] = 2046 - 2 * tid;
-      found[1] = above + hi;
+    int unused;
+    int above = incl - mine + before_wave<kWaves>(sums[0], wave, &unused);
+#pragma unroll
+    for (int i = 0; i < kBins; i++) {
+      if (above < want && want <= above + bin[i]) {
+        found[0] = 2047 - kBins * tid - i;
+        found[1] = above;
+      }
+      above += bin[i];
     }
     __syncthreads();
     prefix = (prefix << bits) | found[0];
@@ -179,15 +196,15 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   const uint32_t edge = prefix;  // keys above it stay, and the first `want` that equal it
 
   // ---- slots in order: a wave takes a run of whole 64s
-  const int run = (L + kEvictThreads - 1) / kEvictThreads * 64;
+  const int run = (L + kThreads - 1) / kThreads * 64;
   const int j0 = wave * run, j1 = j0 + run < L ? j0 + run : L;
   const uint64_t below = ((uint64_t)1 << lane) - 1;
   int ties = 0;
   for (int j = j0 + lane; j - lane < j1; j += 64) ties += __popcll(__ballot(j < j1 && key_of(j) == edge));
   if (lane == 0) sums[0][wave] = ties;
   __syncthreads();
-  int tie0 = 0;
-  for (int w = 0; w < wave; w++) tie0 += sums[0][w];
+  int all_ties;
+  const int tie0 = before_wave<kWaves>(sums[0], wave, &all_ties);
   int hole0 = 0, come0 = 0, moves = 0;
   __shared__ int32_t own_moves[kMoveD > 0 ? 2 * kMovesPerGroup : 1];
   int32_t* const holes = kMoveD > 0 ? own_moves : p.moves + (int64_t)blockIdx.x * 2 * p.cap;
@@ -217,13 +234,9 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
         sums[1][wave] = come;
       }
       __syncthreads();
-      for (int w = 0; w < kEvictWaves; w++) {
-        if (w < wave) {
-          hole0 += sums[0][w];
-          come0 += sums[1][w];
-        }
-        moves += sums[0][w];
-      }
+      int all_come;
+      hole0 = before_wave<kWaves>(sums[0], wave, &moves);
+      come0 = before_wave<kWaves>(sums[1], wave, &all_come);
       moves = moves < cap ? moves : cap;  // (as many as the cap, by its definition)
       if (kMoveD == 0 && tid == 0) p.counts[blockIdx.x] = moves;
     }
@@ -231,7 +244,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   if constexpr (kMoveD > 0) {
     __shared__ MoveSpots spots;
     __syncthreads();
-    move_keys<kMoveD, kEvictThreads>(p, b, h, holes, holes + cap, moves, spots);
+    move_keys<kMoveD, kThreads>(p, b, h, holes, holes + cap, moves, spots);
   }
 }
 
@@ -263,11 +276,11 @@ template <int D>
 hipError_t launch_evict_d(const EvictParams& p, hipStream_t stream) {
   const dim3 pairs((unsigned)(p.c.B * p.c.HK));
   const bool few = p.cap <= kMovesPerGroup;  // (decoding: a step or a few of them over the budget)
-  // (LDS decides how many heads a compute unit selects for at once: two of 16 waves, at more than 16384 keys one)
-#define FA_EVICT(CAP)                                                                                                         \
-  do {                                                                                                                        \
-    if (few) hipLaunchKernelGGL((paged_evict_kernel<CAP, D>), pairs, dim3(kEvictThreads), 0, stream, p);                      \
-    else hipLaunchKernelGGL((paged_evict_kernel<CAP, 0>), pairs, dim3(kEvictThreads), 0, stream, p);                          \
+  // (LDS decides how many heads a compute unit selects for at once: two, at more than 16384 keys one)
+#define FA_EVICT(CAP)                                                                                             \
+  do {                                                                                                            \
+    if (few) hipLaunchKernelGGL((paged_evict_kernel<CAP, D>), pairs, dim3(kEvictThreads), 0, stream, p);          \
+    else hipLaunchKernelGGL((paged_evict_kernel<CAP, 0>), pairs, dim3(kEvictThreads), 0, stream, p);              \
   } while (0)
   if (p.c.max_keys <= 4096) FA_EVICT(4096);
   else if (p.c.max_keys <= 16384) FA_EVICT(16384);

@@ -2,10 +2,13 @@
 //   w[h, j] += sum over rows r of exp(scale q_r . k_j - lse_r)      (rows: the tokens and heads of the group, fa_paged_fwd.h)
 // the probabilities formed again from the forward's lse: no second pass over V, no maxima.
 //
-// A wave owns 32 keys, their fragments in registers (read once, straight from the pages), and streams the rows past them in tiles of 32 that the
-// workgroup's four waves share through LDS: S = Q K^T leaves a key in a lane, so that its sum stays in the lane's register and has one
-// owner.  Few rows: bound by the read of K.  Many: by the exponentials, one per score.
-#include "fa_paged_fwd.h"
+// Two kernels.  Few rows (at most 32 a key head; a decode step): K streams past them, bound by HBM; waves stage 32-key tiles of their own as in
+// fa_paged_decode.hip, over the same line of units.  Many: a wave owns 32 keys, their fragments in registers, and streams the rows past them in tiles of 64
+// or 128 that the workgroup's four waves share through LDS; bound by the exponentials, one per score.  Both form S = Q K^T, which leaves a key in a lane, so
+// that its sum stays in the lane and has one owner.
+#include <type_traits>
+
+#include "fa_paged_line.h"
 
 namespace fa {
 
@@ -16,21 +19,24 @@ struct WeightsParams {
   uint32_t group_magic;  // ceil(2^32 / G), for numbers of at most 2^16: x / G = x * magic >> 32 (G = 1: not used)
 };
 
-template <int D>
+template <int D, int BM_>
 struct WCfg {
-  static constexpr int kTile = 32 * D * 2;
-  static constexpr int kRowOff = 2 * kTile;  // per buffer: 32 lse, 32 limits
-  static constexpr int kLds = 2 * kTile + 2 * 256;
+  static constexpr int BM = BM_;
+  static constexpr int kTile = BM * D * 2;
+  static constexpr int kRowOff = 2 * kTile;  // per buffer: BM lse, BM limits
+  static constexpr int kRow = BM * 8;
+  static constexpr int kLds = 2 * kTile + 2 * kRow;
 };
 
 }  // namespace
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) fa_paged_weights_kernel(const WeightsParams wp) {
-  using C = WCfg<D>;
+// (four waves a SIMD at least: with fewer the compiler puts the products into accumulation registers and moves them out one by one)
+template <typename T, int D, int BM_>
+__global__ void __launch_bounds__(256, 4) fa_paged_weights_kernel(const WeightsParams wp) {
+  using C = WCfg<D, BM_>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
-  constexpr int CH = D / 8;
+  constexpr int CH = D / 8, BM = C::BM;
   const PagedFwdParams& p = wp.f;
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[C::kLds];
 
@@ -72,11 +78,11 @@ __global__ void __launch_bounds__(256) fa_paged_weights_kernel(const WeightsPara
     const int tok = kblock * 128 - past + 1;
     row_first = tok > 0 ? tok * G : 0;
   }
-  const int tile0 = row_first >> 5, ntiles = (rows + 31) >> 5;
+  const int tile0 = row_first / BM, ntiles = (rows + BM - 1) / BM;
   // the next tile's first row as (token, head of the group)
-  int tok0 = __builtin_amdgcn_readfirstlane((tile0 * 32) / G), head0 = __builtin_amdgcn_readfirstlane(tile0 * 32 - tok0 * G);
+  int tok0 = __builtin_amdgcn_readfirstlane((tile0 * BM) / G), head0 = __builtin_amdgcn_readfirstlane(tile0 * BM - tok0 * G);
   constexpr int RPI = 64 / CH;                        // rows per direct-to-LDS instruction
-  constexpr int TI = 32 / RPI > 0 ? 32 / RPI : 1;     // instructions of a tile
+  constexpr int TI = BM / RPI;                        // instructions of a tile
   const int rl = lane / CH, pch = lane % CH;
   auto stage = [&](int it, int buf) {
     const char* const qb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + (int64_t)(q_begin + tok0) * p.q_rs + (int64_t)h * G * p.q_hs);
@@ -85,7 +91,7 @@ __global__ void __launch_bounds__(256) fa_paged_weights_kernel(const WeightsPara
       if (TI >= 4 ? (i & 3) != wave : i != wave) continue;
       int r = i * RPI + rl;
       const int sw = tile_swz<D, kSwzRow>(r);
-      const int most = rows - 1 - it * 32;
+      const int most = rows - 1 - it * BM;
       r = r < most ? r : most;
       const int x = head0 + r, t = per_group(x), g = x - t * G;
       dma16(qb, (uint32_t)(t * p.q_rs * 2 + g * p.q_hs * 2) + 16u * (uint32_t)(pch ^ sw), lds_raw + buf * C::kTile + i * 1024);
@@ -94,26 +100,26 @@ __global__ void __launch_bounds__(256) fa_paged_weights_kernel(const WeightsPara
   // a row's lse (in log2 units; +inf: no row, or one that sees nothing) and limit
   float lse_next = INFINITY;
   int limit_next = 0;
-  auto fetch_row = [&](int it) {  // wave 0, lanes below 32
-    const int r = it * 32 + c;
+  auto fetch_row = [&](int it) {  // a thread a row
+    const int r = it * BM + tid;
     lse_next = INFINITY;
     limit_next = 0;
-    if (wave == 0 && hf == 0 && r < rows) {
-      const int x = head0 + c, t = per_group(x), g = x - t * G;
+    if (tid < BM && r < rows) {
+      const int x = head0 + tid, t = per_group(x), g = x - t * G;
       const float v = p.lse[((int64_t)b * p.c.H + h * G + g) * p.sq_r + tok0 + t];
       lse_next = v == -INFINITY ? INFINITY : v * kLog2e;
       limit_next = p.causal ? past + tok0 + t : Lk;
     }
   };
   auto store_row = [&](int buf) {
-    if (wave == 0 && hf == 0) {
-      reinterpret_cast<float*>(lds_raw + C::kRowOff + buf * 256)[c] = lse_next;
-      reinterpret_cast<int*>(lds_raw + C::kRowOff + buf * 256 + 128)[c] = limit_next;
+    if (tid < BM) {
+      reinterpret_cast<float*>(lds_raw + C::kRowOff + buf * C::kRow)[tid] = lse_next;
+      reinterpret_cast<int*>(lds_raw + C::kRowOff + buf * C::kRow + BM * 4)[tid] = limit_next;
     }
   };
   int first_tok = tok0;  // of the tile in hand
   auto advance = [&]() {
-    const int x = head0 + 32, t = __builtin_amdgcn_readfirstlane(per_group(x));
+    const int x = head0 + BM, t = __builtin_amdgcn_readfirstlane(per_group(x));
     tok0 += t;
     head0 = x - t * G;
   };
@@ -121,7 +127,7 @@ __global__ void __launch_bounds__(256) fa_paged_weights_kernel(const WeightsPara
 #pragma unroll
   for (int ks = 0; ks < D / 16; ks++) qoff[ks] = frag_off<D, kSwzRow>(c, ks * 2 + hf);
 
-  float sum = 0.f;
+  float sum[2] = {0.f, 0.f};
   int it = tile0, buf = 0;
   if (it < ntiles) {
     stage(it, 0);
@@ -139,58 +145,230 @@ __global__ void __launch_bounds__(256) fa_paged_weights_kernel(const WeightsPara
       store_row(buf ^ 1);
       advance();
     }
-    const int* const limits = reinterpret_cast<const int*>(lds_raw + C::kRowOff + buf * 256 + 128);
-    const float* const lses = reinterpret_cast<const float*>(lds_raw + C::kRowOff + buf * 256);
+    const int* const limits = reinterpret_cast<const int*>(lds_raw + C::kRowOff + buf * C::kRow + BM * 4);
+    const float* const lses = reinterpret_cast<const float*>(lds_raw + C::kRowOff + buf * C::kRow);
     const T* const Qs = reinterpret_cast<const T*>(lds_raw + buf * C::kTile);
     if (live) {
-      f32x16 s;
+      auto tile = [&](auto masked) {
 #pragma unroll
-      for (int r = 0; r < 16; r++) s[r] = 0.f;
+        for (int half = 0; half < BM / 32; half++) {
+          f32x16 s;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ks++) s = E::mfma32(*reinterpret_cast<const vec8*>(Qs + qoff[ks]), kreg[ks], s);
-      const bool mask = p.causal && past + first_tok < key0 + 32;  // the tile's first row does not see all of the wave's keys
+          for (int r = 0; r < 16; r++) s[r] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(lses + 8 * j + 4 * hf);
-        f32x4 e;
+          for (int ks = 0; ks < D / 16; ks++) s = E::mfma32(*reinterpret_cast<const vec8*>(Qs + half * 32 * D + qoff[ks]), kreg[ks], s);
+          #pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(lses + half * 32 + 8 * j + 4 * hf);
+            f32x4 e;
 #pragma unroll
-        for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(s[4 * j + i], cs, -l4[i]));
-        if (mask) {
+            for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(s[4 * j + i], cs, -l4[i]));
+            if constexpr (decltype(masked)::value) {
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (key >= limits[8 * j + 4 * hf + i]) e[i] = 0.f;
+              for (int i = 0; i < 4; i++)
+                if (key >= limits[half * 32 + 8 * j + 4 * hf + i]) e[i] = 0.f;
+            }
+            sum[j & 1] += (e[0] + e[1]) + (e[2] + e[3]);
+          }
         }
-        sum += (e[0] + e[1]) + (e[2] + e[3]);
-      }
+      };
+      // (whether the tile's first row does not see all of the wave's keys)
+      if (p.causal && past + first_tok < key0 + 32) tile(std::true_type{});
+      else tile(std::false_type{});
     }
     first_tok = next_tok;
     buf ^= 1;
     it++;
   }
-  sum = half_sum(sum);
+  const float all = half_sum(sum[0] + sum[1]);
   if (hf == 0 && key0 + c < Lk) {
     const int page = table[key >> p.c.page_log2];
     if (page_is_one(page, p.c.n_pages)) {
       float* const w = p.c.weights + (((int64_t)page * p.c.HK + h) << p.c.page_log2) + (key & ((1 << p.c.page_log2) - 1));
-      *w += sum;
+      *w += all;
     }
   }
 }
 
 namespace {
-template <typename T>
-hipError_t launch_t(const WeightsParams& p, int head_dim, hipStream_t stream) {
-  const int64_t n = (int64_t)p.f.c.B * p.f.c.HK * ((p.f.c.max_keys + 127) / 128);
-  if (n >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)n);
-  switch (head_dim) {
-    case 16: hipLaunchKernelGGL((fa_paged_weights_kernel<T, 16>), grid, dim3(256), 0, stream, p); break;
-    case 32: hipLaunchKernelGGL((fa_paged_weights_kernel<T, 32>), grid, dim3(256), 0, stream, p); break;
-    case 64: hipLaunchKernelGGL((fa_paged_weights_kernel<T, 64>), grid, dim3(256), 0, stream, p); break;
-    case 128: hipLaunchKernelGGL((fa_paged_weights_kernel<T, 128>), grid, dim3(256), 0, stream, p); break;
-    default: return hipErrorInvalidValue;
+
+template <int D>
+struct FewCfg {
+  static constexpr int NW = 4, BN = 32;
+  static constexpr int kTile = BN * D * 2;
+  static constexpr int kWave = 2 * kTile;      // two stages
+  static constexpr int kKeys = 2048;           // keys whose sums wait in LDS to be added to the weights
+  static constexpr int kLds = NW * kWave + kKeys * 4;
+};
+// Workgroups resident at once: 72 KB of LDS at d = 128, 40 at 64; below, as many as the waves fill the SIMDs with
+constexpr int few_resident(int D) { return 256 * (D == 128 ? 2 : 4); }
+
+}  // namespace
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) fa_paged_weights_few_kernel(const PagedFwdParams p) {
+  using C = FewCfg<D>;
+  using E = Elem<T>;
+  using vec8 = typename E::vec8;
+  using Stager = GroupStager<D, kSwzRow>;
+  constexpr int NW = C::NW, BN = C::BN, NI = 2 * Stager::NI;
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[C::kLds];
+  float* const sums = reinterpret_cast<float*>(lds_raw + NW * C::kWave);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hf = lane >> 5;
+  const float cs = p.scale_log2;
+  Stager st;
+  st.init(lane, p.c.k_ss);
+  unsigned char* const lds_wave = lds_raw + wave * C::kWave;
+  int koff[D / 16];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ks++) koff[ks] = frag_off<D, kSwzRow>(c, ks * 2 + hf);
+
+  const int sums0 = unit_sums(p.c, 0);
+  const int64_t units = all_units(p.c, sums0);
+  const int n = sharers(p, units);
+  if ((int)blockIdx.x >= n || units == 0) return;
+  int64_t u = share_begin(units, blockIdx.x, n);
+  const int64_t u_end = share_begin(units, blockIdx.x + 1, n);
+  Spot at = spot_of(p.c, u, sums0);
+
+  while (u < u_end) {
+    const int b = __builtin_amdgcn_readfirstlane(at.b), h = __builtin_amdgcn_readfirstlane(at.h);
+    const int unit0 = __builtin_amdgcn_readfirstlane(at.unit), pair_units = __builtin_amdgcn_readfirstlane(at.units);
+    int unit1 = u_end - u < pair_units - unit0 ? unit0 + (int)(u_end - u) : pair_units;
+    unit1 = unit1 - unit0 <= C::kKeys / kDecodeUnit ? unit1 : unit0 + C::kKeys / kDecodeUnit;
+    int q_begin = 0, Lq = 0;
+    if (!paged_rows(p.c, b, &q_begin, &Lq)) return;  // (never: such a sequence has no units)
+    const int Lk = paged_len(p.c, b), G = p.c.G, rows = Lq * G;
+    const int k_lo = unit0 * kDecodeUnit;
+    const int k_hi = Lk < unit1 * kDecodeUnit ? Lk : unit1 * kDecodeUnit;
+    const int ntiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
+    const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
+    const char* const kb = p.c.k + h * p.c.k_hs;
+    const int last_group = (Lk - 1) >> 4;
+    int page[2];
+    auto ask = [&](int t) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int g = (k_lo >> 4) + 2 * t + j;
+        page[j] = page_of_group(p.c, table, g < last_group ? g : last_group);
+      }
+    };
+    auto issue = [&](int t, int stage) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int g0 = (k_lo >> 4) + 2 * t + j, g = g0 < last_group ? g0 : last_group;
+        st.issue(kb + page[j] * p.c.k_ps + slot_of_group(p.c, g) * p.c.k_ss, p.c.k_ss, g < last_group ? 15 : (Lk - 1) & 15,
+                 lds_wave + stage * C::kTile + j * Stager::kBytes);
+      }
+    };
+    int t = wave, stage = 0;
+    if (t < ntiles) {
+      ask(t);
+      issue(t, 0);
+    }
+    if (t + NW < ntiles) {
+      ask(t + NW);
+      issue(t + NW, 1);
+    }
+    // the rows: lane c holds row c's fragments; of the 16 that a lane's results belong to, lse (log2 units; +inf: no row, or one that sees nothing)
+    // and limit.  Waited for here, with the first two tiles: the main loop counts this wave's outstanding loads.
+    const int row = c < rows ? c : rows - 1, tok = row / G;
+    vec8 qreg[D / 16];
+    const T* const qp = reinterpret_cast<const T*>(p.q) + (int64_t)(q_begin + tok) * p.q_rs + (int64_t)(h * G + (row - tok * G)) * p.q_hs + hf * 8;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) qreg[ks] = bitcast<vec8>(ld_global16(qp + ks * 16));
+    float lse[16];
+    int limit[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int x = 8 * (r >> 2) + 4 * hf + (r & 3), xc = x < rows ? x : rows - 1, xt = xc / G;
+      const float v = p.lse[((int64_t)b * p.c.H + h * G + (xc - xt * G)) * p.sq_r + xt];
+      lse[r] = x >= rows || v == -INFINITY ? INFINITY : v * kLog2e;
+      limit[r] = p.causal ? Lk - Lq + 1 + xt : Lk;
+    }
+    wait_vmcnt<0>();
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) asm volatile("" : "+v"(qreg[ks]));
+#pragma unroll
+    for (int r = 0; r < 16; r++) asm volatile("" : "+v"(lse[r]));
+    const int least_limit = p.causal ? Lk - Lq + 1 : Lk;  // of row 0
+
+    for (; t < ntiles; t += NW) {
+      if (t + NW < ntiles) wait_vmcnt<NI>();  // (its NI loads were issued after this tile's)
+      else wait_vmcnt<0>();
+      if (t + 2 * NW < ntiles) ask(t + 2 * NW);
+      const T* const Ks = reinterpret_cast<const T*>(lds_wave + stage * C::kTile);
+      f32x16 s;
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ks++) s = E::mfma32(qreg[ks], *reinterpret_cast<const vec8*>(Ks + koff[ks]), s);
+      if (t + 2 * NW < ntiles) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage has been read before it is refilled
+        issue(t + 2 * NW, stage);
+      }
+      const int key = k_lo + t * BN + c;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = fast_exp2(__builtin_fmaf(s[r], cs, -lse[r]));
+      if (k_lo + t * BN + BN > least_limit) {
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (key >= limit[r]) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) sum += (s[r] + s[r + 1]) + (s[r + 2] + s[r + 3]);
+      sum = half_sum(sum);
+      if (hf == 0) sums[t * BN + c] = sum;
+      stage ^= 1;
+    }
+    __syncthreads();
+    for (int i = tid; i < k_hi - k_lo; i += 64 * NW) {
+      const int key = k_lo + i, pg = table[key >> p.c.page_log2];
+      if (page_is_one(pg, p.c.n_pages)) {
+        float* const w = p.c.weights + (((int64_t)pg * p.c.HK + h) << p.c.page_log2) + (key & ((1 << p.c.page_log2) - 1));
+        *w += sums[i];
+      }
+    }
+    u += unit1 - unit0;
+    if (u >= u_end) return;
+    if (unit1 < pair_units) at.unit = unit1;
+    else if (!next_pair(p.c, &at)) return;  // (never: the line does not end here)
+    __syncthreads();  // the sums have been read
+  }
+}
+
+namespace {
+
+template <typename T, int D>
+hipError_t launch_d(const WeightsParams& p, hipStream_t stream) {
+  const int64_t blocks = (int64_t)p.f.c.B * p.f.c.HK * ((p.f.c.max_keys + 127) / 128);
+  if (blocks >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
+  if (p.f.c.max_sq * p.f.c.G <= kDecodeMaxQ) {
+    PagedFwdParams f = p.f;
+    f.least = 1;
+    f.groups = (int)(blocks < few_resident(D) ? blocks : few_resident(D));  // (a block of 128 keys is a unit)
+    hipLaunchKernelGGL((fa_paged_weights_few_kernel<T, D>), dim3((unsigned)f.groups), dim3(256), 0, stream, f);
+  } else {
+    // rows of a tile: work enough to cover the next one's loads, where there are as many (4 x 16 heads x 509 tokens, d = 64 33.6 us, in tiles of 64 36.8, of 32 40.9)
+    constexpr int kMost = D == 128 ? 64 : 128;
+    if (p.f.c.max_sq * p.f.c.G <= 64) hipLaunchKernelGGL((fa_paged_weights_kernel<T, D, 64>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((fa_paged_weights_kernel<T, D, kMost>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
   }
   return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_t(const WeightsParams& p, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 16: return launch_d<T, 16>(p, stream);
+    case 32: return launch_d<T, 32>(p, stream);
+    case 64: return launch_d<T, 64>(p, stream);
+    case 128: return launch_d<T, 128>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 }  // namespace
 
