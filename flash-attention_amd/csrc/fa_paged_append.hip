@@ -61,57 +61,76 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p)
 #pragma unroll
     for (int i = 0; i < ROWS; i++) seq[i] += __popcll(__ballot(s < p.c.B && end <= row0 + i));
   }
+  // (loads and what is made of them in loops of their own, without branches: the rows' loads are on their way together)
+  int len[ROWS], begin[ROWS], end[ROWS];
+  bool there[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; i++) {
-    const int b = __builtin_amdgcn_readfirstlane(seq[i]), row = row0 + i;
-    seq[i] = b < p.c.B ? b : p.c.B - 1;  // (no branches here and below: the rows' loads are on their way together)
-    slot[i] = append_slot(ld_scalar(p.c.seqlens, seq[i]), ld_scalar(p.c.cu_q, seq[i]), ld_scalar(p.c.cu_q, seq[i] + 1), row, p.c.max_sq, p.c.max_keys);
-    if (b >= p.c.B || row >= p.c.total_q) slot[i] = -1;  // (rows behind the last sequence)
+    const int b = __builtin_amdgcn_readfirstlane(seq[i]);
+    there[i] = b < p.c.B && row0 + i < p.c.total_q;  // (else: behind the last sequence)
+    seq[i] = b < p.c.B ? b : p.c.B - 1;
+    len[i] = ld_scalar(p.c.seqlens, seq[i]);
+    begin[i] = ld_scalar(p.c.cu_q, seq[i]);
+    end[i] = ld_scalar(p.c.cu_q, seq[i] + 1);
   }
 #pragma unroll
   for (int i = 0; i < ROWS; i++) {
-    const int row = row0 + i < p.c.total_q ? row0 + i : p.c.total_q - 1;
+    slot[i] = append_slot(len[i], begin[i], end[i], row0 + i, p.c.max_sq, p.c.max_keys);
+    if (!there[i]) slot[i] = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
     page[i] = ld_scalar(p.c.table + (int64_t)seq[i] * p.c.table_rs, (slot[i] < 0 ? 0 : slot[i]) >> p.c.page_log2);
-    pos[i] = p.given_positions ? ld_scalar(p.given_positions, row) : slot[i];
+    pos[i] = slot[i];
+  }
+  if (p.given_positions) {
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) pos[i] = ld_scalar(p.given_positions, row0 + i < p.c.total_q ? row0 + i : p.c.total_q - 1);
   }
 #pragma unroll
   for (int i = 0; i < ROWS; i++)
     if (slot[i] < 0) page[i] = -1;
-  typename Elem<T>::vec4 c4[ROWS], s4[ROWS];
+  // What an address has of the lane, once; the rest of it, a row's, is wave-uniform.
+  typedef typename Elem<T>::vec4 vec4;
+  const bool moves_only = !norm && !rot;
+  const int64_t lane_to = part == 0 ? (int64_t)h * p.qo_hs * 2 + ch * 16 : (part == 1 ? h * p.c.k_hs : h * p.c.v_hs) + ch * 16;
+  char* const base = part == 0 ? reinterpret_cast<char*>(p.q_out) + lane_to : (part == 1 ? p.c.k : p.c.v) + lane_to;
+  vec4 c4[ROWS], s4[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; i++) {
-    if (on && rot && page_is_one(page[i], p.c.n_pages)) {
-      const int64_t at = (int64_t)table_row(pos[i], p.table_rows) * (D / 2) + ch * 4;
-      c4[i] = *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.cos) + at);
-      s4[i] = *reinterpret_cast<const typename Elem<T>::vec4*>(reinterpret_cast<const T*>(p.sin) + at);
+    const int64_t row_at = (int64_t)table_row(pos[i], p.table_rows) * (D / 2);
+    if (on && rot) {
+      c4[i] = reinterpret_cast<const vec4*>(reinterpret_cast<const T*>(p.cos) + row_at)[ch];
+      s4[i] = reinterpret_cast<const vec4*>(reinterpret_cast<const T*>(p.sin) + row_at)[ch];
     }
   }
 #pragma unroll
   for (int i = 0; i < ROWS; i++) {
     if (!page_is_one(page[i], p.c.n_pages)) continue;  // (wave-uniform)
+    const int at = slot[i] & ((1 << p.c.page_log2) - 1);
+    const int64_t to_q = (int64_t)(row0 + i) * p.qo_rs * 2, to_k = page[i] * p.c.k_ps + at * p.c.k_ss, to_v = page[i] * p.c.v_ps + at * p.c.v_ss;
+    const int64_t m0 = ((int64_t)page[i] * p.c.HK << p.c.page_log2) + at;
     if (on) {
-      float x[8];
+      char* const dst = base + (part == 0 ? to_q : (part == 1 ? to_k : to_v));
+      vec8 y = x8[i];
+      if (!moves_only) {
+        float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = (float)x8[i][e];
-      if (norm) {
-        const float r = inverse_rms<CH>(x, p.eps);
+        for (int e = 0; e < 8; e++) x[e] = (float)x8[i][e];
+        if (norm) {
+          const float r = inverse_rms<CH>(x, p.eps);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = x[e] * r * w[e];
+          for (int e = 0; e < 8; e++) x[e] = x[e] * r * w[e];
+        }
+        if (rot) turn(x, c4[i], s4[i]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = (T)x[e];
       }
-      if (rot) turn(x, c4[i], s4[i]);
-      vec8 y;
-#pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = (T)x[e];
-      const int at = slot[i] & ((1 << p.c.page_log2) - 1);
-      char* dst;
-      if (part == 0) dst = reinterpret_cast<char*>(reinterpret_cast<T*>(p.q_out) + (int64_t)(row0 + i) * p.qo_rs + (int64_t)h * p.qo_hs);
-      else if (part == 1) dst = p.c.k + page[i] * p.c.k_ps + at * p.c.k_ss + h * p.c.k_hs;
-      else dst = p.c.v + page[i] * p.c.v_ps + at * p.c.v_ss + h * p.c.v_hs;
-      st_global16(dst + ch * 16, bitcast<u32x4>(y));
+      st_global16(dst, bitcast<u32x4>(y));
       if (part == 1 && ch == 0) {
-        const int64_t m = ((int64_t)page[i] * p.c.HK + h) << p.c.page_log2;
-        if (p.c.weights) p.c.weights[m + at] = 0.f;
-        if (p.c.positions) p.c.positions[m + at] = pos[i];
+        const int64_t m = m0 + ((int64_t)h << p.c.page_log2);
+        if (p.c.weights) p.c.weights[m] = 0.f;
+        if (p.c.positions) p.c.positions[m] = pos[i];
       }
     }
   }
@@ -119,12 +138,13 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p)
 
 template <typename T, int D>
 hipError_t launch_append_d(const AppendParams& p, hipStream_t stream) {
-  // A decode step's few rows: one a workgroup, so that as many as there are run side by side; prompts: eight a thread in flight.
+  // A decode step's few rows: one a workgroup, so that as many as there are run side by side; prompts: several a thread in flight.
+  constexpr int kRows = 4;  // (8 x 2500 tokens of 16 + 16 heads, d = 64, 251 MB: 64 us, eight 69: with their scalar registers full)
   const bool few = (int64_t)p.c.total_q * p.pieces <= 2048;
-  const int rows = few ? 1 : 8;
+  const int rows = few ? 1 : kRows;
   const dim3 grid((unsigned)((p.c.total_q + rows - 1) / rows * p.pieces)), block((unsigned)p.threads);
   if (few) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((paged_append_kernel<T, D, 8>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((paged_append_kernel<T, D, kRows>), grid, block, 0, stream, p);
   return hipGetLastError();
 }
 template <typename T>
