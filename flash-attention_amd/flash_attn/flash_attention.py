@@ -5,7 +5,9 @@ import torch.nn as nn
 
 from . import flash_attn_gfx950 as _backend
 from .bert_padding import pad_input, unpad_input
-from .flash_attn_interface import flash_attn_unpadded_qkvpacked_func, flash_attn_unpadded_qkvpacked_rotary_func
+from .flash_attn_interface import (flash_attn_unpadded_qkvpacked_func, flash_attn_unpadded_qkvpacked_norm_rotary_func,
+                                   flash_attn_unpadded_qkvpacked_rotary_func)
+from .rotary import apply_qk_norm_rotary
 
 
 class _PaddedAttention(torch.autograd.Function):
@@ -31,7 +33,7 @@ class FlashAttention(nn.Module):
         self.dropout_p = attention_dropout
 
     def forward(self, qkv, attn_mask=None, key_padding_mask=None, causal=False, cu_seqlens=None, max_s=None,
-                need_weights=False, alibi_slopes=None, attn_bias=None, rotary=None):
+                need_weights=False, alibi_slopes=None, attn_bias=None, rotary=None, qk_norm=None):
         """qkv is (B, S, 3, H, D) when cu_seqlens is None, else already packed (nnz, 3, H, D) with cu_seqlens / max_s.
         key_padding_mask, if given, is an object whose `.bool_matrix` is a (B, S) bool tensor, True = keep.
         alibi_slopes (not in the reference): (H,) fp32 slopes of the in-kernel attention bias -slope * |i - j|.
@@ -40,6 +42,8 @@ class FlashAttention(nn.Module):
         rotary (not in the reference): (cos_half, sin_half) tables of RotaryEmbedding.half_tables: q and k are turned by
         their position inside their sequence within the attention kernels (not with key_padding_mask, alibi_slopes or
         attn_bias).
+        qk_norm (not in the reference): (q_weight, k_weight) of headdim each: q and k are first divided by their root mean square, head by head,
+        and multiplied by them (in front of the rotation; like rotary not with key_padding_mask, alibi_slopes or attn_bias).
         Returns (output, None); output has the layout of the input's token dimensions."""
         assert not need_weights
         assert attn_mask is None
@@ -47,17 +51,22 @@ class FlashAttention(nn.Module):
         assert qkv.is_cuda
         p = self.dropout_p if self.training else 0.0
 
-        if rotary is not None:
+        if rotary is not None or qk_norm is not None:
             assert key_padding_mask is None and alibi_slopes is None and attn_bias is None
+            if qk_norm is not None:
+                def attend(x, cu, longest):
+                    return flash_attn_unpadded_qkvpacked_norm_rotary_func(x, *qk_norm, *(rotary or (None, None)), cu, longest, p,
+                                                                          softmax_scale=self.softmax_scale, causal=causal)
+            else:
+                def attend(x, cu, longest):
+                    return flash_attn_unpadded_qkvpacked_rotary_func(x, *rotary, cu, longest, p, softmax_scale=self.softmax_scale, causal=causal)
             if cu_seqlens is not None:
                 assert max_s is not None
-                return flash_attn_unpadded_qkvpacked_rotary_func(qkv, *rotary, cu_seqlens, max_s, p,
-                                                                 softmax_scale=self.softmax_scale, causal=causal), None
+                return attend(qkv, cu_seqlens, max_s), None
             batch, seqlen = qkv.shape[0], qkv.shape[1]
             packed = qkv.reshape(batch * seqlen, *qkv.shape[2:])
             cu = torch.arange(0, (batch + 1) * seqlen, step=seqlen, dtype=torch.int32, device=qkv.device)
-            out = flash_attn_unpadded_qkvpacked_rotary_func(packed, *rotary, cu, seqlen, p,
-                                                            softmax_scale=self.softmax_scale, causal=causal)
+            out = attend(packed, cu, seqlen)
             return out.reshape(batch, seqlen, *out.shape[1:]), None
 
         if cu_seqlens is not None:
@@ -92,10 +101,11 @@ class FlashAttention(nn.Module):
 
 
 class FlashMHA(nn.Module):
-    """Multi-head self-attention block: fused QKV projection, FlashAttention, output projection."""
+    """Multi-head self-attention block: fused QKV projection, FlashAttention, output projection.
+    qk_norm (not in the reference): queries and keys are normalised head by head, with learned weights, in front of the rotation."""
 
     def __init__(self, embed_dim, num_heads, bias=True, batch_first=True, attention_dropout=0.0, causal=False,
-                 use_rotary_emb=None, device=None, dtype=None, **kwargs) -> None:
+                 use_rotary_emb=None, device=None, dtype=None, qk_norm=False, **kwargs) -> None:
         assert batch_first
         factory_kwargs = {"device": device, "dtype": dtype}
         super().__init__()
@@ -110,6 +120,10 @@ class FlashMHA(nn.Module):
         if use_rotary_emb is not None:
             from .rotary import RotaryEmbedding, RotaryEmbedding2D
             self.rotary_emb = RotaryEmbedding(self.head_dim) if use_rotary_emb == "1d" else RotaryEmbedding2D(self.head_dim)
+        self.qk_norm = qk_norm
+        if qk_norm:
+            self.q_norm_weight = nn.Parameter(torch.ones(self.head_dim, **factory_kwargs))
+            self.k_norm_weight = nn.Parameter(torch.ones(self.head_dim, **factory_kwargs))
         self.Wqkv = nn.Linear(embed_dim, 3 * embed_dim, bias=bias, **factory_kwargs)
         self.inner_attn = FlashAttention(attention_dropout=attention_dropout, **factory_kwargs)
         self.out_proj = nn.Linear(embed_dim, embed_dim, bias=bias, **factory_kwargs)
@@ -117,6 +131,18 @@ class FlashMHA(nn.Module):
     def forward(self, x, x_ignored_, x_ignored_1_, attn_mask=None, key_padding_mask=None, need_weights=False):
         b, s = x.shape[0], x.shape[1]
         qkv = self.Wqkv(x).reshape(b, s, 3, self.num_heads, self.head_dim)
+        if self.qk_norm and key_padding_mask is None and self.use_rotary_emb != "2d":
+            rotary = self.rotary_emb.half_tables(qkv) if self.use_rotary_emb else None
+            context, attn_weights = self.inner_attn(qkv, need_weights=need_weights, causal=self.causal, rotary=rotary, qk_norm=self._norm_weights())
+            return self.out_proj(context.reshape(b, s, self.embed_dim)), attn_weights
+        if self.qk_norm:
+            tables = self.rotary_emb.half_tables(qkv) if self.use_rotary_emb == "1d" else (None, None)
+            query, key = apply_qk_norm_rotary(qkv[:, :, 0], qkv[:, :, 1], *self._norm_weights(), *tables)
+            qkv = torch.stack([query, key, qkv[:, :, 2]], dim=2)
+            if self.use_rotary_emb == "2d":
+                qkv = self.rotary_emb.rotate_qkv_(qkv)
+            context, attn_weights = self.inner_attn(qkv, key_padding_mask=key_padding_mask, need_weights=need_weights, causal=self.causal)
+            return self.out_proj(context.reshape(b, s, self.embed_dim)), attn_weights
         if (self.use_rotary_emb == "1d" and key_padding_mask is None and qkv.is_cuda and qkv.dtype == torch.float16):
             # the rotation happens inside the attention kernels (q as it is loaded, dq and dk as they are stored)
             context, attn_weights = self.inner_attn(qkv, need_weights=need_weights, causal=self.causal,
@@ -132,3 +158,22 @@ class FlashMHA(nn.Module):
         context, attn_weights = self.inner_attn(qkv, key_padding_mask=key_padding_mask, need_weights=need_weights,
                                                 causal=self.causal)
         return self.out_proj(context.reshape(b, s, self.embed_dim)), attn_weights
+
+    def _norm_weights(self):
+        return self.q_norm_weight, self.k_norm_weight
+
+    def forward_cached(self, x, step, layer=0):
+        """The block on the new tokens of a serving step (not in the reference): x (total, embed_dim), packed as `step` (PagedKVCache.step) has them.
+        Their keys and values go into the cache's pages of `layer`, normalised and turned as in forward(), and they attend to all that their sequences
+        have there (causal).  Evaluation only."""
+        assert self.causal and self.use_rotary_emb != "2d"
+        total = x.shape[0]
+        q, k, v = self.Wqkv(x).reshape(total, 3, self.num_heads, self.head_dim).unbind(1)
+        opt = {}
+        if self.qk_norm:
+            opt.update(q_weight=self.q_norm_weight, k_weight=self.k_norm_weight)
+        if self.use_rotary_emb:
+            opt.update(zip(("cos_half", "sin_half"), self.rotary_emb.tables_to(step.max_position, q)))
+        q = step.append(layer, q, k, v, **opt)
+        out = step.attend(layer, q, softmax_scale=self.inner_attn.softmax_scale)
+        return self.out_proj(out.reshape(total, self.embed_dim))

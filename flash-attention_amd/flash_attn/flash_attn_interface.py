@@ -65,11 +65,14 @@ def _split(packing, tensors):
 
 
 def _forward(ctx, packing, tensors, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, dropout_p,
-             softmax_scale, causal, return_softmax, alibi_slopes=None, attn_bias=None, rotary=None):
+             softmax_scale, causal, return_softmax, alibi_slopes=None, attn_bias=None, rotary=None, qk=None, more=()):
+    """qk: None, or the (total, 2, nheads, headdim) queries and keys to attend with instead of those in tensors; more: further tensors to save, last."""
     q, k, v = _split(packing, tensors)
     # rotary embedding inside the kernels (packed qkv only): the keys are rotated into a side buffer by the rotary kernel,
     # the queries by the attention kernel as it loads them, which also leaves them in the side buffer for the backward
-    rot = q_rot = None
+    rot, q_rot = qk, None
+    if rot is not None:
+        q, k = rot[:, 0], rot[:, 1]
     if rotary is not None:
         rot = _rotated_keys(tensors[0], cu_seqlens_q, int(max_seqlen_q), *rotary)
         q_rot, k = rot[:, 0], rot[:, 1]
@@ -92,7 +95,7 @@ def _forward(ctx, packing, tensors, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
                                                     dropout_p, softmax_scale, causal, return_softmax, alibi_slopes,
                                                     keep_words, bias_t, rotary, q_rot, philox)
     dropout_saved, ctx.dropout_kept = _backend.pack_dropout(keep_words, philox)
-    ctx.save_for_backward(*tensors, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, bias_t, rot, *dropout_saved)
+    ctx.save_for_backward(*tensors, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, bias_t, rot, *dropout_saved, *more)
     ctx.rotary = rotary  # constant tables, not differentiated
     ctx.bias_shape = tuple(attn_bias.shape) if attn_bias is not None else None
     ctx.bias_needs_grad = attn_bias is not None and attn_bias.requires_grad
@@ -189,6 +192,33 @@ class FlashAttnRotaryQKVPackedFunc(torch.autograd.Function):
         return _extra_grads(ctx, _backward(ctx, dout))
 
 
+class FlashAttnNormRotaryQKVPackedFunc(torch.autograd.Function):
+    """apply(qkv, q_weight, k_weight, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale, causal, eps): self-attention on a packed qkv
+    whose q and k are first normalised head by head and turned (no counterpart in the reference).  The backward of the attention leaves dq and dk in
+    their places of dqkv, and that of the norm turns them there into the gradients of the unnormalised ones."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale, causal, eps):
+        _backend._check(qkv.is_cuda and qkv.dim() == 4 and qkv.shape[1] == 3, "qkv must be a (total, 3, nheads, headdim) GPU tensor")
+        total, batch = qkv.shape[0], cu_seqlens.numel() - 1
+        positions = None
+        if cos_half is not None and total != batch * int(max_seqlen):
+            positions = _backend.token_positions(cu_seqlens, total)
+        qk = torch.empty((total, 2) + tuple(qkv.shape[2:]), dtype=qkv.dtype, device=qkv.device)
+        ctx.norm_args = (int(max_seqlen), eps)
+        _backend.qk_norm_rotary(qkv[:, 0], qkv[:, 1], qk[:, 0], qk[:, 1], q_weight, k_weight, cos_half, sin_half, positions, *ctx.norm_args)
+        return _forward(ctx, "qkv", (qkv,), cu_seqlens, cu_seqlens, max_seqlen, max_seqlen, dropout_p, softmax_scale, causal, False, qk=qk,
+                        more=(q_weight, k_weight, cos_half, sin_half, positions))
+
+    @staticmethod
+    def backward(ctx, dout, *args):
+        dqkv, = _backward(ctx, dout)
+        qkv, norm = ctx.saved_tensors[0], ctx.saved_tensors[-5:]
+        dq, dk = dqkv[:, 0], dqkv[:, 1]
+        dqw, dkw = _backend.qk_norm_rotary_bwd(dq, dk, qkv[:, 0], qkv[:, 1], dq, dk, *norm, *ctx.norm_args)
+        return (dqkv, dqw, dkw) + (None,) * 8
+
+
 class FlashAttnKVPackedFunc(torch.autograd.Function):
     """apply(q, kv, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, dropout_p, softmax_scale, causal,
     return_softmax)"""
@@ -266,6 +296,16 @@ def flash_attn_unpadded_qkvpacked_rotary_func(qkv, cos_half, sin_half, cu_seqlen
     takes a pass of its own.  Differentiable with respect to qkv."""
     return FlashAttnRotaryQKVPackedFunc.apply(qkv, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale,
                                               causal)
+
+
+def flash_attn_unpadded_qkvpacked_norm_rotary_func(qkv, q_weight, k_weight, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale=None,
+                                                   causal=False, eps=1e-6):
+    """flash_attn_unpadded_qkvpacked_func on a qkv whose q and k are first normalised and turned as by apply_qk_norm_rotary (rotary.py): every head's
+    vector divided by its root mean square, times q_weight / k_weight ((headdim,), qkv's dtype or fp32), then turned by its position in its sequence
+    (cos_half, sin_half: (>= max_seqlen, headdim / 2) tables in qkv's dtype; None: not turned).  One pass in front of the attention and one behind its
+    backward, in place.  qkv itself is left as it is.  Differentiable with respect to qkv and the weights."""
+    return FlashAttnNormRotaryQKVPackedFunc.apply(qkv, q_weight, k_weight, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale, causal,
+                                                  eps)
 
 
 def flash_attn_unpadded_kvpacked_func(q, kv, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,

@@ -82,3 +82,153 @@ def paged_evict_func(k_cache, v_cache, key_weights, key_positions, page_table, s
         return done
     _inference(k_cache, v_cache)
     return _backend.paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k)
+
+
+class PagedKVCache:
+    """A pool of pages for the keys and values of a model's layers, and the book of which pages each sequence has.  All layers of a sequence use the
+    same page numbers, each in a pool of its own.
+
+        cache = PagedKVCache(layers, pages, page_size, nheads_k, headdim, dtype, device)
+        a, b = cache.add(), cache.add()
+        step = cache.step([a, b], [prompt_a, prompt_b])            # numbers of new tokens; then, layer by layer:
+        q = step.append(layer, q, k, v, ...)                       # packed (total, heads, headdim) tensors of the new tokens
+        out = step.attend(layer, q)
+        cache.evict([a, b], budget, recent)                        # if made with key_weights=True
+        cache.remove(a)
+
+    A page holds a head's tokens one after the other.  Everything is enqueued on the current stream in the order of the calls; a removed sequence's pages may be
+    given to another at once, so steps of one cache belong on one stream."""
+
+    def __init__(self, layers, pages, page_size, nheads_k, headdim, dtype=torch.float16, device=None, key_weights=False):
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise RuntimeError("page_size must be a power of two from 16 to 1024, got %d" % page_size)
+        if layers < 1 or pages < 1 or nheads_k < 1 or headdim not in (16, 32, 64, 128) or dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError("layers, pages and nheads_k must be positive, headdim 16, 32, 64 or 128, dtype fp16 or bf16")
+        self.page_size = page_size
+        shape = (layers, pages, nheads_k, page_size, headdim)
+        device = torch.device("cuda" if device is None else device)
+        # zeros: what lies behind a sequence's last key is read with its page's, and only then left out
+        self._k, self._v = (torch.zeros(shape, dtype=dtype, device=device).transpose(2, 3) for _ in range(2))
+        self.key_weights = torch.zeros(shape[:4], dtype=torch.float32, device=device) if key_weights else None
+        self.key_positions = torch.zeros(shape[:4], dtype=torch.int32, device=device) if key_weights else None
+        self.device = self._k.device
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages, self._len, self._seen = {}, {}, {}
+        self._next_id = 0
+
+    def layer(self, i):
+        """(k_cache, v_cache) of layer i: (pages, page size, nheads_k, headdim)"""
+        return self._k[i], self._v[i]
+
+    def add(self):
+        """A new, empty sequence."""
+        seq, self._next_id = self._next_id, self._next_id + 1
+        self._pages[seq], self._len[seq], self._seen[seq] = [], 0, 0
+        return seq
+
+    def remove(self, seq):
+        self._free.extend(reversed(self._pages.pop(seq)))
+        del self._len[seq], self._seen[seq]
+
+    def length(self, seq):
+        """Tokens of the sequence that the cache holds"""
+        return self._len[seq]
+
+    def free_pages(self):
+        return len(self._free)
+
+    def _book(self, seqs):
+        if not seqs or len(set(seqs)) != len(seqs) or any(s not in self._pages for s in seqs):
+            raise RuntimeError("a step takes different sequences of this cache, one at least")
+
+    def _device_ints(self, *lists):
+        """int32 tensors on the device, by way of one copy"""
+        flat = torch.tensor([x for l in lists for x in l], dtype=torch.int32)
+        flat = flat.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else flat
+        out, at = [], 0
+        for l in lists:
+            out.append(flat[at:at + len(l)])
+            at += len(l)
+        return out
+
+    def step(self, seqs, new_tokens):
+        """Makes room for new_tokens[i] further tokens of seqs[i] and returns the PagedStep that stores them and attends."""
+        seqs, new = list(seqs), [int(n) for n in new_tokens]
+        self._book(seqs)
+        if len(new) != len(seqs) or min(new) < 0 or sum(new) == 0:
+            raise RuntimeError("a number of new tokens for each sequence, one token at least")
+        need = {s: -(-(self._len[s] + n) // self.page_size) - len(self._pages[s]) for s, n in zip(seqs, new)}
+        if sum(max(0, n) for n in need.values()) > len(self._free):
+            raise RuntimeError("the cache has %d free pages, the step needs %d" % (len(self._free), sum(max(0, n) for n in need.values())))
+        positions = []
+        for s, n in zip(seqs, new):
+            self._pages[s].extend(self._free.pop() for _ in range(max(0, need[s])))
+            positions.extend(range(self._seen[s], self._seen[s] + n))
+            self._len[s] += n
+            self._seen[s] += n
+        return PagedStep(self, seqs, new, positions)
+
+    def evict(self, seqs, budget, recent):
+        """Cuts the sequences to `budget` tokens a key head in every layer (paged_evict_func); pages that become empty are free again."""
+        seqs = list(seqs)
+        self._book(seqs)
+        if self.key_weights is None:
+            raise RuntimeError("eviction goes by key_weights: make the cache with key_weights=True")
+        if budget < 1 or recent < 0:
+            raise RuntimeError("budget must be positive, recent not negative")
+        longest = max(self._len[s] for s in seqs)
+        if longest <= budget:
+            return
+        table, lens, seen = self._tables(seqs)
+        with torch.no_grad():
+            for i in range(self._k.shape[0]):
+                paged_evict_func(*self.layer(i), self.key_weights[i], self.key_positions[i], table, lens, seen, budget, recent, longest)
+        for s in seqs:
+            self._len[s] = min(self._len[s], budget)
+            keep = -(-self._len[s] // self.page_size)
+            self._free.extend(reversed(self._pages[s][keep:]))
+            del self._pages[s][keep:]
+
+    def _tables(self, seqs, *more):
+        cols = max(1, max(len(self._pages[s]) for s in seqs))
+        rows = [p for s in seqs for p in self._pages[s] + [-1] * (cols - len(self._pages[s]))]
+        table, lens, seen, *rest = self._device_ints(rows, [self._len[s] for s in seqs], [self._seen[s] for s in seqs], *more)
+        return (table.view(len(seqs), cols), lens, seen, *rest)
+
+
+class PagedStep:
+    """New tokens of some sequences of a PagedKVCache: the tensors that the functions above take.  The layers' calls are made while the step is the
+    cache's last one for its sequences."""
+
+    def __init__(self, cache, seqs, new, positions):
+        self.cache = cache
+        ends, at = [0], 0
+        for n in new:
+            at += n
+            ends.append(at)
+        self.page_table, self.seqlens_k, _, self.cu_seqlens, self.positions = cache._tables(seqs, ends, positions)
+        self.total, self.max_seqlen_q = at, max(new)
+        self.max_seqlen_k = max(cache._len[s] for s in seqs)
+        self.max_position = max(cache._seen[s] for s in seqs)
+
+    def append(self, layer, q, k, v, **norm_and_rotary):
+        """paged_append_func into the layer's pages (q_weight, k_weight, cos_half, sin_half, eps); tokens are turned by their numbers in their sequences,
+        which go on where an eviction has cut the cache."""
+        c = self.cache
+        weights = (None, None) if c.key_weights is None else (c.key_weights[layer], c.key_positions[layer])
+        if k.shape[0] != self.total:
+            raise RuntimeError("the step has %d tokens, not %d" % (self.total, k.shape[0]))
+        return paged_append_func(q, k, v, *c.layer(layer), self.page_table, self.cu_seqlens, self.seqlens_k,
+                                 positions=self.positions, key_weights=weights[0], key_positions=weights[1],
+                                 **norm_and_rotary)
+
+    def attend(self, layer, q, softmax_scale=None):
+        """flash_attn_paged_func over the layer's pages, causal; a cache with key_weights counts what its keys receive"""
+        c = self.cache
+        k, v = c.layer(layer)
+        where = (self.page_table, self.cu_seqlens, self.seqlens_k, self.max_seqlen_q, self.max_seqlen_k, softmax_scale)
+        if c.key_weights is None:
+            return flash_attn_paged_func(q, k, v, *where)
+        out, lse = flash_attn_paged_func(q, k, v, *where, return_softmax_lse=True)
+        paged_key_weights_func(q, lse, k, c.key_weights[layer], *where)
+        return out

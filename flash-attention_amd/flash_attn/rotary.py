@@ -143,6 +143,17 @@ class RotaryEmbedding(torch.nn.Module):
             self._half_of = cos
         return self._half
 
+    def tables_to(self, positions, like):
+        """(cos, sin) of shape (>= positions, headdim / 2) in `like`'s dtype on its device: tables that grow (to a power of two of rows) and are kept, for
+        positions that grow from call to call."""
+        have = getattr(self, "_grown", None)
+        if have is None or have[0].shape[0] < positions or have[0].device != like.device or have[0].dtype != like.dtype:
+            rows = max(256, 1 << (max(int(positions), 1) - 1).bit_length())
+            pos = torch.arange(rows, device=like.device, dtype=self.inv_freq.dtype)
+            angles = torch.outer(pos, self.inv_freq.to(like.device))  # fp32, as in _update_cos_sin_tables
+            self._grown = have = (torch.cos(angles).to(like.dtype), torch.sin(angles).to(like.dtype))
+        return have
+
     def rotate_qkv_(self, qkv):
         """q and k of a packed (batch, seqlen, 3, nheads, headdim) GPU tensor rotated in place (one HIP kernel); returns
         qkv.  Same tables as forward()."""
