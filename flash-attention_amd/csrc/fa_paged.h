@@ -83,8 +83,10 @@ FA_DEVICE int paged_len(const PagedCache& c, int b) {  // keys of sequence b tha
   return keys_in_reach(ld_scalar(c.seqlens, b), c.max_keys);
 }
 // The page that holds keys 16 g .. 16 g + 15 of a sequence (pages are 16 slots or a power of two times that), inside the pool whatever the table holds.
+// Groups behind the last that is looked at stand for that one, whatever the sequence's length: a tile's pages can be asked for while that is on its way.
 FA_DEVICE int page_of_group(const PagedCache& c, const int32_t* table_b, int g) {
-  return page_in_pool(ld_scalar(table_b, g >> (c.page_log2 - 4)), c.n_pages);
+  const int at = g >> (c.page_log2 - 4), last = (c.max_keys - 1) >> c.page_log2;
+  return page_in_pool(ld_scalar(table_b, at < last ? at : last), c.n_pages);
 }
 FA_DEVICE int slot_of_group(const PagedCache& c, int g) { return (g << 4) & ((1 << c.page_log2) - 1); }
 

@@ -78,50 +78,44 @@ __global__ void __launch_bounds__(64 * NW_) fa_paged_decode_kernel(const PagedFw
     const int b = __builtin_amdgcn_readfirstlane(at.b), h = __builtin_amdgcn_readfirstlane(at.h);
     const int unit0 = __builtin_amdgcn_readfirstlane(at.unit), pair_units = __builtin_amdgcn_readfirstlane(at.units);
     const int unit1 = u_end - u < pair_units - unit0 ? unit0 + (int)(u_end - u) : pair_units;
+    // a tile's two groups of 16 keys: their pages are asked for a step before they are needed, those of the first two tiles together with the lengths
+    const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
+    const int k_lo = unit0 * kDecodeUnit;
+    int page[2], page2[2];
+    auto ask = [&](int t, int (&to)[2]) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) to[j] = page_of_group(p.c, table, (k_lo >> 4) + 2 * t + j);
+    };
+    ask(wave, page);
+    ask(wave + NW, page2);
     int q_begin = 0, Lq = 0;
     if (!paged_rows(p.c, b, &q_begin, &Lq)) return;  // (on the line such a sequence has no units)
     const int Lk = paged_len(p.c, b), G = p.c.G, rows = Lq * G;
-    const int k_lo = unit0 * kDecodeUnit;
     const int k_hi = Lk < unit1 * kDecodeUnit ? Lk : unit1 * kDecodeUnit;
     const int ntiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
-    const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
     const char* const kb = p.c.k + h * p.c.k_hs;
     const char* const vb = p.c.v + h * p.c.v_hs;
     const int last_group = (Lk - 1) >> 4;
 
-    // a tile's two groups of 16 keys: their pages are asked for a step before they are needed
-    int page[2];
-    auto ask = [&](int t) {
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int g = (k_lo >> 4) + 2 * t + j;
-        page[j] = page_of_group(p.c, table, g < last_group ? g : last_group);
-      }
-    };
-    auto issue = [&](int t, int stage) {
+    auto issue = [&](int t, int stage, const int (&pages)[2]) {
       unsigned char* const dst = lds_wave + stage * 2 * C::kTile;
-      int slot[2], last[2];
+      const int g0 = (k_lo >> 4) + 2 * t;
+      const bool both = g0 < last_group;  // (else the tile's second half repeats the last key, in the first one's page)
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        const int g0 = (k_lo >> 4) + 2 * t + j, g = g0 < last_group ? g0 : last_group;
-        slot[j] = slot_of_group(p.c, g);
-        last[j] = g < last_group ? 15 : (Lk - 1) & 15;
+        const int g = both ? g0 + j : g0, pg = both ? pages[j] : pages[0];
+        ks_.issue(kb + pg * p.c.k_ps + slot_of_group(p.c, g) * p.c.k_ss, p.c.k_ss, g < last_group ? 15 : (Lk - 1) & 15, dst + j * KStager::kBytes);
       }
 #pragma unroll
-      for (int j = 0; j < 2; j++) ks_.issue(kb + page[j] * p.c.k_ps + slot[j] * p.c.k_ss, p.c.k_ss, last[j], dst + j * KStager::kBytes);
-#pragma unroll
-      for (int j = 0; j < 2; j++) vs_.issue(vb + page[j] * p.c.v_ps + slot[j] * p.c.v_ss, p.c.v_ss, last[j], dst + C::kTile + j * VStager::kBytes);
+      for (int j = 0; j < 2; j++) {
+        const int g = both ? g0 + j : g0, pg = both ? pages[j] : pages[0];
+        vs_.issue(vb + pg * p.c.v_ps + slot_of_group(p.c, g) * p.c.v_ss, p.c.v_ss, g < last_group ? 15 : (Lk - 1) & 15, dst + C::kTile + j * VStager::kBytes);
+      }
     };
 
     int t = wave, stage = 0;
-    if (t < ntiles) {
-      ask(t);
-      issue(t, 0);
-    }
-    if (t + NW < ntiles) {
-      ask(t + NW);
-      issue(t + NW, 1);
-    }
+    if (t < ntiles) issue(t, 0, page);
+    if (t + NW < ntiles) issue(t + NW, 1, page2);
     const int row = c < rows ? c : rows - 1;  // (columns past the last row repeat it and are dropped at the end)
     const int tok = row / G;
     vec8 qreg[D / 16];
@@ -148,7 +142,7 @@ __global__ void __launch_bounds__(64 * NW_) fa_paged_decode_kernel(const PagedFw
       const bool next = t + NW < ntiles;  // its 2 * NI loads were issued after this tile's
       if (next) wait_vmcnt<3 * NI>();
       else wait_vmcnt<NI>();
-      if (t + 2 * NW < ntiles) ask(t + 2 * NW);
+      if (t + 2 * NW < ntiles) ask(t + 2 * NW, page);
       const T* const Ks = reinterpret_cast<const T*>(lds_wave + stage * 2 * C::kTile);
       const T* const Vs = Ks + BN * D;
       f32x16 s;
@@ -201,7 +195,7 @@ __global__ void __launch_bounds__(64 * NW_) fa_paged_decode_kernel(const PagedFw
         }
       if (t + 2 * NW < ntiles) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage has been read before it is refilled
-        issue(t + 2 * NW, stage);
+        issue(t + 2 * NW, stage, page);
       }
       stage ^= 1;
     }

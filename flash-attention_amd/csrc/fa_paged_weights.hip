@@ -239,40 +239,36 @@ __global__ void __launch_bounds__(256) fa_paged_weights_few_kernel(const PagedFw
     const int unit0 = __builtin_amdgcn_readfirstlane(at.unit), pair_units = __builtin_amdgcn_readfirstlane(at.units);
     int unit1 = u_end - u < pair_units - unit0 ? unit0 + (int)(u_end - u) : pair_units;
     unit1 = unit1 - unit0 <= C::kKeys / kDecodeUnit ? unit1 : unit0 + C::kKeys / kDecodeUnit;
+    // a tile's two groups of 16 keys: their pages are asked for a step before they are needed, those of the first two tiles together with the lengths
+    const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
+    const int k_lo = unit0 * kDecodeUnit;
+    int page[2], page2[2];
+    auto ask = [&](int t, int (&to)[2]) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) to[j] = page_of_group(p.c, table, (k_lo >> 4) + 2 * t + j);
+    };
+    ask(wave, page);
+    ask(wave + NW, page2);
     int q_begin = 0, Lq = 0;
     if (!paged_rows(p.c, b, &q_begin, &Lq)) return;  // (never: such a sequence has no units)
     const int Lk = paged_len(p.c, b), G = p.c.G, rows = Lq * G;
-    const int k_lo = unit0 * kDecodeUnit;
     const int k_hi = Lk < unit1 * kDecodeUnit ? Lk : unit1 * kDecodeUnit;
     const int ntiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
-    const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
     const char* const kb = p.c.k + h * p.c.k_hs;
     const int last_group = (Lk - 1) >> 4;
-    int page[2];
-    auto ask = [&](int t) {
+    auto issue = [&](int t, int stage, const int (&pages)[2]) {
+      const int g0 = (k_lo >> 4) + 2 * t;
+      const bool both = g0 < last_group;  // (else the tile's second half repeats the last key, in the first one's page)
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        const int g = (k_lo >> 4) + 2 * t + j;
-        page[j] = page_of_group(p.c, table, g < last_group ? g : last_group);
-      }
-    };
-    auto issue = [&](int t, int stage) {
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int g0 = (k_lo >> 4) + 2 * t + j, g = g0 < last_group ? g0 : last_group;
-        st.issue(kb + page[j] * p.c.k_ps + slot_of_group(p.c, g) * p.c.k_ss, p.c.k_ss, g < last_group ? 15 : (Lk - 1) & 15,
+        const int g = both ? g0 + j : g0, pg = both ? pages[j] : pages[0];
+        st.issue(kb + pg * p.c.k_ps + slot_of_group(p.c, g) * p.c.k_ss, p.c.k_ss, g < last_group ? 15 : (Lk - 1) & 15,
                  lds_wave + stage * C::kTile + j * Stager::kBytes);
       }
     };
     int t = wave, stage = 0;
-    if (t < ntiles) {
-      ask(t);
-      issue(t, 0);
-    }
-    if (t + NW < ntiles) {
-      ask(t + NW);
-      issue(t + NW, 1);
-    }
+    if (t < ntiles) issue(t, 0, page);
+    if (t + NW < ntiles) issue(t + NW, 1, page2);
     // the rows: lane c holds row c's fragments; of the 16 that a lane's results belong to, lse (log2 units; +inf: no row, or one that sees nothing)
     // and limit.  Waited for here, with the first two tiles: the main loop counts this wave's outstanding loads.
     const int row = c < rows ? c : rows - 1, tok = row / G;
@@ -299,7 +295,7 @@ __global__ void __launch_bounds__(256) fa_paged_weights_few_kernel(const PagedFw
     for (; t < ntiles; t += NW) {
       if (t + NW < ntiles) wait_vmcnt<NI>();  // (its NI loads were issued after this tile's)
       else wait_vmcnt<0>();
-      if (t + 2 * NW < ntiles) ask(t + 2 * NW);
+      if (t + 2 * NW < ntiles) ask(t + 2 * NW, page);
       const T* const Ks = reinterpret_cast<const T*>(lds_wave + stage * C::kTile);
       f32x16 s;
 #pragma unroll
@@ -308,7 +304,7 @@ __global__ void __launch_bounds__(256) fa_paged_weights_few_kernel(const PagedFw
       for (int ks = 0; ks < D / 16; ks++) s = E::mfma32(qreg[ks], *reinterpret_cast<const vec8*>(Ks + koff[ks]), s);
       if (t + 2 * NW < ntiles) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage has been read before it is refilled
-        issue(t + 2 * NW, stage);
+        issue(t + 2 * NW, stage, page);
       }
       const int key = k_lo + t * BN + c;
       float sum = 0.f;
