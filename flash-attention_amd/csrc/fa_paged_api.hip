@@ -13,7 +13,7 @@ namespace {
 // How a forward is cut, from the call's integers alone (the lengths are on the device).
 struct Plan {
   bool decode;
-  int groups, least;       // decode (fa_paged_decode.hip)
+  int groups;              // decode (fa_paged_decode.hip)
   bool wide;               // ... eight (d = 128: four) waves a workgroup
   int nq_tiles, n_splits;  // chunk (fa_paged_chunk.hip)
   bool deal;
@@ -30,12 +30,18 @@ Plan plan_of(const fa_paged_cache& c) {
   const int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
   pl.decode = rows <= fa::kDecodeMaxQ;
   if (pl.decode) {
-    const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
-    pl.wide = pairs <= 256 && max_keys <= 128 * fa::kDecodeWide(c.head_dim);
-    pl.least = 2;
-    if (units <= pl.least || pl.wide) pl.least = 0;  // a workgroup a pair
-    else {
-      pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim), (pairs * units + pl.least - 1) / pl.least);
+    // Pairs that about fill the device once: a workgroup each, of as many waves as LDS allows, that nobody has to join.  us with the line of shares / so
+    // (one new token, all lengths equal; d = 128, 64, 32): 128 pairs of 2000 keys 35.4 / 29.8, 30.4 / 18.1, 23.3 / 15.2; of 8000 108 / 101, 65.9 / 57.2,
+    // 38.5 / 38.3; 256 pairs of 8000 194 / 186, 110 / 96, 65 / 52.  Lengths from a quarter of that on: 128 pairs up to 4000 46.3 / 49.3, 34.1 / 27.0,
+    // 30.8 / 22.0, up to 8000 77.6 / 90.2: the longest sequence decides.  Fewer pairs have too few readers: 8 of 2000 keys (d = 128) 15 / 25.
+    pl.wide = pairs <= 256 && max_keys <= (pairs >= 192 ? 8192 : pairs >= 128 ? 4096 : 128 * fa::kDecodeWide(c.head_dim));
+    // More pairs than that, of few keys: a workgroup each, of the usual number of waves.  us with the line / so, lengths equal and from a quarter on:
+    // d = 128, 512 pairs of 1000 55 / 52, 46 / 37; of 2000 101 / 99, 77 / 71; 320 pairs of 4000 129 / 139, 91 / 100.  d = 64, 1024 of 500 28 / 25;
+    // 320 of 2000 43 / 51, 33 / 45.  d = 32, 512 of 500 19 / 11; of 4000 61 / 52, 47 / 42; of 8000 110 / 100, 78 / 80.
+    const bool whole = pl.wide || max_keys <= 128 || (pairs > 256 && max_keys <= (c.head_dim <= 32 ? 4096 : 1024));
+    if (!whole) {
+      const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
+      pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim), pairs * units);
       pl.bytes = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
     }
     return pl;
@@ -109,7 +115,6 @@ int fa_paged_fwd(const fa_paged_fwd_args* a) {
     return fa::fail(FA_ERR_WORKSPACE, "fa_paged_fwd: needs %zu bytes of 16-byte aligned workspace", pl.bytes);
   fa::PagedFwdParams p = params(a);
   p.groups = pl.groups;
-  p.least = pl.least;
   p.wide = pl.wide;
   p.nq_tiles = pl.nq_tiles;
   p.n_splits = pl.n_splits;

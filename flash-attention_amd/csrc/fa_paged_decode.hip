@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(64 * NW_) fa_paged_decode_kernel(const PagedFw
   // ---- this workgroup's share of the line: [u, u_end), from `at` on
   int64_t u, u_end;
   Spot at;
-  if (p.least > 0) {
+  if (p.groups > 0) {
     const int sums0 = unit_sums(p.c, 0);
     const int64_t units = all_units(p.c, sums0);
     const int n = sharers(p, units);
@@ -265,71 +265,72 @@ __global__ void __launch_bounds__(64 * NW_) fa_paged_decode_kernel(const PagedFw
 
 namespace {
 
-// The pairs that several workgroups' shares have cut: a workgroup joins one row of one, D / 4 threads over its elements times 1024 / D over the parts.
+// The pairs that the ends of the workgroups' shares have cut, each joined by the workgroup whose number is that of the first share that begins inside it: D / 4
+// threads over a row's elements times 1024 / D over the parts, the rows one after the other (blockIdx.y, blockIdx.y + gridDim.y, ...).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_decode_join_kernel(const PagedFwdParams p) {
   constexpr int kCols = D / 4, kLanes = 256 / kCols;
   __shared__ f32x4 os[256];
   __shared__ PartRow ms[256];
-  const int pair = blockIdx.x, r = blockIdx.y;
-  const int b = pair / p.c.HK, h = pair - b * p.c.HK;
-  const int own = units_of(p.c, b);
-  if (own == 0) return;
-  int64_t units = 0, begin = 0;  // of the line; of this pair
-  for (int first = 0; first < p.c.B; first += 64) {
-    const int sums = unit_sums(p.c, first);
-    if (b >= first && b < first + 64) {
-      const int upto = __builtin_amdgcn_readlane(sums, b - first) - own;
-      begin = (units + upto) * p.c.HK + (int64_t)h * own;
-    }
-    units += __builtin_amdgcn_readlane(sums, 63);
-  }
-  units *= p.c.HK;
-  const int n = sharers(p, units);
-  const int w0 = share_of(units, begin, n), w1 = share_of(units, begin + own - 1, n);
+  const int sums0 = unit_sums(p.c, 0);
+  const int64_t units = all_units(p.c, sums0);
+  const int n = sharers(p, units), w = (int)blockIdx.x + 1;
+  if (w >= n || units == 0) return;
+  const Spot at = spot_of(p.c, share_begin(units, w, n), sums0);
+  const int64_t begin = share_begin(units, w, n) - at.unit;  // of the pair
+  if (at.unit == 0 || share_begin(units, w - 1, n) > begin) return;
+  const int b = __builtin_amdgcn_readfirstlane(at.b), h = __builtin_amdgcn_readfirstlane(at.h);
+  const int w0 = w - 1;
+  int w1 = w;
+  while (w1 + 1 < n && share_begin(units, w1 + 1, n) < begin + at.units) w1++;
   int q_begin = 0, Lq = 0;
-  if (w0 == w1 || !paged_rows(p.c, b, &q_begin, &Lq) || r >= Lq * p.c.G) return;
+  if (!paged_rows(p.c, b, &q_begin, &Lq)) return;
   const float cs = p.scale_log2;
   constexpr int kEach = kPartRows * (D + 3);
-  // the pair is the last of workgroup w0's share, and its first, too, if the share begins with it; it is the first of the others'
+  // the pair is the last of share w0, and its first, too, if the share begins with it; it is the first of the others'
   const int first_slot = share_begin(units, w0, n) == begin ? 0 : 1;
   const int col = threadIdx.x % kCols, lane = threadIdx.x / kCols;
-  PartRow a{-INFINITY, 0.f, 0.f};
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int w = w0 + lane; w <= w1; w += kLanes) {
-    const float* const s = p.part + ((int64_t)w * 2 + (w == w0 ? first_slot : 0)) * kEach;
-    const float* const ml = s + kPartRows * D + r;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(s + r * D + col * 4);
-    const float m = ml[0], l = ml[kPartRows], u = ml[2 * kPartRows];
-    const float top = fmaxf(a.m, m), ref = top == -INFINITY ? 0.f : top;
-    const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((m - ref) * cs);
-    a = PartRow{top, a.l * fa + l * fb, a.u * fa + u * fb};
-    o = o * fa + x * fb;
+  for (int r = blockIdx.y; r < Lq * p.c.G; r += gridDim.y) {
+    PartRow a{-INFINITY, 0.f, 0.f};
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    auto join = [&](float m, float l, float u, f32x4 x) {
+      const float top = fmaxf(a.m, m), ref = top == -INFINITY ? 0.f : top;
+      const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((m - ref) * cs);
+      a = PartRow{top, a.l * fa + l * fb, a.u * fa + u * fb};
+      o = o * fa + x * fb;
+    };
+    for (int i = w0 + lane; i <= w1; i += kLanes) {
+      const float* const s = p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
+      const float* const ml = s + kPartRows * D + r;
+      join(ml[0], ml[kPartRows], ml[2 * kPartRows], *reinterpret_cast<const f32x4*>(s + r * D + col * 4));
+    }
+    os[threadIdx.x] = o;
+    ms[threadIdx.x] = a;
+    __syncthreads();
+    if (lane == 0) {
+      for (int i = 1; i < kLanes && i <= w1 - w0; i++) {
+        const PartRow x = ms[i * kCols + col];
+        join(x.m, x.l, x.u, os[i * kCols + col]);
+      }
+      store_row_piece<T>(p, q_begin, h, r, col * 4, o * (a.l > 0.f ? fast_rcp(a.l) : 1.f));
+      if (col == 0) store_lse(p, b, h, r, lse_of(a.m, a.u, cs));
+    }
+    __syncthreads();
   }
-  os[threadIdx.x] = o;
-  ms[threadIdx.x] = a;
-  __syncthreads();
-  if (lane > 0) return;
-  for (int i = 1; i < kLanes && i <= w1 - w0; i++) {
-    const PartRow x = ms[i * kCols + col];
-    const float top = fmaxf(a.m, x.m), ref = top == -INFINITY ? 0.f : top;
-    const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((x.m - ref) * cs);
-    a = PartRow{top, a.l * fa + x.l * fb, a.u * fa + x.u * fb};
-    o = o * fa + os[i * kCols + col] * fb;
-  }
-  store_row_piece<T>(p, q_begin, h, r, col * 4, o * (a.l > 0.f ? fast_rcp(a.l) : 1.f));
-  if (col == 0) store_lse(p, b, h, r, lse_of(a.m, a.u, cs));
 }
 
 template <typename T, int D>
 hipError_t launch_d(const PagedFwdParams& p, hipStream_t stream) {
   const unsigned pairs = (unsigned)(p.c.B * p.c.HK);
-  const dim3 grid(p.least > 0 ? (unsigned)p.groups : pairs);
+  const dim3 grid(p.groups > 0 ? (unsigned)p.groups : pairs);
   if (p.wide) hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWide(D)>), grid, dim3(64 * kDecodeWide(D)), 0, stream, p);
   else hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWaves(D)>), grid, dim3(64 * kDecodeWaves(D)), 0, stream, p);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.least == 0) return e;
-  hipLaunchKernelGGL((paged_decode_join_kernel<T, D>), dim3(pairs, (unsigned)(p.c.max_sq * p.c.G)), dim3(256), 0, stream, p);
+  if (e != hipSuccess || p.groups == 0) return e;
+  // (few pairs have many parts: their rows side by side)
+  const int rows = p.c.max_sq * p.c.G;
+  const unsigned gy = pairs >= 64 ? 1u : (unsigned)rows;
+  if (p.groups > 1) hipLaunchKernelGGL((paged_decode_join_kernel<T, D>), dim3((unsigned)p.groups - 1, gy), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 template <typename T>

@@ -19,8 +19,8 @@ struct PagedFwdParams {
   int sq_r;
   int causal;
   float scale_log2;
-  // decode: workgroups, and the fewest units of keys one of them takes (0: a workgroup a pair).  chunk: query tiles and key splits
-  int groups, least, wide;
+  // decode: the workgroups that share the line of units (0: a workgroup a pair), and whether they are wide.  chunk: query tiles and key splits
+  int groups, wide;
   int nq_tiles, n_splits, deal;
   float* part;  // partial results
 };
@@ -56,7 +56,7 @@ FA_DEVICE float lse_of(float m, float u, float cs) { return u > 0.f ? (m * cs + 
 // ---- decode: keys are dealt out in units of kUnit; a pair (sequence, key head) has ceil(keys / kUnit), one at least, so that its rows are written
 constexpr int kDecodeUnit = 128;
 constexpr int kPartRows = 32;
-// Waves of a workgroup that has a pair to itself where pairs are few and short: as many as their tiles' LDS allows.
+// Waves of a workgroup that has a pair to itself where pairs about fill the device: as many as their tiles' LDS allows.
 constexpr int kDecodeWide(int head_dim) { return head_dim == 128 ? 4 : 8; }
 
 // floats of a workgroup's two partial results: [2][32][D] outputs, [2][3][32] m, l, u

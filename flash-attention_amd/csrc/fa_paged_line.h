@@ -53,16 +53,9 @@ FA_DEVICE Spot spot_of(const PagedCache& c, int64_t u, int sums0) {
 }
 // Workgroups that share the line, and the first unit of workgroup w
 FA_DEVICE int sharers(const PagedFwdParams& p, int64_t units) {
-  const int64_t most = (units + p.least - 1) / p.least;
-  return (int)(most < p.groups ? (most > 0 ? most : 1) : p.groups);
+  return units >= p.groups ? p.groups : units > 0 ? (int)units : 1;
 }
 FA_DEVICE int64_t share_begin(int64_t units, int w, int sharers) { return units * w / sharers; }
-FA_DEVICE int share_of(int64_t units, int64_t u, int sharers) {  // the workgroup whose share holds unit u
-  int w = (int)((u * sharers) / units);
-  while (w + 1 < sharers && share_begin(units, w + 1, sharers) <= u) w++;
-  while (w > 0 && share_begin(units, w, sharers) > u) w--;
-  return w;
-}
 // The first unit of the pair after (b, h): false if there is none
 FA_DEVICE bool next_pair(const PagedCache& c, Spot* at) {
   at->unit = 0;

@@ -345,7 +345,6 @@ hipError_t launch_d(const WeightsParams& p, hipStream_t stream) {
   if (blocks >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
   if (p.f.c.max_sq * p.f.c.G <= kDecodeMaxQ) {
     PagedFwdParams f = p.f;
-    f.least = 1;
     f.groups = (int)(blocks < few_resident(D) ? blocks : few_resident(D));  // (a block of 128 keys is a unit)
     hipLaunchKernelGGL((fa_paged_weights_few_kernel<T, D>), dim3((unsigned)f.groups), dim3(256), 0, stream, f);
   } else {
