@@ -42,6 +42,7 @@ struct NormParams {
   const void* cos;
   const void* sin;
   const int32_t* positions;
+  const int32_t* rows_end;  // null, or where the rows that count end
   int n_rows, seqlen, table_rows;
   float eps;
   int w_fp32;
@@ -82,6 +83,7 @@ struct Place {  // of a thread in its part
   int row0, step, head, ch;
   bool on;
 };
+FA_DEVICE int rows_of(const NormParams& p) { return p.rows_end ? keys_in_reach(*p.rows_end, p.n_rows) : p.n_rows; }
 template <int CH>
 FA_DEVICE Place place_of(const NormPart& q, int block) {
   const int tid = threadIdx.x;
@@ -104,17 +106,18 @@ __global__ void __launch_bounds__(512) qk_norm_rotary_kernel(const NormParams p)
   const NormPart& q = p.part[second];
   const Place pl = place_of<CH>(q, (int)blockIdx.x - q.first_block);
   if (!pl.on) return;
+  const int n_rows = rows_of(p);
   float w[8];
   load_weights<T>(q.w, p.w_fp32 != 0, pl.ch, w);
   const T* const src = reinterpret_cast<const T*>(q.x) + (int64_t)pl.head * q.x_hs + pl.ch * 8;
   T* const dst = reinterpret_cast<T*>(q.out) + (int64_t)pl.head * q.out_hs + pl.ch * 8;
-  for (int64_t row0 = pl.row0; row0 < p.n_rows; row0 += (int64_t)kRows * pl.step) {
+  for (int64_t row0 = pl.row0; row0 < n_rows; row0 += (int64_t)kRows * pl.step) {
     typename Elem<T>::vec8 v[kRows];
     Turned<T> t[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
       const int64_t row = row0 + (int64_t)i * pl.step;
-      if (row < p.n_rows) {
+      if (row < n_rows) {
         v[i] = bitcast<typename Elem<T>::vec8>(ld_global16(src + row * q.x_rs));
         if (kTurn) t[i].load(p, (int)row, pl.ch, D / 2);
       }
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(512) qk_norm_rotary_kernel(const NormParams p)
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
       const int64_t row = row0 + (int64_t)i * pl.step;
-      if (row < p.n_rows) {
+      if (row < n_rows) {
         float x[8];
         to_float(v[i], x);
         const float r = inverse_rms<CH>(x, p.eps);
@@ -147,18 +150,19 @@ __global__ void __launch_bounds__(512) qk_norm_rotary_bwd_kernel(const NormParam
   const Place pl = place_of<CH>(q, (int)blockIdx.x - q.first_block);
   float dw[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (pl.on) {
+    const int n_rows = rows_of(p);
     float w[8];
     load_weights<T>(q.w, p.w_fp32 != 0, pl.ch, w);
     const T* const xs = reinterpret_cast<const T*>(q.x) + (int64_t)pl.head * q.x_hs + pl.ch * 8;
     const T* const gs = reinterpret_cast<const T*>(q.dy) + (int64_t)pl.head * q.dy_hs + pl.ch * 8;
     T* const dst = reinterpret_cast<T*>(q.out) + (int64_t)pl.head * q.out_hs + pl.ch * 8;
-    for (int64_t row0 = pl.row0; row0 < p.n_rows; row0 += (int64_t)kNormBwdRows * pl.step) {
+    for (int64_t row0 = pl.row0; row0 < n_rows; row0 += (int64_t)kNormBwdRows * pl.step) {
       typename Elem<T>::vec8 vx[kNormBwdRows], vg[kNormBwdRows];
       Turned<T> t[kNormBwdRows];
 #pragma unroll
       for (int i = 0; i < kNormBwdRows; i++) {
         const int64_t row = row0 + (int64_t)i * pl.step;
-        if (row < p.n_rows) {
+        if (row < n_rows) {
           vx[i] = bitcast<typename Elem<T>::vec8>(ld_global16(xs + row * q.x_rs));
           vg[i] = bitcast<typename Elem<T>::vec8>(ld_global16(gs + row * q.dy_rs));
           if (kTurn) t[i].load(p, (int)row, pl.ch, D / 2);
@@ -167,7 +171,7 @@ __global__ void __launch_bounds__(512) qk_norm_rotary_bwd_kernel(const NormParam
 #pragma unroll
       for (int i = 0; i < kNormBwdRows; i++) {
         const int64_t row = row0 + (int64_t)i * pl.step;
-        if (row < p.n_rows) {
+        if (row < n_rows) {
           float x[8], g[8];
           to_float(vx[i], x);
           to_float(vg[i], g);
@@ -282,6 +286,7 @@ int check(const fa_qk_norm_args* a, bool bwd, const char* name) {
   const int rc = check_sizes(a, name);
   if (rc) return rc;
   FA_REQUIRE(a->eps >= 0.f, "%s: eps must not be negative", name);
+  FA_REQUIRE(((reinterpret_cast<uintptr_t>(a->rows_end) | reinterpret_cast<uintptr_t>(a->positions)) & 3) == 0, "%s: integers must be 4-byte aligned", name);
   if (a->n_rows == 0) return FA_OK;
   FA_REQUIRE((a->cos_table == nullptr) == (a->sin_table == nullptr), "%s: cos_table and sin_table come together", name);
   if (a->cos_table) {
@@ -328,6 +333,7 @@ NormParams params(const fa_qk_norm_args* a, bool bwd) {
   p.cos = a->cos_table;
   p.sin = a->sin_table;
   p.positions = a->positions;
+  p.rows_end = a->rows_end;
   p.n_rows = (int)a->n_rows;
   p.seqlen = a->seqlen > 0 ? a->seqlen : 1;
   p.table_rows = a->table_rows;

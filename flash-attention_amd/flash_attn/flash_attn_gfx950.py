@@ -123,7 +123,7 @@ class QkNormArgs(ctypes.Structure):
     """struct fa_qk_norm_args, field for field."""
     _fields_ = (
         [("struct_bytes", ctypes.c_uint32), ("dtype", ctypes.c_int32)] +
-        [(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "cos_table", "sin_table", "positions", "dq_out", "dk_out",
+        [(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "cos_table", "sin_table", "positions", "rows_end", "dq_out", "dk_out",
                                         "dq", "dk", "dq_weight", "dk_weight")] +
         [(n + s, ctypes.c_int64) for n in ("q", "k", "q_out", "k_out", "dq_out", "dk_out", "dq", "dk") for s in ("_row_stride", "_head_stride")] +
         [("n_rows", ctypes.c_int64), ("nheads_q", ctypes.c_int32), ("nheads_k", ctypes.c_int32), ("head_dim", ctypes.c_int32),
@@ -1072,7 +1072,7 @@ def _check_positions(positions, like, rows):
                "positions must be a contiguous int32 tensor with one entry per row")
 
 
-def _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps):
+def _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps, cu_seqlens):
     _check(q.is_cuda and q.dim() == 3, "q must be a (rows, heads, head_dim) GPU tensor")
     rows, _, D = q.shape
     a = QkNormArgs()
@@ -1090,17 +1090,21 @@ def _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps):
     if cos is not None:
         a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
     a.positions = positions.data_ptr() if positions is not None else None
+    if cu_seqlens is not None:
+        _check(cu_seqlens.numel() > 1 and cu_seqlens.device == q.device, "cu_seqlens must be on the tensors' device, for one sequence at least")
+        _check_cu("cu_seqlens", cu_seqlens, cu_seqlens.numel() - 1)
+        a.rows_end = cu_seqlens.data_ptr() + 4 * (cu_seqlens.numel() - 1)
     a.n_rows, a.nheads_q, a.nheads_k, a.head_dim = rows, q.shape[1], k.shape[1], D
     a.seqlen, a.eps = seqlen, eps
     a.stream = _stream_handle(q.device)
     return a
 
 
-def qk_norm_rotary(q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions=None, seqlen=0, eps=1e-6):
+def qk_norm_rotary(q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions=None, seqlen=0, eps=1e-6, cu_seqlens=None):
     """Every head's vector of q and k (rows, heads, head_dim) normalised by its root mean square, times q_weight / k_weight, turned by its position (cos and
     sin None: not turned), into q_out and k_out (which may be q and k) in one pass of fa_qk_norm_rotary.  positions: int32 table rows, or None: row %
-    seqlen."""
-    a = _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps)
+    seqlen.  cu_seqlens: of a packed batch; rows behind its last sequence are left out."""
+    a = _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps, cu_seqlens)
     for name, t, like in (("q_out", q_out, q), ("k_out", k_out, k)):
         _check_heads(name, t, q, q.shape[0], q.shape[2])
         _check(t.shape == like.shape, "%s must have the shape of what it is made of" % name)
@@ -1114,10 +1118,10 @@ def qk_norm_rotary(q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions=N
     return q_out, k_out
 
 
-def qk_norm_rotary_bwd(dq_out, dk_out, q, k, dq, dk, q_weight, k_weight, cos, sin, positions=None, seqlen=0, eps=1e-6):
+def qk_norm_rotary_bwd(dq_out, dk_out, q, k, dq, dk, q_weight, k_weight, cos, sin, positions=None, seqlen=0, eps=1e-6, cu_seqlens=None):
     """Gradients through qk_norm_rotary(): q and k as it read them, dq_out and dk_out those of its results; fills dq and dk (which may be dq_out and
     dk_out) and returns (dq_weight, dk_weight)."""
-    a = _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps)
+    a = _qk_norm_args(q, k, q_weight, k_weight, cos, sin, positions, seqlen, eps, cu_seqlens)
     for name, t, like in (("dq_out", dq_out, q), ("dk_out", dk_out, k), ("dq", dq, q), ("dk", dk, k)):
         _check_heads(name, t, q, q.shape[0], q.shape[2])
         _check(t.shape == like.shape, "%s must have the shape of the tensor it belongs to" % name)
@@ -1144,10 +1148,18 @@ def _check_seqlens(name, t, batch, device):
            "%s must be a contiguous int32 tensor with one entry per sequence on the cache's device" % name)
 
 
+def _int32(name, v):
+    """An int for a 32-bit field"""
+    v = int(v)
+    _check(-2 ** 31 <= v < 2 ** 31, "%s is %d, which 32 bits do not hold" % (name, v))
+    return v
+
+
 def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_weights=None, key_positions=None):
     """Fills a PagedCacheArgs from a cache's tensors; v_cache may be None where it is not read."""
     _check(k_cache.is_cuda and k_cache.dim() == 4, "k_cache must be a (pages, page size, heads, head_dim) GPU tensor")
     n_pages, page_size, heads, D = k_cache.shape
+    _check(min(k_cache.shape) > 0 and n_pages < 2 ** 31, "k_cache must have pages, slots and heads, less than 2^31 pages")
     _dtype_code(k_cache)
     for name, t in (("k", k_cache), ("v", v_cache)):
         if t is None:
@@ -1161,11 +1173,11 @@ def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_w
     _check(page_table.device == k_cache.device and page_table.dtype == torch.int32 and page_table.dim() == 2 and
            (page_table.stride(1) == 1 or page_table.shape[1] == 1), "page_table must be a (batch, pages) int32 tensor with contiguous rows on the cache's device")
     batch, cols = page_table.shape
-    _check(batch > 0 and cols > 0, "page_table must have a row for each sequence and a page in each")
+    _check(0 < batch < 2 ** 31 and 0 < cols < 2 ** 31, "page_table must have a row for each sequence and a page in each")
     _check_seqlens("seqlens_k", seqlens_k, batch, k_cache.device)
     a.page_table, a.table_row_stride, a.table_cols = page_table.data_ptr(), (page_table.stride(0) if batch > 1 else cols), cols
     a.seqlens_k = seqlens_k.data_ptr()
-    a.n_pages, a.page_size, a.batch, a.nheads_k, a.head_dim, a.max_seqlen_k = n_pages, page_size, batch, heads, D, int(max_seqlen_k)
+    a.n_pages, a.page_size, a.batch, a.nheads_k, a.head_dim, a.max_seqlen_k = n_pages, page_size, batch, heads, D, _int32("max_seqlen_k", max_seqlen_k)
     for name, t, dtype in (("key_weights", key_weights, torch.float32), ("key_positions", key_positions, torch.int32)):
         if t is not None:
             _check(t.device == k_cache.device and t.dtype == dtype and tuple(t.shape) == (n_pages, heads, page_size) and t.is_contiguous(),
@@ -1179,7 +1191,8 @@ def _paged_queries(a, q, k_cache, cu_seqlens_q, max_seqlen_q):
     _check(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "the query heads must be a multiple of the key heads")
     _check_cu("cu_seqlens_q", cu_seqlens_q, a.batch)
     _check(cu_seqlens_q.device == k_cache.device, "cu_seqlens_q must be on the cache's device")
-    a.cu_seqlens_q, a.nheads_q, a.total_q, a.max_seqlen_q = cu_seqlens_q.data_ptr(), q.shape[1], q.shape[0], int(max_seqlen_q)
+    a.cu_seqlens_q, a.nheads_q, a.total_q = cu_seqlens_q.data_ptr(), _int32("the number of heads", q.shape[1]), _int32("the number of new tokens", q.shape[0])
+    a.max_seqlen_q = _int32("max_seqlen_q", max_seqlen_q)
 
 
 def paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, q_out=None, q_weight=None, k_weight=None, cos=None, sin=None,
@@ -1191,7 +1204,8 @@ def paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k,
     c = a.cache
     _check(k_cache.dim() == 4, "k_cache must be a (pages, page size, heads, head_dim) GPU tensor")
     total, D = k.shape[0], k_cache.shape[3]
-    _paged_cache(c, k_cache, v_cache, page_table, seqlens_k, page_table.shape[-1] * k_cache.shape[1], key_weights, key_positions)
+    _paged_cache(c, k_cache, v_cache, page_table, seqlens_k, min(page_table.shape[-1] * k_cache.shape[1], 2 ** 31 - 1), key_weights, key_positions)
+    _int32("the number of new tokens", total)
     a.dtype = _dtype_code(k_cache)
     for name, t in (("k", k), ("v", v)):
         _check_heads(name, t, k_cache, total, D)
@@ -1292,7 +1306,7 @@ def paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlen
     _check(k_cache.dim() == 4 and v_cache is not None, "k_cache and v_cache must be (pages, page size, heads, head_dim) GPU tensors")
     _paged_cache(a.cache, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_weights, key_positions)
     _check_seqlens("next_positions", next_positions, a.cache.batch, k_cache.device)
-    a.budget, a.recent = int(budget), int(recent)
+    a.budget, a.recent = _int32("budget", budget), _int32("recent", recent)
     dev = k_cache.device
     with _OnDevice(dev):
         new_seqlens = torch.empty_like(seqlens_k)

@@ -200,12 +200,10 @@ class FlashAttnNormRotaryQKVPackedFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale, causal, eps):
         _backend._check(qkv.is_cuda and qkv.dim() == 4 and qkv.shape[1] == 3, "qkv must be a (total, 3, nheads, headdim) GPU tensor")
-        total, batch = qkv.shape[0], cu_seqlens.numel() - 1
-        positions = None
-        if cos_half is not None and total != batch * int(max_seqlen):
-            positions = _backend.token_positions(cu_seqlens, total)
+        total = qkv.shape[0]
+        positions = None if cos_half is None else _backend.token_positions(cu_seqlens, total)
         qk = torch.empty((total, 2) + tuple(qkv.shape[2:]), dtype=qkv.dtype, device=qkv.device)
-        ctx.norm_args = (int(max_seqlen), eps)
+        ctx.norm_args = (int(max_seqlen), eps, cu_seqlens)
         _backend.qk_norm_rotary(qkv[:, 0], qkv[:, 1], qk[:, 0], qk[:, 1], q_weight, k_weight, cos_half, sin_half, positions, *ctx.norm_args)
         return _forward(ctx, "qkv", (qkv,), cu_seqlens, cu_seqlens, max_seqlen, max_seqlen, dropout_p, softmax_scale, causal, False, qk=qk,
                         more=(q_weight, k_weight, cos_half, sin_half, positions))
@@ -303,7 +301,8 @@ def flash_attn_unpadded_qkvpacked_norm_rotary_func(qkv, q_weight, k_weight, cos_
     """flash_attn_unpadded_qkvpacked_func on a qkv whose q and k are first normalised and turned as by apply_qk_norm_rotary (rotary.py): every head's
     vector divided by its root mean square, times q_weight / k_weight ((headdim,), qkv's dtype or fp32), then turned by its position in its sequence
     (cos_half, sin_half: (>= max_seqlen, headdim / 2) tables in qkv's dtype; None: not turned).  One pass in front of the attention and one behind its
-    backward, in place.  qkv itself is left as it is.  Differentiable with respect to qkv and the weights."""
+    backward, in place.  qkv itself is left as it is.  Differentiable with respect to qkv and the weights; rows behind the last sequence have no part in
+    it, and their gradients hold nothing."""
     return FlashAttnNormRotaryQKVPackedFunc.apply(qkv, q_weight, k_weight, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale, causal,
                                                   eps)
 

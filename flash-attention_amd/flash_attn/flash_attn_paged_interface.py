@@ -13,8 +13,10 @@ find new lengths, tables and tokens in the same tensors.  max_seqlen_k then has 
 that is cut, not the memory that is read.
 
 What lies in page_table and seqlens_k is never trusted with an address: entries outside the pool are read as its first or last page and never written to,
-lengths count as far as the table goes.  Pages that several sequences list (a common prompt) may be read by all of them and must not be appended to,
-weighted or evicted from."""
+lengths count as far as the table goes.  Pages that several sequences list (a common prompt), or one lists twice, may be read by all of them and must not be
+appended to, weighted or evicted from: the order in which several workgroups write one slot is not defined.  Keys and values behind a sequence's length are not
+read.  A value that is inf or NaN reaches every new token of its sequence that is handled together with one that sees it, as in the package's other
+attention functions: a weight of 0 does not cancel it."""
 import torch
 
 from . import flash_attn_gfx950 as _backend

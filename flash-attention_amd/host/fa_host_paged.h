@@ -198,7 +198,7 @@ bool fill_cache(fa_paged_cache* c, const at::Tensor* k, const at::Tensor* v, boo
   if (!table || table->device() != k->device() || table->scalar_type() != at::kInt || table->dim() != 2 || (table->stride(1) != 1 && table->size(1) != 1)) return false;
   const int64_t batch = table->size(0), cols = table->size(1);
   if (batch <= 0 || cols <= 0 || !small(batch) || !small(cols) || !lens || lens->device() != k->device() || lens->scalar_type() != at::kInt || lens->dim() != 1 ||
-      lens->size(0) != batch || !lens->is_contiguous() || !small(k->size(0)) || !small(k->size(1)) || !small(k->size(2)) || max_k <= 0)
+      lens->size(0) != batch || !lens->is_contiguous() || !small(k->size(0)) || !small(k->size(1)) || !small(k->size(2)) || k->numel() == 0 || max_k <= 0)
     return false;
   auto beside = [&](const at::Tensor* t, at::ScalarType type) {
     return !t || (t->device() == k->device() && t->scalar_type() == type && t->dim() == 3 && t->size(0) == k->size(0) && t->size(1) == k->size(2) &&

@@ -327,7 +327,8 @@ int fa_token_positions(const int32_t* cu_seqlens, int32_t batch, int32_t total, 
  * by the heads) and R_t the rotation of fa_rotary by table row t.  fp32 between one read and one rounding.  q, k, q_out, k_out: [n_rows,
  * nheads_q or nheads_k, head_dim], strides in elements, innermost 1, multiples of 8; 16-byte aligned; q_out / k_out may be q / k with the same
  * strides.  weight_dtype: enum fa_dtype, or FA_FP32.  Tables as in fa_rotary, or both NULL (no rotation); t = positions[row], clamped to
- * the table, or row % seqlen.  The backward takes q, k (as the forward read them) and dq_out, dk_out, and writes dq, dk (which may be dq_out,
+ * the table, or row % seqlen.  rows_end: NULL, or an int32 in device memory (the last entry of a packed batch's cu_seqlens): rows from it on are
+ * neither read nor written.  The backward takes q, k (as the forward read them) and dq_out, dk_out, and writes dq, dk (which may be dq_out,
  * dk_out with the same strides) and dq_weight, dk_weight ([head_dim], weight_dtype; summed in fp32 in a fixed order).  workspace: of
  * fa_qk_norm_rotary_bwd_workspace_bytes() bytes, 16-byte aligned; the forward needs none. */
 #define FA_FP32 2 /* weights only */
@@ -339,6 +340,7 @@ typedef struct fa_qk_norm_args {
   const void *q_weight, *k_weight;
   const void *cos_table, *sin_table;
   const int32_t* positions;
+  const int32_t* rows_end;
   const void *dq_out, *dk_out;
   void *dq, *dk;
   void *dq_weight, *dk_weight;

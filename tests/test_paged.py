@@ -495,6 +495,28 @@ def test_attention_and_weights(dtype, causal, lens, new, H, HK, D, PS, head_majo
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mk", [640, 1300, 5000, 9000])  # the bound chooses the launch: a workgroup a pair, or shares of the line of all keys
+@pytest.mark.parametrize("lens, HK, D", [
+    ([1, 200, 127, 0, 640] * 7, 4, 64), ([600, 3] * 33, 4, 32), ([129, 128, 300, 5, 640, 1, 1] * 10, 5, 16), ([513, 70] * 33, 5, 128)])
+def test_few_rows_however_the_pairs_are_dealt_out(lens, HK, D, mk):
+    from flash_attn.flash_attn_paged_interface import flash_attn_paged_func
+    c = Cache(lens, HK, D, 16, torch.float16, 21, cols=600).gpu()
+    new = [0 if i % 9 == 8 else 1 + (i % 4 == 1) for i in range(len(lens))]
+    q = torch.randn(sum(new), 2 * HK, D, generator=torch.Generator().manual_seed(22)).half()
+    want, lse64, _, tol, ds = ref_attention(q, c, new, True, D ** -0.5)
+    call = lambda: flash_attn_paged_func(q.cuda(), c.dk, c.dv, c.dtable, cumulative(new).cuda(), c.dlens, 2, mk, return_softmax_lse=True)  # noqa: E731
+    out, lse = call()
+    assert ((out.cpu().double() - want).abs() <= tol + 1e-7).all()
+    for (b, h), x in lse64.items():
+        have = lse[b, h, :new[b]].cpu().double()
+        dead = x == -math.inf
+        assert torch.equal(have == -math.inf, dead)
+        assert ((have - x)[~dead].abs() <= ds + (lens[b] + 16) * E32 + 8 * E32 * (x[~dead].abs() + 8)).all()
+    for _ in range(3):
+        assert torch.equal(call()[0], out)  # the same bits each time
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new, mk", [([1, 1], 5000), ([40, 70], 400)])
 def test_attention_ignores_what_lies_behind(new, mk):
     """strided queries and outputs, rows behind the last sequence, a longer table and bound than needed: the same bits, nothing else written"""

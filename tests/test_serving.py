@@ -265,6 +265,46 @@ def test_attention_with_norm_and_rotation(dtype, lens, H, D, causal, p, turn, fp
 
 
 @pytest.mark.gpu
+def test_rows_behind_the_last_sequence_have_no_part_in_attention_with_norm():
+    """as many rows as sequences of the longest length would have, and only some of them in sequences"""
+    from flash_attn.flash_attn_interface import flash_attn_unpadded_qkvpacked_norm_rotary_func
+    cu, w = cumulative([5, 10]).cuda(), torch.ones(64, dtype=torch.float16, device="cuda").requires_grad_()
+    cos, sin = (t.cuda() for t in tables(10, 64, torch.float16))
+    full = randn(20, 3, 2, 64, seed=1).cuda()
+    full[15:] = math.nan
+    dout = randn(20, 2, 64, seed=2).cuda()
+    got = []
+    for rows in (15, 20):
+        torch.empty(4096, dtype=torch.float16, device="cuda").fill_(math.nan)  # (what fresh tensors may hold)
+        qkv = full[:rows].clone().requires_grad_()
+        out = flash_attn_unpadded_qkvpacked_norm_rotary_func(qkv, w, w, cos, sin, cu, 10, 0.0, causal=True)
+        dqkv, dw = torch.autograd.grad(out, (qkv, w), dout[:rows])
+        got.append((out[:15], dqkv[:15], dw))
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][2].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_sizes_that_no_field_holds_are_refused():
+    """no head, no slot, and numbers beyond 32 bits: errors, not other numbers"""
+    from flash_attn import flash_attn_paged_interface as p
+    c = Cache([20, 9], 2, 64, 16, torch.float16, 1).gpu()
+    q, cu = randn(3, 4, 64, seed=0).cuda(), cumulative([2, 1]).cuda()
+    where = (c.dtable, cu, c.dlens)
+    evict = lambda k, v, *n: p.paged_evict_func(k, v, c.dweights, c.dpositions, c.dtable, c.dlens, c.dlens, *n)  # noqa: E731
+    none, empty = c.dk[:, :, :0], q[:, :0]
+    calls = (lambda: p.flash_attn_paged_func(q, none, none, *where, 2, 20), lambda: p.paged_append_func(q, empty, empty, none, none, *where),
+             lambda: p.paged_append_func(None, empty, empty, none, none, *where), lambda: p.flash_attn_paged_func(q, c.dk[:0], c.dv[:0], *where, 2, 20),
+             lambda: p.paged_key_weights_func(q, torch.zeros(2, 4, 16, device="cuda"), none, c.dweights[:, :0].contiguous(), *where, 2, 20),
+             lambda: p.flash_attn_paged_func(q, c.dk, c.dv, *where, 2 ** 32 + 2, 20), lambda: p.flash_attn_paged_func(q, c.dk, c.dv, *where, 2, 2 ** 32 + 20),
+             lambda: evict(c.dk, c.dv, 2 ** 32 + 5, 2, 20), lambda: evict(c.dk, c.dv, 5, 2 ** 32, 20), lambda: evict(c.dk, c.dv, 5, 2, 2 ** 32 + 20),
+             lambda: evict(none, none, 5, 2, 20))
+    for i, call in enumerate(calls):
+        print(i, flush=True)  # (shown with a failure)
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rotary", [None, "1d", "2d"])
 @pytest.mark.parametrize("padded", [False, True])
 def test_mha_with_norm(rotary, padded):
