@@ -109,7 +109,7 @@ class PagedKVCache:
         self.page_size = page_size
         shape = (layers, pages, nheads_k, page_size, headdim)
         device = torch.device("cuda" if device is None else device)
-        # zeros: what lies behind a sequence's last key is read with its page's, and only then left out
+        # (zeros: entries of a page table that are no pages are read as the first or last one)
         self._k, self._v = (torch.zeros(shape, dtype=dtype, device=device).transpose(2, 3) for _ in range(2))
         self.key_weights = torch.zeros(shape[:4], dtype=torch.float32, device=device) if key_weights else None
         self.key_positions = torch.zeros(shape[:4], dtype=torch.int32, device=device) if key_weights else None
