@@ -3,8 +3,10 @@
 // the probabilities formed again from the forward's lse: no second pass over V, no maxima.
 //
 // Two kernels.  Few rows (at most 32 a key head; a decode step): K streams past them, bound by HBM; waves stage 32-key tiles of their own as in
-// fa_paged_decode.hip, over the same line of units.  Many: a wave owns 32 keys, their fragments in registers, and streams the rows past them in tiles of 64
-// or 128 that the workgroup's four waves share through LDS; bound by the exponentials, one per score.  Both form S = Q K^T, which leaves a key in a lane, so
+// fa_paged_decode.hip, over the same line of units.  Many: a workgroup takes one unit of that line (the launch's last ones find none), a wave owns 32 of its keys, their fragments in registers, and streams the rows past them in tiles of 64
+// or 128 that the workgroup's four waves share through LDS; bound by vector instructions, three per 64 scores (4 sequences of 2000 .. 4001 keys, 8 key
+// heads, 2 x 509 rows, d = 64: 29.6 us, 78 % of the loaded SIMDs' issue; one unit a workgroup by number instead of by the line 34, since a compute unit then
+// has up to four workgroups of long sequences and another two).  Both form S = Q K^T, which leaves a key in a lane, so
 // that its sum stays in the lane and has one owner.
 #include <type_traits>
 
@@ -40,9 +42,13 @@ __global__ void __launch_bounds__(256, 4) fa_paged_weights_kernel(const WeightsP
   const PagedFwdParams& p = wp.f;
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[C::kLds];
 
-  const int blocks = (p.c.max_keys + 127) / 128;
-  const int pair = blockIdx.x / blocks, kblock = (int)blockIdx.x - pair * blocks;
-  const int b = pair / p.c.HK, h = pair - b * p.c.HK;
+  // Workgroups go to the eight XCDs in turn: each XCD takes a contiguous piece of the line of units, whose pairs' rows stay in its L2.
+  const int sums0 = unit_sums(p.c, 0);
+  const int64_t units = all_units(p.c, sums0), each = (units + 7) / 8;
+  const int64_t u = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= each || u >= units) return;
+  const Spot at_unit = spot_of(p.c, u, sums0);
+  const int b = __builtin_amdgcn_readfirstlane(at_unit.b), h = __builtin_amdgcn_readfirstlane(at_unit.h), kblock = __builtin_amdgcn_readfirstlane(at_unit.unit);
   int q_begin = 0, Lq = 0;
   if (!paged_rows(p.c, b, &q_begin, &Lq)) return;
   const int Lk = paged_len(p.c, b), G = p.c.G, rows = Lq * G;
@@ -79,8 +85,9 @@ __global__ void __launch_bounds__(256, 4) fa_paged_weights_kernel(const WeightsP
     row_first = tok > 0 ? tok * G : 0;
   }
   const int tile0 = row_first / BM, ntiles = (rows + BM - 1) / BM;
-  // the next tile's first row as (token, head of the group)
+  // the first rows, as (token, head of the group), of the tile that is staged next and of the one whose lse and limits are asked for next
   int tok0 = __builtin_amdgcn_readfirstlane((tile0 * BM) / G), head0 = __builtin_amdgcn_readfirstlane(tile0 * BM - tok0 * G);
+  int ask_tok = tok0, ask_head = head0;
   constexpr int RPI = 64 / CH;                        // rows per direct-to-LDS instruction
   constexpr int TI = BM / RPI;                        // instructions of a tile
   const int rl = lane / CH, pch = lane % CH;
@@ -102,26 +109,27 @@ __global__ void __launch_bounds__(256, 4) fa_paged_weights_kernel(const WeightsP
   int limit_next = 0;
   auto fetch_row = [&](int it) {  // a thread a row
     const int r = it * BM + tid;
-    lse_next = INFINITY;
+    lse_next = -INFINITY;
     limit_next = 0;
     if (tid < BM && r < rows) {
-      const int x = head0 + tid, t = per_group(x), g = x - t * G;
-      const float v = p.lse[((int64_t)b * p.c.H + h * G + g) * p.sq_r + tok0 + t];
-      lse_next = v == -INFINITY ? INFINITY : v * kLog2e;
-      limit_next = p.causal ? past + tok0 + t : Lk;
+      const int x = ask_head + tid, t = per_group(x), g = x - t * G;
+      lse_next = p.lse[((int64_t)b * p.c.H + h * G + g) * p.sq_r + ask_tok + t];
+      limit_next = p.causal ? past + ask_tok + t : Lk;
     }
   };
   auto store_row = [&](int buf) {
     if (tid < BM) {
-      reinterpret_cast<float*>(lds_raw + C::kRowOff + buf * C::kRow)[tid] = lse_next;
+      reinterpret_cast<float*>(lds_raw + C::kRowOff + buf * C::kRow)[tid] = lse_next == -INFINITY ? INFINITY : lse_next * kLog2e;
       reinterpret_cast<int*>(lds_raw + C::kRowOff + buf * C::kRow + BM * 4)[tid] = limit_next;
     }
   };
   int first_tok = tok0;  // of the tile in hand
   auto advance = [&]() {
-    const int x = head0 + BM, t = __builtin_amdgcn_readfirstlane(per_group(x));
-    tok0 += t;
-    head0 = x - t * G;
+    const int x = ask_head + BM, t = __builtin_amdgcn_readfirstlane(per_group(x));
+    tok0 = ask_tok;
+    head0 = ask_head;
+    ask_tok += t;
+    ask_head = x - t * G;
   };
   int qoff[D / 16];
 #pragma unroll
@@ -130,39 +138,78 @@ __global__ void __launch_bounds__(256, 4) fa_paged_weights_kernel(const WeightsP
   float sum[2] = {0.f, 0.f};
   int it = tile0, buf = 0;
   if (it < ntiles) {
-    stage(it, 0);
     fetch_row(it);
+    stage(it, 0);
     store_row(0);
+    advance();
+    fetch_row(it + 1);
     advance();
   }
   while (it < ntiles) {
-    if (it + 1 < ntiles) fetch_row(it + 1);
     wait_vmem();
     __syncthreads();
     const int next_tok = tok0;
     if (it + 1 < ntiles) {
-      stage(it + 1, buf ^ 1);
       store_row(buf ^ 1);
+      stage(it + 1, buf ^ 1);
+      fetch_row(it + 2);
       advance();
     }
     const int* const limits = reinterpret_cast<const int*>(lds_raw + C::kRowOff + buf * C::kRow + BM * 4);
     const float* const lses = reinterpret_cast<const float*>(lds_raw + C::kRowOff + buf * C::kRow);
     const T* const Qs = reinterpret_cast<const T*>(lds_raw + buf * C::kTile);
     if (live) {
+      // d = 64: a half's exponentials in four groups, the next half's products between them, what either reads from LDS asked for a group before: a wave
+      // alone on its SIMD does not wait for its chain of products (4 x 8 heads of 1024 keys, 2 x 1018 rows 33.7 -> 29.5 us; with four waves there 29.7 -> 29.5).
+      // d = 128 has no registers for it, d = 32 loses a wave to it (22.7 -> 24.5).
       auto tile = [&](auto masked) {
+        constexpr bool kBetween = D == 64;
+        constexpr int KS = D / 16, NH = BM / 32;
+        vec8 q[KS];
+        f32x16 next;
+        f32x4 l4;
+        auto ask_q = [&](int half) {
 #pragma unroll
-        for (int half = 0; half < BM / 32; half++) {
-          f32x16 s;
+          for (int ks = 0; ks < KS; ks++) q[ks] = *reinterpret_cast<const vec8*>(Qs + half * 32 * D + qoff[ks]);
+        };
+        auto ask_lse = [&](int group) { l4 = *reinterpret_cast<const f32x4*>(lses + 8 * group + 4 * hf); };
+        auto products = [&](int ks0, int ks1) {
+          if (ks0 == 0) {
 #pragma unroll
-          for (int r = 0; r < 16; r++) s[r] = 0.f;
+            for (int r = 0; r < 16; r++) next[r] = 0.f;
+          }
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ks++) s = E::mfma32(*reinterpret_cast<const vec8*>(Qs + half * 32 * D + qoff[ks]), kreg[ks], s);
-          #pragma unroll
+          for (int ks = ks0; ks < ks1; ks++) next = E::mfma32(q[ks], kreg[ks], next);
+        };
+        if (kBetween) {
+          ask_q(0);
+          ask_lse(0);
+          products(0, KS);
+          if (NH > 1) ask_q(1);
+        }
+#pragma unroll
+        for (int half = 0; half < NH; half++) {
+          if (!kBetween) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) next[r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) next = E::mfma32(*reinterpret_cast<const vec8*>(Qs + half * 32 * D + qoff[ks]), kreg[ks], next);
+          }
+          const f32x16 s = next;
+#pragma unroll
           for (int j = 0; j < 4; j++) {
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(lses + half * 32 + 8 * j + 4 * hf);
+            if (kBetween) {
+              __builtin_amdgcn_sched_barrier(0);
+              if (half + 1 < NH) products(j * KS / 4, (j + 1) * KS / 4);
+              if (j == 3 && half + 2 < NH) ask_q(half + 2);
+            } else {
+              ask_lse(half * 4 + j);
+            }
+            const f32x4 lj = l4;
+            if (kBetween && half * 4 + j + 1 < NH * 4) ask_lse(half * 4 + j + 1);
             f32x4 e;
 #pragma unroll
-            for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(s[4 * j + i], cs, -l4[i]));
+            for (int i = 0; i < 4; i++) e[i] = fast_exp2(__builtin_fmaf(s[4 * j + i], cs, -lj[i]));
             if constexpr (decltype(masked)::value) {
 #pragma unroll
               for (int i = 0; i < 4; i++)
@@ -348,10 +395,10 @@ hipError_t launch_d(const WeightsParams& p, hipStream_t stream) {
     f.groups = (int)(blocks < few_resident(D) ? blocks : few_resident(D));  // (a block of 128 keys is a unit)
     hipLaunchKernelGGL((fa_paged_weights_few_kernel<T, D>), dim3((unsigned)f.groups), dim3(256), 0, stream, f);
   } else {
-    // rows of a tile: work enough to cover the next one's loads, where there are as many (4 x 16 heads x 509 tokens, d = 64 33.6 us, in tiles of 64 36.8, of 32 40.9)
+    // rows of a tile: work enough to cover the next one's loads, where there are as many (1 x 8 heads, 2 x 1000 rows, d = 64 30.4 us, in tiles of 64 32.9; d = 32 23.2, 26.7)
     constexpr int kMost = D == 128 ? 64 : 128;
-    if (p.f.c.max_sq * p.f.c.G <= 64) hipLaunchKernelGGL((fa_paged_weights_kernel<T, D, 64>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((fa_paged_weights_kernel<T, D, kMost>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    if (p.f.c.max_sq * p.f.c.G <= 64) hipLaunchKernelGGL((fa_paged_weights_kernel<T, D, 64>), dim3((unsigned)(blocks + 7) / 8 * 8), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((fa_paged_weights_kernel<T, D, kMost>), dim3((unsigned)(blocks + 7) / 8 * 8), dim3(256), 0, stream, p);
   }
   return hipGetLastError();
 }
