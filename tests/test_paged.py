@@ -377,7 +377,8 @@ def test_norm_rotary_keeps_special_values_apart():
     ([40, 17, 1], [1, 1, 1], 8, 2, 64, 16, True, True, True, False),
     ([33, 64, 100, 16], [33, 0, 7, 16], 6, 3, 128, 32, False, True, True, True),
     ([700] + list(range(1, 80)), [650] + [1] * 79, 4, 4, 32, 64, True, True, True, False),  # more sequences than a wave has lanes; several rows a workgroup
-    ([300, 90], [290, 61], 20, 20, 128, 16, False, False, True, False)])
+    ([300, 90], [290, 61], 20, 20, 128, 16, False, False, True, False),
+    ([900, 3, 710], [880, 1, 700], 20, 20, 128, 16, True, True, True, False)])  # more rows than the launch has workgroups for
 def test_append(dtype, lens, new, H, HK, D, PS, head_major, norm, turn, fp32):
     from flash_attn.flash_attn_paged_interface import paged_append_func
     c = Cache(lens, HK, D, PS, dtype, 1, head_major).gpu()
