@@ -265,57 +265,68 @@ __global__ void __launch_bounds__(64 * NW_) fa_paged_decode_kernel(const PagedFw
 
 namespace {
 
-// The pairs that the ends of the workgroups' shares have cut, each joined by the workgroup whose number is that of the first share that begins inside it: D / 4
-// threads over a row's elements times 1024 / D over the parts, the rows one after the other (blockIdx.y, blockIdx.y + gridDim.y, ...).
+// The pairs that the ends of the workgroups' shares have cut (blockIdx.x: a pair; blockIdx.y and the threads share its rows): D / 4 threads over a row's
+// elements, times lanes over its parts - as many as there are, rounded up to a power of two -, times rows side by side.  The lanes' results are
+// joined in LDS, in the same order each time.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_decode_join_kernel(const PagedFwdParams p) {
   constexpr int kCols = D / 4, kLanes = 256 / kCols;
   __shared__ f32x4 os[256];
   __shared__ PartRow ms[256];
-  const int sums0 = unit_sums(p.c, 0);
-  const int64_t units = all_units(p.c, sums0);
-  const int n = sharers(p, units), w = (int)blockIdx.x + 1;
-  if (w >= n || units == 0) return;
-  const Spot at = spot_of(p.c, share_begin(units, w, n), sums0);
-  const int64_t begin = share_begin(units, w, n) - at.unit;  // of the pair
-  if (at.unit == 0 || share_begin(units, w - 1, n) > begin) return;
-  const int b = __builtin_amdgcn_readfirstlane(at.b), h = __builtin_amdgcn_readfirstlane(at.h);
-  const int w0 = w - 1;
-  int w1 = w;
-  while (w1 + 1 < n && share_begin(units, w1 + 1, n) < begin + at.units) w1++;
+  const int b = blockIdx.x / p.c.HK, h = (int)blockIdx.x - b * p.c.HK;
+  int64_t units = 0, begin = 0;  // of all pairs; where this one's lie
+  int pair_units = 0;
+  for (int first = 0; first < p.c.B; first += 64) {
+    const int sums = unit_sums(p.c, first), k = b - first;
+    if (k >= 0 && k < 64) {
+      const int upto = k > 0 ? __builtin_amdgcn_readlane(sums, k > 0 ? k - 1 : 0) : 0;
+      pair_units = __builtin_amdgcn_readlane(sums, k) - upto;
+      begin = (units + upto) * p.c.HK + (int64_t)h * pair_units;
+    }
+    units += __builtin_amdgcn_readlane(sums, 63);
+  }
+  units *= p.c.HK;
   int q_begin = 0, Lq = 0;
-  if (!paged_rows(p.c, b, &q_begin, &Lq)) return;
+  if (pair_units == 0 || !paged_rows(p.c, b, &q_begin, &Lq)) return;
+  const int n = sharers(p, units);
+  const auto share_of = [&](int64_t u) { return (int)(((u + 1) * n - 1) / units); };  // (the last w with units * w / n <= u)
+  const int w0 = share_of(begin), w1 = share_of(begin + pair_units - 1);
+  if (w0 == w1) return;  // whole
   const float cs = p.scale_log2;
   constexpr int kEach = kPartRows * (D + 3);
   // the pair is the last of share w0, and its first, too, if the share begins with it; it is the first of the others'
   const int first_slot = share_begin(units, w0, n) == begin ? 0 : 1;
-  const int col = threadIdx.x % kCols, lane = threadIdx.x / kCols;
-  for (int r = blockIdx.y; r < Lq * p.c.G; r += gridDim.y) {
+  int lanes = 2;
+  while (lanes < kLanes && lanes < w1 - w0 + 1) lanes *= 2;
+  const int col = threadIdx.x % kCols, at = threadIdx.x / kCols, lane = at & (lanes - 1), side = at / lanes, beside = kLanes / lanes;
+  const int rows = Lq * p.c.G;
+  for (int r0 = blockIdx.y * beside; r0 < rows; r0 += gridDim.y * beside) {
+    const int r = r0 + side;
     PartRow a{-INFINITY, 0.f, 0.f};
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    auto join = [&](float m, float l, float u, f32x4 x) {
-      const float top = fmaxf(a.m, m), ref = top == -INFINITY ? 0.f : top;
-      const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((m - ref) * cs);
-      a = PartRow{top, a.l * fa + l * fb, a.u * fa + u * fb};
-      o = o * fa + x * fb;
+    auto join = [&](PartRow x, f32x4 xo) {
+      const float top = fmaxf(a.m, x.m), ref = top == -INFINITY ? 0.f : top;
+      const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((x.m - ref) * cs);
+      a = PartRow{top, a.l * fa + x.l * fb, a.u * fa + x.u * fb};
+      o = o * fa + xo * fb;
     };
-    for (int i = w0 + lane; i <= w1; i += kLanes) {
-      const float* const s = p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
-      const float* const ml = s + kPartRows * D + r;
-      join(ml[0], ml[kPartRows], ml[2 * kPartRows], *reinterpret_cast<const f32x4*>(s + r * D + col * 4));
-    }
-    os[threadIdx.x] = o;
-    ms[threadIdx.x] = a;
-    __syncthreads();
-    if (lane == 0) {
-      for (int i = 1; i < kLanes && i <= w1 - w0; i++) {
-        const PartRow x = ms[i * kCols + col];
-        join(x.m, x.l, x.u, os[i * kCols + col]);
+    if (r < rows)
+      for (int i = w0 + lane; i <= w1; i += lanes) {
+        const float* const s = p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
+        const float* const ml = s + kPartRows * D + r;
+        join(PartRow{ml[0], ml[kPartRows], ml[2 * kPartRows]}, *reinterpret_cast<const f32x4*>(s + r * D + col * 4));
       }
+    for (int half = lanes / 2; half > 0; half /= 2) {
+      os[threadIdx.x] = o;
+      ms[threadIdx.x] = a;
+      __syncthreads();
+      if (lane < half) join(ms[threadIdx.x + half * kCols], os[threadIdx.x + half * kCols]);
+      __syncthreads();
+    }
+    if (lane == 0 && r < rows) {
       store_row_piece<T>(p, q_begin, h, r, col * 4, o * (a.l > 0.f ? fast_rcp(a.l) : 1.f));
       if (col == 0) store_lse(p, b, h, r, lse_of(a.m, a.u, cs));
     }
-    __syncthreads();
   }
 }
 
@@ -327,10 +338,8 @@ hipError_t launch_d(const PagedFwdParams& p, hipStream_t stream) {
   else hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWaves(D)>), grid, dim3(64 * kDecodeWaves(D)), 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.groups == 0) return e;
-  // (few pairs have many parts: their rows side by side)
-  const int rows = p.c.max_sq * p.c.G;
-  const unsigned gy = pairs >= 64 ? 1u : (unsigned)rows;
-  if (p.groups > 1) hipLaunchKernelGGL((paged_decode_join_kernel<T, D>), dim3((unsigned)p.groups - 1, gy), dim3(256), 0, stream, p);
+  const unsigned rows = (unsigned)(p.c.max_sq * p.c.G), side = pairs < 1024 ? 1024 / pairs : 1;  // (workgroups beside each other for a pair's rows)
+  hipLaunchKernelGGL((paged_decode_join_kernel<T, D>), dim3(pairs, rows < side ? rows : side), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 template <typename T>
