@@ -30,15 +30,19 @@ Plan plan_of(const fa_paged_cache& c) {
   const int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
   pl.decode = rows <= fa::kDecodeMaxQ;
   if (pl.decode) {
-    // Pairs that about fill the device once: a workgroup each, of as many waves as LDS allows, that nobody has to join.  us with the line of shares / so
-    // (one new token, all lengths equal; d = 128, 64, 32): 128 pairs of 2000 keys 35.4 / 29.8, 30.4 / 18.1, 23.3 / 15.2; of 8000 108 / 101, 65.9 / 57.2,
-    // 38.5 / 38.3; 256 pairs of 8000 194 / 186, 110 / 96, 65 / 52.  Lengths from a quarter of that on: 128 pairs up to 4000 46.3 / 49.3, 34.1 / 27.0,
-    // 30.8 / 22.0, up to 8000 77.6 / 90.2: the longest sequence decides.  Fewer pairs have too few readers: 8 of 2000 keys (d = 128) 15 / 25.
-    pl.wide = pairs <= 256 && max_keys <= (pairs >= 192 ? 8192 : pairs >= 128 ? 4096 : 128 * fa::kDecodeWide(c.head_dim));
-    // More pairs than that, of few keys: a workgroup each, of the usual number of waves.  us with the line / so, lengths equal and from a quarter on:
-    // d = 128, 512 pairs of 1000 55 / 52, 46 / 37; of 2000 101 / 99, 77 / 71; 320 pairs of 4000 129 / 139, 91 / 100.  d = 64, 1024 of 500 28 / 25;
-    // 320 of 2000 43 / 51, 33 / 45.  d = 32, 512 of 500 19 / 11; of 4000 61 / 52, 47 / 42; of 8000 110 / 100, 78 / 80.
-    const bool whole = pl.wide || max_keys <= 128 || (pairs > 256 && max_keys <= (c.head_dim <= 32 ? 4096 : 1024));
+    // A pair to itself, or shares of the line of all keys and a join behind them: the join is another launch and the line's beginning a chain of loads, 14 us
+    // at the least; a workgroup alone with a pair reads 26 (d = 128) or 34 keys a wave and us, and the longest sequence decides.  us of a workgroup a pair / of
+    // the line, one new token, all lengths equal | from a quarter on:
+    // few pairs, wide workgroups: 32 pairs of 600 keys, d = 128 13.1 / 16.5, of 1000 17.2 / 15.1; d = 64 1000 11.4 / 15.2, 2000 17.5 / 15.1; d = 32 2000 13.5 / 14.8
+    // 128 pairs: d = 128 1000 19.1 / 22.5 | 20.0 / 22.4, 2000 29.9 / 32.2 | 29.5 / 26.4; d = 64 4000 29.1 / 30.2 | 26.8 / 26.0, 8000 61 / 59 | 53 / 40
+    // 256 pairs: d = 128 4000 101 / 104 | 72 / 72, 8000 187 / 191 | 134 / 131; d = 64 8000 98 / 106 | 72 / 73; d = 32 8000 53 / 59 | 41 / 41
+    pl.wide = pairs <= 256 && max_keys <= (pairs >= 192 ? 1024 : pairs >= 96 ? 512 : 192) * fa::kDecodeWide(c.head_dim);
+    // short keys at d <= 32, more pairs than the device holds at once: the usual number of waves.  d = 32, 256 pairs of 500 8.2 / 14.7, wide 9.1; 320 of 2000 24 / 25 |
+    // 22 / 22, of 4000 41 / 40 | 36 / 30; d = 64, 320 of 500 18 / 22 | 17 / 16, of 1000 29 / 26 | 26 / 22, 1024 of 1000 53 / 56 | 39 / 43; d = 128, 320 of 1000 37 / 40 |
+    // 29 / 30, of 2000 71 / 71 | 54 / 53, 1024 of 1000 100 / 104 | 68 / 78
+    const bool small = c.head_dim <= 32;
+    if (small && max_keys <= 512) pl.wide = false;
+    const bool whole = pl.wide || max_keys <= (small ? 512 : 128) || (pairs > 256 && max_keys <= (small ? 2048 : c.head_dim == 64 && pairs < 1024 ? 512 : 1024));
     if (!whole) {
       const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
       pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim), pairs * units);
