@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   __shared__ __attribute__((aligned(16))) uint32_t keys[kCap > 0 ? kCap : 4];
   __shared__ int hist[2048];
   __shared__ int sums[2][kWaves];
-  __shared__ uint32_t found[2];  // digit, keys above it
+  __shared__ uint32_t found[3];  // digit, keys above it, keys of it
   const int b = blockIdx.x / p.c.HK, h = (int)blockIdx.x - b * p.c.HK;
   const int L = paged_len(p.c, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -118,6 +118,13 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
     return p.c.positions[at] >= newest ? kNewest : k;
   };
   auto key_of = [&](int j) { return kCap > 0 ? keys[j] : read_key(j); };
+  // (the lanes whose digit is the first one's count as one: keys of equal weight, such as those that have received nothing yet, would queue up)
+  auto count = [&](uint32_t digit) {
+    const bool like_first = digit == (uint32_t)__builtin_amdgcn_readfirstlane((int)digit);
+    const uint64_t same = __ballot(like_first);
+    if (!like_first) atomicAdd(&hist[digit], 1);
+    else if (lane == (int)__builtin_ctzll(same)) atomicAdd(&hist[digit], __popcll(same));
+  };
 
   // ---- the budget-th largest key
   uint32_t prefix = 0;
@@ -153,7 +160,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               k[e] = pos[i][e] >= newest ? kNewest : ordered(w[i][e]);
-              if (q + e < L) atomicAdd(&hist[k[e] >> 21], 1);
+              if (q + e < L) count(k[e] >> 21);
             }
             *reinterpret_cast<u32x4*>(keys + q) = k;
           }
@@ -163,7 +170,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
 #pragma unroll 4
       for (int j = tid; j < L; j += kThreads) {
         const uint32_t k = key_of(j);
-        if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
+        if (pass == 0 || (k >> (shift + bits)) == prefix) count((k >> shift) & ((1 << bits) - 1));
       }
     }
     __syncthreads();
@@ -185,6 +192,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
       if (above < want && want <= above + bin[i]) {
         found[0] = 2047 - kBins * tid - i;
         found[1] = above;
+        found[2] = bin[i];
       }
       above += bin[i];
     }
@@ -199,47 +207,58 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   const int run = (L + kThreads - 1) / kThreads * 64;
   const int j0 = wave * run, j1 = j0 + run < L ? j0 + run : L;
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  int ties = 0;
-  for (int j = j0 + lane; j - lane < j1; j += 64) ties += __popcll(__ballot(j < j1 && key_of(j) == edge));
-  if (lane == 0) sums[0][wave] = ties;
+  int ties_end = INT32_MAX;  // keys that equal the edge stay below this slot
+  if ((int)found[2] > want) {
+    int ties = 0;
+    for (int j = j0 + lane; j < j1; j += 64) ties += key_of(j) == edge;
+    ties = __builtin_amdgcn_readlane(wave_prefix_sum(ties), 63);
+    if (lane == 0) sums[0][wave] = ties;
+    __syncthreads();
+    int unused;
+    int tie = before_wave<kWaves>(sums[0], wave, &unused);
+    if (tie < want && want <= tie + ties) {
+      for (int j = j0 + lane; j - lane < j1; j += 64) {
+        const bool tied = j < j1 && key_of(j) == edge;
+        const uint64_t all = __ballot(tied);
+        if (tied && tie + __popcll(all & below) == want - 1) found[0] = (uint32_t)j + 1;
+        tie += __popcll(all);
+      }
+    }
+    __syncthreads();
+    ties_end = (int)found[0];
+  }
+  const auto stays = [&](int j, uint32_t k) { return k > edge || (k == edge && j < ties_end); };
+  int holes_here = 0, come_here = 0;
+  for (int j = j0 + lane; j < j1; j += 64) {
+    const bool stay = stays(j, key_of(j));
+    holes_here += !stay && j < p.budget;
+    come_here += stay && j >= p.budget;
+  }
+  holes_here = __builtin_amdgcn_readlane(wave_prefix_sum(holes_here), 63);
+  come_here = __builtin_amdgcn_readlane(wave_prefix_sum(come_here), 63);
+  __syncthreads();  // (the ties have been read)
+  if (lane == 0) {
+    sums[0][wave] = holes_here;
+    sums[1][wave] = come_here;
+  }
   __syncthreads();
-  int all_ties;
-  const int tie0 = before_wave<kWaves>(sums[0], wave, &all_ties);
-  int hole0 = 0, come0 = 0, moves = 0;
   __shared__ int32_t own_moves[kMoveD > 0 ? 2 * kMovesPerGroup : 1];
   int32_t* const holes = kMoveD > 0 ? own_moves : p.moves + (int64_t)blockIdx.x * 2 * p.cap;
   const int cap = kMoveD > 0 ? kMovesPerGroup : p.cap;
-  for (int round = 0; round < 2; round++) {  // counted, then written
-    int tie = tie0, hole = hole0, come = come0;
-    for (int j = j0 + lane; j - lane < j1; j += 64) {
-      const bool in = j < j1;
-      const uint32_t k = in ? key_of(j) : 0;
-      const uint64_t tied = __ballot(in && k == edge);
-      const bool stays = in && (k > edge || (k == edge && tie + __popcll(tied & below) < want));
-      tie += __popcll(tied);
-      const bool is_hole = in && !stays && j < p.budget, comes = stays && j >= p.budget;
-      const uint64_t hb = __ballot(is_hole), cb = __ballot(comes);
-      if (round == 1) {
-        const int nh = hole + __popcll(hb & below), nc = come + __popcll(cb & below);
-        if (is_hole && nh < cap) holes[nh] = j;
-        if (comes && nc < cap) holes[cap + nc] = j;
-      }
-      hole += __popcll(hb);
-      come += __popcll(cb);
-    }
-    if (round == 0) {
-      __syncthreads();  // (the ties have been read)
-      if (lane == 0) {
-        sums[0][wave] = hole;
-        sums[1][wave] = come;
-      }
-      __syncthreads();
-      int all_come;
-      hole0 = before_wave<kWaves>(sums[0], wave, &moves);
-      come0 = before_wave<kWaves>(sums[1], wave, &all_come);
-      moves = moves < cap ? moves : cap;  // (as many as the cap, by its definition)
-      if (kMoveD == 0 && tid == 0) p.counts[blockIdx.x] = moves;
-    }
+  int moves, all_come;
+  int hole = before_wave<kWaves>(sums[0], wave, &moves), come = before_wave<kWaves>(sums[1], wave, &all_come);
+  moves = moves < cap ? moves : cap;  // (as many as the cap, by its definition)
+  if (kMoveD == 0 && tid == 0) p.counts[blockIdx.x] = moves;
+  for (int j = j0 + lane; j - lane < j1; j += 64) {
+    const bool in = j < j1;
+    const bool stay = in && stays(j, key_of(in ? j : j0));
+    const bool is_hole = in && !stay && j < p.budget, comes = stay && j >= p.budget;
+    const uint64_t hb = __ballot(is_hole), cb = __ballot(comes);
+    const int nh = hole + __popcll(hb & below), nc = come + __popcll(cb & below);
+    if (is_hole && nh < cap) holes[nh] = j;
+    if (comes && nc < cap) holes[cap + nc] = j;
+    hole += __popcll(hb);
+    come += __popcll(cb);
   }
   if constexpr (kMoveD > 0) {
     __shared__ MoveSpots spots;
