@@ -323,37 +323,48 @@ __global__ void __launch_bounds__(256, ChunkCfg<D>::kWaves - (kLse ? 1 : 0)) fa_
 
 namespace {
 
-// The splits' partial results joined: D / 4 threads a row.
-template <typename T>
-__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedFwdParams p, int D) {
-  const int per_row = D / 4;
+// Threads of a row's elements times lanes over its splits, four of them each where there are lanes enough (62 splits of 64 rows, 8 key heads, d = 128
+// 7 us, with one lane 34).
+template <int D>
+constexpr int kJoinCols = D / 4;
+template <int D>
+int join_lanes(int n_splits) {
+  int lanes = 1;
+  while (lanes < 256 / kJoinCols<D> && lanes * 4 < n_splits) lanes *= 2;
+  return lanes;
+}
+// The splits' partial results joined.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedFwdParams p, int lanes) {
+  constexpr int kCols = kJoinCols<D>;
+  __shared__ f32x4 os[256];
+  __shared__ PartRow ms[256];
   const int64_t all = (int64_t)p.c.B * p.c.HK * p.nq_tiles * kChunkRows;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t at = idx / per_row;
-  if (at >= all) return;
-  const int d0 = (int)(idx - at * per_row) * 4;
+  const int col = threadIdx.x % kCols, in = threadIdx.x / kCols, lane = in & (lanes - 1);
+  const int64_t at = (int64_t)blockIdx.x * (256 / kCols / lanes) + in / lanes;
   const int pair = (int)(at / (p.nq_tiles * kChunkRows)), r = (int)(at - (int64_t)pair * p.nq_tiles * kChunkRows);
   const int b = pair / p.c.HK, h = pair - b * p.c.HK;
-  const int s = p.c.cu_q[b], e = p.c.cu_q[b + 1];
-  if (s < 0 || e <= s || e > p.c.total_q) return;
-  const int Lq = e - s < p.c.max_sq ? e - s : p.c.max_sq;
-  if (r >= Lq * p.c.G) return;
-  const float cs = p.scale_log2;
-  float m = -INFINITY;
-  for (int i = 0; i < p.n_splits; i++) m = fmaxf(m, p.part[(int64_t)i * all * (D + 3) + all * D + at * 3]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f, u = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < p.n_splits; i++) {
-    const float* const x = p.part + (int64_t)i * all * (D + 3);
-    const float* const ml = x + all * D + at * 3;
-    const float f = fast_exp2((ml[0] - mu) * cs);
-    l = __builtin_fmaf(ml[1], f, l);
-    u = __builtin_fmaf(ml[2], f, u);
-    o = o + *reinterpret_cast<const f32x4*>(x + at * D + d0) * f;
+  int s = 0, e = 0;
+  if (at < all) {
+    s = p.c.cu_q[b];
+    e = p.c.cu_q[b + 1];
   }
-  store_row_piece<T>(p, s, h, r, d0, o * (l > 0.f ? fast_rcp(l) : 1.f));
-  if (d0 == 0) store_lse(p, b, h, r, lse_of(m, u, cs));
+  const bool on = s >= 0 && e > s && e <= p.c.total_q && r < (e - s < p.c.max_sq ? e - s : p.c.max_sq) * p.c.G;
+  const float cs = p.scale_log2;
+  JoinedRow x;
+  if (on) {
+#pragma unroll 4
+    for (int i = lane; i < p.n_splits; i += lanes) {
+      const float* const from = p.part + (int64_t)i * all * (D + 3);
+      const float* const ml = from + all * D + at * 3;
+      x.add(PartRow{ml[0], ml[1], ml[2]}, *reinterpret_cast<const f32x4*>(from + at * D + col * 4), cs);
+    }
+  }
+  x.across<kCols>(lane, lanes, cs, os, ms);
+  if (on && lane == 0) {
+    store_row_piece<T>(p, s, h, r, col * 4, x.o * (x.a.l > 0.f ? fast_rcp(x.a.l) : 1.f));
+    if (col == 0) store_lse(p, b, h, r, lse_of(x.a.m, x.a.u, cs));
+  }
 }
 
 template <typename T, int D>
@@ -365,8 +376,9 @@ hipError_t launch_d(const PagedFwdParams& p, hipStream_t stream) {
   else hipLaunchKernelGGL((fa_paged_chunk_kernel<T, D, false>), grid, dim3(256), 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.n_splits <= 1) return e;
-  const int64_t n = items * kChunkRows * (D / 4);
-  hipLaunchKernelGGL(paged_chunk_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, p, D);
+  const int lanes = join_lanes<D>(p.n_splits);
+  const int64_t n = items * kChunkRows * kJoinCols<D> * lanes;
+  hipLaunchKernelGGL((paged_chunk_join_kernel<T, D>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, p, lanes);
   return hipGetLastError();
 }
 template <typename T>

@@ -302,30 +302,17 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const PagedFwdPa
   const int rows = Lq * p.c.G;
   for (int r0 = blockIdx.y * beside; r0 < rows; r0 += gridDim.y * beside) {
     const int r = r0 + side;
-    PartRow a{-INFINITY, 0.f, 0.f};
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    auto join = [&](PartRow x, f32x4 xo) {
-      const float top = fmaxf(a.m, x.m), ref = top == -INFINITY ? 0.f : top;
-      const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((x.m - ref) * cs);
-      a = PartRow{top, a.l * fa + x.l * fb, a.u * fa + x.u * fb};
-      o = o * fa + xo * fb;
-    };
+    JoinedRow x;
     if (r < rows)
       for (int i = w0 + lane; i <= w1; i += lanes) {
         const float* const s = p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
         const float* const ml = s + kPartRows * D + r;
-        join(PartRow{ml[0], ml[kPartRows], ml[2 * kPartRows]}, *reinterpret_cast<const f32x4*>(s + r * D + col * 4));
+        x.add(PartRow{ml[0], ml[kPartRows], ml[2 * kPartRows]}, *reinterpret_cast<const f32x4*>(s + r * D + col * 4), cs);
       }
-    for (int half = lanes / 2; half > 0; half /= 2) {
-      os[threadIdx.x] = o;
-      ms[threadIdx.x] = a;
-      __syncthreads();
-      if (lane < half) join(ms[threadIdx.x + half * kCols], os[threadIdx.x + half * kCols]);
-      __syncthreads();
-    }
+    x.across<kCols>(lane, lanes, cs, os, ms);
     if (lane == 0 && r < rows) {
-      store_row_piece<T>(p, q_begin, h, r, col * 4, o * (a.l > 0.f ? fast_rcp(a.l) : 1.f));
-      if (col == 0) store_lse(p, b, h, r, lse_of(a.m, a.u, cs));
+      store_row_piece<T>(p, q_begin, h, r, col * 4, x.o * (x.a.l > 0.f ? fast_rcp(x.a.l) : 1.f));
+      if (col == 0) store_lse(p, b, h, r, lse_of(x.a.m, x.a.u, cs));
     }
   }
 }

@@ -32,6 +32,29 @@ struct PartRow {
   float m, l, u;
 };
 
+// Four elements of a row, joined from parts.
+struct JoinedRow {
+  PartRow a{-INFINITY, 0.f, 0.f};
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  FA_DEVICE void add(PartRow x, f32x4 xo, float cs) {
+    const float top = fmaxf(a.m, x.m), ref = top == -INFINITY ? 0.f : top;
+    const float fa = fast_exp2((a.m - ref) * cs), fb = fast_exp2((x.m - ref) * cs);
+    a = PartRow{top, a.l * fa + x.l * fb, a.u * fa + x.u * fb};
+    o = o * fa + xo * fb;
+  }
+  // A workgroup's `lanes` (a power of two) partial joins of each row, kCols threads apart, in a fixed order; lane 0 has the result.
+  template <int kCols>
+  FA_DEVICE void across(int lane, int lanes, float cs, f32x4* os, PartRow* ms) {
+    for (int half = lanes / 2; half > 0; half /= 2) {
+      os[threadIdx.x] = o;
+      ms[threadIdx.x] = a;
+      __syncthreads();
+      if (lane < half) add(ms[threadIdx.x + half * kCols], os[threadIdx.x + half * kCols], cs);
+      __syncthreads();
+    }
+  }
+};
+
 FA_DEVICE bool paged_rows(const PagedCache& c, int b, int* begin, int* len) {  // the new tokens of sequence b
   const int s = ld_scalar(c.cu_q, b), e = ld_scalar(c.cu_q, b + 1);
   if (s < 0 || e <= s || e > c.total_q) return false;
