@@ -54,11 +54,14 @@ Plan plan_of(const fa_paged_cache& c) {
   const int64_t items = pairs * pl.nq_tiles;
   const int tiles = (max_keys + 63) / 64;
   pl.deal = pairs % 8 == 0 || pairs >= 48;  // (else one XCD would have a quarter more of them than another, or none)
-  // Row tiles that do not fill the compute units share their keys, at least 512 of them each, so that there are two workgroups a compute unit.  us with
-  // 512 workgroups and 512 keys / 768 and 256 (d = 128, 8 key heads of 32 heads): 64 tokens behind 16000 49.5 / 59.2, 512 behind 7700 101 / 99.5;
-  // d = 64: 3 x 100 tokens behind 6000, 12 heads 29.4 / 35.9, 2 x 200 behind 1800 28.6 / 31.3.
-  int64_t n = items >= 384 ? 1 : (512 + items - 1) / items;
-  n = std::min<int64_t>({n, tiles / 8, 64});
+  // Row tiles that do not fill the compute units share their keys: at most two workgroups a compute unit (another would be a third for some),
+  // at least 256 keys each, where there are many tiles 512.  us of at least 512 keys / so: 12 heads, d = 128, 33 tokens behind 3000 25.8 / 19.0, 40 behind 460
+  // 19.0 / 15.9, d = 64 18.9 / 15.9, 100 behind 900 16.8 / 15.1; 8 x 4 key heads of 16, 64 rows, 2000 keys 18.9 / 15.5; 3 x 12 heads, 100 behind 5900 27.8 / 29.9.
+  // Two tiles of 512 keys, d = 64: 12.9 in one launch, 15.0 in two; 216 tiles of 700 keys 17.1 in one, 25.2 in two.  One workgroup more a tile than fits: 112 tiles,
+  // d = 128 39 / 44.  256 tiles undivided 122, two each 103 (d = 128, 4000 keys).
+  const int64_t n_fit = items >= 384 ? 1 : items > 256 ? 2 : 512 / items;
+  const int least = items > 128 ? 8 : c.head_dim < 128 && tiles < 12 ? tiles : 4;  // tiles of 64 keys
+  const int64_t n = std::min<int64_t>({n_fit, tiles / least, 64});
   pl.n_splits = n < 2 ? 1 : (int)n;
   if (pl.n_splits > 1) pl.bytes = (size_t)pl.n_splits * items * fa::kChunkRows * (c.head_dim + 3) * 4;
   return pl;
