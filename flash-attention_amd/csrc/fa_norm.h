@@ -11,6 +11,12 @@
 
 namespace fa {
 
+// Workgroups of `waves` waves each that walk over rows, for the whole device: whole ones a compute unit, about `most` waves of them.
+inline int walking_workgroups(int waves, int most) {
+  const int each = (most + waves / 2) / waves;
+  return 256 * (each > 0 ? each : 1);
+}
+
 // Sum over the CH lanes (2, 4, 8 or 16, aligned) that hold a vector, in each of them.
 template <int CH>
 FA_DEVICE float vector_sum(float x) {

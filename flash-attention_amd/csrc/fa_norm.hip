@@ -228,9 +228,12 @@ __global__ void __launch_bounds__(1024) norm_weights_kernel(const NormParams p, 
   }
 }
 
-// How the launches are cut.  At most kNormBlocks workgroups for both parts, shared by their sizes, which walk on over the rows: the forward of 32768 rows
-// of 20 heads, d = 128 71 us (4.7 TB/s), with 2048 of them 78, a workgroup for every four rows 85; and the backward's each leave a row of sums.
-constexpr int kNormBlocks = 1024;
+// How the launches are cut.  The workgroups of both parts, shared by their sizes, walk on over the rows: as many as give a compute unit about 20 waves in the
+// forward and 16 in the backward (whose workgroups each leave a row of sums, too).  us of the forward with four workgroups a compute unit whatever their size / so: 32768
+// rows of 16 + 4 heads, d = 128 71.6 / 67.9 (4.9 TB/s; a workgroup for every four rows 85.8), 16000 of 32 + 8 (eight waves a workgroup) 91 / 77, 65536 of 2 x 12,
+// d = 64 86.5 / 78.4, 24000 of 2 x 12 63 / 55; with 24 waves 69.8, -, 77.5, 53.8.  Backward, 16 waves / 20: 64000 rows of 2 x 8 heads, d = 32 48 / 63, 11200 of
+// 2 x 20, d = 128 74 / 100, 48000 of 24 + 8, d = 64 118 / 141, the others alike.
+constexpr int kForwardWaves = 20, kBackwardWaves = 16;
 
 void cut(NormPart* part, int heads, int D, int n_rows, int rows_in_flight, int most_blocks, int first_block) {
   part->heads = heads;
@@ -261,7 +264,9 @@ int block_threads(const NormParams& p) {
 int cut_parts(NormParams* p, const fa_qk_norm_args* a, bool bwd) {
   const int n = (int)a->n_rows, D = a->head_dim, all = std::max(1, a->nheads_q + a->nheads_k);
   // (pieces of a row are 256 threads wide: parts that share a launch with a wider one keep to rows of their own)
-  const int64_t most = kNormBlocks;
+  const int per_row = std::max(1, std::max(a->nheads_q, a->nheads_k) * (D / 8));
+  const int threads = per_row > 512 ? 256 : (per_row >= 256 ? 1 : 256 / per_row) * per_row;
+  const int64_t most = walking_workgroups((threads + 63) / 64, bwd ? kBackwardWaves : kForwardWaves);
   const int64_t q_share = std::max<int64_t>(1, most * a->nheads_q / all), k_share = std::max<int64_t>(1, most * a->nheads_k / all);
   const int rows = bwd ? kNormBwdRows : norm_rows(n, all, D);
   cut(&p->part[0], a->nheads_q, D, n, rows, (int)q_share, 0);

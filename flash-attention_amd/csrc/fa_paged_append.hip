@@ -145,10 +145,10 @@ hipError_t launch_append_d(AppendParams p, hipStream_t stream) {
   const bool few = (int64_t)p.c.total_q * p.pieces <= 2048;
   const int rows = few ? 1 : kRows;
   p.groups = (p.c.total_q + rows - 1) / rows;
-  // Prompts: whole workgroups a compute unit, 20 waves of them at most, which walk on over the rows.  us of so many waves / as many workgroups as rows want: 20000
+  // Prompts: whole workgroups a compute unit, about 20 waves of them, which walk on over the rows.  us of so many waves / as many workgroups as rows want: 20000
   // rows of 3 x 16 heads, d = 64 (six waves a workgroup, three of them a compute unit) 56 / 65, d = 32 35 / 33, 18000 of 3 x 12 40 / 49; 21000 of 40 heads 46 / 58, d = 128
   // 98 / 108; 15000 of 3 x 32, d = 128 (a row six workgroups) 158 / 153.  24 waves: 65 and 46 for the first and the third.
-  if (!few) p.groups = std::min(p.groups, std::max(1, 256 * std::max(1, 20 / (p.threads / 64)) / p.pieces));
+  if (!few) p.groups = std::min(p.groups, std::max(1, walking_workgroups(p.threads / 64, 20) / p.pieces));
   const dim3 grid((unsigned)(p.groups * p.pieces)), block((unsigned)p.threads);
   if (few) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((paged_append_kernel<T, D, kRows>), grid, block, 0, stream, p);

@@ -1,8 +1,8 @@
 // The calls of the paged cache and of the norm in front of it, made natively (included by fa_host.cpp, whose rules hold here: a call that fails a
 // check returns None and the binding runs it, and raises what it has to).  A decode step is a handful of such calls whose kernels take 4 to 15 us: what
 // the host takes decides.  us of a pass among others with the binding's own calls / with these:
-//   norm of a prompt of 61 tokens 28.0 / 5.6, its training step on 8 x 511 .. 1021 tokens 194 / 81 (kernels 38), a decode step of 32 sequences stored
-//   29.1 / 5.9, attention of one token 23.9 / 13.3, eviction of 32 sequences' one key with two copies 28.7 / 19.1.
+//   norm of a prompt of 61 tokens 28.0 / 6.1, its training step on 8 x 511 .. 1021 tokens 194 / 79 (kernels 30; an empty native function's takes 54), a
+//   decode step of 32 sequences stored 29.1 / 5.9, attention of one token 23.9 / 7.8, eviction of 32 sequences' one key with two copies 28.7 / 16.1.
 #pragma once
 
 #include <ATen/core/grad_mode.h>
