@@ -292,7 +292,8 @@ def _norm_case(rows, H, HK, D, dtype, wdtype, seed, packed):
     (1, 1, 1, 16, False, False, True), (61, 12, 12, 64, False, False, True), (7, 3, 1, 32, True, True, True), (130, 8, 2, 128, False, True, True),
     (5, 40, 40, 128, True, False, True),  # rows wider than a workgroup
     (33, 33, 1, 128, False, False, True),  # ... beside one that is not
-    (2500, 4, 4, 64, False, True, True), (300, 1, 5, 16, True, False, False), (17, 6, 6, 128, False, False, False)])
+    (2500, 4, 4, 64, False, True, True), (300, 1, 5, 16, True, False, False), (17, 6, 6, 128, False, False, False),
+    (6000, 20, 3, 128, False, True, True), (12000, 8, 8, 64, True, True, True)])  # more rows than the launch has workgroups for
 def test_norm_rotary_forward_and_backward(dtype, rows, H, HK, D, fp32, packed, turn):
     from flash_attn.rotary import apply_qk_norm_rotary
     eps = 1e-5
