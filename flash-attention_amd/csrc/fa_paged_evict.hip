@@ -166,6 +166,13 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
           }
         }
       }
+    } else if (kCap > 0) {
+      for (int q = tid * 4; q < L; q += kThreads * 4) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(keys + q);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (q + e < L && (k[e] >> (shift + bits)) == prefix) count((k[e] >> shift) & ((1 << bits) - 1));
+      }
     } else {
 #pragma unroll 4
       for (int j = tid; j < L; j += kThreads) {
@@ -227,38 +234,37 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
     __syncthreads();
     ties_end = (int)found[0];
   }
-  const auto stays = [&](int j, uint32_t k) { return k > edge || (k == edge && j < ties_end); };
-  int holes_here = 0, come_here = 0;
-  for (int j = j0 + lane; j < j1; j += 64) {
-    const bool stay = stays(j, key_of(j));
-    holes_here += !stay && j < p.budget;
-    come_here += stay && j >= p.budget;
-  }
-  holes_here = __builtin_amdgcn_readlane(wave_prefix_sum(holes_here), 63);
-  come_here = __builtin_amdgcn_readlane(wave_prefix_sum(come_here), 63);
-  __syncthreads();  // (the ties have been read)
-  if (lane == 0) {
-    sums[0][wave] = holes_here;
-    sums[1][wave] = come_here;
-  }
+  // A slot takes part in a move if it is below the budget and its key goes, or behind it and its key stays.  There are as many of the one kind as of the other, and
+  // all of the first come before the second: one count in slot order numbers both.
+  const auto moves_at = [&](int j) {
+    const uint32_t k = key_of(j);
+    return (k > edge || (k == edge && j < ties_end)) == (j >= p.budget);
+  };
+  int here = 0;
+#pragma unroll 4
+  for (int j = j0 + lane; j < j1; j += 64) here += moves_at(j);
+  here = __builtin_amdgcn_readlane(wave_prefix_sum(here), 63);
+  if (lane == 0) sums[1][wave] = here;
   __syncthreads();
   __shared__ int32_t own_moves[kMoveD > 0 ? 2 * kMovesPerGroup : 1];
   int32_t* const holes = kMoveD > 0 ? own_moves : p.moves + (int64_t)blockIdx.x * 2 * p.cap;
   const int cap = kMoveD > 0 ? kMovesPerGroup : p.cap;
-  int moves, all_come;
-  int hole = before_wave<kWaves>(sums[0], wave, &moves), come = before_wave<kWaves>(sums[1], wave, &all_come);
-  moves = moves < cap ? moves : cap;  // (as many as the cap, by its definition)
+  int all;
+  int rank = before_wave<kWaves>(sums[1], wave, &all);
+  const int moves = all / 2 < cap ? all / 2 : cap;  // (as many as the cap, by its definition)
   if (kMoveD == 0 && tid == 0) p.counts[blockIdx.x] = moves;
   for (int j = j0 + lane; j - lane < j1; j += 64) {
-    const bool in = j < j1;
-    const bool stay = in && stays(j, key_of(in ? j : j0));
-    const bool is_hole = in && !stay && j < p.budget, comes = stay && j >= p.budget;
-    const uint64_t hb = __ballot(is_hole), cb = __ballot(comes);
-    const int nh = hole + __popcll(hb & below), nc = come + __popcll(cb & below);
-    if (is_hole && nh < cap) holes[nh] = j;
-    if (comes && nc < cap) holes[cap + nc] = j;
-    hole += __popcll(hb);
-    come += __popcll(cb);
+    const bool one = j < j1 && moves_at(j);
+    const uint64_t ones = __ballot(one);
+    const int n = rank + __popcll(ones & below);
+    if (one) {
+      if (j < p.budget) {
+        if (n < cap) holes[n] = j;
+      } else if ((unsigned)(n - all / 2) < (unsigned)cap) {
+        holes[cap + n - all / 2] = j;
+      }
+    }
+    rank += __popcll(ones);
   }
   if constexpr (kMoveD > 0) {
     __shared__ MoveSpots spots;
