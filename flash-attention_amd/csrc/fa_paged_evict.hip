@@ -253,18 +253,18 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const EvictP
   int rank = before_wave<kWaves>(sums[1], wave, &all);
   const int moves = all / 2 < cap ? all / 2 : cap;  // (as many as the cap, by its definition)
   if (kMoveD == 0 && tid == 0) p.counts[blockIdx.x] = moves;
-  for (int j = j0 + lane; j - lane < j1; j += 64) {
-    const bool one = j < j1 && moves_at(j);
-    const uint64_t ones = __ballot(one);
-    const int n = rank + __popcll(ones & below);
-    if (one) {
-      if (j < p.budget) {
-        if (n < cap) holes[n] = j;
-      } else if ((unsigned)(n - all / 2) < (unsigned)cap) {
-        holes[cap + n - all / 2] = j;
-      }
+  constexpr int kAtOnce = 4;
+  for (int j = j0 + lane; j - lane < j1; j += 64 * kAtOnce) {
+    bool one[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; i++) one[i] = j + i * 64 < j1 && moves_at(j + i * 64);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; i++) {
+      const uint64_t ones = __ballot(one[i]);
+      const int at = j + i * 64, n = rank + __popcll(ones & below), to = at < p.budget ? n : n - all / 2;
+      if (one[i] && (unsigned)to < (unsigned)cap) holes[at < p.budget ? to : cap + to] = at;
+      rank += __popcll(ones);
     }
-    rank += __popcll(ones);
   }
   if constexpr (kMoveD > 0) {
     __shared__ MoveSpots spots;
