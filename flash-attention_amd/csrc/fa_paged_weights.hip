@@ -253,7 +253,7 @@ constexpr int few_resident(int D) { return 256 * (D == 128 ? 2 : 4); }
 }  // namespace
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) fa_paged_weights_few_kernel(const PagedFwdParams p) {
+__global__ void __launch_bounds__(256, D == 128 ? 2 : 4) fa_paged_weights_few_kernel(const PagedFwdParams p) {
   using C = FewCfg<D>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
