@@ -31,6 +31,8 @@ inline int check_paged_cache(const fa_paged_cache* c, bool needs_k, bool needs_v
   FA_REQUIRE(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0,
              "%s: page_size must be a power of two from 16 to 1024, got %d", name, c->page_size);
   FA_REQUIRE(c->batch > 0 && c->nheads_k > 0 && c->n_pages > 0 && c->table_cols > 0 && c->max_seqlen_k > 0, "%s: sizes must be positive", name);
+  const int64_t room = (int64_t)c->table_cols * c->page_size;
+  FA_REQUIRE((room < c->max_seqlen_k ? room : c->max_seqlen_k) <= ((int64_t)1 << 30), "%s: more than 2^30 keys of a sequence", name);  // (counted in 32 bits)
   FA_REQUIRE(c->nheads_k <= 65536 && c->batch <= (1 << 20) && (int64_t)c->batch * c->nheads_k < ((int64_t)1 << 24), "%s: too many sequences or heads", name);
   FA_REQUIRE(c->page_table && c->seqlens_k && c->table_row_stride >= c->table_cols, "%s: null pointer, or page table rows that overlap", name);
   FA_REQUIRE(((reinterpret_cast<uintptr_t>(c->page_table) | reinterpret_cast<uintptr_t>(c->seqlens_k) | reinterpret_cast<uintptr_t>(c->cu_seqlens_q) |

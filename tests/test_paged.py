@@ -194,7 +194,8 @@ ENTRY = {"norm": "fa_qk_norm_rotary", "append": "fa_paged_append", "fwd": "fa_pa
         ({"cache.max_seqlen_k": 0}, "positive"), ({"cache.page_table": None}, "null"), ({"cache.seqlens_k": None}, "null"), ({"cache.table_row_stride": 3}, "overlap"),
         ({"cache.seqlens_k": (1 << 20) + 2}, "4-byte"), ({"cache.k_cache": None}, "k_cache"), ({"cache.k_cache": (1 << 20) + 8}, "16-byte"),
         ({"cache.k_slot_stride": 60}, "multiples of 8"), ({"cache.k_slot_stride": 1 << 24}, "multiples of 8"), ({"cache.k_head_stride": -64}, "multiples of 8"),
-        ({"cache.k_page_stride": 4}, "multiples of 8")]
+        ({"cache.k_page_stride": 4}, "multiples of 8"),
+        ({"cache.page_size": 1024, "cache.table_cols": 1 << 21, "cache.table_row_stride": 1 << 21, "cache.max_seqlen_k": 2 ** 31 - 1}, "2^30 keys")]
 ] + [
     (k, *r) for k in ("append", "fwd", "weights") for r in [
         ({"cache.nheads_q": 3}, "multiple of nheads_k"), ({"cache.nheads_q": 4096}, "multiple of nheads_k"), ({"cache.cu_seqlens_q": None}, "cu_seqlens_q"),
