@@ -31,8 +31,8 @@ struct Cfg {
 }  // namespace
 
 // Waves per SIMD that registers are to allow: without a bound the compiler puts the products into accumulation registers and moves them out one by one (d = 64, 32 x 8
-// pairs of 4096 .. 16384 keys 135 us, with the bound 132; d = 32 75.6, 73.4).  At d = 128 LDS allows one, and it does so whatever is asked for.
-constexpr int decode_bound(int head_dim, int waves) { return head_dim == 128 || waves == 8 ? 2 : (head_dim == 64 ? 3 : 4); }
+// pairs of 4096 .. 16384 keys 135 us, with the bound 132; d = 32 75.6, 73.4).  At d = 128 LDS allows one.
+constexpr int decode_bound(int head_dim, int waves) { return head_dim == 128 ? 1 : (waves == 8 ? 2 : (head_dim == 64 ? 3 : 4)); }
 
 template <typename T, int D, int NW_>
 __global__ void __launch_bounds__(64 * NW_, decode_bound(D, NW_)) fa_paged_decode_kernel(const PagedFwdParams p) {
