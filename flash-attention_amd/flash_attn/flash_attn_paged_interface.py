@@ -17,6 +17,8 @@ lengths count as far as the table goes.  Pages that several sequences list (a co
 appended to, weighted or evicted from: the order in which several workgroups write one slot is not defined.  Keys and values behind a sequence's length are not
 read.  A value that is inf or NaN reaches every new token of its sequence that is handled together with one that sees it, as in the package's other
 attention functions: a weight of 0 does not cancel it."""
+from array import array
+
 import torch
 
 from . import flash_attn_gfx950 as _backend
@@ -125,7 +127,7 @@ class PagedKVCache:
     def add(self):
         """A new, empty sequence."""
         seq, self._next_id = self._next_id, self._next_id + 1
-        self._pages[seq], self._len[seq], self._seen[seq] = [], 0, 0
+        self._pages[seq], self._len[seq], self._seen[seq] = array("i"), 0, 0
         return seq
 
     def remove(self, seq):
@@ -145,8 +147,11 @@ class PagedKVCache:
 
     def _device_ints(self, *lists):
         """int32 tensors on the device, by way of one copy"""
-        flat = torch.tensor([x for l in lists for x in l], dtype=torch.int32)
-        flat = flat.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else flat
+        flat = array("i")
+        for l in lists:
+            flat.extend(l)
+        flat = torch.frombuffer(flat, dtype=torch.int32)
+        flat = flat.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else flat.clone()
         out, at = [], 0
         for l in lists:
             out.append(flat[at:at + len(l)])
@@ -193,7 +198,10 @@ class PagedKVCache:
 
     def _tables(self, seqs, *more):
         cols = max(1, max(len(self._pages[s]) for s in seqs))
-        rows = [p for s in seqs for p in self._pages[s] + [-1] * (cols - len(self._pages[s]))]
+        rows = array("i")
+        for s in seqs:
+            rows.extend(self._pages[s])
+            rows.extend(array("i", [-1]) * (cols - len(self._pages[s])))
         table, lens, seen, *rest = self._device_ints(rows, [self._len[s] for s in seqs], [self._seen[s] for s in seqs], *more)
         return (table.view(len(seqs), cols), lens, seen, *rest)
 
