@@ -471,6 +471,66 @@ def test_calls_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_calls_of_two_threads_on_their_own_streams():
+    """scratch belongs to a call: two threads' calls overlap and give what each gives alone"""
+    import threading
+    from flash_attn import flash_attn_paged_interface as p
+    jobs = []
+    for i, (lens, new) in enumerate((([9000, 5000, 100], 1), ([3000, 2500], 20))):
+        c = Cache(lens, 2, 64, 64, torch.float16, 30 + i).gpu()
+        q, cu = randn(len(lens) * new, 8, 64, seed=i).cuda(), cumulative([new] * len(lens)).cuda()
+        jobs.append(lambda q=q, c=c, cu=cu, new=new, n=max(lens): p.flash_attn_paged_func(q, c.dk, c.dv, c.dtable, cu, c.dlens, new, n))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(job, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [job() for _ in range(30)]
+            torch.cuda.current_stream().synchronize()
+        wrong.extend(i for i, x in enumerate(outs) if not torch.equal(x, want))
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(jobs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 30])
+def test_views_give_what_copies_give(new):
+    """queries, keys and values of a packed tensor, a page table inside a wider one, lengths and offsets inside longer tensors, pools inside larger ones"""
+    from flash_attn import flash_attn_paged_interface as p
+    got = []
+    for views in (False, True):
+        c = Cache([130, 90, 61], 2, 64, 32, torch.bfloat16, 8).gpu()
+        k, v, w, pos = c.dk.nan_to_num(0.5), c.dv.nan_to_num(0.25), c.dweights, c.dpositions
+        qkv = randn(3 * new, 8, 64, seed=2, dtype=torch.bfloat16).cuda()
+        q, kn, vn = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+        cu, table, lens = cumulative([new] * 3).cuda(), c.dtable, c.dlens
+        if views:
+            pools = torch.full((2, c.n_pages + 2, 3, 32, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+            pools[0, 1:-1, :2], pools[1, 1:-1, :2] = k.transpose(1, 2), v.transpose(1, 2)
+            k, v = (x[1:-1, :2].transpose(1, 2) for x in pools)
+            wide = torch.full((3, table.shape[1] + 5), 7, dtype=torch.int32, device="cuda")
+            wide[:, 2:-3] = table
+            table = wide[:, 2:-3]
+            lens, cu = torch.cat([lens[:1], lens, lens])[1:4], torch.cat([cu[:1], cu, cu])[1:5]
+        else:
+            q, kn, vn = q.contiguous(), kn.contiguous(), vn.contiguous()
+        q = p.paged_append_func(q, kn, vn, k, v, table, cu, lens, key_weights=w, key_positions=pos)
+        out, lse = p.flash_attn_paged_func(q, k, v, table, cu, lens, new, 130, return_softmax_lse=True)
+        p.paged_key_weights_func(q, lse, k, w, table, cu, lens, new, 130)
+        n = p.paged_evict_func(k, v, w, pos, table, lens, lens, 70, 8, 130)
+        got.append((q, out, lse[..., :new], k, v, w, pos, n))
+        if views:
+            assert (pools[:, :, 2] == 9).all() and (pools[:, 0] == 9).all() and (pools[:, -1] == 9).all()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 50])
 def test_a_cache_beyond_32_bit_offsets(new):
     """pages whose offsets pass 2^32 bytes (and 2^31 elements) give what pages at the front give"""
