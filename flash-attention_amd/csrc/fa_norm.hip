@@ -372,7 +372,7 @@ hipError_t launch_norm(const NormParams& p, int D, int blocks, bool bwd, hipStre
 #undef FA_NORM_D
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !bwd) return e;
-  const int parts = p.part[1].heads > 0 ? 2 : 1;
+  const int parts = p.part[1].dw != nullptr ? 2 : 1;  // (keys without heads: no workgroup, a gradient of zeros)
   hipLaunchKernelGGL(norm_weights_kernel<T>, dim3((unsigned)(parts * (D / 16))), dim3(1024), 0, stream, p, D);
   return hipGetLastError();
 }

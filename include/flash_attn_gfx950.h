@@ -329,7 +329,8 @@ int fa_token_positions(const int32_t* cu_seqlens, int32_t batch, int32_t total, 
  * strides.  weight_dtype: enum fa_dtype, or FA_FP32.  Tables as in fa_rotary, or both NULL (no rotation); t = positions[row], clamped to
  * the table, or row % seqlen.  rows_end: NULL, or an int32 in device memory (the last entry of a packed batch's cu_seqlens): rows from it on are
  * neither read nor written.  The backward takes q, k (as the forward read them) and dq_out, dk_out, and writes dq, dk (which may be dq_out,
- * dk_out with the same strides) and dq_weight, dk_weight ([head_dim], weight_dtype; summed in fp32 in a fixed order).  workspace: of
+ * dk_out with the same strides) and dq_weight, dk_weight ([head_dim], weight_dtype; summed in fp32 in a fixed order; of keys
+ * without heads: dk_weight, if given, becomes zeros).  workspace: of
  * fa_qk_norm_rotary_bwd_workspace_bytes() bytes, 16-byte aligned; the forward needs none. */
 #define FA_FP32 2 /* weights only */
 typedef struct fa_qk_norm_args {
