@@ -20,13 +20,18 @@ attention functions: a weight of 0 does not cancel it."""
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import flash_attn_gfx950 as _backend
 
 
-def _inference(*tensors):
+def _inference(*tensors, constants=()):
+    """constants: tensors that no gradient is formed of, but whose tangents would be lost just as well"""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("the paged cache has no backward: call it under torch.no_grad()")
+    # (a tangent is there under no_grad, too)
+    if torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (*tensors, *constants)):
+        raise RuntimeError("the paged cache has no derivative in forward mode")
 
 
 def paged_append_func(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, q_weight=None, k_weight=None, cos_half=None, sin_half=None,
@@ -41,7 +46,7 @@ def paged_append_func(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens
                                           key_weights, key_positions)
     if done is not None:
         return None if q is None else done
-    _inference(q, k, v, q_weight, k_weight)
+    _inference(q, k, v, q_weight, k_weight, constants=(k_cache, v_cache, cos_half, sin_half, key_weights))
     return _backend.paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, None, q_weight, k_weight, cos_half, sin_half, positions, eps,
                                  key_weights, key_positions)
 
@@ -71,7 +76,7 @@ def paged_key_weights_func(q, softmax_lse, k_cache, key_weights, page_table, cu_
     if _backend.passes().paged_key_weights(q, softmax_lse, k_cache, key_weights, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale,
                                            causal):
         return key_weights
-    _inference(q, k_cache)
+    _inference(q, k_cache, constants=(softmax_lse, key_weights))
     scale = q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale
     return _backend.paged_key_weights(q, softmax_lse, k_cache, key_weights, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal)
 
@@ -84,7 +89,7 @@ def paged_evict_func(k_cache, v_cache, key_weights, key_positions, page_table, s
     done = _backend.passes().paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k)
     if done is not None:
         return done
-    _inference(k_cache, v_cache)
+    _inference(k_cache, v_cache, constants=(key_weights,))
     return _backend.paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k)
 
 

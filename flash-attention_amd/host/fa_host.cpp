@@ -3,7 +3,7 @@
 //
 // Every check the Python binding makes is made here too, but nothing is reported: a call that fails one, or that is of a kind
 // handled there (probabilities returned, profiling events, a device that is not current, tensors without memory of their own such as those of
-// functorch and of fake-tensor tracing), returns None and the binding runs it - and raises what it has to.  What the library itself refuses
+// functorch and of fake-tensor tracing, tensors with a forward-mode tangent), returns None and the binding runs it - and raises what it has to.  What the library itself refuses
 // is raised here with the binding's text.
 //
 // Bound by the interpreter.  us with the binding's own calls / with these: one forward of 12 heads x 61 tokens (kernel 6) 21.4 / 14.2; training
@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/gil.h>
@@ -59,7 +60,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// A tensor argument; null for None.  ok is cleared for anything but a plain tensor (or parameter) with memory of its own.
+// A tensor argument; null for None.  ok is cleared for anything but a plain tensor (or parameter) with memory of its own, and where a tangent would be lost.
 const at::Tensor* tensor(PyObject* o, bool& ok) {
   if (o == Py_None) return nullptr;
   if (!THPVariable_Check(o)) {
@@ -70,6 +71,7 @@ const at::Tensor* tensor(PyObject* o, bool& ok) {
   constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchGradWrapper,
                                          c10::DispatchKey::FuncTorchBatched});
   if (!t.defined() || !t.has_storage() || t.key_set().has_any(wrapped) || t.layout() != at::kStrided) ok = false;
+  else if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined()) ok = false;
   return &t;
 }
 bool as_int(PyObject* o, int64_t* v) {  // a Python int (what int() of anything else gives is left to the binding)

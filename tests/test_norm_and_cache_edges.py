@@ -33,3 +33,55 @@ def test_keys_without_heads_leave_their_weight_a_gradient_of_zeros(fp32):
     got = torch.autograd.grad((q2, k2), (q, k, *w), (dq, torch.zeros_like(k2)))
     assert torch.equal(got[0], want[0]) and got[1].shape == k.shape and torch.equal(got[2], want[1])
     assert torch.equal(got[3], torch.zeros_like(got[3]))
+
+
+# ---- forward-mode tangents: nothing here has a rule for them
+
+def test_forward_tangents_are_refused_by_the_cache(lib):
+    """also under no_grad, which forward mode does not heed; a tensor whose tangents are switched off is a plain one (and refused for its device here)"""
+    from flash_attn import flash_attn_paged_interface as p
+    q, c = torch.zeros(3, 2, 64).half(), torch.zeros(4, 16, 2, 64).half()
+    i32, meta, lse = torch.zeros(2, dtype=torch.int32), torch.zeros(4, 2, 16), torch.zeros(1, 2, 16)
+    w = torch.ones(64).half()
+    with forward_ad.dual_level(), torch.no_grad():
+        d = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda q=q, k=q, v=q, w=w: p.paged_append_func(q, k, v, c, c, i32[:1, None], i32, i32[:1], w, w),
+                 lambda q=q, k=c, v=c: p.flash_attn_paged_func(q, k, v, i32[:1, None], i32, i32[:1], 3, 3),
+                 lambda q=q, l=lse, k=c: p.paged_key_weights_func(q, l, k, meta, i32[:1, None], i32, i32[:1], 3, 3),
+                 lambda k=c, v=c: p.paged_evict_func(k, v, meta, meta.int(), i32[:1, None], i32[:1], i32[:1], 2, 1, 3)]
+        for call in calls:
+            for i, t in enumerate(call.__defaults__):
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call(*call.__defaults__[:i], d(t))
+            with pytest.raises(RuntimeError, match="GPU"):
+                call()
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="GPU"):
+            calls[1](d(q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_tangents_do_not_pass_the_native_calls(lib, grad):
+    from flash_attn import flash_attn_paged_interface as p
+    from flash_attn.rotary import apply_qk_norm_rotary
+    c = Cache([20, 9], 2, 64, 16, torch.float16, 1).gpu()
+    q, cu = randn(3, 4, 64, seed=0).cuda(), cumulative([2, 1]).cuda()
+    w = torch.ones(64, dtype=torch.float16, device="cuda")
+    before = [t.clone() for t in (c.dk, c.dv, c.dweights, c.dpositions)]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        d = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        where = (c.dtable, cu, c.dlens)
+        out, lse = p.flash_attn_paged_func(q, c.dk, c.dv, *where, 2, 20, return_softmax_lse=True)
+        for args in ((d(q), q, w, w), (q, d(q), w, w), (q, q, d(w), w), (q, q, w, d(w)), (d(q)[:, :2], q, w, w)):
+            with pytest.raises(NotImplementedError):
+                apply_qk_norm_rotary(*args)
+        for call in (lambda: p.paged_append_func(d(q), q[:, :2], q[:, 2:], c.dk, c.dv, *where), lambda: p.paged_append_func(None, q[:, :2], d(q)[:, 2:], c.dk, c.dv, *where),
+                     lambda: p.paged_append_func(q, q[:, :2], q[:, 2:], c.dk, c.dv, *where, w, d(w)), lambda: p.flash_attn_paged_func(d(q), c.dk, c.dv, *where, 2, 20),
+                     lambda: p.flash_attn_paged_func(q, d(c.dk), c.dv, *where, 2, 20), lambda: p.paged_key_weights_func(d(q), lse, c.dk, c.dweights, *where, 2, 20),
+                     lambda: p.paged_evict_func(c.dk, d(c.dv), c.dweights, c.dpositions, c.dtable, c.dlens, c.dlens, 8, 2, 20)):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                call()
+        with forward_ad._set_fwd_grad_enabled(False):
+            assert torch.equal(p.flash_attn_paged_func(d(q), c.dk, c.dv, *where, 2, 20), out)
+    same = [torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(before, (c.dk, c.dv, c.dweights, c.dpositions))]
+    assert all(same)  # (nothing was stored)
