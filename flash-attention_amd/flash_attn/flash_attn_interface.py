@@ -200,6 +200,9 @@ class FlashAttnNormRotaryQKVPackedFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, cos_half, sin_half, cu_seqlens, max_seqlen, dropout_p, softmax_scale, causal, eps):
         _backend._check(qkv.is_cuda and qkv.dim() == 4 and qkv.shape[1] == 3, "qkv must be a (total, 3, nheads, headdim) GPU tensor")
+        # (positions are formed on the device, where the kernels clamp them to the tables)
+        if cos_half is not None and cos_half.shape[0] < int(max_seqlen):
+            raise RuntimeError("the tables have %d rows, the sequences up to %d positions" % (cos_half.shape[0], int(max_seqlen)))
         total = qkv.shape[0]
         positions = None if cos_half is None else _backend.token_positions(cu_seqlens, total)
         qk = torch.empty((total, 2) + tuple(qkv.shape[2:]), dtype=qkv.dtype, device=qkv.device)

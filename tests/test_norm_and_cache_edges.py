@@ -85,3 +85,19 @@ def test_forward_tangents_do_not_pass_the_native_calls(lib, grad):
             assert torch.equal(p.flash_attn_paged_func(d(q), c.dk, c.dv, *where, 2, 20), out)
     same = [torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(before, (c.dk, c.dv, c.dweights, c.dpositions))]
     assert all(same)  # (nothing was stored)
+
+
+# ---- rotation tables that end before the positions do
+
+@pytest.mark.gpu
+def test_attention_with_norm_refuses_tables_shorter_than_its_sequences():
+    from flash_attn.flash_attn_interface import flash_attn_unpadded_qkvpacked_norm_rotary_func as f
+    qkv, cu = randn(50, 3, 2, 64, seed=1).cuda(), cumulative([20, 30]).cuda()
+    w = torch.ones(64, dtype=torch.float16, device="cuda")
+    cos, sin = (t.cuda() for t in tables(30, 64, torch.float16))
+    want = f(qkv, w, w, cos, sin, cu, 30, 0.0, causal=True)
+    for rows, longest in ((29, 30), (1, 30), (30, 31)):
+        with pytest.raises(RuntimeError, match="rows"):
+            f(qkv, w, w, cos[:rows], sin[:rows], cu, longest, 0.0, causal=True)
+    longer = (t.cuda() for t in tables(64, 64, torch.float16))
+    assert torch.equal(f(qkv, w, w, *longer, cu, 30, 0.0, causal=True), want)
