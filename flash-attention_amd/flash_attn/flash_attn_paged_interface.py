@@ -38,7 +38,8 @@ def paged_append_func(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens
                       positions=None, eps=1e-6, key_weights=None, key_positions=None):
     """Stores the new tokens' k and v (total, nheads_k, headdim) into the pages of their sequences, behind what is there: row i of sequence b goes to
     slot seqlens_k[b] - (its new tokens) + i.  In the same pass k, and q (total, nheads, headdim) if it is given, are normalised (q_weight, k_weight: see
-    apply_qk_norm_rotary) and turned by their positions (cos_half, sin_half) - positions[row], or the slot.  Returns the new q, or None.
+    apply_qk_norm_rotary) and turned by their positions (cos_half, sin_half) - positions[row], or the slot, clamped to the tables: they are on the device, and what
+    the tables have to reach is the caller's to know (PagedStep does).  Returns the new q, or None.
     key_weights, key_positions (pages, nheads_k, page size): set to 0 and the position for the new tokens (for paged_key_weights_func and
     paged_evict_func).  Rows behind the last sequence, and tokens for which the page table has no room, are not stored; their rows of the returned q
     hold nothing."""
@@ -224,15 +225,18 @@ class PagedStep:
         self.page_table, self.seqlens_k, _, self.cu_seqlens, self.positions = cache._tables(seqs, ends, positions)
         self.total, self.max_seqlen_q = at, max(new)
         self.max_seqlen_k = max(cache._len[s] for s in seqs)
-        self.max_position = max(cache._seen[s] for s in seqs)
+        self.max_position = max(cache._seen[s] for s, n in zip(seqs, new) if n > 0)  # table rows that the new tokens' positions reach
 
     def append(self, layer, q, k, v, **norm_and_rotary):
         """paged_append_func into the layer's pages (q_weight, k_weight, cos_half, sin_half, eps); tokens are turned by their numbers in their sequences,
-        which go on where an eviction has cut the cache."""
+        which go on where an eviction has cut the cache: tables of max_position rows at least."""
         c = self.cache
         weights = (None, None) if c.key_weights is None else (c.key_weights[layer], c.key_positions[layer])
         if k.shape[0] != self.total:
             raise RuntimeError("the step has %d tokens, not %d" % (self.total, k.shape[0]))
+        cos = norm_and_rotary.get("cos_half")
+        if cos is not None and cos.shape[0] < self.max_position:  # (the kernels clamp positions to the tables: the keys would stay turned wrongly)
+            raise RuntimeError("the tables have %d rows, the step's tokens positions up to %d" % (cos.shape[0], self.max_position - 1))
         return paged_append_func(q, k, v, *c.layer(layer), self.page_table, self.cu_seqlens, self.seqlens_k,
                                  positions=self.positions, key_weights=weights[0], key_positions=weights[1],
                                  **norm_and_rotary)

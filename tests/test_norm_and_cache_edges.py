@@ -101,3 +101,24 @@ def test_attention_with_norm_refuses_tables_shorter_than_its_sequences():
             f(qkv, w, w, cos[:rows], sin[:rows], cu, longest, 0.0, causal=True)
     longer = (t.cuda() for t in tables(64, 64, torch.float16))
     assert torch.equal(f(qkv, w, w, *longer, cu, 30, 0.0, causal=True), want)
+
+
+def test_a_step_refuses_tables_that_its_positions_outgrow(lib):
+    """before anything is stored; sequences of the step without a new token do not count"""
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    c = PagedKVCache(1, 8, 16, 2, 64, device="cpu")
+    a, b = c.add(), c.add()
+    c.step([a], [40])
+    s = c.step([a, b], [0, 5])
+    assert s.max_position == 5
+    q = torch.zeros(5, 2, 64).half()
+    for rows in (1, 4):
+        with pytest.raises(RuntimeError, match="rows"):
+            s.append(0, q, q, q, **dict(zip(("cos_half", "sin_half"), tables(rows, 64, torch.float16))))
+    for rows in (5, 41):  # (long enough: what is refused is the host's tensors)
+        with pytest.raises(RuntimeError, match="GPU"):
+            s.append(0, q, q, q, **dict(zip(("cos_half", "sin_half"), tables(rows, 64, torch.float16))))
+    s = c.step([a, b], [1, 0])
+    assert s.max_position == 41
+    with pytest.raises(RuntimeError, match="rows"):
+        s.append(0, q[:1], q[:1], q[:1], **dict(zip(("cos_half", "sin_half"), tables(40, 64, torch.float16))))
