@@ -111,16 +111,42 @@ def apply_qk_norm_rotary(q, k, q_weight, k_weight, cos_half=None, sin_half=None,
     return _QkNormRotary.apply(_kernel_rows(q), _kernel_rows(k), q_weight, k_weight, cos_half, sin_half, positions, q.shape[0], eps)
 
 
+def _inverse_frequencies(dim, device=None):
+    return 1.0 / (10000 ** (torch.arange(0, dim, 2, device=device).float() / dim))
+
+
 class RotaryEmbedding(torch.nn.Module):
-    """Rotary embedding of RoFormer (Su et al., arXiv:2104.09864) for queries and keys."""
+    """Rotary embedding of RoFormer (Su et al., arXiv:2104.09864) for queries and keys.  Angles are formed in fp32 at least, also where .half() or .bfloat16()
+    have rounded the module's buffer of frequencies."""
 
     def __init__(self, dim_model: int, *_, **__):
         super().__init__()
-        exponent = torch.arange(0, dim_model, 2).float() / dim_model
-        self.register_buffer("inv_freq", 1.0 / (10000 ** exponent))
+        self.register_buffer("inv_freq", _inverse_frequencies(dim_model))
         self._seq_len_cached = None
         self._cos_cached = None
         self._sin_cached = None
+
+    def _apply(self, *args, **kwargs):
+        was = self.inv_freq.dtype
+        out = super()._apply(*args, **kwargs)
+        if was in (torch.float16, torch.bfloat16) and self.inv_freq.dtype != was:  # (back from 16 bits)
+            self.inv_freq = _inverse_frequencies(2 * self.inv_freq.numel(), "cpu").to(self.inv_freq)
+        self._frequencies(self.inv_freq.device)  # (made here and not at the first use, which a graph may capture)
+        return out
+
+    def _frequencies(self, device):
+        """The frequencies on `device` in fp32 or more: the buffer's, or, where that has been rounded to 16 bits, what it was made of"""
+        if self.inv_freq.dtype in (torch.float32, torch.float64):
+            return self.inv_freq.to(device)
+        have = getattr(self, "_wide_freq", None)
+        if have is None or have.device != device:
+            self._wide_freq = have = _inverse_frequencies(2 * self.inv_freq.numel(), "cpu").to(device)
+        return have
+
+    def _angles(self, positions, device):
+        """(positions, dim / 2): an angle for each position 0, 1, .. and each frequency"""
+        freq = self._frequencies(device)
+        return torch.outer(torch.arange(positions, device=device, dtype=freq.dtype), freq)
 
     def _update_cos_sin_tables(self, x, seq_dimension=-2):
         seq_len = x.shape[seq_dimension]
@@ -128,8 +154,7 @@ class RotaryEmbedding(torch.nn.Module):
                  or self._cos_cached.dtype != x.dtype)
         if stale:
             self._seq_len_cached = seq_len
-            pos = torch.arange(seq_len, device=x.device, dtype=self.inv_freq.dtype)
-            angles = torch.outer(pos, self.inv_freq.to(x.device))  # fp32 (seq, dim/2)
+            angles = self._angles(seq_len, x.device)
             self._cos_cached = torch.cos(angles).to(x.dtype).repeat_interleave(2, dim=-1)
             self._sin_cached = torch.sin(angles).to(x.dtype).repeat_interleave(2, dim=-1)
         return self._cos_cached, self._sin_cached
@@ -149,8 +174,7 @@ class RotaryEmbedding(torch.nn.Module):
         have = getattr(self, "_grown", None)
         if have is None or have[0].shape[0] < positions or have[0].device != like.device or have[0].dtype != like.dtype:
             rows = max(256, 1 << (max(int(positions), 1) - 1).bit_length())
-            pos = torch.arange(rows, device=like.device, dtype=self.inv_freq.dtype)
-            angles = torch.outer(pos, self.inv_freq.to(like.device))  # fp32, as in _update_cos_sin_tables
+            angles = self._angles(rows, like.device)  # as in _update_cos_sin_tables
             self._grown = have = (torch.cos(angles).to(like.dtype), torch.sin(angles).to(like.dtype))
         return have
 

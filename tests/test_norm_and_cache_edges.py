@@ -122,3 +122,57 @@ def test_a_step_refuses_tables_that_its_positions_outgrow(lib):
     assert s.max_position == 41
     with pytest.raises(RuntimeError, match="rows"):
         s.append(0, q[:1], q[:1], q[:1], **dict(zip(("cos_half", "sin_half"), tables(40, 64, torch.float16))))
+
+
+# ---- modules in 16 bits
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [16, 64, 128])
+def test_tables_of_a_module_in_16_bits_are_formed_in_32(dtype, dim):
+    """.half() and .bfloat16() round the buffer of frequencies too.  An angle is a position times a frequency: three roundings in fp32 (power, reciprocal, product) of at
+    most two steps each, so off by 6 * 2^-23 of itself; cosines by that, their own few steps, and one rounding."""
+    from flash_attn.rotary import RotaryEmbedding
+    N = 5000
+    plain = RotaryEmbedding(dim)
+    like = torch.zeros(1, N, 3, 1, dim, dtype=dtype)
+    emb = RotaryEmbedding(dim).to(dtype)
+    angle = torch.outer(torch.arange(N, dtype=torch.float64), 10000.0 ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim))
+    for got, same, exact in zip(emb.tables_to(N, like), emb.half_tables(like), (torch.cos(angle), torch.sin(angle))):
+        assert got.dtype == dtype and got.shape[0] >= N and torch.equal(got[:N], same)
+        assert ((got[:N].double() - exact).abs() <= half_step(dtype) + 6 * 2.0 ** -23 * angle + 2.0 ** -21).all()
+    # a module in 32 bits: what its buffer says, as before
+    want = torch.outer(torch.arange(N, dtype=torch.float32), plain.inv_freq)
+    assert torch.equal(plain.tables_to(N, like)[0][:N], torch.cos(want).to(dtype)) and torch.equal(plain.half_tables(like)[1], torch.sin(want).to(dtype))
+    back = RotaryEmbedding(dim).to(dtype).float()
+    assert torch.equal(back.inv_freq, plain.inv_freq) and back.inv_freq.dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_a_module_in_16_bits_serves_far_positions_as_one_in_32_bits_does():
+    """the same projections: a module made in fp16 (frequencies in fp32) and one turned to fp16, at positions beyond 2048"""
+    from flash_attn.flash_attention import FlashMHA
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    torch.manual_seed(2)
+    made = FlashMHA(128, 2, causal=True, use_rotary_emb="1d", device="cuda", dtype=torch.float16).eval()
+    turned = FlashMHA(128, 2, causal=True, use_rotary_emb="1d", device="cuda").half().eval()
+    turned.load_state_dict(made.state_dict())
+    x = torch.randn(2101, 128, device="cuda", dtype=torch.float16)
+    outs = []
+    with torch.no_grad():
+        for m in (made, turned):
+            cache = PagedKVCache(1, 140, 16, 2, 64)
+            seq = cache.add()
+            outs.append([m.forward_cached(x[a:b], cache.step([seq], [b - a])) for a, b in ((0, 2100), (2100, 2101))])
+        tables = [m.rotary_emb.tables_to(2101, x) for m in (made, turned)]
+        whole = [m(x[None], None, None)[0] for m in (made, turned)]
+    # the frequencies of both are fp32 numbers, at most two steps apart: angles by 2 * 2^-23 of themselves, and a rounding to 16 bits on each side
+    gap = 2 * half_step(torch.float16) + 2 * 2.0 ** -23 * 4096 + 2.0 ** -21
+    assert all((a.float() - b.float()).abs().max() <= gap for a, b in zip(*tables))
+    # a vector turned by tables off by g is off by at most 2 g of its length, a score by 4 g |q| |k| / 8, and an output by that (twice) of the largest value
+    with torch.no_grad():
+        qkv = (x.float() @ made.Wqkv.weight.float().t() + made.Wqkv.bias.float()).view(-1, 3, 2, 64)
+        size = qkv.norm(dim=-1).amax(0)  # (3, heads)
+        step = 2 * 4 * gap * (size[0] * size[1]).max().item() / 8 * qkv[:, 2].abs().max().item() + 6 * half_step(torch.float16) * qkv[:, 2].abs().max().item()
+        bound = made.out_proj.weight.float().abs().sum(1) * step + 1e-3
+    for a, b in zip(outs[0] + whole[:1], outs[1] + whole[1:]):
+        assert ((a.float() - b.float()).abs() <= bound).all()
