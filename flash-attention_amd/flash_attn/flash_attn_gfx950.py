@@ -463,6 +463,12 @@ def _raise(rc, lib):
     raise RuntimeError("flash_attn_gfx950 error %d: %s" % (rc, msg))
 
 
+def contiguous16(t):
+    """t, or a copy of it that is contiguous and lies where the kernels' 16-byte loads reach it: a gradient can be a piece of another tensor"""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _check_alibi(alibi_slopes, nheads, device, sparse):
     """alibi_slopes: None or nheads fp32 slopes on the tensors' device (an extension: the reference has no attention bias)."""
     if alibi_slopes is None:

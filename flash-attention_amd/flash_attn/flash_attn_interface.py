@@ -124,7 +124,7 @@ def _backward(ctx, dout):
         if cu_seqlens_q.numel() - 1 <= 65535 and q.shape[1] <= 65535:  # (the grid of the kernel that knows what was written)
             written = (cu_seqlens_q, cu_seqlens_k, q.shape[0], k.shape[0], ctx.causal)
         dbias = new_bias_grad(q, cu_seqlens_q.numel() - 1, ctx.max_seqlen_q, ctx.max_seqlen_k, cleared=written is None)
-    _flash_attn_backward(dout.contiguous(), q, k, v, out, softmax_lse, dq, dk, dv, cu_seqlens_q, cu_seqlens_k,
+    _flash_attn_backward(_backend.contiguous16(dout), q, k, v, out, softmax_lse, dq, dk, dv, cu_seqlens_q, cu_seqlens_k,
                          ctx.max_seqlen_q, ctx.max_seqlen_k, ctx.dropout_p, ctx.softmax_scale, ctx.causal,
                          ctx.alibi_slopes, keep_words, bias_t, dbias, ctx.rotary, philox)
     ctx.dbias = None

@@ -106,7 +106,7 @@ def _flash_blocksparse_attn_forward(qkv, cu_seqlens, blockmask, dropout_p, max_s
 def _flash_blocksparse_attn_backward(dout, qkv, out, S_dmask, softmax_lse, cu_seqlens, blockmask, dropout_p, max_s,
                                      softmax_scale, causal, alibi_slopes=None, attn_bias=None, dbias=None, gen=None, row_order=None):
     dqkv = torch.empty_like(qkv)
-    _backend.bwd_block(dout.contiguous(), qkv[:, 0], qkv[:, 1], qkv[:, 2], out, softmax_lse, dqkv[:, 0], dqkv[:, 1],
+    _backend.bwd_block(_backend.contiguous16(dout), qkv[:, 0], qkv[:, 1], qkv[:, 2], out, softmax_lse, dqkv[:, 0], dqkv[:, 1],
                        dqkv[:, 2], cu_seqlens, cu_seqlens, blockmask, max_s, max_s, dropout_p, softmax_scale, causal,
                        gen, row_order=row_order, alibi_slopes=alibi_slopes, attn_bias=attn_bias,
                        dbias=dbias)

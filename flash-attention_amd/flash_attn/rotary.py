@@ -44,7 +44,7 @@ class _ApplyRotaryQKV(torch.autograd.Function):
     def backward(ctx, grad):
         from . import flash_attn_gfx950 as backend
         cos_half, sin_half = ctx.saved_tensors
-        grad = grad.contiguous()
+        grad = backend.contiguous16(grad)
         return backend.rotary(grad, torch.empty_like(grad), cos_half, sin_half, n_rotated=2, conjugate=True), None, None
 
 
@@ -84,7 +84,7 @@ class _QkNormRotary(torch.autograd.Function):
 def _kernel_rows(t):
     """t as the kernels read a (rows, heads, headdim) tensor: itself, or a contiguous copy where its strides or its address are not theirs."""
     ok = t.stride(2) == 1 and all(0 <= s < 1 << 24 and s % 8 == 0 for s in t.stride()[:2]) and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)  # (contiguous() would hand back one whose address is the fault)
 
 
 def apply_qk_norm_rotary(q, k, q_weight, k_weight, cos_half=None, sin_half=None, positions=None, eps=1e-6):

@@ -134,8 +134,9 @@ struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
     const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3];
     Rows rq, rk, gq, gk;
     at::Tensor dqo = grads[0], dko = grads[1];
-    if (!rows_of(dqo, q, &gq)) dqo = dqo.contiguous();
-    if (!rows_of(dko, q, &gk)) dko = dko.contiguous();
+    // (a clone: contiguous() hands a contiguous tensor back whose address is the fault)
+    if (!rows_of(dqo, q, &gq)) dqo = dqo.clone(at::MemoryFormat::Contiguous);
+    if (!rows_of(dko, q, &gk)) dko = dko.clone(at::MemoryFormat::Contiguous);
     TORCH_CHECK(rows_of(q, q, &rq) && rows_of(k, q, &rk) && rows_of(dqo, q, &gq) && rows_of(dko, q, &gk), "apply_qk_norm_rotary: gradients of another dtype or device");
     at::Tensor dq = at::empty(q.sizes(), plain(q)), dk = at::empty(k.sizes(), plain(k)), dqw = at::empty(qw.sizes(), plain(qw)), dkw = at::empty(kw.sizes(), plain(kw));
     fa_qk_norm_args f;

@@ -176,3 +176,71 @@ def test_a_module_in_16_bits_serves_far_positions_as_one_in_32_bits_does():
         bound = made.out_proj.weight.float().abs().sum(1) * step + 1e-3
     for a, b in zip(outs[0] + whole[:1], outs[1] + whole[1:]):
         assert ((a.float() - b.float()).abs() <= bound).all()
+
+
+# ---- tensors at odd addresses
+
+def odd_address(t):
+    """the same values, contiguous, one element behind an aligned address"""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    flat[1:] = t.reshape(-1)
+    got = flat[1:].view(t.shape)
+    assert got.is_contiguous() and got.data_ptr() % 16
+    return got
+
+
+def test_rows_at_an_odd_address_are_copied_to_an_even_one():
+    from flash_attn.rotary import _kernel_rows
+    t = odd_address(randn(3, 2, 64, seed=0))
+    got = _kernel_rows(t)
+    assert got.data_ptr() % 16 == 0 and got.is_contiguous() and torch.equal(got, t)
+    view = randn(3, 4, 64, seed=1)[:, :2]
+    assert _kernel_rows(view) is view
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("four", [False, True])
+def test_norm_of_tensors_at_odd_addresses(four):
+    """as input (the Python function) and as incoming gradient (the native one, and Python's)"""
+    from flash_attn.rotary import apply_qk_norm_rotary
+    q, k = randn(6, 4, 64, seed=0).cuda(), randn(6, 2, 64, seed=1).cuda()
+    dq, dk = randn(6, 4, 64, seed=2).cuda(), randn(6, 2, 64, seed=3).cuda()
+    if four:
+        q, k, dq, dk = (t.view(2, 3, *t.shape[1:]) for t in (q, k, dq, dk))
+    w = torch.ones(64, dtype=torch.float16, device="cuda").requires_grad_()
+    cos, sin = (t.cuda() for t in tables(6, 64, torch.float16))
+
+    def step(q, k, dq, dk):
+        q, k = q.detach().requires_grad_(), k.detach().requires_grad_()
+        y = apply_qk_norm_rotary(q, k, w, w, cos, sin)
+        return y + torch.autograd.grad(y, (q, k, w), (dq, dk))
+
+    want = step(q, k, dq, dk)
+    for odd in ((0,), (1,), (2,), (3,), (0, 3), (2, 3)):
+        got = step(*(odd_address(t) if i in odd else t for i, t in enumerate((q, k, dq, dk))))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), odd
+    # a gradient as autograd makes it: a piece of a longer one
+    x, y = q.detach().requires_grad_(), k.detach().requires_grad_()
+    out = apply_qk_norm_rotary(x, y, w, w, cos, sin)
+    joined = torch.cat([torch.zeros(1, dtype=torch.float16, device="cuda"), out[0].flatten()])
+    up = torch.cat([torch.zeros(1, dtype=torch.float16, device="cuda"), dq.flatten()])
+    got = torch.autograd.grad((joined, out[1]), (x, y, w), (up, dk))
+    assert all(torch.equal(a, b) for a, b in zip(got, want[2:]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["plain", "rotary", "norm", "blocks"])
+def test_attention_takes_a_gradient_at_an_odd_address(which):
+    from flash_attn import flash_attn_interface as f
+    from flash_attn.flash_blocksparse_attn_interface import flash_blocksparse_attn_func
+    qkv, cu = randn(50, 3, 2, 64, seed=1).cuda().requires_grad_(), cumulative([20, 30]).cuda()
+    w = torch.ones(64, dtype=torch.float16, device="cuda")
+    cos, sin = (t.cuda() for t in tables(30, 64, torch.float16))
+    dout = randn(50, 2, 64, seed=2).cuda()
+    call = {"plain": lambda: f.flash_attn_unpadded_qkvpacked_func(qkv, cu, 30, 0.0, causal=True),
+            "blocks": lambda: flash_blocksparse_attn_func(qkv, cu, torch.ones(2, 1, device="cuda"), 0.0, 32),
+            "rotary": lambda: f.flash_attn_unpadded_qkvpacked_rotary_func(qkv, cos, sin, cu, 30, 0.0, causal=True),
+            "norm": lambda: f.flash_attn_unpadded_qkvpacked_norm_rotary_func(qkv, w, w, cos, sin, cu, 30, 0.0, causal=True)}[which]
+    want, = torch.autograd.grad(call(), qkv, dout)
+    got, = torch.autograd.grad(call(), qkv, odd_address(dout))
+    assert torch.equal(got, want)
