@@ -30,8 +30,10 @@
 // 100 MB.
 // The hand-over needs no atomics and no cache write-back: the key tiles of a (batch, head) run on one XCD (map_tile), whose L2
 // is the point of coherence for them.  Stores are complete (vmcnt) when the L2 has them; the counter is written after that;
-// the next owner reads counter and block with device-scope loads, which bypass its compute unit's L1.  Every workgroup checks
-// that it runs on the XCD its id implies (workgroup ids are dealt to the XCDs in turn) and poisons its dq with NaN if not.
+// the next owner reads counter and block with device-scope loads, which bypass its compute unit's L1.  Workgroup ids are dealt to the
+// XCDs in turn, from an XCD on that is the hardware queue's (measured: 0 in a process of one queue; 0, 7, 6, 5 on four queues of another, each constant
+// over its launches), so ids that are equal modulo 8 share one, whichever it is.  The counter carries its writer's XCD, and an owner on another poisons the
+// block with NaN.
 // A wave that waits for its turn gives up after a bounded number of polls and poisons its block with NaN: the grid always
 // drains, and a schedule that broke the assumptions above shows instead of hanging.  The front end only launches the kernel
 // when all key tiles of a (batch, head) fit one XCD at once with room to spare (fused_bwd_bytes in fa_api.hip).
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(256, 2) fa_bwd_fused_kernel(const BwdParams p)
   const int n0 = kt * BN;
   if (n0 >= Lk) return;
   const int nkt = (Lk + BN - 1) / BN, nqt = (Lq + BM - 1) / BM;  // key tiles that add to dQ, query tiles
-  const bool xcd_ok = xcc_id() == (int)(blockIdx.x & 7u);
+  const int xcc = xcc_id();
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(256, 2) fa_bwd_fused_kernel(const BwdParams p)
   int rel_mt = -1, rel_rank = 0;
   auto release = [&]() {  // the block's stores have been acknowledged: pass it on
     if (rel_mt < 0) return;
-    if (lane == 0) __hip_atomic_store(flagbase + rel_mt * 4, rel_rank + 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (lane == 0) __hip_atomic_store(flagbase + rel_mt * 4, (xcc << 16) | (rel_rank + 1), __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_WORKGROUP);
     rel_mt = -1;
   };
   auto load_sum = [&](int mt_) {
@@ -257,6 +259,8 @@ __global__ void __launch_bounds__(256, 2) fa_bwd_fused_kernel(const BwdParams p)
     for (int bq = 0; bq < 2; bq++)
       ld[bq] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(acc_rsrc, toff + bq * 1024, 0, 16));
   };
+
+  auto arrived = [&](int seen, int rank) { return (seen & 0xffff) >= rank; };  // (16 bits for the rank, the writer's XCD above them)
 
   int buf = 0;
   int mt = o_j, pend = -1;
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(256, 2) fa_bwd_fused_kernel(const BwdParams p)
           dq_pend[bq] = E::mfma16(bitcast<vec8>(u32x4{lo[0], lo[1], hi[0], hi[1]}), ktf[kk], dq_pend[bq]);
         }
       }
-      if (kMode == 0 && rank > 0 && !loaded && seen >= rank) {
+      if (kMode == 0 && rank > 0 && !loaded && arrived(seen, rank)) {
         load_sum(pend);
         loaded = true;
       }
@@ -359,11 +363,11 @@ __global__ void __launch_bounds__(256, 2) fa_bwd_fused_kernel(const BwdParams p)
       for (int bq = 0; bq < 2; bq++) *reinterpret_cast<f32x4*>(dst + bq * 1024) = dq_pend[bq];
     }
     if (pend >= 0 && kMode < 2) {
-      bool ok = xcd_ok;
+      bool ok = true;
       if (kMode == 0 && rank > 0 && !loaded) {  // its turn had not come at the top of the step
         int polls = 0;
 #pragma unroll 1
-        while (seen < rank) {
+        while (!arrived(seen, rank)) {
           if (++polls > kFusedPollLimit) { ok = false; break; }
           __builtin_amdgcn_s_sleep(2);
           seen = __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -371,10 +375,11 @@ __global__ void __launch_bounds__(256, 2) fa_bwd_fused_kernel(const BwdParams p)
         load_sum(pend);
       }
       if (kMode == 0 && rank > 0) {
+        ok = ok && seen >> 16 == xcc;
 #pragma unroll
         for (int bq = 0; bq < 2; bq++) dq_pend[bq] = dq_pend[bq] + ld[bq];
       }
-      if (!ok) {  // wrong XCD, or the block's turn never came
+      if (!ok) {  // handed over on another XCD, or the block's turn never came
 #pragma unroll
         for (int bq = 0; bq < 2; bq++)
 #pragma unroll
