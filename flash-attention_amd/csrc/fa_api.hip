@@ -506,7 +506,7 @@ int bwd_impl(const fa_bwd_args* a, bool want_block, void* ev_main_start = nullpt
 
   // the whole backward in one kernel, if the caller brought the scratch for it
   const size_t fused_need = fused_bwd_bytes(a);
-  if (fused_need > 0 && !a->dbias && a->workspace && a->workspace_bytes >= fused_need && aligned16(a->workspace)) {
+  if (fused_need > 0 && !a->dbias && a->workspace && a->workspace_bytes >= fused_need && aligned16(a->workspace) && fa::fused_bwd_possible(stream)) {
     p.nqt_ring = (a->max_seqlen_q + fa::kFusedBM - 1) / fa::kFusedBM;
     p.dq_acc = reinterpret_cast<float*>(a->workspace);
     p.dq_flags = reinterpret_cast<int*>(ws + (size_t)a->batch * a->nheads * p.nqt_ring * fa::kFusedBM * a->head_dim * 4);

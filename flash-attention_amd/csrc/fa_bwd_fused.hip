@@ -1,5 +1,12 @@
 // Launcher of the one-kernel backward (fa_bwd_fused_kernel.h): softmax_d pass (which also clears the hand-over counters),
 // then the kernel.
+//
+// A workgroup waits for others of its launch, so those have to find a place: one launch at a time on a device.  Two launches' workgroups leave each
+// other room (an XCD holds 64, and at most 31 of a launch wait for a pair of which a part has not begun), three do not: each would wait for what the others
+// keep out until its polls are used up, and poison its blocks.  A launch therefore waits for the one before it, whatever their streams; under capture, where that
+// is not known, the two-kernel backward runs.
+#include <mutex>
+
 #include "fa_bwd_fused_kernel.h"
 
 #ifdef FA_FUSED_EXPERIMENTS
@@ -41,10 +48,32 @@ hipError_t launch_fused_t(const BwdParams& p0, hipStream_t stream, hipEvent_t ev
 }
 }  // namespace
 
+namespace {
+constexpr int kMostDevices = 64;
+std::mutex g_in_turn;
+hipEvent_t g_last_done[kMostDevices];  // of a device's last launch; created with its first one and kept
+}  // namespace
+
+bool fused_bwd_possible(hipStream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &status) == hipSuccess) return status == hipStreamCaptureStatusNone;
+  (void)hipGetLastError();
+  return false;
+}
+
 hipError_t launch_bwd_fused(const BwdParams& p, int dtype, hipStream_t stream, hipEvent_t ev_start, hipEvent_t ev_stop) {
   if (p.B * p.H == 0) return hipSuccess;
-  if (dtype == 0) return launch_fused_t<_Float16>(p, stream, ev_start, ev_stop);
-  return launch_fused_t<__bf16>(p, stream, ev_start, ev_stop);
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  if (e != hipSuccess) return e;
+  if (device < 0 || device >= kMostDevices) return hipErrorInvalidDevice;
+  const std::lock_guard<std::mutex> lock(g_in_turn);
+  hipEvent_t& done = g_last_done[device];
+  if (done) e = hipStreamWaitEvent(stream, done, 0);
+  else e = hipEventCreateWithFlags(&done, hipEventDisableTiming);
+  if (e != hipSuccess) return e;
+  e = dtype == 0 ? launch_fused_t<_Float16>(p, stream, ev_start, ev_stop) : launch_fused_t<__bf16>(p, stream, ev_start, ev_stop);
+  return e != hipSuccess ? e : hipEventRecord(done, stream);
 }
 
 }  // namespace fa

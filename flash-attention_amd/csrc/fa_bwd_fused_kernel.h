@@ -36,7 +36,7 @@
 // block with NaN.
 // A wave that waits for its turn gives up after a bounded number of polls and poisons its block with NaN: the grid always
 // drains, and a schedule that broke the assumptions above shows instead of hanging.  The front end only launches the kernel
-// when all key tiles of a (batch, head) fit one XCD at once with room to spare (fused_bwd_bytes in fa_api.hip).
+// when all key tiles of a (batch, head) fit one XCD at once with room to spare (fused_bwd_bytes in fa_api.hip), one launch at a time (fa_bwd_fused.hip).
 #pragma once
 
 #include "fa_bwd_kernel.h"

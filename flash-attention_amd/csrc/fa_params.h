@@ -628,6 +628,7 @@ hipError_t launch_dq_combine(const BwdParams& p, int dtype, int head_dim, hipStr
 // The whole backward in one kernel (fa_bwd_fused_kernel.h; head_dim 64, dense, no mask, no dropout, no bias): softmax_d pass, then
 // the kernel.  ev_start / ev_stop: null, or events recorded around the main kernel.
 hipError_t launch_bwd_fused(const BwdParams& p, int dtype, hipStream_t stream, hipEvent_t ev_start, hipEvent_t ev_stop);
+bool fused_bwd_possible(hipStream_t stream);  // (not under capture)
 // fa_rotary: rotate the first n_rotated of n_parts (row, part, head, head_dim) slices, copy the others
 struct RotaryParams {
   const void* src;

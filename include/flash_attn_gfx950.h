@@ -469,7 +469,8 @@ int fa_blocksparse_row_order(const uint8_t* layout, int32_t n_row_blocks, int32_
  * short launches at head_dim 64 (few workgroups that find query rows), as one launch that holds both kinds of
  * workgroup, with bit-identical results; 0x10: always two launches; 0x20: one kernel
  * that also passes dQ from key tile to key tile through fp32 scratch, where it exists (head_dim 64, no blockmask, mask,
- * dropout or bias, max_seqlen_k <= 4096) and only if the caller brings the scratch fa_bwd_workspace_bytes() then asks for.
+ * dropout or bias, max_seqlen_k <= 4096) and only if the caller brings the scratch fa_bwd_workspace_bytes() then asks for
+ * (a process's launches of it take turns on a device; a call under stream capture runs the two kernels).
  * Bit 6 (0x40): at head_dim 128 without dropout, blockmask or bias the dK/dV kernel runs as wave pairs (one wave holds K and
  * owns dV, its partner holds V and owns dK; 64 keys per workgroup) instead of four waves with 32 keys each and V in LDS.
  * The defaults are the faster choices on the shapes measured; the others are kept for parts and shapes where the balance differs.

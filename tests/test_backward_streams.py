@@ -46,3 +46,39 @@ def test_one_kernel_backward_on_every_stream(dtype, lens_q, lens_k, H, one_kerne
     u = torch.finfo(dtype).eps / 2
     for a, b in zip(want, run()):
         assert (a.float() - b.float()).abs().max() <= 4 * u * b.float().abs().max()  # (a few fp32 sums in another order, and a rounding on each side)
+
+
+@pytest.mark.gpu
+def test_one_kernel_backwards_of_several_streams_take_turns(one_kernel):
+    """a launch's workgroups wait for each other and need places side by side: launches of more streams at once, 32 key tiles each, give what each gives alone"""
+    runs = [setup([256, 700], [4096, 3000], 8, seed=i) for i in range(5)]
+    want = [run() for run in runs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in runs], []
+    for _ in range(6):
+        for run, s in zip(runs, streams):
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for i, grads in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(grads, want[i % len(runs)])), i
+
+
+@pytest.mark.gpu
+def test_the_one_kernel_backward_is_not_captured(one_kernel):
+    """a graph's replays could not take their turn: it holds the two kernels"""
+    be = one_kernel
+    run = setup([300, 77], [300, 77], 3)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    be.set_launch_policy(0x10)
+    want = run()
+    for _ in range(3):
+        for t in got:
+            t.fill_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
