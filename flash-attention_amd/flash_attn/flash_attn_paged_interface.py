@@ -85,7 +85,7 @@ def paged_key_weights_func(q, softmax_lse, k_cache, key_weights, page_table, cu_
 def paged_evict_func(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k):
     """Cuts every sequence's cache to `budget` keys a head, in place, and returns the new lengths min(seqlens_k, budget).  Of a longer sequence stay
     the keys whose position is at least next_positions[b] - recent, and then those with the largest key_weights (NaN counts as -inf; ties: the lower
-    slot).  Each key head chooses for itself; a kept key from behind the budget takes the place, and the weight and position, of one that goes.  Slots
+    slot; of more than `budget` recent keys those in the lowest slots stay, whatever their positions).  Each key head chooses for itself; a kept key from behind the budget takes the place, and the weight and position, of one that goes.  Slots
     from `budget` on are left as they were.  next_positions: (batch,) int32, the position that each sequence's next token would have."""
     done = _backend.passes().paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k)
     if done is not None:
@@ -182,13 +182,14 @@ class PagedKVCache:
         return PagedStep(self, seqs, new, positions)
 
     def evict(self, seqs, budget, recent):
-        """Cuts the sequences to `budget` tokens a key head in every layer (paged_evict_func); pages that become empty are free again."""
+        """Cuts the sequences to `budget` tokens a key head in every layer, the `recent` newest among them (paged_evict_func); pages that become empty are free
+        again."""
         seqs = list(seqs)
         self._book(seqs)
         if self.key_weights is None:
             raise RuntimeError("eviction goes by key_weights: make the cache with key_weights=True")
-        if budget < 1 or recent < 0:
-            raise RuntimeError("budget must be positive, recent not negative")
+        if budget < 1 or recent < 0 or recent > budget:  # (of more recent keys than the budget the lowest slots' would stay, not the newest)
+            raise RuntimeError("budget must be positive, recent not negative and at most the budget")
         longest = max(self._len[s] for s in seqs)
         if longest <= budget:
             return

@@ -244,3 +244,18 @@ def test_attention_takes_a_gradient_at_an_odd_address(which):
     want, = torch.autograd.grad(call(), qkv, dout)
     got, = torch.autograd.grad(call(), qkv, odd_address(dout))
     assert torch.equal(got, want)
+
+
+# ---- the book
+
+def test_eviction_keeps_no_more_recent_keys_than_its_budget():
+    """the newest could not all stay, and the budget would go to the lowest slots: refused, whatever the lengths"""
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    c = PagedKVCache(1, 10, 16, 2, 64, device="cpu", key_weights=True)
+    a = c.add()
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="recent"):
+            c.evict([a], 30, 31)
+        c.evict([a], 41, 41)  # (nothing to cut)
+        c.step([a], [20])
+    assert c.length(a) == 40
