@@ -175,7 +175,9 @@ class RotaryEmbedding(torch.nn.Module):
         if have is None or have[0].shape[0] < positions or have[0].device != like.device or have[0].dtype != like.dtype:
             rows = max(256, 1 << (max(int(positions), 1) - 1).bit_length())
             angles = self._angles(rows, like.device)  # as in _update_cos_sin_tables
-            self._grown = have = (torch.cos(angles).to(like.dtype), torch.sin(angles).to(like.dtype))
+            have = (torch.cos(angles).to(like.dtype), torch.sin(angles).to(like.dtype))
+            if not (like.is_cuda and torch.cuda.is_current_stream_capturing()):  # (a graph's own: there is nothing in them before it is replayed)
+                self._grown = have
         return have
 
     def rotate_qkv_(self, qkv):

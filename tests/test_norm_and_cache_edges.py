@@ -246,6 +246,29 @@ def test_attention_takes_a_gradient_at_an_odd_address(which):
     assert torch.equal(got, want)
 
 
+# ---- the tables that a module keeps, and graphs
+
+@pytest.mark.gpu
+def test_tables_made_under_capture_are_the_graphs_own():
+    """a graph's memory holds nothing before its first replay: tables that a capture made are not handed to other calls"""
+    from flash_attn.rotary import RotaryEmbedding
+    like = torch.zeros(1, device="cuda", dtype=torch.float16)
+    want = RotaryEmbedding(64).cuda().tables_to(300, like)
+    emb = RotaryEmbedding(64).cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cos, sin = emb.tables_to(300, like)
+        out = cos + 0
+    got = emb.tables_to(300, like)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0])
+        assert torch.equal(emb.tables_to(300, like)[0], want[0])
+
+
 # ---- the book
 
 def test_eviction_keeps_no_more_recent_keys_than_its_budget():
