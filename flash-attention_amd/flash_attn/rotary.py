@@ -161,24 +161,25 @@ class RotaryEmbedding(torch.nn.Module):
 
     def half_tables(self, qkv):
         """(cos, sin) of shape (seqlen, headdim / 2) for a (batch, seqlen, 3, nheads, headdim) tensor: one entry per rotated
-        pair, the form the HIP kernels read.  Same values as forward()'s tables; kept until those change."""
-        cos, sin = self._update_cos_sin_tables(qkv[:, :, 0], seq_dimension=-3)
-        if getattr(self, "_half_of", None) is not cos:
-            self._half = (cos[:, ::2].contiguous(), sin[:, ::2].contiguous())
-            self._half_of = cos
+        pair, the form the HIP kernels read.  Same values as forward()'s tables."""
+        n, tables = qkv.shape[1], self.tables_to(qkv.shape[1], qkv)
+        if getattr(self, "_half_of", None) is not tables or self._half[0].shape[0] != n:
+            self._half, self._half_of = (tables[0][:n], tables[1][:n]), tables
         return self._half
 
     def tables_to(self, positions, like):
-        """(cos, sin) of shape (>= positions, headdim / 2) in `like`'s dtype on its device: tables that grow (to a power of two of rows) and are kept, for
-        positions that grow from call to call."""
-        have = getattr(self, "_grown", None)
-        if have is None or have[0].shape[0] < positions or have[0].device != like.device or have[0].dtype != like.dtype:
+        """(cos, sin) of shape (>= positions, headdim / 2) in `like`'s dtype on its device: tables that grow (to a power of two of rows), for
+        positions that grow from call to call.  Those they outgrow are kept, too (all together as many rows again): graphs that read them may be replayed."""
+        loaded = 0 if self.inv_freq.is_inference() else self.inv_freq._version  # (load_state_dict() may bring other frequencies)
+        kept = self.__dict__.setdefault("_tables", {}).setdefault((like.device, like.dtype, loaded), [])
+        if not kept or kept[-1][0].shape[0] < positions:
             rows = max(256, 1 << (max(int(positions), 1) - 1).bit_length())
             angles = self._angles(rows, like.device)  # as in _update_cos_sin_tables
             have = (torch.cos(angles).to(like.dtype), torch.sin(angles).to(like.dtype))
-            if not (like.is_cuda and torch.cuda.is_current_stream_capturing()):  # (a graph's own: there is nothing in them before it is replayed)
-                self._grown = have
-        return have
+            if like.is_cuda and torch.cuda.is_current_stream_capturing():  # (a graph's own: there is nothing in them before it is replayed)
+                return have
+            kept.append(have)
+        return kept[-1]
 
     def rotate_qkv_(self, qkv):
         """q and k of a packed (batch, seqlen, 3, nheads, headdim) GPU tensor rotated in place (one HIP kernel); returns

@@ -143,7 +143,11 @@ def test_tables_of_a_module_in_16_bits_are_formed_in_32(dtype, dim):
     # a module in 32 bits: what its buffer says, as before
     want = torch.outer(torch.arange(N, dtype=torch.float32), plain.inv_freq)
     assert torch.equal(plain.tables_to(N, like)[0][:N], torch.cos(want).to(dtype)) and torch.equal(plain.half_tables(like)[1], torch.sin(want).to(dtype))
+    other = {"inv_freq": plain.inv_freq / 2}
+    plain.load_state_dict(other)
+    assert torch.equal(plain.half_tables(like)[0], torch.cos(want / 2).to(dtype))
     back = RotaryEmbedding(dim).to(dtype).float()
+    plain = RotaryEmbedding(dim)
     assert torch.equal(back.inv_freq, plain.inv_freq) and back.inv_freq.dtype == torch.float32
 
 
@@ -267,6 +271,49 @@ def test_tables_made_under_capture_are_the_graphs_own():
         torch.cuda.synchronize()
         assert torch.equal(out, want[0])
         assert torch.equal(emb.tables_to(300, like)[0], want[0])
+
+
+@pytest.mark.gpu
+def test_tables_that_a_graph_reads_outlive_their_growth():
+    from flash_attn.rotary import RotaryEmbedding
+    like = torch.zeros(1, device="cuda", dtype=torch.float16)
+    emb = RotaryEmbedding(64).cuda()
+    want = [t.clone() for t in emb.tables_to(300, like)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cos, sin = emb.tables_to(300, like)
+        out = cos + sin
+    for n in (600, 5000):
+        assert emb.tables_to(n, like)[0].shape[0] >= n
+        emb.tables_to(n, like.bfloat16())
+        fresh = [torch.full_like(want[0], math.nan) for _ in range(64)]  # (the memory of tensors that are gone)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0] + want[1])
+        del fresh
+    assert emb.tables_to(300, like)[0] is emb.tables_to(4000, like)[0]
+
+
+@pytest.mark.gpu
+def test_half_tables_that_a_graph_reads_outlive_those_of_other_lengths():
+    from flash_attn.rotary import RotaryEmbedding
+    emb = RotaryEmbedding(64).cuda()
+    x = [torch.zeros(1, n, 3, 1, 64, device="cuda", dtype=torch.float16) for n in (300, 301, 40, 5000)]
+    want = [t.clone() for t in emb.half_tables(x[0])]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cos, sin = emb.half_tables(x[0])
+        out = cos + sin
+    for y in x[1:]:
+        assert [t.shape[0] for t in emb.half_tables(y)] == [y.shape[1]] * 2
+        fresh = [torch.full_like(want[0], math.nan) for _ in range(64)]  # (the memory of tensors that are gone)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0] + want[1])
+        del fresh
+    # the values of forward()'s tables
+    cos, sin = emb._update_cos_sin_tables(x[3][:, :, 0], seq_dimension=-3)
+    assert all(torch.equal(a, b[:, ::2]) for a, b in zip(emb.half_tables(x[3]), (cos, sin)))
 
 
 # ---- the book
