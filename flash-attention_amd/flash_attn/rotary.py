@@ -111,6 +111,13 @@ def apply_qk_norm_rotary(q, k, q_weight, k_weight, cos_half=None, sin_half=None,
     return _QkNormRotary.apply(_kernel_rows(q), _kernel_rows(k), q_weight, k_weight, cos_half, sin_half, positions, q.shape[0], eps)
 
 
+_SHORT = (torch.float16, torch.bfloat16)
+
+
+def _version(t):
+    return 0 if t.is_inference() else t._version
+
+
 def _inverse_frequencies(dim, device=None):
     return 1.0 / (10000 ** (torch.arange(0, dim, 2, device=device).float() / dim))
 
@@ -127,21 +134,35 @@ class RotaryEmbedding(torch.nn.Module):
         self._sin_cached = None
 
     def _apply(self, *args, **kwargs):
-        was = self.inv_freq.dtype
+        values, wide, was_short = self._values(), self._frequencies(self.inv_freq.device), self.inv_freq.dtype in _SHORT
         out = super()._apply(*args, **kwargs)
-        if was in (torch.float16, torch.bfloat16) and self.inv_freq.dtype != was:  # (back from 16 bits)
-            self.inv_freq = _inverse_frequencies(2 * self.inv_freq.numel(), "cpu").to(self.inv_freq)
-        self._frequencies(self.inv_freq.device)  # (made here and not at the first use, which a graph may capture)
+        if wide.is_meta or self.inv_freq.is_meta:
+            return out
+        if self.inv_freq.dtype in _SHORT:
+            self._wide_freq, self._wide_of = wide.to(self.inv_freq.device), values
+        elif was_short:  # (back from 16 bits)
+            self.inv_freq = wide.to(self.inv_freq)
+        self._seen = (self.inv_freq, _version(self.inv_freq))  # (moved or cast: the same values)
         return out
 
+    def _values(self):
+        """A number for the values of the buffer: another one when it has been loaded or set"""
+        seen = self.__dict__.get("_seen")
+        if seen is None or seen[0] is not self.inv_freq or seen[1] != _version(self.inv_freq):
+            self._seen = (self.inv_freq, _version(self.inv_freq))
+            self._count = self.__dict__.get("_count", 0) + 1
+        return self._count
+
     def _frequencies(self, device):
-        """The frequencies on `device` in fp32 or more: the buffer's, or, where that has been rounded to 16 bits, what it was made of"""
-        if self.inv_freq.dtype in (torch.float32, torch.float64):
-            return self.inv_freq.to(device)
-        have = getattr(self, "_wide_freq", None)
-        if have is None or have.device != device:
-            self._wide_freq = have = _inverse_frequencies(2 * self.inv_freq.numel(), "cpu").to(device)
-        return have
+        """The frequencies on `device` in fp32 or more: the buffer's, or, where that has been rounded to 16 bits, what was rounded"""
+        freq = self.inv_freq
+        if freq.dtype not in _SHORT or freq.is_meta:
+            return freq.to(device)
+        if self.__dict__.get("_wide_of") != self._values():  # (loaded, or cast past the module: the usual ones rounded, or others)
+            wide = _inverse_frequencies(2 * freq.numel(), "cpu").to(freq.device)
+            usual = torch.allclose(freq.float(), wide, rtol=torch.finfo(freq.dtype).eps, atol=0.0)
+            self._wide_freq, self._wide_of = wide if usual else freq.float(), self._values()
+        return self._wide_freq.to(device)
 
     def _angles(self, positions, device):
         """(positions, dim / 2): an angle for each position 0, 1, .. and each frequency"""
@@ -151,9 +172,9 @@ class RotaryEmbedding(torch.nn.Module):
     def _update_cos_sin_tables(self, x, seq_dimension=-2):
         seq_len = x.shape[seq_dimension]
         stale = (seq_len != self._seq_len_cached or self._cos_cached.device != x.device
-                 or self._cos_cached.dtype != x.dtype)
+                 or self._cos_cached.dtype != x.dtype or self.__dict__.get("_cached_values") != self._values())
         if stale:
-            self._seq_len_cached = seq_len
+            self._seq_len_cached, self._cached_values = seq_len, self._values()
             angles = self._angles(seq_len, x.device)
             self._cos_cached = torch.cos(angles).to(x.dtype).repeat_interleave(2, dim=-1)
             self._sin_cached = torch.sin(angles).to(x.dtype).repeat_interleave(2, dim=-1)
@@ -170,8 +191,7 @@ class RotaryEmbedding(torch.nn.Module):
     def tables_to(self, positions, like):
         """(cos, sin) of shape (>= positions, headdim / 2) in `like`'s dtype on its device: tables that grow (to a power of two of rows), for
         positions that grow from call to call.  Those they outgrow are kept, too (all together as many rows again): graphs that read them may be replayed."""
-        loaded = 0 if self.inv_freq.is_inference() else self.inv_freq._version  # (load_state_dict() may bring other frequencies)
-        kept = self.__dict__.setdefault("_tables", {}).setdefault((like.device, like.dtype, loaded), [])
+        kept = self.__dict__.setdefault("_tables", {}).setdefault((like.device, like.dtype, self._values()), [])
         if not kept or kept[-1][0].shape[0] < positions:
             rows = max(256, 1 << (max(int(positions), 1) - 1).bit_length())
             angles = self._angles(rows, like.device)  # as in _update_cos_sin_tables

@@ -3,6 +3,7 @@ bits, tensors at odd addresses, tables and steps under capture.
 
 Tolerances are counted: u is half a step of the element type, 2^-24 a rounding in fp32."""
 import math
+import pickle
 
 import pytest
 import torch
@@ -149,6 +150,34 @@ def test_tables_of_a_module_in_16_bits_are_formed_in_32(dtype, dim):
     back = RotaryEmbedding(dim).to(dtype).float()
     plain = RotaryEmbedding(dim)
     assert torch.equal(back.inv_freq, plain.inv_freq) and back.inv_freq.dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_other_frequencies_stay_through_16_bits(dtype):
+    """loaded before a cast: not rounded at all; loaded into a module in 16 bits: as they were loaded"""
+    from flash_attn.rotary import RotaryEmbedding
+    like, other = torch.zeros(1, 9, 3, 1, 64), RotaryEmbedding(64).inv_freq * 0.3
+    emb = RotaryEmbedding(64)
+    emb.half_tables(like), emb(like[:, :, 0], like[:, :, 0], seq_dimension=-3)
+    emb.load_state_dict({"inv_freq": other})
+    want = torch.cos(torch.outer(torch.arange(9.0), other))
+    assert torch.equal(emb._update_cos_sin_tables(like[:, :, 0], seq_dimension=-3)[0][:, ::2], want)
+    assert torch.equal(emb.to(dtype).half_tables(like)[0], want) and torch.equal(emb.to(dtype).cpu().half_tables(like)[0], want)
+    assert torch.equal(emb.float().inv_freq, other) and torch.equal(emb.half_tables(like)[0], want)
+    emb = RotaryEmbedding(64).to(dtype)
+    emb.half_tables(like)
+    emb.load_state_dict({"inv_freq": other})
+    want = torch.cos(torch.outer(torch.arange(9.0), other.to(dtype).float()))
+    assert torch.equal(emb.half_tables(like)[0], want) and torch.equal(emb.float().inv_freq, other.to(dtype).float())
+    emb.inv_freq = RotaryEmbedding(64).inv_freq
+    assert torch.equal(emb.half_tables(like)[0], RotaryEmbedding(64).half_tables(like)[0])
+    copy = pickle.loads(pickle.dumps(RotaryEmbedding(64).to(dtype)))
+    assert torch.equal(copy.half_tables(like)[0], RotaryEmbedding(64).half_tables(like)[0])
+    with torch.device("meta"):
+        emb = RotaryEmbedding(64).to(dtype)
+    emb = emb.to_empty(device="cpu")
+    emb.load_state_dict(RotaryEmbedding(64).to(dtype).state_dict())
+    assert torch.equal(emb.half_tables(like)[0], RotaryEmbedding(64).half_tables(like)[0])
 
 
 @pytest.mark.gpu
