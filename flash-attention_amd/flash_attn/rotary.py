@@ -198,6 +198,8 @@ class RotaryEmbedding(torch.nn.Module):
             have = (torch.cos(angles).to(like.dtype), torch.sin(angles).to(like.dtype))
             if like.is_cuda and torch.cuda.is_current_stream_capturing():  # (a graph's own: there is nothing in them before it is replayed)
                 return have
+            if like.is_cuda:  # (the next call may be on another stream; they grow a few times in a process)
+                torch.cuda.current_stream(like.device).synchronize()
             kept.append(have)
         return kept[-1]
 

@@ -345,6 +345,25 @@ def test_half_tables_that_a_graph_reads_outlive_those_of_other_lengths():
     assert all(torch.equal(a, b[:, ::2]) for a, b in zip(emb.half_tables(x[3]), (cos, sin)))
 
 
+@pytest.mark.gpu
+def test_tables_made_on_one_stream_are_whole_on_another():
+    from flash_attn.rotary import RotaryEmbedding
+    like = torch.zeros(1, device="cuda", dtype=torch.float16)
+    want = RotaryEmbedding(128).cuda().tables_to(1 << 16, like)
+    emb = RotaryEmbedding(128).cuda()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    x = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        for _ in range(20):
+            x = x @ x * 1e-3  # (work in front of the tables)
+        emb.tables_to(1 << 16, like)
+    with torch.cuda.stream(b):
+        got = [t.clone() for t in emb.tables_to(1 << 16, like)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 # ---- the book
 
 def test_eviction_keeps_no_more_recent_keys_than_its_budget():
