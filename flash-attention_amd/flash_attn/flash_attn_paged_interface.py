@@ -8,8 +8,8 @@ theirs in a page table.
     cu_seqlens_q       (batch + 1,) int32: where each sequence's new tokens begin in the packed (total, heads, headdim) tensors
 
 A step of a model advances seqlens_k by the new tokens once; every layer then stores them (paged_append_func) and attends
-(flash_attn_paged_func).  Nothing here waits for the GPU or reads its memory on the host: calls can be captured into a graph, whose replays
-find new lengths, tables and tokens in the same tensors.  max_seqlen_k then has to hold for all of them; it bounds the work
+(flash_attn_paged_func).  Nothing here waits for the GPU or reads its memory on the host: the functions' calls can be captured into a graph, whose replays
+find new lengths, tables and tokens in the same tensors (PagedKVCache's book is the host's: its steps are made, and its evictions called, outside).  max_seqlen_k then has to hold for all of them; it bounds the work
 that is cut, not the memory that is read.
 
 What lies in page_table and seqlens_k is never trusted with an address: entries outside the pool are read as its first or last page and never written to,
@@ -164,8 +164,13 @@ class PagedKVCache:
             at += len(l)
         return out
 
+    def _not_under_capture(self, what):
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("%s is made of the host's numbers, which a graph's replays would not find again: not while a stream is captured" % what)
+
     def step(self, seqs, new_tokens):
         """Makes room for new_tokens[i] further tokens of seqs[i] and returns the PagedStep that stores them and attends."""
+        self._not_under_capture("a step")
         seqs, new = list(seqs), [int(n) for n in new_tokens]
         self._book(seqs)
         if len(new) != len(seqs) or min(new) < 0 or sum(new) == 0:
@@ -184,6 +189,7 @@ class PagedKVCache:
     def evict(self, seqs, budget, recent):
         """Cuts the sequences to `budget` tokens a key head in every layer, the `recent` newest among them (paged_evict_func); pages that become empty are free
         again."""
+        self._not_under_capture("an eviction of whole sequences")
         seqs = list(seqs)
         self._book(seqs)
         if self.key_weights is None:

@@ -364,6 +364,23 @@ def test_tables_made_on_one_stream_are_whole_on_another():
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.gpu
+def test_steps_and_evictions_are_not_made_under_capture():
+    """their numbers are the host's: a replay would find those of another step"""
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    cache = PagedKVCache(1, 8, 16, 2, 64, key_weights=True)
+    seq = cache.add()
+    cache.step([seq], [40])
+    graph, y = torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.step([seq], [1]), lambda: cache.evict([seq], 20, 2)):
+            with pytest.raises(RuntimeError, match="captur"):
+                call()
+        y += 1
+    assert cache.length(seq) == 40 and cache.free_pages() == 5
+    assert cache.step([seq], [1]).seqlens_k.tolist() == [41]
+
+
 # ---- the book
 
 def test_eviction_keeps_no_more_recent_keys_than_its_budget():
