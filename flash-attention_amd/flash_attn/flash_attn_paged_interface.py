@@ -234,13 +234,16 @@ class PagedStep:
         self.max_seqlen_k = max(cache._len[s] for s in seqs)
         self.max_position = max(cache._seen[s] for s, n in zip(seqs, new) if n > 0)  # table rows that the new tokens' positions reach
 
+    def _own(self, t):
+        if t.shape[0] != self.total:
+            raise RuntimeError("the step has %d tokens, not %d" % (self.total, t.shape[0]))
+
     def append(self, layer, q, k, v, **norm_and_rotary):
         """paged_append_func into the layer's pages (q_weight, k_weight, cos_half, sin_half, eps); tokens are turned by their numbers in their sequences,
         which go on where an eviction has cut the cache: tables of max_position rows at least."""
         c = self.cache
         weights = (None, None) if c.key_weights is None else (c.key_weights[layer], c.key_positions[layer])
-        if k.shape[0] != self.total:
-            raise RuntimeError("the step has %d tokens, not %d" % (self.total, k.shape[0]))
+        self._own(k)
         cos = norm_and_rotary.get("cos_half")
         if cos is not None and cos.shape[0] < self.max_position:  # (the kernels clamp positions to the tables: the keys would stay turned wrongly)
             raise RuntimeError("the tables have %d rows, the step's tokens positions up to %d" % (cos.shape[0], self.max_position - 1))
@@ -250,6 +253,7 @@ class PagedStep:
 
     def attend(self, layer, q, softmax_scale=None):
         """flash_attn_paged_func over the layer's pages, causal; a cache with key_weights counts what its keys receive"""
+        self._own(q)
         c = self.cache
         k, v = c.layer(layer)
         where = (self.page_table, self.cu_seqlens, self.seqlens_k, self.max_seqlen_q, self.max_seqlen_k, softmax_scale)

@@ -394,3 +394,14 @@ def test_eviction_keeps_no_more_recent_keys_than_its_budget():
         c.evict([a], 41, 41)  # (nothing to cut)
         c.step([a], [20])
     assert c.length(a) == 40
+
+
+def test_a_step_attends_with_its_own_number_of_tokens(lib):
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    c = PagedKVCache(1, 10, 16, 2, 64, device="cpu")
+    s = c.step([c.add()], [5])
+    for n in (4, 6, 0):
+        with pytest.raises(RuntimeError, match="5 tokens"):
+            s.attend(0, torch.zeros(n, 2, 64).half())
+    with pytest.raises(RuntimeError, match="GPU"):
+        s.attend(0, torch.zeros(5, 2, 64).half())
