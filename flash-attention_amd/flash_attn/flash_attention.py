@@ -27,6 +27,8 @@ class FlashAttention(nn.Module):
         attention_dropout: dropout probability applied to the attention weights while training (default 0.0)
     """
 
+    dtypes = (torch.float16,)  # the reference's module restriction (:41); the functional API takes bf16, too, and so does qk_norm
+
     def __init__(self, softmax_scale=None, attention_dropout=0.0, device=None, dtype=None):
         super().__init__()
         self.softmax_scale = softmax_scale
@@ -47,7 +49,7 @@ class FlashAttention(nn.Module):
         Returns (output, None); output has the layout of the input's token dimensions."""
         assert not need_weights
         assert attn_mask is None
-        assert qkv.dtype == torch.float16  # the reference's module restriction (:41); the functional API takes bf16 too
+        assert qkv.dtype in self.dtypes or (qk_norm is not None and qkv.dtype == torch.bfloat16)
         assert qkv.is_cuda
         p = self.dropout_p if self.training else 0.0
 
@@ -102,7 +104,8 @@ class FlashAttention(nn.Module):
 
 class FlashMHA(nn.Module):
     """Multi-head self-attention block: fused QKV projection, FlashAttention, output projection.
-    qk_norm (not in the reference): queries and keys are normalised head by head, with learned weights, in front of the rotation."""
+    qk_norm (not in the reference): queries and keys are normalised head by head, with learned weights, in front of the rotation; fp16 or
+    bf16 then, else forward() takes fp16, as the reference's does."""
 
     def __init__(self, embed_dim, num_heads, bias=True, batch_first=True, attention_dropout=0.0, causal=False,
                  use_rotary_emb=None, device=None, dtype=None, qk_norm=False, **kwargs) -> None:
@@ -126,6 +129,8 @@ class FlashMHA(nn.Module):
             self.k_norm_weight = nn.Parameter(torch.ones(self.head_dim, **factory_kwargs))
         self.Wqkv = nn.Linear(embed_dim, 3 * embed_dim, bias=bias, **factory_kwargs)
         self.inner_attn = FlashAttention(attention_dropout=attention_dropout, **factory_kwargs)
+        if qk_norm:  # (whose queries and keys reach it normalised where there is a mask: in bf16 as forward_cached() takes them)
+            self.inner_attn.dtypes = (torch.float16, torch.bfloat16)
         self.out_proj = nn.Linear(embed_dim, embed_dim, bias=bias, **factory_kwargs)
 
     def forward(self, x, x_ignored_, x_ignored_1_, attn_mask=None, key_padding_mask=None, need_weights=False):

@@ -405,3 +405,42 @@ def test_a_step_attends_with_its_own_number_of_tokens(lib):
             s.attend(0, torch.zeros(n, 2, 64).half())
     with pytest.raises(RuntimeError, match="GPU"):
         s.attend(0, torch.zeros(5, 2, 64).half())
+
+
+# ---- the module in bf16
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [None, "1d", "2d"])
+@pytest.mark.parametrize("padded", [False, True])
+def test_mha_with_norm_in_bf16(rotary, padded):
+    """what forward_cached() serves, forward() runs and trains: against the definition in 64 bits from the module's own projections"""
+    from flash_attn.flash_attention import FlashMHA
+    torch.manual_seed(0)
+    m = FlashMHA(128, 4, causal=rotary != "2d", use_rotary_emb=rotary, qk_norm=True, device="cuda", dtype=torch.bfloat16)
+    x = torch.randn(2, 49, 128, device="cuda", dtype=torch.bfloat16)
+    keep = torch.ones(2, 49, dtype=torch.bool, device="cuda")
+    mask = None
+    if padded:
+        keep[1, 30:] = False
+        mask = type("Mask", (), {"bool_matrix": keep})
+    y, _ = m(x, None, None, key_padding_mask=mask)
+    y.float().square().sum().backward()
+    assert y.dtype == torch.bfloat16 and all(p.grad is not None and p.grad.isfinite().all() and p.grad.abs().sum() > 0 for p in m.parameters())
+    with torch.no_grad():
+        qkv = m.Wqkv(x).reshape(2, 49, 3, 4, 32)
+        q, k = (t / (t.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt() for t in (qkv[:, :, 0].double(), qkv[:, :, 1].double()))
+        if rotary:
+            q, k = m.rotary_emb(q, k, seq_dimension=-3)
+        s = (q.transpose(1, 2) @ k.permute(0, 2, 3, 1).contiguous()) * 32 ** -0.5
+        s = s.masked_fill(~keep[:, None, None, :], -math.inf)
+        if m.causal:
+            s = s.masked_fill(torch.ones(49, 49, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+        v = qkv[:, :, 2].double().transpose(1, 2).contiguous()
+        ctx = (torch.softmax(s, -1) @ v).transpose(1, 2).reshape(2, 49, 128)
+        want = ctx @ m.out_proj.weight.double().t() + m.out_proj.bias.double()
+        # q and k: one rounding of the norm (2d: and one of each turn), tables rounded (2 u of a vector): 6 u of |q| |k| = 32 in a score, times the scale; attention
+        # rounds probabilities and its result; the projection rounds once
+        u = half_step(torch.bfloat16)
+        vmax = v.abs().max().item()
+        bound = m.out_proj.weight.double().abs().sum(1) * vmax * (2 * 2 * 6 * u * 32 * 32 ** -0.5 + 4 * u) + u * want.abs() + 1e-3
+        assert ((y.double() - want).abs() <= bound)[keep].all()
