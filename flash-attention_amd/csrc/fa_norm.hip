@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(1024) norm_weights_kernel(const NormParams p, 
 
 // How the launches are cut.  The workgroups of both parts, shared by their sizes, walk on over the rows: as many as give a compute unit about 20 waves in the
 // forward and 16 in the backward (whose workgroups each leave a row of sums, too).  us of the forward with four workgroups a compute unit whatever their size / so: 32768
-// rows of 16 + 4 heads, d = 128 71.6 / 67.9 (4.9 TB/s; a workgroup for every four rows 85.8), 16000 of 32 + 8 (eight waves a workgroup) 91 / 77, 65536 of 2 x 12,
+// rows of 16 + 4 heads, d = 128 71.6 / 67.9 (a workgroup for every four rows 85.8; as it is now 63, 5.4 TB/s), 16000 of 32 + 8 (eight waves a workgroup) 91 / 77, 65536 of 2 x 12,
 // d = 64 86.5 / 78.4, 24000 of 2 x 12 63 / 55; with 24 waves 69.8, -, 77.5, 53.8.  Backward, 16 waves / 20: 64000 rows of 2 x 8 heads, d = 32 48 / 63, 11200 of
 // 2 x 20, d = 128 74 / 100, 48000 of 24 + 8, d = 64 118 / 141, the others alike.
 constexpr int kForwardWaves = 20, kBackwardWaves = 16;

@@ -1,5 +1,5 @@
 // fa_paged_append: the new tokens' k and v go into their sequences' pages, k (and q, into q_out) normalised and turned on the way (fa_norm.h).
-// HBM-bound for prompts (each vector read once, written once: 4.4 TB/s, of 5.3 that a copy reaches; without norm and rotation 5.1), whose workgroups
+// HBM-bound for prompts (each vector read once, written once: 4.5 TB/s, of 5.3 that a copy reaches; without norm and rotation 5.1), whose workgroups
 // walk over the rows; for a decode step's few rows bound by latency: the row's sequence, its
 // length, its page and the store depend on each other, so the rows are loaded before any of them is asked for, and a wave finds a row's sequence
 // with one load and a ballot for 64 sequences.

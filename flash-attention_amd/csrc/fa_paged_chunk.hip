@@ -43,7 +43,7 @@ FA_DEVICE int longest_sequence(const PagedCache& c, int rank) {
 
 // Workgroup id -> (sequence, key head, row tile).  Ids go to the eight XCDs in turn; the tiles of a pair should run on one of them, side by side, since
 // they read the same keys, and the longest sequences should begin first.  With pairs enough (p.deal) those are dealt to the XCDs one by one, longest
-// sequences first: 4 sequences of 4096 .. 8192 keys, 8 key heads, 1024 new tokens each, d = 128 417 us, in contiguous pieces, which give an XCD
+// sequences first: 4 sequences of 4096 .. 8192 keys, 8 key heads, 1024 new tokens each, d = 128 421 us (to 429 on other boxes), in contiguous pieces, which give an XCD
 // one sequence's heads, 516.  Few pairs: each XCD takes a contiguous piece of the line of all tiles.  Tiles of a pair from the last (longest walk under the mask) on.
 FA_DEVICE bool place(const PagedFwdParams& p, int id, int* b, int* h, int* tile) {
   const int pairs = p.c.B * p.c.HK, x = id & 7, j = id >> 3;

@@ -24,7 +24,7 @@ struct EvictParams {
   int32_t* moves;           // [B * HK][2][cap]: holes, keys that come
 };
 
-constexpr int kEvictThreads = 1024;  // (8 x 8 heads of 4915 .. 16384 keys, the whole operator 60.5 us; 512 threads 67.8)
+constexpr int kEvictThreads = 1024;  // (8 x 8 heads of 4915 .. 16384 keys to 4096, two caches in turn, the copies of weights and positions that a pass begins with included: 60.1 us; 512 threads 67.2)
 constexpr uint32_t kNewest = 0xffffffffu;
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
@@ -35,7 +35,8 @@ FA_DEVICE uint32_t ordered(float w) {
 }
 
 // Copies `moves` (at most kMovesPerGroup) of a head's keys and values: first where each comes from and goes to, into LDS, then 16 bytes a thread at a time,
-// four of them in flight (8 x 8 heads cut from 4915 .. 16384 keys to 4096, d = 128, 149 MB: the whole operator 60.5 us, with two 61.6, with eight 95.9).
+// four of them in flight (8 x 8 heads cut from 4915 .. 16384 keys to 4096, d = 128, 149 MB: the pass of above 60.1 us, with two 60.9,
+// with eight 95.4; as the case of perf/operators.py is timed 62.9).
 constexpr int kMovesPerGroup = 64;
 struct MoveSpots {
   int64_t at[kMovesPerGroup][4];  // k from, k to (negative: nowhere), v from, v to: bytes

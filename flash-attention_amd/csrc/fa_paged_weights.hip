@@ -5,8 +5,8 @@
 // Two kernels.  Few rows (at most 32 a key head; a decode step): K streams past them, bound by HBM; waves stage 32-key tiles of their own as in
 // fa_paged_decode.hip, over the same line of units.  Many: a workgroup takes one unit of that line (the launch's last ones find none), a wave owns 32 of its keys, their fragments in registers, and streams the rows past them in tiles of 64
 // or 128 that the workgroup's four waves share through LDS; bound by vector instructions, three per 64 scores (4 sequences of 2000 .. 4001 keys, 8 key
-// heads, 2 x 509 rows, d = 64: 29.6 us, 78 % of the loaded SIMDs' issue; one unit a workgroup by number instead of by the line 34, since a compute unit then
-// has up to four workgroups of long sequences and another two).  Both form S = Q K^T, which leaves a key in a lane, so
+// heads, 2 x 509 rows, d = 64: 26 us, vector instructions in 55 % of all SIMDs' cycles; one unit a workgroup by number instead of by the line 34, when this took
+// 29.6, since a compute unit then has up to four workgroups of long sequences and another two).  Both form S = Q K^T, which leaves a key in a lane, so
 // that its sum stays in the lane and has one owner.
 #include <type_traits>
 
