@@ -183,16 +183,17 @@ class RotaryEmbedding(torch.nn.Module):
     def half_tables(self, qkv):
         """(cos, sin) of shape (seqlen, headdim / 2) for a (batch, seqlen, 3, nheads, headdim) tensor: one entry per rotated
         pair, the form the HIP kernels read.  Same values as forward()'s tables."""
-        n, tables = qkv.shape[1], self.tables_to(qkv.shape[1], qkv)
-        if getattr(self, "_half_of", None) is not tables or self._half[0].shape[0] != n:
-            self._half, self._half_of = (tables[0][:n], tables[1][:n]), tables
-        return self._half
+        n, tables, half = qkv.shape[1], self.tables_to(qkv.shape[1], qkv), self.__dict__.get("_half")
+        if half is None or half[0] is not tables or half[1] != n:
+            self._half = half = (tables, n, (tables[0][:n], tables[1][:n]))  # (in one piece: other threads may ask for other lengths)
+        return half[2]
 
     def tables_to(self, positions, like):
         """(cos, sin) of shape (>= positions, headdim / 2) in `like`'s dtype on its device: tables that grow (to a power of two of rows), for
         positions that grow from call to call.  Those they outgrow are kept, too (all together as many rows again): graphs that read them may be replayed."""
         kept = self.__dict__.setdefault("_tables", {}).setdefault((like.device, like.dtype, self._values()), [])
-        if not kept or kept[-1][0].shape[0] < positions:
+        have = kept[-1] if kept else None
+        if have is None or have[0].shape[0] < positions:
             rows = max(256, 1 << (max(int(positions), 1) - 1).bit_length())
             angles = self._angles(rows, like.device)  # as in _update_cos_sin_tables
             have = (torch.cos(angles).to(like.dtype), torch.sin(angles).to(like.dtype))
@@ -201,7 +202,7 @@ class RotaryEmbedding(torch.nn.Module):
             if like.is_cuda:  # (the next call may be on another stream; they grow a few times in a process)
                 torch.cuda.current_stream(like.device).synchronize()
             kept.append(have)
-        return kept[-1]
+        return have
 
     def rotate_qkv_(self, qkv):
         """q and k of a packed (batch, seqlen, 3, nheads, headdim) GPU tensor rotated in place (one HIP kernel); returns

@@ -211,6 +211,27 @@ def test_a_module_in_16_bits_serves_far_positions_as_one_in_32_bits_does():
         assert ((a.float() - b.float()).abs() <= bound).all()
 
 
+def test_tables_of_two_threads():
+    """threads that ask one module for tables of different lengths get theirs"""
+    import threading
+    from flash_attn.rotary import RotaryEmbedding
+    emb, wrong = RotaryEmbedding(16), []
+
+    def ask(lengths):
+        x = {n: torch.zeros(1, n, 1, 1, 16) for n in lengths}
+        for _ in range(300):
+            for n in lengths:
+                if emb.half_tables(x[n])[0].shape[0] != n or emb.tables_to(n, x[n])[0].shape[0] < n:
+                    wrong.append(n)
+
+    threads = [threading.Thread(target=ask, args=(n,)) for n in ((3, 300, 5000), (7, 900), (2000, 20000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 # ---- tensors at odd addresses
 
 def odd_address(t):
