@@ -171,14 +171,18 @@ class RotaryEmbedding(torch.nn.Module):
 
     def _update_cos_sin_tables(self, x, seq_dimension=-2):
         seq_len = x.shape[seq_dimension]
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():  # (a graph's own: those that are kept go with the next length)
+            return self._cos_sin(seq_len, x)
         stale = (seq_len != self._seq_len_cached or self._cos_cached.device != x.device
                  or self._cos_cached.dtype != x.dtype or self.__dict__.get("_cached_values") != self._values())
         if stale:
             self._seq_len_cached, self._cached_values = seq_len, self._values()
-            angles = self._angles(seq_len, x.device)
-            self._cos_cached = torch.cos(angles).to(x.dtype).repeat_interleave(2, dim=-1)
-            self._sin_cached = torch.sin(angles).to(x.dtype).repeat_interleave(2, dim=-1)
+            self._cos_cached, self._sin_cached = self._cos_sin(seq_len, x)
         return self._cos_cached, self._sin_cached
+
+    def _cos_sin(self, seq_len, x):
+        angles = self._angles(seq_len, x.device)
+        return tuple(f(angles).to(x.dtype).repeat_interleave(2, dim=-1) for f in (torch.cos, torch.sin))
 
     def half_tables(self, qkv):
         """(cos, sin) of shape (seqlen, headdim / 2) for a (batch, seqlen, 3, nheads, headdim) tensor: one entry per rotated
@@ -261,14 +265,20 @@ class RotaryEmbedding2D(torch.nn.Module):
         assert seqlen == side * side
         grid = qkv[:, :side, 0, :, :qkv.shape[-1] // 2]  # (b, side, nheads, headdim / 2): `side` positions per axis
         cos, sin = self.rotary_emb1d._update_cos_sin_tables(grid, seq_dimension=-3)
-        key = (b, side, qkv.device)
-        if self._pos_cached is None or self._pos_cached[0] != key:
-            tok = torch.arange(seqlen, device=qkv.device, dtype=torch.int32)
+        return _ApplyRotaryQKV2D.apply(qkv, cos[:, ::2].contiguous(), sin[:, ::2].contiguous(), *self._grid_positions(b, side, qkv))
+
+    def _grid_positions(self, b, side, qkv):
+        """(column, row) of every token of b grids"""
+        key, have = (b, side, qkv.device), self._pos_cached
+        capturing = qkv.is_cuda and torch.cuda.is_current_stream_capturing()
+        if capturing or have is None or have[0] != key:
+            tok = torch.arange(side * side, device=qkv.device, dtype=torch.int32)
             col = (tok % side).repeat(b).contiguous()
             row = torch.div(tok, side, rounding_mode="floor").to(torch.int32).repeat(b).contiguous()
-            self._pos_cached = (key, col, row)
-        _, col, row = self._pos_cached
-        return _ApplyRotaryQKV2D.apply(qkv, cos[:, ::2].contiguous(), sin[:, ::2].contiguous(), col, row)
+            have = (key, col, row)
+            if not capturing:  # (a graph's own, as in RotaryEmbedding)
+                self._pos_cached = have
+        return have[1:]
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, seq_dimension=-2):
         assert seq_dimension in [-2, -3]

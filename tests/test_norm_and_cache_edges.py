@@ -367,6 +367,38 @@ def test_half_tables_that_a_graph_reads_outlive_those_of_other_lengths():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["2d", "1d", "elementwise"])
+@pytest.mark.parametrize("warm", [False, True])
+def test_rotations_in_a_graph_and_beside_it(kind, warm):
+    """captured before or after the module has tables, replayed behind eager calls of other lengths: the graph and the eager calls give what a new module gives"""
+    from flash_attn.rotary import RotaryEmbedding, RotaryEmbedding2D
+    make = lambda: (RotaryEmbedding2D if kind == "2d" else RotaryEmbedding)(64).cuda()  # noqa: E731
+
+    def turn(emb, x):
+        if kind == "elementwise":
+            return torch.stack([*emb(x[:, :, 0], x[:, :, 1], seq_dimension=-3), x[:, :, 2]], 2)
+        return emb.rotate_qkv_(x.clone())
+
+    x = {n: randn(2, n, 3, 2, 64, seed=n).cuda() for n in (49, 64, 2025)}
+    want = {n: turn(make(), t) for n, t in x.items()}
+    emb, still = make(), x[49].clone()
+    if warm:
+        turn(emb, x[49])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = turn(emb, still)
+    assert torch.equal(turn(emb, x[49]), want[49])
+    for n in (64, 2025, 49):
+        assert torch.equal(turn(emb, x[n]), want[n])
+        fresh = [torch.full((m,), math.nan, device="cuda", dtype=torch.float16) for m in (64, 98, 1568, 3136, 6272) * 16]  # (the memory of tensors that are gone)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[49])
+        del fresh
+
+
+@pytest.mark.gpu
 def test_tables_made_on_one_stream_are_whole_on_another():
     from flash_attn.rotary import RotaryEmbedding
     like = torch.zeros(1, device="cuda", dtype=torch.float16)
