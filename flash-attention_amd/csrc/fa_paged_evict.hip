@@ -24,7 +24,8 @@ struct EvictParams {
   int32_t* moves;           // [B * HK][2][cap]: holes, keys that come
 };
 
-constexpr int kEvictThreads = 1024;  // (8 x 8 heads of 4915 .. 16384 keys to 4096, two caches in turn, the copies of weights and positions that a pass begins with included: 60.1 us; 512 threads 67.2)
+// (8 x 8 heads of 4915 .. 16384 keys to 4096, two caches in turn, the copies of weights and positions that a pass begins with included: 60.1 us; 512 threads 67.2)
+constexpr int kEvictThreads = 1024;
 constexpr uint32_t kNewest = 0xffffffffu;
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 

@@ -9,8 +9,8 @@ theirs in a page table.
 
 A step of a model advances seqlens_k by the new tokens once; every layer then stores them (paged_append_func) and attends
 (flash_attn_paged_func).  Nothing here waits for the GPU or reads its memory on the host: the functions' calls can be captured into a graph, whose replays
-find new lengths, tables and tokens in the same tensors (PagedKVCache's book is the host's: its steps are made, and its evictions called, outside).  max_seqlen_k then has to hold for all of them; it bounds the work
-that is cut, not the memory that is read.
+find new lengths, tables and tokens in the same tensors (PagedKVCache's book is the host's: its steps are made, and its evictions called, outside).
+max_seqlen_k then has to hold for all of them; it bounds the work that is cut, not the memory that is read.
 
 What lies in page_table and seqlens_k is never trusted with an address: entries outside the pool are read as its first or last page and never written to,
 lengths count as far as the table goes.  Pages that several sequences list (a common prompt), or one lists twice, may be read by all of them and must not be
@@ -85,8 +85,8 @@ def paged_key_weights_func(q, softmax_lse, k_cache, key_weights, page_table, cu_
 def paged_evict_func(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k):
     """Cuts every sequence's cache to `budget` keys a head, in place, and returns the new lengths min(seqlens_k, budget).  Of a longer sequence stay
     the keys whose position is at least next_positions[b] - recent, and then those with the largest key_weights (NaN counts as -inf; ties: the lower
-    slot; of more than `budget` recent keys those in the lowest slots stay, whatever their positions).  Each key head chooses for itself; a kept key from behind the budget takes the place, and the weight and position, of one that goes.  Slots
-    from `budget` on are left as they were.  next_positions: (batch,) int32, the position that each sequence's next token would have."""
+    slot; of more than `budget` recent keys those in the lowest slots stay, whatever their positions).  Each key head chooses for itself; a kept key
+    from behind the budget takes the place, and the weight and position, of one that goes.  Slots from `budget` on are left as they were.  next_positions: (batch,) int32, the position that each sequence's next token would have."""
     done = _backend.passes().paged_evict(k_cache, v_cache, key_weights, key_positions, page_table, seqlens_k, next_positions, budget, recent, max_seqlen_k)
     if done is not None:
         return done
