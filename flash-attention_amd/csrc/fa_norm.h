@@ -30,6 +30,19 @@ FA_DEVICE float vector_sum(float x) {
   return x;
 }
 
+// ... and the largest of values that are numbers
+template <int CH>
+FA_DEVICE float vector_max(float x) {
+  const auto other = [](float v, auto ctrl) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  x = fmaxf(x, other(x, std::integral_constant<int, 0xB1>{}));
+  if constexpr (CH >= 4) x = fmaxf(x, other(x, std::integral_constant<int, 0x4E>{}));
+  if constexpr (CH >= 8) x = fmaxf(x, other(x, std::integral_constant<int, 0x141>{}));
+  if constexpr (CH >= 16) x = fmaxf(x, other(x, std::integral_constant<int, 0x140>{}));
+  return x;
+}
+
 template <typename T>
 FA_DEVICE void load_weights(const void* w, bool fp32, int ch, float (&out)[8]) {
 #pragma unroll

@@ -22,10 +22,17 @@ struct PagedCache {
   int total_q, max_sq;
   float* weights;      // [n_pages][HK][page size]
   int32_t* positions;
+  // a cache in 8 bits (fa_paged_8bit.h): the rows' exponents, [n_pages][HK][page size]
+  uint8_t* k_exps;
+  uint8_t* v_exps;
+  // sequences that share a prefix (fa_paged_fwd.h): how many keys of each
+  const int32_t* prefix;
+  int max_prefix;
 };
 
-// Everything about a cache's tensors that the entry points have in common.  needs_v / needs_q: whether v_cache / cu_seqlens_q are used.
-inline int check_paged_cache(const fa_paged_cache* c, bool needs_k, bool needs_v, bool needs_q, const char* name) {
+// Everything about a cache's tensors that the entry points have in common.  needs_v / needs_q: whether v_cache / cu_seqlens_q are used.  scales: of a cache
+// in 8 bits, or null.
+inline int check_paged_cache(const fa_paged_cache* c, bool needs_k, bool needs_v, bool needs_q, const char* name, const fa_paged_scales* scales = nullptr) {
   FA_REQUIRE(c->head_dim == 16 || c->head_dim == 32 || c->head_dim == 64 || c->head_dim == 128, "%s: head_dim must be 16, 32, 64 or 128, got %d", name,
              c->head_dim);
   FA_REQUIRE(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0,
@@ -44,6 +51,14 @@ inline int check_paged_cache(const fa_paged_cache* c, bool needs_k, bool needs_v
     FA_REQUIRE(c->total_q >= 0 && c->max_seqlen_q > 0 && (int64_t)c->max_seqlen_q * (c->nheads_q / c->nheads_k) < ((int64_t)1 << 30), "%s: bad number of new tokens", name);
   }
   const auto page_ok = [](int64_t s) { return s % 8 == 0 && s >= 0 && s < ((int64_t)1 << 40); };
+  if (scales) {
+    FA_REQUIRE(scales->struct_bytes == sizeof(fa_paged_scales), "%s: scales' struct size mismatch", name);
+    FA_REQUIRE((!needs_k || (scales->k_scales && aligned16(scales->k_scales))) && (!needs_v || (scales->v_scales && aligned16(scales->v_scales))),
+               "%s: k_scales and v_scales must be there and 16-byte aligned", name);
+    FA_REQUIRE((!needs_k || (c->k_page_stride % 16 == 0 && c->k_slot_stride % 16 == 0 && c->k_head_stride % 16 == 0)) &&
+                   (!needs_v || (c->v_page_stride % 16 == 0 && c->v_slot_stride % 16 == 0 && c->v_head_stride % 16 == 0)),
+               "%s: the strides of a cache in 8 bits must be multiples of 16 elements", name);
+  }
   if (needs_k)
     FA_REQUIRE(c->k_cache && aligned16(c->k_cache) && page_ok(c->k_page_stride) && stride_ok(c->k_slot_stride) && stride_ok(c->k_head_stride),
                "%s: k_cache must be 16-byte aligned, its strides multiples of 8 elements (slots and heads below 2^24)", name);
@@ -53,12 +68,13 @@ inline int check_paged_cache(const fa_paged_cache* c, bool needs_k, bool needs_v
   return FA_OK;
 }
 
-inline PagedCache paged_cache(const fa_paged_cache* c) {
+inline PagedCache paged_cache(const fa_paged_cache* c, const fa_paged_scales* scales = nullptr) {
   PagedCache p{};
+  const int64_t size = scales ? 1 : 2;  // bytes of an element
   p.k = reinterpret_cast<char*>(c->k_cache);
   p.v = reinterpret_cast<char*>(c->v_cache);
-  p.k_ps = c->k_page_stride * 2; p.k_ss = c->k_slot_stride * 2; p.k_hs = c->k_head_stride * 2;
-  p.v_ps = c->v_page_stride * 2; p.v_ss = c->v_slot_stride * 2; p.v_hs = c->v_head_stride * 2;
+  p.k_ps = c->k_page_stride * size; p.k_ss = c->k_slot_stride * size; p.k_hs = c->k_head_stride * size;
+  p.v_ps = c->v_page_stride * size; p.v_ss = c->v_slot_stride * size; p.v_hs = c->v_head_stride * size;
   p.table = c->page_table;
   p.table_rs = c->table_row_stride;
   p.seqlens = c->seqlens_k;
@@ -72,6 +88,10 @@ inline PagedCache paged_cache(const fa_paged_cache* c) {
   p.total_q = c->total_q; p.max_sq = c->max_seqlen_q;
   p.weights = c->key_weights;
   p.positions = c->key_positions;
+  if (scales) {
+    p.k_exps = reinterpret_cast<uint8_t*>(scales->k_scales);
+    p.v_exps = reinterpret_cast<uint8_t*>(scales->v_scales);
+  }
   return p;
 }
 
@@ -88,6 +108,11 @@ FA_DEVICE int paged_len(const PagedCache& c, int b) {  // keys of sequence b tha
 // Groups behind the last that is looked at stand for that one, whatever the sequence's length: a tile's pages can be asked for while that is on its way.
 FA_DEVICE int page_of_group(const PagedCache& c, const int32_t* table_b, int g) {
   const int at = g >> (c.page_log2 - 4), last = (c.max_keys - 1) >> c.page_log2;
+  return page_in_pool(ld_scalar(table_b, at < last ? at : last), c.n_pages);
+}
+// The same for a table whose first `skipped` pages are not looked at (table_b: from there on)
+FA_DEVICE int page_of_group(const PagedCache& c, const int32_t* table_b, int g, int skipped) {
+  const int at = g >> (c.page_log2 - 4), last = ((c.max_keys - 1) >> c.page_log2) - skipped;
   return page_in_pool(ld_scalar(table_b, at < last ? at : last), c.n_pages);
 }
 FA_DEVICE int slot_of_group(const PagedCache& c, int g) { return (g << 4) & ((1 << c.page_log2) - 1); }

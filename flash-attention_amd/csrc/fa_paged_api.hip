@@ -18,16 +18,31 @@ struct Plan {
   int nq_tiles, n_splits;  // chunk (fa_paged_chunk.hip)
   bool deal;
   size_t bytes;
+  // a shared prefix (fa_paged_chunk_kernel.h): whether its keys are read once for all, its row tiles and key splits, and the bytes of its parts, which come first
+  bool share;
+  int pre_tiles, pre_splits;
+  size_t pre_bytes;
 };
 
-// Workgroups of the decode kernel that are resident at once: two a compute unit at d = 128 (64 KB of tiles each), four else.
-int decode_resident(int head_dim) { return 256 * (head_dim == 128 ? 2 : 4); }
+// Workgroups of the decode kernel that are resident at once: two a compute unit at d = 128 (64 KB of tiles each), four else; over pages in 8 bits, whose workgroups
+// have four waves, three at d = 64 (registers).
+int decode_resident(int head_dim, bool k8) { return 256 * (head_dim == 128 ? 2 : k8 && head_dim == 64 ? 3 : 4); }
 
-Plan plan_of(const fa_paged_cache& c) {
+Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* prefix = nullptr) {
   Plan pl{};
   const int rows = c.max_seqlen_q * (c.nheads_q / c.nheads_k);
   const int64_t pairs = (int64_t)c.batch * c.nheads_k;
-  const int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
+  int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
+  const int shared = prefix ? std::min(prefix->max_prefix_len, max_keys) / c.page_size * c.page_size : 0;
+  pl.share = shared > 0;
+  if (pl.share) {
+    const int64_t all_rows = (int64_t)c.total_q * (c.nheads_q / c.nheads_k);
+    pl.pre_tiles = (int)((all_rows + fa::kChunkRows - 1) / fa::kChunkRows) + prefix->n_groups - 1;
+    const int64_t items = (int64_t)c.nheads_k * pl.pre_tiles, tiles = (shared + 63) / 64;
+    pl.pre_splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / items, tiles / 4, 64}));
+    pl.pre_bytes = fa::align16((size_t)pl.pre_splits * c.nheads_k * all_rows * (c.head_dim + 3) * 4);
+    max_keys = std::max(max_keys - shared, 1);  // (what comes behind the longest prefix: how the rest is cut goes by it)
+  }
   pl.decode = rows <= fa::kDecodeMaxQ;
   if (pl.decode) {
     // A pair to itself, or shares of the line of all keys and a join behind them: the join is another launch and the line's beginning a chain of loads, 14 us
@@ -45,7 +60,7 @@ Plan plan_of(const fa_paged_cache& c) {
     const bool whole = pl.wide || max_keys <= (small ? 512 : 128) || (pairs > 256 && max_keys <= (small ? 2048 : c.head_dim == 64 && pairs < 1024 ? 512 : 1024));
     if (!whole) {
       const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
-      pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim), pairs * units);
+      pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim, k8), pairs * units);
       pl.bytes = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
     }
     return pl;
@@ -63,14 +78,14 @@ Plan plan_of(const fa_paged_cache& c) {
   const int least = items > 128 ? 8 : c.head_dim < 128 && tiles < 12 ? tiles : 4;  // tiles of 64 keys
   const int64_t n = std::min<int64_t>({n_fit, tiles / least, 64});
   pl.n_splits = n < 2 ? 1 : (int)n;
-  if (pl.n_splits > 1) pl.bytes = (size_t)pl.n_splits * items * fa::kChunkRows * (c.head_dim + 3) * 4;
+  if (pl.n_splits > 1 || pl.share) pl.bytes = (size_t)pl.n_splits * items * fa::kChunkRows * (c.head_dim + 3) * 4;
   return pl;
 }
 
-int check(const fa_paged_fwd_args* a, bool weights, const char* name) {
+int check(const fa_paged_fwd_args* a, bool weights, const char* name, const fa_paged_scales* scales = nullptr) {
   FA_REQUIRE(a && a->struct_bytes == sizeof(fa_paged_fwd_args), "%s: struct size mismatch", name);
   FA_REQUIRE(a->dtype == FA_FP16 || a->dtype == FA_BF16, "%s: dtype must be fp16 or bf16", name);
-  const int rc = fa::check_paged_cache(&a->cache, true, !weights, true, name);
+  const int rc = fa::check_paged_cache(&a->cache, true, !weights, true, name, scales);
   if (rc) return rc;
   const fa_paged_cache& c = a->cache;
   FA_REQUIRE(std::isfinite(a->softmax_scale) && a->softmax_scale > 0.f, "%s: softmax_scale must be positive and finite", name);
@@ -92,9 +107,19 @@ int check(const fa_paged_fwd_args* a, bool weights, const char* name) {
   return FA_OK;
 }
 
-fa::PagedFwdParams params(const fa_paged_fwd_args* a) {
+int check_prefix(const fa_paged_fwd_args* a, const fa_paged_prefix* x, const char* name) {
+  FA_REQUIRE(x->struct_bytes == sizeof(fa_paged_prefix), "%s: prefix's struct size mismatch", name);
+  FA_REQUIRE(x->n_groups > 0 && x->n_groups <= a->cache.batch && x->max_prefix_len >= 0, "%s: from one group to a group for each sequence, max_prefix_len not negative", name);
+  FA_REQUIRE(x->cu_groups && x->prefix_lens && ((reinterpret_cast<uintptr_t>(x->cu_groups) | reinterpret_cast<uintptr_t>(x->prefix_lens)) & 3) == 0,
+             "%s: cu_groups and prefix_lens must be there and 4-byte aligned", name);
+  const int64_t rows = (int64_t)a->cache.total_q * (a->cache.nheads_q / a->cache.nheads_k);
+  FA_REQUIRE(rows < ((int64_t)1 << 30) && (rows / fa::kChunkRows + x->n_groups) * a->cache.nheads_k < ((int64_t)1 << 24), "%s: too many rows", name);
+  return FA_OK;
+}
+
+fa::PagedFwdParams params(const fa_paged_fwd_args* a, const fa_paged_scales* scales = nullptr) {
   fa::PagedFwdParams p{};
-  p.c = fa::paged_cache(&a->cache);
+  p.c = fa::paged_cache(&a->cache, scales);
   p.q = a->q;
   p.o = a->o;
   p.lse = a->softmax_lse;
@@ -109,29 +134,51 @@ fa::PagedFwdParams params(const fa_paged_fwd_args* a) {
 
 extern "C" {
 
-size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_args* a) {
+size_t fa_paged_fwd_with_workspace_bytes(const fa_paged_fwd_args* a, const fa_paged_scales* scales, const fa_paged_prefix* prefix) {
   if (!a || a->struct_bytes != sizeof(fa_paged_fwd_args) || fa::check_paged_cache(&a->cache, false, false, true, "fa_paged_fwd") != FA_OK) return 0;
-  return plan_of(a->cache).bytes;
+  if (prefix && check_prefix(a, prefix, "fa_paged_fwd_with") != FA_OK) return 0;
+  const Plan pl = plan_of(a->cache, scales != nullptr, prefix);
+  return pl.pre_bytes + pl.bytes;
 }
 
-int fa_paged_fwd(const fa_paged_fwd_args* a) {
-  const int rc = check(a, false, "fa_paged_fwd");
+int fa_paged_fwd_with(const fa_paged_fwd_args* a, const fa_paged_scales* scales, const fa_paged_prefix* prefix) {
+  const char* const name = scales || prefix ? "fa_paged_fwd_with" : "fa_paged_fwd";
+  int rc = check(a, false, name, scales);
+  if (!rc && prefix) rc = check_prefix(a, prefix, name);
   if (rc || a->cache.total_q == 0) return rc;
-  const Plan pl = plan_of(a->cache);
-  if (pl.bytes && (!a->workspace || a->workspace_bytes < pl.bytes || !fa::aligned16(a->workspace)))
-    return fa::fail(FA_ERR_WORKSPACE, "fa_paged_fwd: needs %zu bytes of 16-byte aligned workspace", pl.bytes);
-  fa::PagedFwdParams p = params(a);
+  const Plan pl = plan_of(a->cache, scales != nullptr, prefix);
+  const size_t bytes = pl.pre_bytes + pl.bytes;
+  if (bytes && (!a->workspace || a->workspace_bytes < bytes || !fa::aligned16(a->workspace)))
+    return fa::fail(FA_ERR_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace", name, bytes);
+  fa::PagedFwdParams p = params(a, scales);
   p.groups = pl.groups;
   p.wide = pl.wide;
   p.nq_tiles = pl.nq_tiles;
   p.n_splits = pl.n_splits;
   p.deal = pl.deal;
-  p.part = reinterpret_cast<float*>(a->workspace);
+  p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + pl.pre_bytes);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(a->stream);
-  if (pl.decode) FA_LAUNCH(fa::launch_paged_decode(p, a->dtype, a->cache.head_dim, stream));
-  else FA_LAUNCH(fa::launch_paged_chunk(p, a->dtype, a->cache.head_dim, stream));
+  const int dtype = a->dtype, head_dim = a->cache.head_dim;
+  if (pl.share) {
+    p.c.prefix = prefix->prefix_lens;
+    p.c.max_prefix = prefix->max_prefix_len;
+    p.cu_groups = prefix->cu_groups;
+    p.n_groups = prefix->n_groups;
+    p.pre_tiles = pl.pre_tiles;
+    p.pre_splits = pl.pre_splits;
+    p.pre = reinterpret_cast<float*>(a->workspace);
+    FA_LAUNCH((scales ? fa::launch_paged_prefix_8bit : fa::launch_paged_prefix)(p, dtype, head_dim, stream));
+    if (pl.decode) FA_LAUNCH((scales ? fa::launch_paged_decode_own_8bit : fa::launch_paged_decode_own)(p, dtype, head_dim, stream));
+    else FA_LAUNCH((scales ? fa::launch_paged_chunk_own_8bit : fa::launch_paged_chunk_own)(p, dtype, head_dim, stream));
+    return FA_OK;
+  }
+  if (pl.decode) FA_LAUNCH((scales ? fa::launch_paged_decode_8bit : fa::launch_paged_decode)(p, dtype, head_dim, stream));
+  else FA_LAUNCH((scales ? fa::launch_paged_chunk_8bit : fa::launch_paged_chunk)(p, dtype, head_dim, stream));
   return FA_OK;
 }
+
+size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_args* a) { return fa_paged_fwd_with_workspace_bytes(a, nullptr, nullptr); }
+int fa_paged_fwd(const fa_paged_fwd_args* a) { return fa_paged_fwd_with(a, nullptr, nullptr); }
 
 int fa_paged_key_weights(const fa_paged_fwd_args* a) {
   const int rc = check(a, true, "fa_paged_key_weights");

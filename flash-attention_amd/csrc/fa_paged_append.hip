@@ -9,7 +9,8 @@
 #include <cstdint>
 
 #include "fa_norm.h"
-#include "fa_paged.h"
+#include "fa_paged_8bit.h"
+#include "fa_paged_rows.h"
 
 namespace fa {
 
@@ -29,8 +30,9 @@ struct AppendParams {
   int per_row, pieces, threads, groups;
 };
 
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p) {
+// kQuant: into pages in 8 bits (fa_paged_8bit.h), k straight from 32 bits
+template <typename T, int D, int ROWS, bool kQuant>
+FA_DEVICE void paged_append(const AppendParams p) {
   constexpr int CH = D / 8;
   using vec8 = typename Elem<T>::vec8;
   const int group = blockIdx.x / p.pieces, piece = blockIdx.x - group * p.pieces;
@@ -51,55 +53,18 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p)
 #pragma unroll
     for (int i = 0; i < ROWS; i++)
       if (on && row0 + i < p.c.total_q) x8[i] = bitcast<vec8>(ld_global16(src + (int64_t)(row0 + i) * rs));
-    // Where the rows go, wave-uniform and for all of them at once: their sequences (cu is non-decreasing: as many as end at or before the row; a load
-    // and a ballot for 64 of them), then lengths, then pages.
-    int seq[ROWS], slot[ROWS], page[ROWS], pos[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) seq[i] = 0;
-    for (int at = 0; at < p.c.B; at += 64) {
-      const int s = at + (threadIdx.x & 63);
-      const int end = p.c.cu_q[s < p.c.B ? s + 1 : p.c.B];
-#pragma unroll
-      for (int i = 0; i < ROWS; i++) seq[i] += __popcll(__ballot(s < p.c.B && end <= row0 + i));
-    }
-    // (loads and what is made of them in loops of their own, without branches: the rows' loads are on their way together)
-    int len[ROWS], begin[ROWS], end[ROWS];
-    bool there[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-      const int b = __builtin_amdgcn_readfirstlane(seq[i]);
-      there[i] = b < p.c.B && row0 + i < p.c.total_q;  // (else: behind the last sequence)
-      seq[i] = b < p.c.B ? b : p.c.B - 1;
-      len[i] = ld_scalar(p.c.seqlens, seq[i]);
-      begin[i] = ld_scalar(p.c.cu_q, seq[i]);
-      end[i] = ld_scalar(p.c.cu_q, seq[i] + 1);
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-      slot[i] = append_slot(len[i], begin[i], end[i], row0 + i, p.c.max_sq, p.c.max_keys);
-      if (!there[i]) slot[i] = -1;
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-      page[i] = ld_scalar(p.c.table + (int64_t)seq[i] * p.c.table_rs, (slot[i] < 0 ? 0 : slot[i]) >> p.c.page_log2);
-      pos[i] = slot[i];
-    }
-    if (p.given_positions) {
-#pragma unroll
-      for (int i = 0; i < ROWS; i++) pos[i] = ld_scalar(p.given_positions, row0 + i < p.c.total_q ? row0 + i : p.c.total_q - 1);
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; i++)
-      if (slot[i] < 0) page[i] = -1;
+    RowPlaces<ROWS> at;
+    at.find(p.c, p.given_positions, row0);
     // What an address has of the lane, once; the rest of it, a row's, is wave-uniform.
     typedef typename Elem<T>::vec4 vec4;
     const bool moves_only = !norm && !rot;
-    const int64_t lane_to = part == 0 ? (int64_t)h * p.qo_hs * 2 + ch * 16 : (part == 1 ? h * p.c.k_hs : h * p.c.v_hs) + ch * 16;
+    const int chunk = kQuant ? 8 : 16;  // bytes of a lane's elements in the cache
+    const int64_t lane_to = part == 0 ? (int64_t)h * p.qo_hs * 2 + ch * 16 : (part == 1 ? h * p.c.k_hs : h * p.c.v_hs) + ch * chunk;
     char* const base = part == 0 ? reinterpret_cast<char*>(p.q_out) + lane_to : (part == 1 ? p.c.k : p.c.v) + lane_to;
     vec4 c4[ROWS], s4[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-      const int64_t row_at = (int64_t)table_row(pos[i], p.table_rows) * (D / 2);
+      const int64_t row_at = (int64_t)table_row(at.pos[i], p.table_rows) * (D / 2);
       if (on && rot) {
         c4[i] = reinterpret_cast<const vec4*>(reinterpret_cast<const T*>(p.cos) + row_at)[ch];
         s4[i] = reinterpret_cast<const vec4*>(reinterpret_cast<const T*>(p.sin) + row_at)[ch];
@@ -107,17 +72,19 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p)
     }
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-      if (!page_is_one(page[i], p.c.n_pages)) continue;  // (wave-uniform)
-      const int at = slot[i] & ((1 << p.c.page_log2) - 1);
-      const int64_t to_q = (int64_t)(row0 + i) * p.qo_rs * 2, to_k = page[i] * p.c.k_ps + at * p.c.k_ss, to_v = page[i] * p.c.v_ps + at * p.c.v_ss;
-      const int64_t m0 = ((int64_t)page[i] * p.c.HK << p.c.page_log2) + at;
+      if (!page_is_one(at.page[i], p.c.n_pages)) continue;  // (wave-uniform)
+      const int slot = at.slot[i] & ((1 << p.c.page_log2) - 1);
+      const int64_t to_q = (int64_t)(row0 + i) * p.qo_rs * 2, to_k = at.page[i] * p.c.k_ps + slot * p.c.k_ss, to_v = at.page[i] * p.c.v_ps + slot * p.c.v_ss;
+      const int64_t m0 = ((int64_t)at.page[i] * p.c.HK << p.c.page_log2) + slot;
       if (on) {
         char* const dst = base + (part == 0 ? to_q : (part == 1 ? to_k : to_v));
         vec8 y = x8[i];
-        if (!moves_only) {
-          float x[8];
+        float x[8];
+        if (!moves_only || kQuant) {
 #pragma unroll
           for (int e = 0; e < 8; e++) x[e] = (float)x8[i][e];
+        }
+        if (!moves_only) {
           if (norm) {
             const float r = inverse_rms<CH>(x, p.eps);
 #pragma unroll
@@ -127,15 +94,40 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p)
 #pragma unroll
           for (int e = 0; e < 8; e++) y[e] = (T)x[e];
         }
-        st_global16(dst, bitcast<u32x4>(y));
+        const int64_t m = m0 + ((int64_t)h << p.c.page_log2);
+        if constexpr (kQuant) {
+          float top = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float a = __builtin_fabsf(x[e]);
+            top = a < INFINITY ? fmaxf(top, a) : top;
+          }
+          const int byte = row_exponent<T>(vector_max<CH>(top));
+          if (part == 0) {
+            st_global16(dst, bitcast<u32x4>(y));
+          } else {
+            *reinterpret_cast<u32x2*>(dst) = quant8<T>(x, byte);
+            if (ch == 0) (part == 1 ? p.c.k_exps : p.c.v_exps)[m] = (uint8_t)byte;
+          }
+        } else {
+          st_global16(dst, bitcast<u32x4>(y));
+        }
         if (part == 1 && ch == 0) {
-          const int64_t m = m0 + ((int64_t)h << p.c.page_log2);
           if (p.c.weights) p.c.weights[m] = 0.f;
-          if (p.c.positions) p.c.positions[m] = pos[i];
+          if (p.c.positions) p.c.positions[m] = at.pos[i];
         }
       }
     }
   }
+}
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(512) paged_append_kernel(const AppendParams p) {
+  paged_append<T, D, ROWS, false>(p);
+}
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(512) paged_append_8bit_kernel(const AppendParams p) {
+  paged_append<T, D, ROWS, true>(p);
 }
 
 template <typename T, int D>
@@ -150,6 +142,11 @@ hipError_t launch_append_d(AppendParams p, hipStream_t stream) {
   // 98 / 108; 15000 of 3 x 32, d = 128 (a row six workgroups) 158 / 153.  24 waves: 65 and 46 for the first and the third.
   if (!few) p.groups = std::min(p.groups, std::max(1, walking_workgroups(p.threads / 64, 20) / p.pieces));
   const dim3 grid((unsigned)(p.groups * p.pieces)), block((unsigned)p.threads);
+  if (p.c.k_exps) {
+    if (few) hipLaunchKernelGGL((paged_append_8bit_kernel<T, D, 1>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((paged_append_8bit_kernel<T, D, kRows>), grid, block, 0, stream, p);
+    return hipGetLastError();
+  }
   if (few) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((paged_append_kernel<T, D, kRows>), grid, block, 0, stream, p);
   return hipGetLastError();
@@ -168,11 +165,13 @@ hipError_t launch_append(const AppendParams& p, int D, hipStream_t stream) {
 }  // namespace
 }  // namespace fa
 
-extern "C" int fa_paged_append(const fa_paged_append_args* a) {
-  const char* const name = "fa_paged_append";
+extern "C" int fa_paged_append(const fa_paged_append_args* a) { return fa_paged_append_with(a, nullptr); }
+
+extern "C" int fa_paged_append_with(const fa_paged_append_args* a, const fa_paged_scales* scales) {
+  const char* const name = scales ? "fa_paged_append_with" : "fa_paged_append";
   FA_REQUIRE(a && a->struct_bytes == sizeof(fa_paged_append_args), "%s: struct size mismatch", name);
   FA_REQUIRE(a->dtype == FA_FP16 || a->dtype == FA_BF16, "%s: dtype must be fp16 or bf16", name);
-  const int rc = fa::check_paged_cache(&a->cache, true, true, true, name);
+  const int rc = fa::check_paged_cache(&a->cache, true, true, true, name, scales);
   if (rc) return rc;
   const fa_paged_cache& c = a->cache;
   FA_REQUIRE(c.k_slot_stride >= c.head_dim && c.v_slot_stride >= c.head_dim && (c.nheads_k == 1 || (c.k_head_stride >= c.head_dim && c.v_head_stride >= c.head_dim)) &&
@@ -194,7 +193,7 @@ extern "C" int fa_paged_append(const fa_paged_append_args* a) {
   FA_REQUIRE((a->cos_table == nullptr) == (a->sin_table == nullptr) && (!a->cos_table || a->table_rows >= 1), "%s: cos_table and sin_table come together, with rows", name);
   FA_REQUIRE(((reinterpret_cast<uintptr_t>(a->cos_table) | reinterpret_cast<uintptr_t>(a->sin_table)) & 7) == 0, "%s: tables must be 8-byte aligned", name);
   fa::AppendParams p{};
-  p.c = fa::paged_cache(&c);
+  p.c = fa::paged_cache(&c, scales);
   p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out;
   p.qw = a->q_weight; p.kw = a->k_weight;
   p.cos = a->cos_table; p.sin = a->sin_table;

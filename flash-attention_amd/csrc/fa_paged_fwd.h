@@ -4,6 +4,11 @@
 // Rows.  The query heads of a group read the same keys: the G heads of the Lq new tokens of a sequence are G * Lq rows of one product, row r being
 // head r % G of token r / G, so that a key head's keys are read once for all of them.  Row r sees the keys below limit(r) = Lk - Lq + r / G + 1
 // under the causal mask (aligned at the end), Lk else; a limit of 0 or less: nothing, o = 0 and lse = -inf.
+//
+// Shared prefixes.  The sequences of a group list the same pages for their first prefix[b] keys (whole pages), which all their new tokens see.  To those keys the
+// group's rows are one product, G times the tokens of all its sequences: the chunk kernel reads them once per 128 rows, as if the group were one sequence without a
+// mask (fa_paged_chunk_kernel.h, kShared), and leaves partial results; the sequences' own keys, from `first` on, are attended as ever, and whatever writes a row's
+// result adds the prefix's parts to its own.
 #pragma once
 
 #include "fa_paged.h"
@@ -23,6 +28,11 @@ struct PagedFwdParams {
   int groups, wide;
   int nq_tiles, n_splits, deal;
   float* part;  // partial results
+  // shared prefixes: groups of sequences (cu_groups[g] .. cu_groups[g + 1]), the splits of a prefix's keys, the row tiles that there can be, and the parts:
+  // [split][key head][G * total_q rows][D], m, l and u behind all of them
+  const int32_t* cu_groups;
+  int n_groups, pre_splits, pre_tiles;
+  float* pre;
 };
 
 // Partial results of a row: its output before the division, the maximum m of its scores (before scaling), the sum l of the probabilities as they are
@@ -55,11 +65,48 @@ struct JoinedRow {
   }
 };
 
+// The keys of sequence b that its group shares: what comes in front of its own ones
+template <bool kPrefix>
+FA_DEVICE int first_own(const PagedCache& c, int b) {
+  if constexpr (!kPrefix) return 0;
+  else return shared_keys(ld_scalar(c.prefix, b), c.max_prefix, c.max_keys, c.page_log2);
+}
+template <bool kPrefix>
+FA_DEVICE int own_len(const PagedCache& c, int b) {
+  if constexpr (!kPrefix) return paged_len(c, b);
+  const int n = paged_len(c, b) - first_own<kPrefix>(c, b);
+  return n > 0 ? n : 0;
+}
+// Adds the prefix's parts lane, lane + lanes, .. of a row (of all the call's rows of key head h) to x.  A part's maximum is one of scores before scaling; `unit`
+// brings it to x's units.
+template <int D>
+FA_DEVICE void add_prefix(const PagedFwdParams& p, JoinedRow* x, int h, int64_t row, int d0, float cs, float unit, int lane = 0, int lanes = 1) {
+  const int64_t rows = (int64_t)p.c.total_q * p.c.G, all = (int64_t)p.c.HK * rows, at = (int64_t)h * rows + row;
+#pragma unroll 4
+  for (int i = lane; i < p.pre_splits; i += lanes) {
+    const float* const from = p.pre + (int64_t)i * all * (D + 3);
+    const float* const ml = from + all * D + at * 3;
+    x->add(PartRow{ml[0] * unit, ml[1], ml[2]}, *reinterpret_cast<const f32x4*>(from + at * D + d0), cs);
+  }
+}
+
 FA_DEVICE bool paged_rows(const PagedCache& c, int b, int* begin, int* len) {  // the new tokens of sequence b
   const int s = ld_scalar(c.cu_q, b), e = ld_scalar(c.cu_q, b + 1);
   if (s < 0 || e <= s || e > c.total_q) return false;
   *begin = s;
   *len = e - s < c.max_sq ? e - s : c.max_sq;
+  return true;
+}
+
+// Group g: its first sequence, where its new tokens begin, and how many all its sequences have
+FA_DEVICE bool group_rows(const PagedFwdParams& p, int g, int* b, int* begin, int* tokens) {
+  const int b0 = p.cu_groups[g], b1 = p.cu_groups[g + 1];
+  if (b0 < 0 || b1 <= b0 || b1 > p.c.B) return false;
+  const int s = p.c.cu_q[b0], e = p.c.cu_q[b1];
+  if (s < 0 || e <= s || e > p.c.total_q) return false;
+  *b = b0;
+  *begin = s;
+  *tokens = e - s;
   return true;
 }
 
@@ -81,12 +128,25 @@ constexpr int kDecodeUnit = 128;
 constexpr int kPartRows = 32;
 // Waves of a workgroup that has a pair to itself where pairs about fill the device: as many as their tiles' LDS allows.
 constexpr int kDecodeWide(int head_dim) { return head_dim == 128 ? 4 : 8; }
+// ... over pages in 8 bits, whose tiles take half the LDS, and of one that has its share of the line
+constexpr int kDecodeWide8 = 8;
+constexpr int kDecodeWaves8 = 4;
 
 // floats of a workgroup's two partial results: [2][32][D] outputs, [2][3][32] m, l, u
 inline size_t decode_part_floats(int D) { return 2 * (size_t)kPartRows * (D + 3); }
 
 hipError_t launch_paged_decode(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 hipError_t launch_paged_chunk(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+// of a cache in 8 bits
+hipError_t launch_paged_decode_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+hipError_t launch_paged_chunk_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+// behind a shared prefix, and over it
+hipError_t launch_paged_decode_own(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+hipError_t launch_paged_decode_own_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+hipError_t launch_paged_chunk_own(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+hipError_t launch_paged_chunk_own_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+hipError_t launch_paged_prefix(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+hipError_t launch_paged_prefix_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 constexpr int kChunkRows = 128;  // rows of a workgroup of the chunk kernel
 
 }  // namespace fa

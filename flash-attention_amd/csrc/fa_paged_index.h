@@ -26,4 +26,9 @@ FA_INDEX int append_slot(int len, int begin, int end, int row, int max_rows, int
 // A table row for a position: the nearest one.
 FA_INDEX int table_row(int pos, int rows) { return pos < 0 ? 0 : (pos < rows ? pos : rows - 1); }
 
+// The keys that a sequence shares with others: whole pages, at most what the table and the caller's bounds hold.
+FA_INDEX int shared_keys(int len, int max_prefix, int max_keys, int page_log2) {
+  return keys_in_reach(len, max_prefix < max_keys ? max_prefix : max_keys) >> page_log2 << page_log2;
+}
+
 }  // namespace fa

@@ -13,31 +13,36 @@ FA_DEVICE void wait_vmcnt() {  // at most N of this wave's global loads (direct-
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
 }
 
-// The line of units.  Sequence b has HK pairs of units(b) each; a sequence without new tokens has none.
+// The line of units.  Sequence b has HK pairs of units(b) each; a sequence without new tokens has none.  kPrefix: of its own keys, behind those that its group shares.
+template <bool kPrefix = false>
 FA_DEVICE int units_of(const PagedCache& c, int b) {
-  const int keys = keys_in_reach(c.seqlens[b], c.max_keys);
+  int keys = keys_in_reach(c.seqlens[b], c.max_keys);
+  if constexpr (kPrefix) keys -= shared_keys(c.prefix[b], c.max_prefix, c.max_keys, c.page_log2);
   const int s = c.cu_q[b], e = c.cu_q[b + 1];
   if (s < 0 || e <= s || e > c.total_q) return 0;
   return keys <= kDecodeUnit ? 1 : (keys + kDecodeUnit - 1) / kDecodeUnit;
 }
 // Units of 64 sequences from `first` on as inclusive sums over the lanes; the same in every wave
+template <bool kPrefix = false>
 FA_DEVICE int unit_sums(const PagedCache& c, int first) {
   const int b = first + (threadIdx.x & 63);
-  return wave_prefix_sum(b < c.B ? units_of(c, b) : 0);
+  return wave_prefix_sum(b < c.B ? units_of<kPrefix>(c, b) : 0);
 }
 // (sums0: the first 64 sequences' sums, made once)
+template <bool kPrefix = false>
 FA_DEVICE int64_t all_units(const PagedCache& c, int sums0) {
   int64_t n = __builtin_amdgcn_readlane(sums0, 63);
-  for (int first = 64; first < c.B; first += 64) n += __builtin_amdgcn_readlane(unit_sums(c, first), 63);
+  for (int first = 64; first < c.B; first += 64) n += __builtin_amdgcn_readlane(unit_sums<kPrefix>(c, first), 63);
   return n * c.HK;
 }
 struct Spot {  // a unit of the line
   int b, h, unit, units;  // units: of each pair of sequence b
 };
+template <bool kPrefix = false>
 FA_DEVICE Spot spot_of(const PagedCache& c, int64_t u, int sums0) {
   int64_t before = 0;
   for (int first = 0; first < c.B; first += 64) {
-    const int sums = first == 0 ? sums0 : unit_sums(c, first);
+    const int sums = first == 0 ? sums0 : unit_sums<kPrefix>(c, first);
     const int all = __builtin_amdgcn_readlane(sums, 63);
     if (u < before + (int64_t)all * c.HK) {
       const int64_t rest = u - before;
@@ -57,6 +62,7 @@ FA_DEVICE int sharers(const PagedFwdParams& p, int64_t units) {
 }
 FA_DEVICE int64_t share_begin(int64_t units, int w, int sharers) { return units * w / sharers; }
 // The first unit of the pair after (b, h): false if there is none
+template <bool kPrefix = false>
 FA_DEVICE bool next_pair(const PagedCache& c, Spot* at) {
   at->unit = 0;
   if (at->h + 1 < c.HK) {
@@ -64,9 +70,9 @@ FA_DEVICE bool next_pair(const PagedCache& c, Spot* at) {
     return true;
   }
   at->h = 0;
-  do at->b++; while (at->b < c.B && units_of(c, at->b) == 0);
+  do at->b++; while (at->b < c.B && units_of<kPrefix>(c, at->b) == 0);
   if (at->b >= c.B) return false;
-  at->units = units_of(c, at->b);
+  at->units = units_of<kPrefix>(c, at->b);
   return true;
 }
 

@@ -162,6 +162,24 @@ class PagedFwdArgs(ctypes.Structure):
          ("stream", ctypes.c_void_p)])
 
 
+class PagedScales(ctypes.Structure):
+    """struct fa_paged_scales, field for field."""
+    _fields_ = [("struct_bytes", ctypes.c_uint32), ("reserved0", ctypes.c_uint32), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p)]
+
+
+class PagedPrefix(ctypes.Structure):
+    """struct fa_paged_prefix, field for field."""
+    _fields_ = [("struct_bytes", ctypes.c_uint32), ("n_groups", ctypes.c_int32), ("max_prefix_len", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+                ("cu_groups", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p)]
+
+
+class PagedReadArgs(ctypes.Structure):
+    """struct fa_paged_read_args, field for field."""
+    _fields_ = (
+        [("struct_bytes", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("cache", PagedCacheArgs), ("k_out", ctypes.c_void_p), ("v_out", ctypes.c_void_p)] +
+        [(n + s, ctypes.c_int64) for n in ("k", "v") for s in ("_row_stride", "_head_stride")] + [("stream", ctypes.c_void_p)])
+
+
 class PagedEvictArgs(ctypes.Structure):
     """struct fa_paged_evict_args, field for field."""
     _fields_ = [("struct_bytes", ctypes.c_uint32), ("budget", ctypes.c_int32), ("recent", ctypes.c_int32), ("reserved0", ctypes.c_int32),
@@ -175,7 +193,8 @@ EXPORTED_SYMBOLS = (
     "fa_gather_rows", "fa_scatter_rows", "fa_scatter_rows_workspace_bytes", "fa_rotary", "fa_set_launch_policy",
     "fa_keep_words_bytes", "fa_blocksparse_row_order", "fa_bias_grad_reduce", "fa_bias_grad_reduce_ragged", "fa_pad_bias_rows", "fa_padding_rows", "fa_fwd_padded",
     "fa_token_positions", "fa_qk_norm_rotary", "fa_qk_norm_rotary_bwd", "fa_qk_norm_rotary_bwd_workspace_bytes", "fa_paged_append", "fa_paged_fwd",
-    "fa_paged_fwd_workspace_bytes", "fa_paged_key_weights", "fa_paged_evict", "fa_paged_evict_workspace_bytes",
+    "fa_paged_fwd_workspace_bytes", "fa_paged_key_weights", "fa_paged_evict", "fa_paged_evict_workspace_bytes", "fa_paged_append_with", "fa_paged_fwd_with",
+    "fa_paged_fwd_with_workspace_bytes", "fa_paged_read",
 )
 # declared in include/flash_attn_gfx950_bench.h: instrumentation for bench.py, not part of the drop-in boundary
 BENCH_SYMBOLS = ("fa_bwd_profiled",)
@@ -199,8 +218,8 @@ def _load_host(lib):
         "fa_fwd", "fa_fwd_block", "fa_bwd", "fa_bwd_block", "fa_fwd_workspace_bytes", "fa_bwd_workspace_bytes", "fa_round_seqlens",
         "fa_last_error", "fa_pad_bias_rows", "fa_bias_grad_reduce_ragged", "fa_rotary", "fa_token_positions")))
     host.bind_paged(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
-        "fa_qk_norm_rotary", "fa_qk_norm_rotary_bwd", "fa_qk_norm_rotary_bwd_workspace_bytes", "fa_paged_append", "fa_paged_fwd", "fa_paged_fwd_workspace_bytes",
-        "fa_paged_key_weights", "fa_paged_evict", "fa_paged_evict_workspace_bytes")))
+        "fa_qk_norm_rotary", "fa_qk_norm_rotary_bwd", "fa_qk_norm_rotary_bwd_workspace_bytes", "fa_paged_append_with", "fa_paged_fwd_with",
+        "fa_paged_fwd_with_workspace_bytes", "fa_paged_read", "fa_paged_key_weights", "fa_paged_evict", "fa_paged_evict_workspace_bytes")))
     return host
 
 
@@ -285,6 +304,10 @@ def load_library():
         for name, args in (("fa_qk_norm_rotary_bwd", QkNormArgs), ("fa_paged_fwd", PagedFwdArgs), ("fa_paged_evict", PagedEvictArgs)):
             getattr(lib, name + "_workspace_bytes").argtypes = [ctypes.POINTER(args)]
             getattr(lib, name + "_workspace_bytes").restype = ctypes.c_size_t
+        for name, args in (("fa_paged_append_with", (PagedAppendArgs, PagedScales)), ("fa_paged_fwd_with", (PagedFwdArgs, PagedScales, PagedPrefix)),
+                           ("fa_paged_fwd_with_workspace_bytes", (PagedFwdArgs, PagedScales, PagedPrefix)), ("fa_paged_read", (PagedReadArgs, PagedScales))):
+            getattr(lib, name).argtypes = [ctypes.POINTER(a) for a in args]
+            getattr(lib, name).restype = ctypes.c_size_t if name.endswith("_bytes") else ctypes.c_int
         lib.fa_set_launch_policy.argtypes = [ctypes.c_int]
         lib.fa_set_launch_policy.restype = ctypes.c_int
         _host = _passes = _load_host(lib)
@@ -1161,12 +1184,16 @@ def _int32(name, v):
     return v
 
 
-def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_weights=None, key_positions=None):
-    """Fills a PagedCacheArgs from a cache's tensors; v_cache may be None where it is not read."""
+def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_weights=None, key_positions=None, k_scales=None, v_scales=None):
+    """Fills a PagedCacheArgs from a cache's tensors; v_cache may be None where it is not read.  Returns the PagedScales of a cache in 8 bits, else None."""
     _check(k_cache.is_cuda and k_cache.dim() == 4, "k_cache must be a (pages, page size, heads, head_dim) GPU tensor")
     n_pages, page_size, heads, D = k_cache.shape
     _check(min(k_cache.shape) > 0 and n_pages < 2 ** 31, "k_cache must have pages, slots and heads, less than 2^31 pages")
-    _dtype_code(k_cache)
+    _check((k_scales is None) == (v_scales is None), "k_scales and v_scales come together")
+    if k_scales is None:
+        _check(k_cache.dtype in (torch.float16, torch.bfloat16), "the cache must be fp16 or bf16, or (storing, reading and attention) float8_e4m3fn with k_scales and v_scales")
+    else:
+        _check(k_cache.dtype == torch.float8_e4m3fn, "k_scales and v_scales are those of a float8_e4m3fn cache")
     for name, t in (("k", k_cache), ("v", v_cache)):
         if t is None:
             continue
@@ -1184,15 +1211,21 @@ def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_w
     a.page_table, a.table_row_stride, a.table_cols = page_table.data_ptr(), (page_table.stride(0) if batch > 1 else cols), cols
     a.seqlens_k = seqlens_k.data_ptr()
     a.n_pages, a.page_size, a.batch, a.nheads_k, a.head_dim, a.max_seqlen_k = n_pages, page_size, batch, heads, D, _int32("max_seqlen_k", max_seqlen_k)
-    for name, t, dtype in (("key_weights", key_weights, torch.float32), ("key_positions", key_positions, torch.int32)):
+    scales = PagedScales() if k_scales is not None else None
+    for name, t, dtype, to in (("key_weights", key_weights, torch.float32, a), ("key_positions", key_positions, torch.int32, a),
+                               ("k_scales", k_scales, torch.uint8, scales), ("v_scales", v_scales, torch.uint8, scales)):
         if t is not None:
             _check(t.device == k_cache.device and t.dtype == dtype and tuple(t.shape) == (n_pages, heads, page_size) and t.is_contiguous(),
                    "%s must be a contiguous (pages, heads, page size) tensor of %s on the cache's device" % (name, dtype))
-            setattr(a, name, t.data_ptr())
+            setattr(to, name, t.data_ptr())
+    if scales is not None:
+        scales.struct_bytes = ctypes.sizeof(scales)
+    return scales
 
 
 def _paged_queries(a, q, k_cache, cu_seqlens_q, max_seqlen_q):
-    _check(q.is_cuda and q.device == k_cache.device and q.dtype == k_cache.dtype and q.dim() == 3 and q.shape[2] == k_cache.shape[3] and q.stride(2) == 1,
+    _dtype_code(q)
+    _check(q.is_cuda and q.device == k_cache.device and (q.dtype == k_cache.dtype or k_cache.dtype == torch.float8_e4m3fn) and q.dim() == 3 and q.shape[2] == k_cache.shape[3] and q.stride(2) == 1,
            "q must be a (total, heads, head_dim) tensor of the cache's dtype and device, contiguous in the last dimension")
     _check(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "the query heads must be a multiple of the key heads")
     _check_cu("cu_seqlens_q", cu_seqlens_q, a.batch)
@@ -1202,19 +1235,21 @@ def _paged_queries(a, q, k_cache, cu_seqlens_q, max_seqlen_q):
 
 
 def paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, q_out=None, q_weight=None, k_weight=None, cos=None, sin=None,
-                 positions=None, eps=1e-6, key_weights=None, key_positions=None):
-    """Stores the new tokens' k and v (total, heads, head_dim) into the pages of their sequences and returns q_out: fa_paged_append.  q may be None."""
+                 positions=None, eps=1e-6, key_weights=None, key_positions=None, k_scales=None, v_scales=None):
+    """Stores the new tokens' k and v (total, heads, head_dim) into the pages of their sequences and returns q_out: fa_paged_append_with.  q may be None."""
     lib = load_library()
     a = PagedAppendArgs()
     a.struct_bytes = ctypes.sizeof(a)
     c = a.cache
     _check(k_cache.dim() == 4, "k_cache must be a (pages, page size, heads, head_dim) GPU tensor")
     total, D = k.shape[0], k_cache.shape[3]
-    _paged_cache(c, k_cache, v_cache, page_table, seqlens_k, min(page_table.shape[-1] * k_cache.shape[1], 2 ** 31 - 1), key_weights, key_positions)
+    scales = _paged_cache(c, k_cache, v_cache, page_table, seqlens_k, min(page_table.shape[-1] * k_cache.shape[1], 2 ** 31 - 1), key_weights, key_positions,
+                          k_scales, v_scales)
     _int32("the number of new tokens", total)
-    a.dtype = _dtype_code(k_cache)
+    a.dtype = _dtype_code(k)
+    _check(k.device == k_cache.device and (scales is not None or k.dtype == k_cache.dtype), "k must be on the cache's device, and of its dtype")
     for name, t in (("k", k), ("v", v)):
-        _check_heads(name, t, k_cache, total, D)
+        _check_heads(name, t, k, total, D)
         _check(t.shape[1] == k_cache.shape[2], "%s must have the cache's heads" % name)
         setattr(a, name, t.data_ptr())
         setattr(a, name + "_row_stride", t.stride(0))
@@ -1224,40 +1259,50 @@ def paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k,
     c.cu_seqlens_q, c.nheads_q, c.total_q, c.max_seqlen_q = cu_seqlens_q.data_ptr(), c.nheads_k, total, max(total, 1)
     _check((q_weight is None) == (k_weight is None), "q_weight and k_weight come together")
     if k_weight is not None:
-        a.weight_dtype = _check_norm(q_weight, k_weight, k_cache, D)
+        a.weight_dtype = _check_norm(q_weight, k_weight, k, D)
         a.q_weight, a.k_weight = q_weight.data_ptr(), k_weight.data_ptr()
-    _check_tables(cos, sin, k_cache, D)
+    _check_tables(cos, sin, k, D)
     if cos is not None:
         a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    _check_positions(positions, k_cache, total)
+    _check_positions(positions, k, total)
     a.positions = positions.data_ptr() if positions is not None else None
     a.eps = eps
     with _OnDevice(k_cache.device):
         if q is not None:
-            _check_heads("q", q, k_cache, total, D)
+            _check_heads("q", q, k, total, D)
             _check(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "the query heads must be a multiple of the key heads")
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            _check_heads("q_out", q_out, k_cache, total, D)
+            _check_heads("q_out", q_out, k, total, D)
             _check(q_out.shape == q.shape, "q_out must have q's shape")
             c.nheads_q, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
             a.q_row_stride, a.q_head_stride, a.q_out_row_stride, a.q_out_head_stride = q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
         a.stream = _stream_handle(k_cache.device)
-        rc = lib.fa_paged_append(ctypes.byref(a))
+        rc = lib.fa_paged_append_with(ctypes.byref(a), None if scales is None else ctypes.byref(scales))
     if rc != 0:
         _raise(rc, lib)
     return q_out
 
 
-def paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, return_lse=False, out=None):
-    """Attention of the new tokens' q (total, heads, head_dim) over a paged cache: [o] or [o, softmax_lse] (fa_paged_fwd)."""
+def paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, return_lse=False, out=None,
+              k_scales=None, v_scales=None, cu_groups=None, prefix_lens=None, max_prefix_len=0):
+    """Attention of the new tokens' q (total, heads, head_dim) over a paged cache: [o] or [o, softmax_lse] (fa_paged_fwd_with).  cu_groups, prefix_lens: of groups of
+    sequences that begin with the same keys."""
     lib = load_library()
     a = PagedFwdArgs()
     a.struct_bytes = ctypes.sizeof(a)
-    _paged_cache(a.cache, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k)
+    scales = _paged_cache(a.cache, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, k_scales=k_scales, v_scales=v_scales)
     _paged_queries(a.cache, q, k_cache, cu_seqlens_q, max_seqlen_q)
     a.dtype = _dtype_code(q)
     dev = q.device
+    prefix = None
+    _check((cu_groups is None) == (prefix_lens is None), "cu_groups and prefix_lens come together")
+    if cu_groups is not None:
+        _check_seqlens("prefix_lens", prefix_lens, a.cache.batch, k_cache.device)
+        _check(cu_groups.device == k_cache.device and cu_groups.dtype == torch.int32 and cu_groups.dim() == 1 and 2 <= cu_groups.numel() <= a.cache.batch + 1 and
+               cu_groups.is_contiguous(), "cu_groups must be a contiguous int32 tensor on the cache's device: where each group's sequences begin, and the batch's end")
+        prefix = PagedPrefix(ctypes.sizeof(PagedPrefix), cu_groups.numel() - 1, _int32("max_prefix_len", max_prefix_len), 0, cu_groups.data_ptr(), prefix_lens.data_ptr())
+    more = [None if x is None else ctypes.byref(x) for x in (scales, prefix)]
     with _OnDevice(dev):
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=dev)
@@ -1270,14 +1315,42 @@ def paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seql
         a.q, a.o = q.data_ptr(), out.data_ptr()
         a.q_row_stride, a.q_head_stride, a.o_row_stride, a.o_head_stride = q.stride(0), q.stride(1), out.stride(0), out.stride(1)
         a.softmax_scale, a.is_causal = float(softmax_scale), int(bool(is_causal))
-        a.workspace_bytes = lib.fa_paged_fwd_workspace_bytes(ctypes.byref(a))
+        a.workspace_bytes = lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), *more)
         ws = torch.empty((a.workspace_bytes,), dtype=torch.uint8, device=dev) if a.workspace_bytes else None
         a.workspace = ws.data_ptr() if ws is not None else None
         a.stream = _stream_handle(dev)
-        rc = lib.fa_paged_fwd(ctypes.byref(a))
+        rc = lib.fa_paged_fwd_with(ctypes.byref(a), *more)
     if rc != 0:
         _raise(rc, lib)
     return [out, lse] if return_lse else [out]
+
+
+def paged_read(k_cache, v_cache, page_table, cu_seqlens, seqlens_k, total, dtype, k_scales=None, v_scales=None):
+    """(k, v) (total, heads, head_dim) in `dtype`: the packed tokens out of the pages of their sequences (fa_paged_read)."""
+    lib = load_library()
+    a = PagedReadArgs()
+    a.struct_bytes = ctypes.sizeof(a)
+    c = a.cache
+    _check(v_cache is not None, "v_cache is required")
+    _check(dtype in (torch.float16, torch.bfloat16), "keys and values are read as fp16 or bf16")
+    scales = _paged_cache(c, k_cache, v_cache, page_table, seqlens_k, min(page_table.shape[-1] * k_cache.shape[1], 2 ** 31 - 1), k_scales=k_scales, v_scales=v_scales)
+    _check(scales is not None or dtype == k_cache.dtype, "a cache in 16 bits is read as what it is")
+    _check_cu("cu_seqlens", cu_seqlens, c.batch)
+    _check(cu_seqlens.device == k_cache.device, "cu_seqlens must be on the cache's device")
+    total = _int32("the number of tokens", total)
+    _check(total >= 0, "the number of tokens is negative")
+    c.cu_seqlens_q, c.total_q = cu_seqlens.data_ptr(), total
+    dev = k_cache.device
+    with _OnDevice(dev):
+        k, v = (torch.empty((total,) + tuple(k_cache.shape[2:]), dtype=dtype, device=dev) for _ in range(2))
+        a.dtype = _dtype_code(k)
+        a.k_out, a.v_out = k.data_ptr(), v.data_ptr()
+        a.k_row_stride, a.k_head_stride, a.v_row_stride, a.v_head_stride = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
+        a.stream = _stream_handle(dev)
+        rc = lib.fa_paged_read(ctypes.byref(a), None if scales is None else ctypes.byref(scales))
+    if rc != 0:
+        _raise(rc, lib)
+    return k, v
 
 
 def paged_key_weights(q, softmax_lse, k_cache, key_weights, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal):

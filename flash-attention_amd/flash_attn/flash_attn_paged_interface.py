@@ -12,6 +12,12 @@ A step of a model advances seqlens_k by the new tokens once; every layer then st
 find new lengths, tables and tokens in the same tensors (PagedKVCache's book is the host's: its steps are made, and its evictions called, outside).
 max_seqlen_k then has to hold for all of them; it bounds the work that is cut, not the memory that is read.
 
+A cache in 8 bits: k_cache and v_cache are torch.float8_e4m3fn, and beside them k_scales and v_scales (pages, nheads_k, page size) uint8 hold an exponent + 127 for every
+slot and key head, of which the row stands for its values times 2^exponent.  paged_append_func rounds each row once, to the nearest values under the smallest exponent
+that brings its largest finite magnitude to 448 or below (-15 to 8 for fp16, -100 to 120 for bf16; under the largest one values end at 240; inf and NaN become NaN):
+a value is off by 2^-4 of itself at most, and by 2^-10 of the scale where it is small.  What a row stands for is exact in the dtype it came from, which is the one to read it
+in and to attend with.  Key weights and eviction are those of caches in 16 bits.
+
 What lies in page_table and seqlens_k is never trusted with an address: entries outside the pool are read as its first or last page and never written to,
 lengths count as far as the table goes.  Pages that several sequences list (a common prompt), or one lists twice, may be read by all of them and must not be
 appended to, weighted or evicted from: the order in which several workgroups write one slot is not defined.  Keys and values behind a sequence's length are not
@@ -35,38 +41,76 @@ def _inference(*tensors, constants=()):
 
 
 def paged_append_func(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, q_weight=None, k_weight=None, cos_half=None, sin_half=None,
-                      positions=None, eps=1e-6, key_weights=None, key_positions=None):
+                      positions=None, eps=1e-6, key_weights=None, key_positions=None, k_scales=None, v_scales=None):
     """Stores the new tokens' k and v (total, nheads_k, headdim) into the pages of their sequences, behind what is there: row i of sequence b goes to
     slot seqlens_k[b] - (its new tokens) + i.  In the same pass k, and q (total, nheads, headdim) if it is given, are normalised (q_weight, k_weight: see
     apply_qk_norm_rotary) and turned by their positions (cos_half, sin_half) - positions[row], or the slot, clamped to the tables: they are on the device, and what
     the tables have to reach is the caller's to know (PagedStep does).  Returns the new q, or None.
     key_weights, key_positions (pages, nheads_k, page size): set to 0 and the position for the new tokens (for paged_key_weights_func and
-    paged_evict_func).  Rows behind the last sequence, and tokens for which the page table has no room, are not stored; their rows of the returned q
+    paged_evict_func).  k_scales, v_scales: of a cache in 8 bits, into which k and v are quantised.  Rows behind the last sequence, and tokens for which the page table has no room, are not stored; their rows of the returned q
     hold nothing."""
     done = _backend.passes().paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, q_weight, k_weight, cos_half, sin_half, positions, eps,
-                                          key_weights, key_positions)
+                                          key_weights, key_positions, k_scales, v_scales)
     if done is not None:
         return None if q is None else done
     _inference(q, k, v, q_weight, k_weight, constants=(k_cache, v_cache, cos_half, sin_half, key_weights))
     return _backend.paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, None, q_weight, k_weight, cos_half, sin_half, positions, eps,
-                                 key_weights, key_positions)
+                                 key_weights, key_positions, k_scales, v_scales)
 
 
 def flash_attn_paged_func(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale=None, causal=True,
-                          return_softmax_lse=False):
+                          return_softmax_lse=False, k_scales=None, v_scales=None):
     """Attention of the new tokens q (total, nheads, headdim) over their sequences' pages; nheads is a multiple of nheads_k, and query head h attends with
     key head h // (nheads // nheads_k).  causal: a sequence's last new token sees all its keys, the one before it one less, and so on (the new tokens'
-    own keys are in the cache); a token that sees no key gives zeros.  max_seqlen_q, max_seqlen_k: at least the longest of each.
+    own keys are in the cache); a token that sees no key gives zeros.  max_seqlen_q, max_seqlen_k: at least the longest of each.  k_scales, v_scales: of a cache in 8 bits.
     Returns out (total, nheads, headdim), or (out, softmax_lse), softmax_lse (batch, nheads, max_seqlen_q rounded up to 16) fp32, -inf for a token
     that sees no key.  Rows of out behind the last sequence hold nothing."""
     done = _backend.passes().paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
-                                       return_softmax_lse)
+                                       return_softmax_lse, k_scales, v_scales)
     if done is not None:
         return done
     _inference(q, k_cache, v_cache)
     scale = q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale
-    r = _backend.paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, return_softmax_lse)
+    r = _backend.paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, return_softmax_lse,
+                           k_scales=k_scales, v_scales=v_scales)
     return (r[0], r[1]) if return_softmax_lse else r[0]
+
+
+def flash_attn_paged_prefix_func(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, cu_groups, prefix_lens, max_prefix_len,
+                                 softmax_scale=None, causal=True, return_softmax_lse=False, k_scales=None, v_scales=None):
+    """flash_attn_paged_func for sequences that begin with the same keys (a system prompt, several answers to one question), which are read once for all of them.
+    cu_groups (groups + 1,) int32: group g is the sequences cu_groups[g] .. cu_groups[g + 1] - 1, from 0 to the batch's end.  prefix_lens (batch,) int32: how many
+    leading keys the sequences of a group have in the same pages - one number within a group, 0 for nothing, and no more keys than the sequence's first new token sees.
+    Whole pages count; what is left of a prefix is read as each sequence's own.  max_prefix_len: at least the longest; prefixes count up to it.  As always each sequence
+    lists all its pages, and its result is that of flash_attn_paged_func, rounded elsewhere; where prefixes are shorter in one sequence of a group than in the next, or the
+    pages are not the same, the first one's keys stand for all."""
+    done = _backend.passes().paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
+                                       return_softmax_lse, k_scales, v_scales, cu_groups, prefix_lens, max_prefix_len)
+    if done is not None:
+        return done
+    _inference(q, k_cache, v_cache)
+    scale = q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale
+    if cu_groups is None or prefix_lens is None:
+        raise RuntimeError("cu_groups and prefix_lens say which sequences share what: flash_attn_paged_func takes those that share nothing")
+    r = _backend.paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, return_softmax_lse,
+                           k_scales=k_scales, v_scales=v_scales, cu_groups=cu_groups, prefix_lens=prefix_lens, max_prefix_len=max_prefix_len)
+    return (r[0], r[1]) if return_softmax_lse else r[0]
+
+
+def paged_read_func(k_cache, v_cache, page_table, cu_seqlens, seqlens_k, total, k_scales=None, v_scales=None, dtype=None):
+    """The keys and values that the cache holds, packed: the counterpart of paged_append_func.  Row i of sequence b's cu_seqlens[b + 1] - cu_seqlens[b] rows is slot
+    seqlens_k[b] - (its rows) + i, so cu_seqlens made of seqlens_k gives whole sequences, and that of the last step what the step stored.  total: rows of the results
+    (total, nheads_k, headdim), cu_seqlens' last entry or more.  dtype: the cache's; for a cache in 8 bits (k_scales, v_scales) fp16 or bf16, whichever it was made from:
+    nothing is rounded.  Rows that stand for no slot are zeros.  Returns (k, v)."""
+    if dtype is None and k_scales is None:
+        dtype = k_cache.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("keys and values are read as fp16 or bf16 (dtype), the one that they came from")
+    done = _backend.passes().paged_read(k_cache, v_cache, page_table, cu_seqlens, seqlens_k, total, 0 if dtype == torch.float16 else 1, k_scales, v_scales)
+    if done is not None:
+        return done
+    _inference(k_cache, v_cache)
+    return _backend.paged_read(k_cache, v_cache, page_table, cu_seqlens, seqlens_k, total, dtype, k_scales, v_scales)
 
 
 def paged_key_weights_func(q, softmax_lse, k_cache, key_weights, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale=None,

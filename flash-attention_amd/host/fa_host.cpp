@@ -454,6 +454,7 @@ PyMethodDef methods[] = {
     {"qk_norm_rotary", (PyCFunction)(void (*)(void))guarded<qk_norm_rotary>, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)(void))guarded<paged_append>, METH_FASTCALL, nullptr},
     {"paged_fwd", (PyCFunction)(void (*)(void))guarded<paged_fwd>, METH_FASTCALL, nullptr},
+    {"paged_read", (PyCFunction)(void (*)(void))guarded<paged_read>, METH_FASTCALL, nullptr},
     {"paged_key_weights", (PyCFunction)(void (*)(void))guarded<paged_key_weights>, METH_FASTCALL, nullptr},
     {"paged_evict", (PyCFunction)(void (*)(void))guarded<paged_evict>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -15,18 +15,19 @@ struct PagedLibrary {
   int (*qk_norm)(const fa_qk_norm_args*);
   int (*qk_norm_bwd)(const fa_qk_norm_args*);
   size_t (*qk_norm_bwd_workspace_bytes)(const fa_qk_norm_args*);
-  int (*append)(const fa_paged_append_args*);
-  int (*fwd)(const fa_paged_fwd_args*);
-  size_t (*fwd_workspace_bytes)(const fa_paged_fwd_args*);
+  int (*append)(const fa_paged_append_args*, const fa_paged_scales*);
+  int (*fwd)(const fa_paged_fwd_args*, const fa_paged_scales*, const fa_paged_prefix*);
+  size_t (*fwd_workspace_bytes)(const fa_paged_fwd_args*, const fa_paged_scales*, const fa_paged_prefix*);
+  int (*read)(const fa_paged_read_args*, const fa_paged_scales*);
   int (*key_weights)(const fa_paged_fwd_args*);
   int (*evict)(const fa_paged_evict_args*);
   size_t (*evict_workspace_bytes)(const fa_paged_evict_args*);
 } g_paged;
 bool g_paged_bound = false;
 
-// bind_paged(addresses of the nine entry points above, in their order)
+// bind_paged(addresses of the ten entry points above, in their order)
 PyObject* py_bind_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  constexpr int kEntries = 9;
+  constexpr int kEntries = 10;
   if (n != kEntries) return PyErr_Format(PyExc_TypeError, "bind_paged takes %d addresses", kEntries);
   void* f[kEntries];
   for (int i = 0; i < kEntries; i++) {
@@ -190,11 +191,21 @@ PyObject* qk_norm_rotary(PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- the paged cache
+// The exponents of a cache in 8 bits, beside its tensors (both or neither)
+struct Scales {
+  const at::Tensor *k = nullptr, *v = nullptr;
+  fa_paged_scales s;
+  const fa_paged_scales* get() {
+    if (!k) return nullptr;
+    s = fa_paged_scales{(uint32_t)sizeof(s), 0, ptr(*k), ptr(*v)};
+    return &s;
+  }
+};
 // Fills a cache's fields; false where the binding would refuse (or copy) something.
 bool fill_cache(fa_paged_cache* c, const at::Tensor* k, const at::Tensor* v, bool needs_v, const at::Tensor* table, const at::Tensor* lens, int64_t max_k,
-                const at::Tensor* weights, const at::Tensor* positions) {
+                const at::Tensor* weights, const at::Tensor* positions, const Scales& scales = Scales()) {
   memset(c, 0, sizeof(*c));
-  if (!g_paged_bound || !on_current_device(k) || dtype_of(*k) < 0 || k->dim() != 4 || k->stride(3) != 1 || !dim_ok(k->size(3)) || (needs_v && !v)) return false;
+  if (!g_paged_bound || !on_current_device(k) || (scales.k ? k->scalar_type() != at::kFloat8_e4m3fn : dtype_of(*k) < 0) || !scales.k != !scales.v || k->dim() != 4 || k->stride(3) != 1 || !dim_ok(k->size(3)) || (needs_v && !v)) return false;
   if (v && (v->device() != k->device() || v->scalar_type() != k->scalar_type() || v->sizes() != k->sizes() || v->stride(3) != 1)) return false;
   if (!table || table->device() != k->device() || table->scalar_type() != at::kInt || table->dim() != 2 || (table->stride(1) != 1 && table->size(1) != 1)) return false;
   const int64_t batch = table->size(0), cols = table->size(1);
@@ -205,7 +216,7 @@ bool fill_cache(fa_paged_cache* c, const at::Tensor* k, const at::Tensor* v, boo
     return !t || (t->device() == k->device() && t->scalar_type() == type && t->dim() == 3 && t->size(0) == k->size(0) && t->size(1) == k->size(2) &&
                   t->size(2) == k->size(1) && t->is_contiguous());
   };
-  if (!beside(weights, at::kFloat) || !beside(positions, at::kInt)) return false;
+  if (!beside(weights, at::kFloat) || !beside(positions, at::kInt) || !beside(scales.k, at::kByte) || !beside(scales.v, at::kByte)) return false;
   c->k_cache = ptr(*k);
   c->k_page_stride = k->stride(0); c->k_slot_stride = k->stride(1); c->k_head_stride = k->stride(2);
   if (v) {
@@ -224,7 +235,7 @@ bool fill_cache(fa_paged_cache* c, const at::Tensor* k, const at::Tensor* v, boo
   return true;
 }
 bool fill_queries(fa_paged_cache* c, const at::Tensor* q, const at::Tensor& k, const at::Tensor* cu, int64_t max_q) {
-  if (!q || !cu || !q->is_cuda() || q->device() != k.device() || q->scalar_type() != k.scalar_type() || q->dim() != 3 || q->size(2) != k.size(3) || q->stride(2) != 1 ||
+  if (!q || !cu || !q->is_cuda() || q->device() != k.device() || dtype_of(*q) < 0 || (k.scalar_type() != at::kFloat8_e4m3fn && q->scalar_type() != k.scalar_type()) || q->dim() != 3 || q->size(2) != k.size(3) || q->stride(2) != 1 ||
       q->size(1) <= 0 || !small(q->size(1)) || q->size(1) % k.size(2) != 0 || !small(q->size(0)) || max_q <= 0 || !is_cu(cu, k) || cu->size(0) != (int64_t)c->batch + 1)
     return false;
   c->cu_seqlens_q = (const int32_t*)ptr(*cu);
@@ -234,27 +245,30 @@ bool fill_queries(fa_paged_cache* c, const at::Tensor* q, const at::Tensor& k, c
   return true;
 }
 
-// paged_append(q, k, v, k_cache, v_cache, table, cu, seqlens, q_weight, k_weight, cos, sin, positions, eps, key_weights, key_positions) -> the new q, True
-// without one, or None
+// paged_append(q, k, v, k_cache, v_cache, table, cu, seqlens, q_weight, k_weight, cos, sin, positions, eps, key_weights, key_positions[, k_scales, v_scales])
+// -> the new q, True without one, or None
 PyObject* paged_append(PyObject* const* a, Py_ssize_t n) {
-  if (n != 16) return PyErr_Format(PyExc_TypeError, "paged_append takes 16 arguments");
+  if (n != 16 && n != 18) return PyErr_Format(PyExc_TypeError, "paged_append takes 16 or 18 arguments");
   bool ok = true;
   const at::Tensor* t[13];
   for (int i = 0; i < 13; i++) t[i] = tensor(a[i], ok);
   const at::Tensor *q = t[0], *k = t[1], *v = t[2], *kc = t[3], *cu = t[6], *qw = t[8], *kw = t[9], *cos = t[10], *sin = t[11], *pos = t[12];
   const at::Tensor *weights = tensor(a[14], ok), *positions = tensor(a[15], ok);
+  Scales scales;
+  if (n == 18) scales.k = tensor(a[16], ok), scales.v = tensor(a[17], ok);
   fa_paged_append_args f;
   memset(&f, 0, sizeof(f));
   double eps;
   Rows rk, rv, rq;
   if (!ok || !as_double(a[13], &eps) || needs_grad({q, k, v, qw, kw}) || !k || !v || !kc || !t[5] || kc->dim() != 4 || t[5]->dim() != 2 ||
-      !fill_cache(&f.cache, kc, t[4], true, t[5], t[7], t[5]->size(1) * kc->size(1), weights, positions) || k->dim() != 3 || v->dim() != 3 || !rows_of(*k, *kc, &rk) ||
-      !rows_of(*v, *kc, &rv) || rk.heads != kc->size(2) || rv.heads != rk.heads || rk.dim != kc->size(3) || rv.dim != rk.dim || rv.rows != rk.rows || !is_cu(cu, *kc) ||
-      cu->size(0) != (int64_t)f.cache.batch + 1 || ((qw || kw) && !norm_ok(qw, kw, *kc, rk.dim)) || !angles_ok(cos, sin, *kc, rk.dim) || !positions_ok(pos, *kc, rk.rows))
+      !fill_cache(&f.cache, kc, t[4], true, t[5], t[7], t[5]->size(1) * kc->size(1), weights, positions, scales) || dtype_of(*k) < 0 || k->device() != kc->device() ||
+      (!scales.k && k->scalar_type() != kc->scalar_type()) || k->dim() != 3 || v->dim() != 3 || !rows_of(*k, *k, &rk) || !rows_of(*v, *k, &rv) || rk.heads != kc->size(2) ||
+      rv.heads != rk.heads || rk.dim != kc->size(3) || rv.dim != rk.dim || rv.rows != rk.rows || !is_cu(cu, *kc) || cu->size(0) != (int64_t)f.cache.batch + 1 ||
+      ((qw || kw) && !norm_ok(qw, kw, *k, rk.dim)) || !angles_ok(cos, sin, *k, rk.dim) || !positions_ok(pos, *k, rk.rows))
     Py_RETURN_NONE;
-  if (q && (q->dim() != 3 || !rows_of(*q, *kc, &rq) || rq.rows != rk.rows || rq.dim != rk.dim || rq.heads <= 0 || rq.heads % rk.heads != 0)) Py_RETURN_NONE;
+  if (q && (q->dim() != 3 || !rows_of(*q, *k, &rq) || rq.rows != rk.rows || rq.dim != rk.dim || rq.heads <= 0 || rq.heads % rk.heads != 0)) Py_RETURN_NONE;
   f.struct_bytes = sizeof(f);
-  f.dtype = dtype_of(*kc);
+  f.dtype = dtype_of(*k);
   f.cache.cu_seqlens_q = (const int32_t*)ptr(*cu);
   f.cache.total_q = (int32_t)rk.rows;
   f.cache.max_seqlen_q = (int32_t)(rk.rows > 0 ? rk.rows : 1);
@@ -277,16 +291,17 @@ PyObject* paged_append(PyObject* const* a, Py_ssize_t n) {
   }
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_paged.append(&f);
+  rc = g_paged.append(&f, scales.get());
   Py_END_ALLOW_THREADS
   if (rc != 0) return refused(rc);
   if (!q) Py_RETURN_TRUE;
   return THPVariable_Wrap(std::move(qo));
 }
 
-// paged_fwd(q, k_cache, v_cache, table, cu, seqlens, max_q, max_k, scale or None, causal, return_lse) -> out, (out, lse) or None
+// paged_fwd(q, k_cache, v_cache, table, cu, seqlens, max_q, max_k, scale or None, causal, return_lse[, k_scales, v_scales[, cu_groups, prefix_lens, max_prefix]])
+// -> out, (out, lse) or None
 PyObject* paged_fwd(PyObject* const* a, Py_ssize_t n) {
-  if (n != 11) return PyErr_Format(PyExc_TypeError, "paged_fwd takes 11 arguments");
+  if (n != 11 && n != 13 && n != 16) return PyErr_Format(PyExc_TypeError, "paged_fwd takes 11, 13 or 16 arguments");
   bool ok = true;
   const at::Tensor* t[6];
   for (int i = 0; i < 6; i++) t[i] = tensor(a[i], ok);
@@ -296,9 +311,20 @@ PyObject* paged_fwd(PyObject* const* a, Py_ssize_t n) {
   int64_t mq, mk;
   double scale = 0;
   int32_t causal, want_lse;
+  Scales scales;
+  if (n > 11) scales.k = tensor(a[11], ok), scales.v = tensor(a[12], ok);
   if (!ok || !as_int(a[6], &mq) || !as_int(a[7], &mk) || (a[8] != Py_None && !as_double(a[8], &scale)) || !as_flag(a[9], &causal) || !as_flag(a[10], &want_lse) ||
-      needs_grad({q, kc, vc}) || !fill_cache(&f.cache, kc, vc, true, t[3], t[5], mk, nullptr, nullptr) || !fill_queries(&f.cache, q, *kc, t[4], mq))
+      needs_grad({q, kc, vc}) || !fill_cache(&f.cache, kc, vc, true, t[3], t[5], mk, nullptr, nullptr, scales) || !fill_queries(&f.cache, q, *kc, t[4], mq))
     Py_RETURN_NONE;
+  fa_paged_prefix prefix;
+  memset(&prefix, 0, sizeof(prefix));
+  if (n == 16) {
+    const at::Tensor *groups = tensor(a[13], ok), *lens = tensor(a[14], ok);
+    int64_t most;
+    const auto ints = [&](const at::Tensor* x) { return x && x->device() == kc->device() && x->scalar_type() == at::kInt && x->dim() == 1 && x->is_contiguous(); };
+    if (!ok || !ints(groups) || !ints(lens) || lens->size(0) != f.cache.batch || groups->size(0) < 2 || groups->size(0) > (int64_t)f.cache.batch + 1 || !as_int(a[15], &most)) Py_RETURN_NONE;
+    prefix = fa_paged_prefix{(uint32_t)sizeof(prefix), (int32_t)(groups->size(0) - 1), (int32_t)most, 0, (const int32_t*)ptr(*groups), (const int32_t*)ptr(*lens)};
+  }
   if (a[8] == Py_None) scale = 1 / std::sqrt((double)f.cache.head_dim);
   at::Tensor o = at::empty(q->sizes(), plain(*q)), lse, ws;
   f.struct_bytes = sizeof(f);
@@ -311,7 +337,9 @@ PyObject* paged_fwd(PyObject* const* a, Py_ssize_t n) {
   }
   f.softmax_scale = (float)scale;
   f.is_causal = causal;
-  f.workspace_bytes = g_paged.fwd_workspace_bytes(&f);
+  const fa_paged_scales* const s8 = scales.get();
+  const fa_paged_prefix* const px = n == 16 ? &prefix : nullptr;
+  f.workspace_bytes = g_paged.fwd_workspace_bytes(&f, s8, px);
   if (f.workspace_bytes) {
     ws = at::empty({(int64_t)f.workspace_bytes}, plain(*q).dtype(at::kByte));
     f.workspace = ptr(ws);
@@ -319,7 +347,7 @@ PyObject* paged_fwd(PyObject* const* a, Py_ssize_t n) {
   f.stream = stream_of(*q);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_paged.fwd(&f);
+  rc = g_paged.fwd(&f, s8, px);
   Py_END_ALLOW_THREADS
   if (rc != 0) return refused(rc);
   PyObject* po = THPVariable_Wrap(std::move(o));
@@ -328,6 +356,47 @@ PyObject* paged_fwd(PyObject* const* a, Py_ssize_t n) {
   PyObject* r = pl ? PyTuple_Pack(2, po, pl) : nullptr;
   Py_DECREF(po);
   Py_XDECREF(pl);
+  return r;
+}
+
+// paged_read(k_cache, v_cache, table, cu, seqlens, total, dtype (0 fp16, 1 bf16), k_scales, v_scales) -> (k, v) or None
+PyObject* paged_read(PyObject* const* a, Py_ssize_t n) {
+  if (n != 9) return PyErr_Format(PyExc_TypeError, "paged_read takes 9 arguments");
+  bool ok = true;
+  const at::Tensor* t[5];
+  for (int i = 0; i < 5; i++) t[i] = tensor(a[i], ok);
+  const at::Tensor *kc = t[0], *vc = t[1], *cu = t[3];
+  Scales scales;
+  scales.k = tensor(a[7], ok);
+  scales.v = tensor(a[8], ok);
+  fa_paged_read_args f;
+  memset(&f, 0, sizeof(f));
+  int64_t total, dtype;
+  if (!ok || !as_int(a[5], &total) || !as_int(a[6], &dtype) || (dtype != FA_FP16 && dtype != FA_BF16) || total < 0 || !kc || !t[2] || kc->dim() != 4 || t[2]->dim() != 2 ||
+      needs_grad({kc, vc}) || !fill_cache(&f.cache, kc, vc, true, t[2], t[4], t[2]->size(1) * kc->size(1), nullptr, nullptr, scales) ||
+      (!scales.k && dtype_of(*kc) != dtype) || !is_cu(cu, *kc) || cu->size(0) != (int64_t)f.cache.batch + 1)
+    Py_RETURN_NONE;
+  const at::TensorOptions as = plain(*kc).dtype(dtype == FA_FP16 ? at::kHalf : at::kBFloat16);
+  at::Tensor k = at::empty({total, kc->size(2), kc->size(3)}, as), v = at::empty({total, kc->size(2), kc->size(3)}, as);
+  f.struct_bytes = sizeof(f);
+  f.dtype = (int32_t)dtype;
+  f.cache.cu_seqlens_q = (const int32_t*)ptr(*cu);
+  f.cache.total_q = (int32_t)total;
+  f.cache.max_seqlen_q = (int32_t)(total > 0 ? total : 1);
+  f.k_out = ptr(k); f.v_out = ptr(v);
+  f.k_row_stride = f.v_row_stride = kc->size(2) * kc->size(3);
+  f.k_head_stride = f.v_head_stride = kc->size(3);
+  f.stream = stream_of(*kc);
+  int rc;
+  const fa_paged_scales* const s8 = scales.get();
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_paged.read(&f, s8);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return refused(rc);
+  PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
+  PyObject* r = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
+  Py_XDECREF(pk);
+  Py_XDECREF(pv);
   return r;
 }
 

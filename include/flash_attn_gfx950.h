@@ -427,6 +427,48 @@ typedef struct fa_paged_fwd_args {
 int fa_paged_fwd(const fa_paged_fwd_args* args);
 size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_args* args);
 
+/* A cache in 8 bits.  A slot's head_dim keys (values) of a key head are e4m3 numbers y_i (one byte each; the strides above count them, multiples of 16) that stand
+ * for y_i * 2^(s - 127), s being the row's byte in k_scales (v_scales): [n_pages, nheads_k, page_size] contiguous, 16-byte aligned.  What fa_paged_append_with
+ * stores: s - 127 is the smallest exponent, from -15 to 8 for FA_FP16 and -100 to 120 for FA_BF16, with 448 * 2^(s - 127) at least the row's largest finite magnitude,
+ * y_i the nearest to x_i * 2^(127 - s) (ties to even; of the largest exponent at most 240 in magnitude; inf and NaN: NaN).  Every such row is exact in that dtype. */
+typedef struct fa_paged_scales {
+  uint32_t struct_bytes;
+  uint32_t reserved0; /* 0 */
+  void* k_scales;
+  void* v_scales;
+} fa_paged_scales;
+
+/* Sequences that begin with the same keys.  Group g is sequences cu_groups[g] .. cu_groups[g + 1] - 1 (n_groups + 1 int32, from 0 to batch); the sequences of a group list
+ * the same pages for their first prefix_lens[b] keys (batch int32, one value within a group, at most the keys that the sequence's first new token sees;
+ * whole pages count, the rest is each sequence's own).  max_prefix_len: at least the longest prefix, 0 if there is none; longer ones count as that. */
+typedef struct fa_paged_prefix {
+  uint32_t struct_bytes;
+  int32_t n_groups, max_prefix_len;
+  int32_t reserved0; /* 0 */
+  const int32_t* cu_groups;
+  const int32_t* prefix_lens;
+} fa_paged_prefix;
+
+/* fa_paged_append into a cache in 8 bits (scales == NULL: fa_paged_append).  k is rounded once, behind norm and rotation. */
+int fa_paged_append_with(const fa_paged_append_args* args, const fa_paged_scales* scales);
+/* fa_paged_fwd over a cache in 8 bits (scales != NULL) and / or with shared prefixes (prefix != NULL), whose keys are read once for all new tokens of a group: what
+ * fa_paged_fwd gives for the same tables, rounded elsewhere. */
+int fa_paged_fwd_with(const fa_paged_fwd_args* args, const fa_paged_scales* scales, const fa_paged_prefix* prefix);
+size_t fa_paged_fwd_with_workspace_bytes(const fa_paged_fwd_args* args, const fa_paged_scales* scales, const fa_paged_prefix* prefix);
+
+/* The tokens that fa_paged_append stored, out of their pages: row i of the cu_seqlens_q[b + 1] - cu_seqlens_q[b] rows of sequence b becomes the key and value of slot
+ * seqlens_k[b] - rows + i.  k_out, v_out: [total_q, nheads_k, head_dim] of `dtype`, exact.  scales == NULL: a cache in 16 bits of that dtype.  Rows that stand
+ * for no slot (behind the last sequence; in front of a sequence's first key) become zeros.  nheads_q and max_seqlen_q are not read. */
+typedef struct fa_paged_read_args {
+  uint32_t struct_bytes;
+  int32_t dtype;
+  fa_paged_cache cache;
+  void *k_out, *v_out;
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+  void* stream;
+} fa_paged_read_args;
+int fa_paged_read(const fa_paged_read_args* args, const fa_paged_scales* scales);
+
 /* key_weights of every key += the sum over the new tokens and the query heads of its group of exp(softmax_scale * q.k - softmax_lse), q and
  * softmax_lse being those of fa_paged_fwd over the same cache (o and workspace are not read).  One owner per key: reproducible bit for bit. */
 int fa_paged_key_weights(const fa_paged_fwd_args* args);
