@@ -52,6 +52,18 @@ FA_DEVICE typename Elem<T>::vec8 dequant8(u32x2 w, float scale) {
   return dequant8(w, scale, static_cast<typename Elem<T>::vec8*>(nullptr));
 }
 
+// The largest finite magnitude of eight values.  Infinities are rare: they are looked for once for the wave, NaN are nobody's maximum anyway.
+FA_DEVICE float finite_top(const float (&x)[8]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = fmaxf(top, __builtin_fabsf(x[i]));
+  if (__builtin_expect(__any(top == INFINITY), 0)) {
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = __builtin_fabsf(x[i]) < INFINITY ? fmaxf(top, __builtin_fabsf(x[i])) : top;
+  }
+  return top;
+}
 // The byte of a row whose largest finite magnitude is `top` (448 = 7/8 * 2^9)
 template <typename T>
 FA_DEVICE int row_exponent(float top) {
@@ -60,15 +72,19 @@ FA_DEVICE int row_exponent(float top) {
   e = e < RowExponent<T>::least ? RowExponent<T>::least : e;  // (zeros, too)
   return (e > RowExponent<T>::most ? RowExponent<T>::most : e) + 127;
 }
-// Eight values of a row with that byte
+// Eight values of a row with that byte.  Finite ones are 448 at most, and what is not becomes NaN as it is converted.
 template <typename T>
 FA_DEVICE u32x2 quant8(const float (&x)[8], int byte) {
-  const float down = power_of_two(254 - byte), most = byte == RowExponent<T>::most + 127 ? 240.f : 448.f;
+  const float down = power_of_two(254 - byte);
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float z = __builtin_amdgcn_fmed3f(x[i] * down, -most, most);
-    y[i] = __builtin_fabsf(x[i]) < INFINITY ? z : NAN;
+  for (int i = 0; i < 8; i++) y[i] = x[i] * down;
+  if (__builtin_expect(__any(byte == RowExponent<T>::most + 127), 0)) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float z = __builtin_amdgcn_fmed3f(y[i], -240.f, 240.f);
+      if (byte == RowExponent<T>::most + 127 && __builtin_fabsf(y[i]) < INFINITY) y[i] = z;
+    }
   }
   u32x2 w;
 #pragma unroll

@@ -37,8 +37,8 @@ FA_DEVICE void paged_append(const AppendParams p) {
   using vec8 = typename Elem<T>::vec8;
   const int group = blockIdx.x / p.pieces, piece = blockIdx.x - group * p.pieces;
   const int j = piece * (int)blockDim.x + threadIdx.x;
-  const int head = j / CH, ch = j % CH;
-  const bool on = j < p.per_row;
+  const bool on = j < p.per_row;  // (a thread without a place loads what the last one does, so that no branch stands between the rows' loads)
+  const int head = (on ? j : p.per_row - 1) / CH, ch = (on ? j : p.per_row - 1) % CH;
   // heads of q, then of k, then of v
   const int part = head < p.q_heads ? 0 : (head < p.q_heads + p.c.HK ? 1 : 2);
   const int h = part == 0 ? head : (part == 1 ? head - p.q_heads : head - p.q_heads - p.c.HK);
@@ -47,14 +47,19 @@ FA_DEVICE void paged_append(const AppendParams p) {
   const int64_t rs = part == 0 ? p.q_rs : (part == 1 ? p.k_rs : p.v_rs);
   const bool norm = p.kw != nullptr && part < 2, rot = p.cos != nullptr && part < 2;
   float w[8];
-  if (on && norm) load_weights<T>(part == 0 ? p.qw : p.kw, p.w_fp32 != 0, ch, w);
+  if (norm) load_weights<T>(part == 0 ? p.qw : p.kw, p.w_fp32 != 0, ch, w);
+#pragma unroll
+  for (int e = 0; e < 8; e++) asm volatile("" : "+v"(w[e]));  // (waited for here: in the loop it would be the last trip's stores that are waited for)
   for (int row0 = group * ROWS; row0 < p.c.total_q; row0 += p.groups * ROWS) {
     vec8 x8[ROWS];
 #pragma unroll
-    for (int i = 0; i < ROWS; i++)
-      if (on && row0 + i < p.c.total_q) x8[i] = bitcast<vec8>(ld_global16(src + (int64_t)(row0 + i) * rs));
+    for (int i = 0; i < ROWS; i++) x8[i] = bitcast<vec8>(ld_global16(src + (int64_t)(row0 + i < p.c.total_q ? row0 + i : p.c.total_q - 1) * rs));
     RowPlaces<ROWS> at;
     at.find(p.c, p.given_positions, row0);
+    // (the rows have come in with what that looked up; said here, since on paths that drop a row its load would count as under way, and the next trip's
+    // loads would wait for all of this one's stores)
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) asm volatile("" : "+v"(x8[i]));
     // What an address has of the lane, once; the rest of it, a row's, is wave-uniform.
     typedef typename Elem<T>::vec4 vec4;
     const bool moves_only = !norm && !rot;
@@ -62,13 +67,15 @@ FA_DEVICE void paged_append(const AppendParams p) {
     const int64_t lane_to = part == 0 ? (int64_t)h * p.qo_hs * 2 + ch * 16 : (part == 1 ? h * p.c.k_hs : h * p.c.v_hs) + ch * chunk;
     char* const base = part == 0 ? reinterpret_cast<char*>(p.q_out) + lane_to : (part == 1 ? p.c.k : p.c.v) + lane_to;
     vec4 c4[ROWS], s4[ROWS];
+    if (rot) {
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-      const int64_t row_at = (int64_t)table_row(at.pos[i], p.table_rows) * (D / 2);
-      if (on && rot) {
+      for (int i = 0; i < ROWS; i++) {
+        const int64_t row_at = (int64_t)table_row(at.pos[i], p.table_rows) * (D / 2);
         c4[i] = reinterpret_cast<const vec4*>(reinterpret_cast<const T*>(p.cos) + row_at)[ch];
         s4[i] = reinterpret_cast<const vec4*>(reinterpret_cast<const T*>(p.sin) + row_at)[ch];
       }
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) asm volatile("" : "+v"(c4[i]), "+v"(s4[i]));  // (all of them before the first store, behind which a load would wait for it)
     }
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
@@ -96,13 +103,7 @@ FA_DEVICE void paged_append(const AppendParams p) {
         }
         const int64_t m = m0 + ((int64_t)h << p.c.page_log2);
         if constexpr (kQuant) {
-          float top = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float a = __builtin_fabsf(x[e]);
-            top = a < INFINITY ? fmaxf(top, a) : top;
-          }
-          const int byte = row_exponent<T>(vector_max<CH>(top));
+          const int byte = row_exponent<T>(vector_max<CH>(finite_top(x)));
           if (part == 0) {
             st_global16(dst, bitcast<u32x4>(y));
           } else {

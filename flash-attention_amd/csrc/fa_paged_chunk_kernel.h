@@ -194,44 +194,72 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p) {
     }
   };
 
-  // ---- staging of pages in 8 bits: this thread's chunks of a tile (d >= 64: one of K and one of V; d < 64: one of either)
-  constexpr int kChunks = BN * D / 16, CH8 = D / 16;
-  constexpr bool kBoth = kChunks >= 256;
-  const int my = kBoth ? tid : tid % kChunks, my_row = my / CH8, my_chunk = my % CH8;
-  const bool mine = kBoth || tid < 2 * kChunks, my_v = !kBoth && tid >= kChunks;
-  const int last_page = ((p.c.max_keys - 1) >> p.c.page_log2) - skipped;
-  u32x4 raw[kBoth ? 2 : 1];
-  int raw_exp[kBoth ? 2 : 1], my_page = 0;
-  auto ask8 = [&](int it) {  // the page of the thread's row of tile `it`, a step before it is needed
-    const int key = it * BN + my_row, at = (key < Lk ? key : Lk - 1) >> p.c.page_log2;
-    my_page = table[at < last_page ? at : last_page];
+  // ---- staging of pages in 8 bits: this thread's chunks of a tile (d >= 64: one of K and one of V; d < 64: one of either).  A wave's rows lie in one or, at d < 64, several
+  // groups of 16 keys, a page each: for one group addresses are a wave-uniform base and the lane's offset.
+  constexpr int kChunks = BN * D / 16, CH8 = D / 16, kMine = kChunks >= 256 ? 2 : 1;
+  constexpr int kWaveRows = 64 / CH8, kGroups = kWaveRows > 16 ? kWaveRows / 16 : 1;
+  const int my = tid % kChunks, my_row = my / CH8, my_chunk = my % CH8;
+  const bool mine = kMine == 2 || tid < 2 * kChunks, my_v = kMine == 1 && tid >= kChunks;
+  const int wave_row = (wave * 64) % kChunks / CH8;  // (kMine == 1: a wave is K's or V's)
+  const uint32_t k_off = (uint32_t)((my_row & 15) * p.c.k_ss) + 16u * my_chunk, v_off = (uint32_t)((my_row & 15) * p.c.v_ss) + 16u * my_chunk;
+  u32x4 raw[kMine];
+  int raw_exp[kMine], page8[kGroups];
+  int to8[kMine][2];
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      to8[i][j] = i == 1 || my_v ? BN * D + frag_off<D, kSwzTr>(my_row, 2 * my_chunk + j) : frag_off<D, kSwzRow>(my_row, 2 * my_chunk + j);
+  auto ask8 = [&](int it) {  // the pages of the wave's rows of tile `it`, a step before they are needed
+#pragma unroll
+    for (int j = 0; j < kGroups; j++) {
+      const int g = it * (BN / 16) + wave_row / 16 + j;
+      page8[j] = page_of_group(p.c, table, g < last_group ? g : last_group, skipped);
+    }
   };
   auto fetch = [&](int it) {
     if (!mine) return;
-    const int key0 = it * BN + my_row, key = key0 < Lk ? key0 : Lk - 1, slot = key & ((1 << p.c.page_log2) - 1);  // (rows behind the last key repeat it)
-    const int page = page_in_pool(my_page, p.c.n_pages);
-    const int64_t at = (((int64_t)page * p.c.HK + h) << p.c.page_log2) + slot;
-    const char* const kp = p.c.k + page * p.c.k_ps + slot * p.c.k_ss + h * p.c.k_hs + 16 * my_chunk;
-    const char* const vp = p.c.v + page * p.c.v_ps + slot * p.c.v_ss + h * p.c.v_hs + 16 * my_chunk;
-    raw[0] = ld_global16(my_v ? vp : kp);
-    raw_exp[0] = (my_v ? p.c.v_exps : p.c.k_exps)[at];
-    if constexpr (kBoth) {
-      raw[1] = ld_global16(vp);
-      raw_exp[1] = p.c.v_exps[at];
+    const int g0 = it * (BN / 16) + wave_row / 16;
+    int64_t page = page8[0];
+    int g = g0 < last_group ? g0 : last_group;
+    if constexpr (kGroups > 1) {
+      const int in = (my_row >> 4) & (kGroups - 1);
+#pragma unroll
+      for (int j = 1; j < kGroups; j++)
+        if (in == j) page = page8[j];
+      g = g0 + in < last_group ? g0 + in : last_group;
+    }
+    const int slot = slot_of_group(p.c, g);
+    const char* const kb = p.c.k + h * p.c.k_hs + page * p.c.k_ps + slot * p.c.k_ss;
+    const char* const vb = p.c.v + h * p.c.v_hs + page * p.c.v_ps + slot * p.c.v_ss;
+    const int64_t xb = ((page * p.c.HK + h) << p.c.page_log2) + slot;
+    uint32_t ko = k_off, vo = v_off, row = my_row & 15;
+    if (__builtin_expect(it * BN + BN > Lk, 0)) {  // (rows behind the last key repeat it)
+      const int key = it * BN + my_row, last = (Lk - 1) & 15;
+      if (key >= Lk) {
+        row = last;
+        ko = (uint32_t)(last * p.c.k_ss) + 16u * my_chunk;
+        vo = (uint32_t)(last * p.c.v_ss) + 16u * my_chunk;
+      }
+    }
+    if constexpr (kMine == 2) {
+      raw[0] = ld_global16(kb + ko);
+      raw_exp[0] = p.c.k_exps[xb + row];
+      raw[1] = ld_global16(vb + vo);
+      raw_exp[1] = p.c.v_exps[xb + row];
+    } else {
+      raw[0] = ld_global16(my_v ? vb + vo : kb + ko);
+      raw_exp[0] = (my_v ? p.c.v_exps : p.c.k_exps)[xb + row];
     }
   };
   auto widen = [&](int buf) {
     if (!mine) return;
+    T* const to = reinterpret_cast<T*>(lds_raw + buf * C::kBuf);
 #pragma unroll
-    for (int i = 0; i < (kBoth ? 2 : 1); i++) {
-      const bool is_v = i == 1 || my_v;
+    for (int i = 0; i < kMine; i++) {
       const float scale = power_of_two(raw_exp[i]);
-      T* const to = reinterpret_cast<T*>(lds_raw + buf * C::kBuf + (is_v ? C::kTile : 0));
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int chunk = 2 * my_chunk + j, at = is_v ? frag_off<D, kSwzTr>(my_row, chunk) : frag_off<D, kSwzRow>(my_row, chunk);
-        *reinterpret_cast<vec8*>(to + at) = dequant8<T>(u32x2{raw[i][2 * j], raw[i][2 * j + 1]}, scale);
-      }
+      for (int j = 0; j < 2; j++) *reinterpret_cast<vec8*>(to + to8[i][j]) = dequant8<T>(u32x2{raw[i][2 * j], raw[i][2 * j + 1]}, scale);
     }
   };
 

@@ -14,7 +14,7 @@
 
 namespace fa {
 
-template <int D, int NW_, bool k8>
+template <int D, int NW_, bool k8, bool kPrefix>
 struct DecodeCfg {
   static constexpr int NW = NW_;
   static constexpr int BN = 32;
@@ -27,12 +27,13 @@ struct DecodeCfg {
   static constexpr int XS = DV + 4;                       // merge: floats per (wave, row)
   static constexpr int kMerge = NW * 32 * XS * 4 + 3 * NW * 32 * 4;
   static constexpr int kTiles = NW * kWave + kSlack;
-  static constexpr int kLds = kTiles > kMerge ? kTiles : kMerge;
+  static constexpr int kEnd = kMerge + (kPrefix ? 64 * NW * 28 : 0);  // (behind a prefix: the threads' joins of its parts)
+  static constexpr int kLds = kTiles > kEnd ? kTiles : kEnd;
 };
 
 template <typename T, int D, int NW_, bool k8, bool kPrefix>
 FA_DEVICE void paged_decode(const PagedFwdParams p) {
-  using C = DecodeCfg<D, NW_, k8>;
+  using C = DecodeCfg<D, NW_, k8, kPrefix>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
   constexpr int NW = C::NW, BN = C::BN, DV = C::DV;
@@ -295,38 +296,59 @@ FA_DEVICE void paged_decode(const PagedFwdParams p) {
     __syncthreads();
     const bool whole = unit0 == 0 && unit1 == pair_units;
     float* const part_o = whole ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * (kPartRows * (D + 3));
-    for (int idx = tid; idx < rows * (D / 4); idx += 64 * NW) {
-      const int r = idx / (D / 4), d0 = idx % (D / 4) * 4;
+    const auto merge_waves = [&](int r, int d0) {  // what the workgroup's waves have of row r
       float m = Xm[r];
 #pragma unroll
       for (int w = 1; w < NW; w++) m = fmaxf(m, Xm[w * 32 + r]);
       const float mu = m == -INFINITY ? 0.f : m;
-      float l = 0.f, us = 0.f;
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      JoinedRow x;
+      x.a = PartRow{m, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; w++) {
         const float f = fast_exp2((Xm[w * 32 + r] - mu) * mcs);  // 0 for a wave without keys
-        l = __builtin_fmaf(Xl[w * 32 + r], f, l);
-        us = __builtin_fmaf(Xu[w * 32 + r], f, us);
-        o = o + *reinterpret_cast<const f32x4*>(X + (w * 32 + r) * C::XS + d0) * f;
+        x.a.l = __builtin_fmaf(Xl[w * 32 + r], f, x.a.l);
+        x.a.u = __builtin_fmaf(Xu[w * 32 + r], f, x.a.u);
+        x.o = x.o + *reinterpret_cast<const f32x4*>(X + (w * 32 + r) * C::XS + d0) * f;
       }
-      if (whole) {
-        if constexpr (kPrefix) {
-          if (first_key > 0) {
-            JoinedRow x{PartRow{m, l, us}, o};
-            add_prefix<D>(p, &x, h, (int64_t)q_begin * G + r, d0, mcs, k8 ? cs : 1.f);
-            m = x.a.m; l = x.a.l; us = x.a.u; o = x.o;
-          }
+      return x;
+    };
+    const auto store = [&](const JoinedRow& x, int r, int d0) {
+      store_row_piece<T>(p, q_begin, h, r, d0, x.o * (x.a.l > 0.f ? fast_rcp(x.a.l) : 1.f));
+      if (d0 == 0) store_lse(p, b, h, r, lse_of(x.a.m, x.a.u, mcs));
+    };
+    if (kPrefix && whole && first_key > 0) {
+      // the parts of the prefix: as many threads to a row's piece as there are, joined through LDS (32 splits, 4 rows, d = 128: one thread a piece reads
+      // 32 parts one after the other)
+      constexpr int kCols = D / 4, kBeside = 64 * NW / kCols;
+      int lanes = 1;
+      while (lanes * 2 * rows <= kBeside && lanes * 2 <= p.pre_splits) lanes *= 2;
+      f32x4* const os = reinterpret_cast<f32x4*>(lds_raw + C::kMerge);
+      PartRow* const ms = reinterpret_cast<PartRow*>(os + 64 * NW);
+      const int at = tid / kCols, d0 = tid % kCols * 4, lane = at & (lanes - 1);
+      for (int r0 = 0; r0 < rows; r0 += kBeside / lanes) {
+        const int r = r0 + at / lanes;
+        JoinedRow x;
+        if (r < rows) {
+          if (lane == 0) x = merge_waves(r, d0);
+          add_prefix<D>(p, &x, h, (int64_t)q_begin * G + r, d0, mcs, k8 ? cs : 1.f, lane, lanes);
         }
-        store_row_piece<T>(p, q_begin, h, r, d0, o * (l > 0.f ? fast_rcp(l) : 1.f));
-        if (d0 == 0) store_lse(p, b, h, r, lse_of(m, us, mcs));
-      } else {
-        *reinterpret_cast<f32x4*>(part_o + r * D + d0) = o;
-        if (d0 == 0) {
-          float* const ml = part_o + kPartRows * D + r;
-          ml[0] = m;
-          ml[kPartRows] = l;
-          ml[2 * kPartRows] = us;
+        x.across<kCols>(lane, lanes, mcs, os, ms);
+        if (lane == 0 && r < rows) store(x, r, d0);
+      }
+    } else {
+      for (int idx = tid; idx < rows * (D / 4); idx += 64 * NW) {
+        const int r = idx / (D / 4), d0 = idx % (D / 4) * 4;
+        const JoinedRow x = merge_waves(r, d0);
+        if (whole) {
+          store(x, r, d0);
+        } else {
+          *reinterpret_cast<f32x4*>(part_o + r * D + d0) = x.o;
+          if (d0 == 0) {
+            float* const ml = part_o + kPartRows * D + r;
+            ml[0] = x.a.m;
+            ml[kPartRows] = x.a.l;
+            ml[2 * kPartRows] = x.a.u;
+          }
         }
       }
     }

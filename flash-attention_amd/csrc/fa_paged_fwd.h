@@ -82,7 +82,7 @@ FA_DEVICE int own_len(const PagedCache& c, int b) {
 template <int D>
 FA_DEVICE void add_prefix(const PagedFwdParams& p, JoinedRow* x, int h, int64_t row, int d0, float cs, float unit, int lane = 0, int lanes = 1) {
   const int64_t rows = (int64_t)p.c.total_q * p.c.G, all = (int64_t)p.c.HK * rows, at = (int64_t)h * rows + row;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = lane; i < p.pre_splits; i += lanes) {
     const float* const from = p.pre + (int64_t)i * all * (D + 3);
     const float* const ml = from + all * D + at * 3;

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "fa_norm.h"
 #include "fa_paged_8bit.h"
@@ -20,32 +21,35 @@ struct ReadParams {
   int per_row, pieces, threads, groups;
 };
 
-// A thread has 16 elements (8 bits; 32 bytes come out) or 8 (16 bits) of a row's place (key or value, head, chunk) and walks over rows.
+// A thread has 8 elements of a row's place (key or value, head, chunk) and walks over rows.  (16 elements of 8 bits, 32 bytes out: 61 us for 46000 rows of 2 x 8 heads,
+// d = 128: the lanes' stores leave gaps that another instruction fills.)
 template <typename T, int D, int ROWS, bool k8>
 __global__ void __launch_bounds__(512) paged_read_kernel(const ReadParams p) {
-  constexpr int N = k8 ? 16 : 8, CH = D / N;
+  constexpr int CH = D / 8, kBytes = k8 ? 8 : 16;
+  using Chunk = std::conditional_t<k8, u32x2, u32x4>;
   const int group = blockIdx.x / p.pieces, piece = blockIdx.x - group * p.pieces;
   const int j = piece * (int)blockDim.x + threadIdx.x;
   const int head = j / CH, ch = j % CH;
   const bool on = j < p.per_row, second = head >= p.c.HK;
   const int h = second ? head - p.c.HK : head;
-  const char* const src = (second ? p.c.v + h * p.c.v_hs : p.c.k + h * p.c.k_hs) + ch * 16;
-  char* const dst = reinterpret_cast<char*>(second ? p.v : p.k) + h * (second ? p.v_hs : p.k_hs) + ch * (2 * N);
+  const char* const src = (second ? p.c.v + h * p.c.v_hs : p.c.k + h * p.c.k_hs) + ch * kBytes;
+  char* const dst = reinterpret_cast<char*>(second ? p.v : p.k) + h * (second ? p.v_hs : p.k_hs) + ch * 16;
   const int64_t to_row = second ? p.v_rs : p.k_rs;
-  const uint8_t* const exps = (second ? p.c.v_exps : p.c.k_exps) + ((int64_t)h << p.c.page_log2);
+  const uint8_t* const exps = second ? p.c.v_exps : p.c.k_exps;
   for (int row0 = group * ROWS; row0 < p.c.total_q; row0 += p.groups * ROWS) {
     RowPlaces<ROWS> at;
     at.find(p.c, nullptr, row0);
-    u32x4 x[ROWS];
+    Chunk x[ROWS];
     int e[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
       const int page = page_in_pool(at.page[i], p.c.n_pages), slot = at.slot[i] & ((1 << p.c.page_log2) - 1);
       const int64_t from_k = page * p.c.k_ps + slot * p.c.k_ss, from_v = page * p.c.v_ps + slot * p.c.v_ss;
-      x[i] = u32x4{0, 0, 0, 0};
+      x[i] = Chunk{};
+      e[i] = 127;
       if (on && at.slot[i] >= 0) {
-        x[i] = ld_global16(src + (second ? from_v : from_k));
-        if constexpr (k8) e[i] = exps[((int64_t)page * p.c.HK << p.c.page_log2) + slot];
+        x[i] = *reinterpret_cast<const Chunk*>(src + (second ? from_v : from_k));
+        if constexpr (k8) e[i] = exps[((int64_t)page * p.c.HK + h << p.c.page_log2) + slot];
       }
     }
 #pragma unroll
@@ -53,9 +57,7 @@ __global__ void __launch_bounds__(512) paged_read_kernel(const ReadParams p) {
       if (!on || row0 + i >= p.c.total_q) continue;
       char* const to = dst + (int64_t)(row0 + i) * to_row;
       if constexpr (k8) {
-        const float scale = at.slot[i] >= 0 ? power_of_two(e[i]) : 1.f;
-        st_global16(to, bitcast<u32x4>(dequant8<T>(u32x2{x[i][0], x[i][1]}, scale)));
-        st_global16(to + 16, bitcast<u32x4>(dequant8<T>(u32x2{x[i][2], x[i][3]}, scale)));
+        st_global16(to, bitcast<u32x4>(dequant8<T>(x[i], power_of_two(e[i]))));
       } else {
         st_global16(to, x[i]);
       }
@@ -65,7 +67,7 @@ __global__ void __launch_bounds__(512) paged_read_kernel(const ReadParams p) {
 
 template <typename T, int D, bool k8>
 hipError_t launch_read_d(ReadParams p, hipStream_t stream) {
-  p.per_row = 2 * p.c.HK * (D / (k8 ? 16 : 8));
+  p.per_row = 2 * p.c.HK * (D / 8);
   p.threads = p.per_row <= 512 ? (p.per_row + 63) / 64 * 64 : 256;
   p.pieces = (p.per_row + p.threads - 1) / p.threads;
   constexpr int kRows = 4;
