@@ -18,10 +18,11 @@ struct Plan {
   int nq_tiles, n_splits;  // chunk (fa_paged_chunk.hip)
   bool deal;
   size_t bytes;
-  // a shared prefix (fa_paged_chunk_kernel.h): whether its keys are read once for all, its row tiles and key splits, and the bytes of its parts, which come first
+  // a shared prefix (fa_paged_prefix_kernel.h): whether its keys are read once for all, its row tiles and key splits, and the bytes of its parts, which come first
   bool share;
   int pre_tiles, pre_splits;
   size_t pre_bytes;
+  size_t whole_at;  // decode: where in the other bytes the parts of whole pairs are
 };
 
 // Workgroups of the decode kernel that are resident at once: two a compute unit at d = 128 (64 KB of tiles each), four else; over pages in 8 bits, whose workgroups
@@ -32,18 +33,35 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
   Plan pl{};
   const int rows = c.max_seqlen_q * (c.nheads_q / c.nheads_k);
   const int64_t pairs = (int64_t)c.batch * c.nheads_k;
-  int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
-  const int shared = prefix ? std::min(prefix->max_prefix_len, max_keys) / c.page_size * c.page_size : 0;
-  pl.share = shared > 0;
-  if (pl.share) {
-    const int64_t all_rows = (int64_t)c.total_q * (c.nheads_q / c.nheads_k);
-    pl.pre_tiles = (int)((all_rows + fa::kChunkRows - 1) / fa::kChunkRows) + prefix->n_groups - 1;
-    const int64_t items = (int64_t)c.nheads_k * pl.pre_tiles, tiles = (shared + 63) / 64;
-    pl.pre_splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / items, tiles / 4, 64}));
-    pl.pre_bytes = fa::align16((size_t)pl.pre_splits * c.nheads_k * all_rows * (c.head_dim + 3) * 4);
-    max_keys = std::max(max_keys - shared, 1);  // (what comes behind the longest prefix: how the rest is cut goes by it)
-  }
+  const int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
   pl.decode = rows <= fa::kDecodeMaxQ;
+  // A shared prefix is read once for all if that saves at least 16 MB of 1024 keys or more: the same pages read again come out of the caches, and splitting and joining
+  // costs a launch.  us so / as if nothing were shared, one new token, 8 x 4 heads, d = 128: 2 sequences behind 2048 keys 12.7 / 13.2, 4 12.8 / 15.5, 48 26 / 48; behind 8192
+  // 2 16.6 / 20.6, 16 22 / 52, 48 35 / 132; behind 512 16 15.2 / 15.7, 48 24.2 / 24.7; in 8 bits 8 behind 2048 13.5 / 17.8, 16 behind 512 13.8 / 12.4, 48 23 / 19; 12
+  // heads, d = 64: 4 behind 2048 12.4 / 12.6, 16 18.5 / 15.9, 48 27 / 35, 2 behind 8192 18.1 / 16.3, 4 18.3 / 20.2; 8 heads, d = 32: 8 behind 2048 11.9 / 13.3, 48 behind 512
+  // 14.7 / 10.8.  More than 32 rows a pair (8 x 4 heads, 24 tokens): 24 sequences behind 8192 keys 243 / 154.
+  const int shared = prefix && pl.decode ? std::min(prefix->max_prefix_len, max_keys) / c.page_size * c.page_size : 0;
+  const int64_t saved = (int64_t)(c.batch - (prefix ? prefix->n_groups : 0)) * c.nheads_k * shared * c.head_dim * (k8 ? 2 : 4);
+  pl.share = shared > 0 && (prefix->always || (shared >= 1024 && saved >= ((int64_t)16 << 20)));
+  if (pl.share) {
+    // Row tiles of all groups, and how a prefix's keys are split: many splits are short ones, and leave as many parts to write and to read.  Of n splits the keys
+    // take t = shared / n * 1.75 us / 64 (d = 128), the parts n times 8 of their bytes at 5 TB/s, beside a stream that wants them, too; together least at n =
+    // sqrt(shared * 160 d / bytes of a split's parts).  At most half of the resident workgroups, and 128 keys each at least.  us with 8 / 16 / 32 splits: 32
+    // sequences of 8 x 4 heads behind 8192 keys 34.2 / 33.0 / 37.9, 64 behind 16384 in 8 bits 81 / 62 / 75; of 128 / 256 / 512 keys: 3 groups of 4 x 4 heads of 3, d = 64, 3
+    // tokens, behind 1667 .. 3333 15.9 / 15.2 / 20.8
+    const int resident = 256 * (c.head_dim == 128 || (c.head_dim == 64 && !k8) ? 2 : 3);
+    const int64_t all_rows = (int64_t)c.total_q * (c.nheads_q / c.nheads_k), part = std::max<int64_t>(all_rows, 1) * (c.head_dim + 3) * 4 * c.nheads_k;
+    pl.pre_tiles = (int)((all_rows + fa::kChunkRows - 1) / fa::kChunkRows) + prefix->n_groups - 1;
+    const int64_t items = (int64_t)c.nheads_k * pl.pre_tiles, best = (int64_t)std::sqrt((double)shared * 160 * c.head_dim / (double)part);
+    pl.pre_splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / 2 / std::max<int64_t>(items, 1), shared / 128, best, 64}));
+    pl.pre_bytes = fa::align16((size_t)pl.pre_splits * part);
+    // ... beside the line of what comes behind it, which has the other resident workgroups, and a part for each pair
+    const int64_t units = (std::max(max_keys - shared, 1) + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
+    pl.groups = (int)std::min<int64_t>(std::max<int64_t>(resident - items * pl.pre_splits, resident / 2), pairs * units);
+    pl.whole_at = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
+    pl.bytes = pl.whole_at + (size_t)pairs * fa::decode_part_floats(c.head_dim) * 2;
+    return pl;
+  }
   if (pl.decode) {
     // A pair to itself, or shares of the line of all keys and a join behind them: the join is another launch and the line's beginning a chain of loads, 14 us
     // at the least; a workgroup alone with a pair reads 26 (d = 128) or 34 keys a wave and us, and the longest sequence decides.  us of a workgroup a pair / of
@@ -78,7 +96,7 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
   const int least = items > 128 ? 8 : c.head_dim < 128 && tiles < 12 ? tiles : 4;  // tiles of 64 keys
   const int64_t n = std::min<int64_t>({n_fit, tiles / least, 64});
   pl.n_splits = n < 2 ? 1 : (int)n;
-  if (pl.n_splits > 1 || pl.share) pl.bytes = (size_t)pl.n_splits * items * fa::kChunkRows * (c.head_dim + 3) * 4;
+  if (pl.n_splits > 1) pl.bytes = (size_t)pl.n_splits * items * fa::kChunkRows * (c.head_dim + 3) * 4;
   return pl;
 }
 
@@ -167,9 +185,8 @@ int fa_paged_fwd_with(const fa_paged_fwd_args* a, const fa_paged_scales* scales,
     p.pre_tiles = pl.pre_tiles;
     p.pre_splits = pl.pre_splits;
     p.pre = reinterpret_cast<float*>(a->workspace);
+    p.whole_part = reinterpret_cast<float*>(reinterpret_cast<char*>(p.part) + pl.whole_at);
     FA_LAUNCH((scales ? fa::launch_paged_prefix_8bit : fa::launch_paged_prefix)(p, dtype, head_dim, stream));
-    if (pl.decode) FA_LAUNCH((scales ? fa::launch_paged_decode_own_8bit : fa::launch_paged_decode_own)(p, dtype, head_dim, stream));
-    else FA_LAUNCH((scales ? fa::launch_paged_chunk_own_8bit : fa::launch_paged_chunk_own)(p, dtype, head_dim, stream));
     return FA_OK;
   }
   if (pl.decode) FA_LAUNCH((scales ? fa::launch_paged_decode_8bit : fa::launch_paged_decode)(p, dtype, head_dim, stream));

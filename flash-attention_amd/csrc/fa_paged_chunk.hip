@@ -12,14 +12,15 @@ namespace fa {
 
 template <typename T, int D, bool kLse>
 __global__ void __launch_bounds__(256, ChunkCfg<D>::kWaves - (kLse ? 1 : 0)) fa_paged_chunk_kernel(const PagedFwdParams p) {
-  paged_chunk<T, D, kLse, false, kAll>(p);
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[ChunkCfg<D>::kLds];
+  paged_chunk<T, D, kLse, false, false>(p, blockIdx.x, blockIdx.y, lds_raw);
 }
 
 namespace {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedFwdParams p, int lanes) {
-  paged_chunk_join<T, D, false>(p, lanes);
+  paged_chunk_join<T, D>(p, lanes);
 }
 
 template <typename T, int D>

@@ -1,10 +1,7 @@
-// Attention of many rows a key head over a paged cache, as a kernel body that fa_paged_chunk*.hip and fa_paged_prefix*.hip make kernels of: over pages in 16 bits, whose tiles
-// go from memory to LDS by themselves, and in 8 bits (k8), whose tiles are widened on the way: a thread holds the next tile's chunks (16 values each) in registers
-// while the waves compute, and writes what they stand for, in 16 bits, into the buffer that nobody reads; each value is widened once for the workgroup's 128 rows, and the main
-// loop is the same.  kMode:
-//   kAll     a sequence's rows over all its keys
-//   kOwn     ... over those behind what its group shares; partial results, which the join adds to the prefix's
-//   kShared  the rows of a group of sequences over the keys that they share, without a mask; partial results
+// Attention of many rows a key head over a paged cache, as a kernel body that fa_paged_chunk.hip, fa_paged_chunk_8bit.hip and fa_paged_prefix_kernel.h make kernels of: over pages in 16
+// bits, whose tiles go from memory to LDS by themselves, and in 8 bits (k8), whose tiles are widened on the way: a thread holds the next tile's chunks (16 values each) in
+// registers while the waves compute, and writes what they stand for, in 16 bits, into the buffer that nobody reads; each value is widened once for the workgroup's 128
+// rows, and the main loop is the same.  kShared: the rows of a group of sequences over the keys that the group shares, without a mask; partial results.
 #pragma once
 
 #include <type_traits>
@@ -14,11 +11,10 @@
 
 namespace fa {
 
-enum { kAll = 0, kOwn = 1, kShared = 2 };
-
-template <int D>
+constexpr int chunk_keys(int head_dim) { return head_dim == 128 ? 32 : 64; }  // keys of a tile
+template <int D, int BN_ = chunk_keys(D)>
 struct ChunkCfg {
-  static constexpr int BN = D == 128 ? 32 : 64;
+  static constexpr int BN = BN_;
   static constexpr int DV = D < 32 ? 32 : D;
   static constexpr int kTile = BN * D * 2;
   static constexpr int kBuf = 2 * kTile;
@@ -97,21 +93,19 @@ FA_DEVICE bool place_shared(const PagedFwdParams& p, int id, int* g, int* h, int
   return false;
 }
 
-template <typename T, int D, bool kLse, bool k8, int kMode>
-FA_DEVICE void paged_chunk(const PagedFwdParams p) {
-  using C = ChunkCfg<D>;
+template <typename T, int D, bool kLse, bool k8, bool kShared, int BN_ = chunk_keys(D)>
+FA_DEVICE void paged_chunk(const PagedFwdParams p, const int wg, const int split, unsigned char* const lds_raw) {
+  using C = ChunkCfg<D, BN_>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
   constexpr int BN = C::BN, DV = C::DV, KB = BN / 32, CH = D / 8;
   constexpr int GW = BN / 32;  // groups of 16 keys that a wave stages (waves 0 and 1: K, 2 and 3: V)
-  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[C::kLds];
 
   int b, h, qt;
-  const int split = blockIdx.y;
-  int q_begin = 0, Lq = 0, Lk = 0, skipped = 0;  // skipped: pages in front of the keys that are counted
-  if constexpr (kMode == kShared) {
+  int q_begin = 0, Lq = 0, Lk = 0;
+  if constexpr (kShared) {
     int g = 0;
-    if (!place_shared(p, blockIdx.x, &g, &h, &qt)) return;
+    if (!place_shared(p, wg, &g, &h, &qt)) return;
     if (!group_rows(p, __builtin_amdgcn_readfirstlane(g), &b, &q_begin, &Lq)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     q_begin = __builtin_amdgcn_readfirstlane(q_begin);
@@ -119,19 +113,14 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p) {
     Lk = first_own<true>(p.c, b);
     if (Lk == 0) return;  // (nothing is shared, nobody looks for a part)
   } else {
-    if (!place(p, blockIdx.x, &b, &h, &qt)) return;
+    if (!place(p, wg, &b, &h, &qt)) return;
     if (!paged_rows(p.c, b, &q_begin, &Lq)) return;
   }
   const int G = p.c.G, rows = Lq * G, m0 = qt * kChunkRows;
   if (m0 >= rows) return;
-  if constexpr (kMode != kShared) Lk = paged_len(p.c, b);
-  if constexpr (kMode == kOwn) {
-    const int first_key = first_own<true>(p.c, b);
-    skipped = first_key >> p.c.page_log2;
-    Lk = Lk > first_key ? Lk - first_key : 0;
-  }
-  const bool masked = kMode != kShared && p.causal;
-  const int n_splits = kMode == kShared ? p.pre_splits : p.n_splits;
+  if constexpr (!kShared) Lk = paged_len(p.c, b);
+  const bool masked = !kShared && p.causal;
+  const int n_splits = kShared ? p.pre_splits : p.n_splits;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -162,7 +151,7 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p) {
 
   // ---- staging
   const bool stages_v = wave >= 2;
-  const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs + skipped;
+  const int32_t* const table = p.c.table + (int64_t)b * p.c.table_rs;
   const int last_group = (Lk - 1) >> 4;
   GroupStager<D, kSwzRow> sk;
   GroupStager<D, kSwzTr> sv;
@@ -178,8 +167,7 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p) {
 #pragma unroll
     for (int j = 0; j < GW; j++) {
       const int g = it * (BN / 16) + group0 + j;
-      if constexpr (kMode == kOwn) page[j] = page_of_group(p.c, table, g < last_group ? g : last_group, skipped);
-      else page[j] = page_of_group(p.c, table, g < last_group ? g : last_group);
+      page[j] = page_of_group(p.c, table, g < last_group ? g : last_group);
     }
   };
   auto stage = [&](int it, int buf) {
@@ -196,71 +184,77 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p) {
 
   // ---- staging of pages in 8 bits: this thread's chunks of a tile (d >= 64: one of K and one of V; d < 64: one of either).  A wave's rows lie in one or, at d < 64, several
   // groups of 16 keys, a page each: for one group addresses are a wave-uniform base and the lane's offset.
-  constexpr int kChunks = BN * D / 16, CH8 = D / 16, kMine = kChunks >= 256 ? 2 : 1;
-  constexpr int kWaveRows = 64 / CH8, kGroups = kWaveRows > 16 ? kWaveRows / 16 : 1;
-  const int my = tid % kChunks, my_row = my / CH8, my_chunk = my % CH8;
+  constexpr int kChunks = BN * D / 16, CH8 = D / 16, kSets = kChunks > 256 ? kChunks / 256 : 1, kMine = kChunks >= 256 ? 2 : 1;
+  constexpr int kWaveRows = 64 / CH8, kGroups = kWaveRows > 16 ? kWaveRows / 16 : 1, kSetRows = kChunks / kSets / CH8;
+  const int my = tid % (kChunks / kSets), my_row = my / CH8, my_chunk = my % CH8;  // (of the first set; the others' rows are kSetRows further)
   const bool mine = kMine == 2 || tid < 2 * kChunks, my_v = kMine == 1 && tid >= kChunks;
-  const int wave_row = (wave * 64) % kChunks / CH8;  // (kMine == 1: a wave is K's or V's)
+  const int wave_row = (wave * 64) % (kChunks / kSets) / CH8;  // (kMine == 1: a wave is K's or V's)
   const uint32_t k_off = (uint32_t)((my_row & 15) * p.c.k_ss) + 16u * my_chunk, v_off = (uint32_t)((my_row & 15) * p.c.v_ss) + 16u * my_chunk;
-  u32x4 raw[kMine];
-  int raw_exp[kMine], page8[kGroups];
-  int to8[kMine][2];
-#pragma unroll
-  for (int i = 0; i < kMine; i++)
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-      to8[i][j] = i == 1 || my_v ? BN * D + frag_off<D, kSwzTr>(my_row, 2 * my_chunk + j) : frag_off<D, kSwzRow>(my_row, 2 * my_chunk + j);
+  u32x4 raw[kSets][kMine];
+  int raw_exp[kSets][kMine], page8[kSets][kGroups];
   auto ask8 = [&](int it) {  // the pages of the wave's rows of tile `it`, a step before they are needed
 #pragma unroll
-    for (int j = 0; j < kGroups; j++) {
-      const int g = it * (BN / 16) + wave_row / 16 + j;
-      page8[j] = page_of_group(p.c, table, g < last_group ? g : last_group, skipped);
-    }
+    for (int i = 0; i < kSets; i++)
+#pragma unroll
+      for (int j = 0; j < kGroups; j++) {
+        const int g = (it * BN + i * kSetRows + wave_row) / 16 + j;
+        page8[i][j] = page_of_group(p.c, table, g < last_group ? g : last_group);
+      }
   };
   auto fetch = [&](int it) {
     if (!mine) return;
-    const int g0 = it * (BN / 16) + wave_row / 16;
-    int64_t page = page8[0];
-    int g = g0 < last_group ? g0 : last_group;
-    if constexpr (kGroups > 1) {
-      const int in = (my_row >> 4) & (kGroups - 1);
 #pragma unroll
-      for (int j = 1; j < kGroups; j++)
-        if (in == j) page = page8[j];
-      g = g0 + in < last_group ? g0 + in : last_group;
-    }
-    const int slot = slot_of_group(p.c, g);
-    const char* const kb = p.c.k + h * p.c.k_hs + page * p.c.k_ps + slot * p.c.k_ss;
-    const char* const vb = p.c.v + h * p.c.v_hs + page * p.c.v_ps + slot * p.c.v_ss;
-    const int64_t xb = ((page * p.c.HK + h) << p.c.page_log2) + slot;
-    uint32_t ko = k_off, vo = v_off, row = my_row & 15;
-    if (__builtin_expect(it * BN + BN > Lk, 0)) {  // (rows behind the last key repeat it)
-      const int key = it * BN + my_row, last = (Lk - 1) & 15;
-      if (key >= Lk) {
-        row = last;
-        ko = (uint32_t)(last * p.c.k_ss) + 16u * my_chunk;
-        vo = (uint32_t)(last * p.c.v_ss) + 16u * my_chunk;
+    for (int i = 0; i < kSets; i++) {
+      const int n0 = it * BN + i * kSetRows, g0 = (n0 + wave_row) / 16;
+      int64_t page = page8[i][0];
+      int g = g0 < last_group ? g0 : last_group;
+      if constexpr (kGroups > 1) {
+        const int in = (my_row >> 4) & (kGroups - 1);
+#pragma unroll
+        for (int j = 1; j < kGroups; j++)
+          if (in == j) page = page8[i][j];
+        g = g0 + in < last_group ? g0 + in : last_group;
       }
-    }
-    if constexpr (kMine == 2) {
-      raw[0] = ld_global16(kb + ko);
-      raw_exp[0] = p.c.k_exps[xb + row];
-      raw[1] = ld_global16(vb + vo);
-      raw_exp[1] = p.c.v_exps[xb + row];
-    } else {
-      raw[0] = ld_global16(my_v ? vb + vo : kb + ko);
-      raw_exp[0] = (my_v ? p.c.v_exps : p.c.k_exps)[xb + row];
+      const int slot = slot_of_group(p.c, g);
+      const char* const kb = p.c.k + h * p.c.k_hs + page * p.c.k_ps + slot * p.c.k_ss;
+      const char* const vb = p.c.v + h * p.c.v_hs + page * p.c.v_ps + slot * p.c.v_ss;
+      const int64_t xb = ((page * p.c.HK + h) << p.c.page_log2) + slot;
+      uint32_t ko = k_off, vo = v_off, row = my_row & 15;
+      if (__builtin_expect(n0 + kSetRows > Lk, 0)) {  // (rows behind the last key repeat it)
+        const int last = (Lk - 1) & 15;
+        if (n0 + my_row >= Lk) {
+          row = last;
+          ko = (uint32_t)(last * p.c.k_ss) + 16u * my_chunk;
+          vo = (uint32_t)(last * p.c.v_ss) + 16u * my_chunk;
+        }
+      }
+      if constexpr (kMine == 2) {
+        raw[i][0] = ld_global16(kb + ko);
+        raw_exp[i][0] = p.c.k_exps[xb + row];
+        raw[i][1] = ld_global16(vb + vo);
+        raw_exp[i][1] = p.c.v_exps[xb + row];
+      } else {
+        raw[i][0] = ld_global16(my_v ? vb + vo : kb + ko);
+        raw_exp[i][0] = (my_v ? p.c.v_exps : p.c.k_exps)[xb + row];
+      }
     }
   };
   auto widen = [&](int buf) {
     if (!mine) return;
     T* const to = reinterpret_cast<T*>(lds_raw + buf * C::kBuf);
 #pragma unroll
-    for (int i = 0; i < kMine; i++) {
-      const float scale = power_of_two(raw_exp[i]);
+    for (int i = 0; i < kSets; i++)
 #pragma unroll
-      for (int j = 0; j < 2; j++) *reinterpret_cast<vec8*>(to + to8[i][j]) = dequant8<T>(u32x2{raw[i][2 * j], raw[i][2 * j + 1]}, scale);
-    }
+      for (int m = 0; m < kMine; m++) {
+        const float scale = power_of_two(raw_exp[i][m]);
+        const bool is_v = m == 1 || my_v;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int row = i * kSetRows + my_row, chunk = 2 * my_chunk + j;
+          *reinterpret_cast<vec8*>(to + (is_v ? BN * D + frag_off<D, kSwzTr>(row, chunk) : frag_off<D, kSwzRow>(row, chunk))) =
+              dequant8<T>(u32x2{raw[i][m][2 * j], raw[i][m][2 * j + 1]}, scale);
+        }
+      }
   };
 
   f32x16 o_acc[DV / 32];
@@ -298,9 +292,6 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p) {
     for (int i = 0; i < DV / 32; i++) asm volatile("" : "+v"(o_acc[i]));  // (see fa_fwd_kernel.h: keeps O from being copied on every trip)
     if constexpr (k8) {
       __syncthreads();  // tile `it` is in LDS, and nobody still reads the other buffer
-      if (it + 1 < ntiles) widen(buf ^ 1);
-      if (it + 2 < ntiles) fetch(it + 2);
-      if (it + 3 < ntiles) ask8(it + 3);
     } else {
       wait_vmem();      // this wave's share of tile `it` is in LDS
       __syncthreads();  // so is everyone else's, and nobody still reads the other buffer
@@ -398,17 +389,22 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p) {
             o_acc[db] = E::mfma32(bitcast<vec8>(u32x4{lo[0], lo[1], hi[0], hi[1]}), pb[kb][t], o_acc[db]);
           }
     }
+    if constexpr (k8) {  // (in front of the products the next tile's writes cost 451 us where they cost 431 here: 4 x 1024 tokens over 4096 .. 8192 keys, 8 heads of 32)
+      if (it + 1 < ntiles) widen(buf);
+      if (it + 2 < ntiles) fetch(it + 2);
+      if (it + 3 < ntiles) ask8(it + 3);
+    }
     it++;
   }
 
   const float l_tot = half_sum(l_i);
   const float u_tot = kLse ? half_sum(u_i) : 0.f;
-  if (kMode != kAll || n_splits > 1) {  // partial result of this split, fp32: [split][pair][row of nq_tiles * 128][D], m, l and u behind all of them
+  if (kShared || n_splits > 1) {  // partial result of this split, fp32: [split][pair][row of nq_tiles * 128][D], m, l and u behind all of them
     if (mw + c < rows) {
       // (of a prefix: [split][key head][row of the call])
-      const int64_t all = kMode == kShared ? (int64_t)p.c.HK * p.c.total_q * G : (int64_t)p.c.B * p.c.HK * p.nq_tiles * kChunkRows;
-      const int64_t at = kMode == kShared ? (int64_t)h * p.c.total_q * G + (int64_t)q_begin * G + mw + c : ((int64_t)b * p.c.HK + h) * p.nq_tiles * kChunkRows + mw + c;
-      float* const parts = kMode == kShared ? p.pre : p.part;
+      const int64_t all = kShared ? (int64_t)p.c.HK * p.c.total_q * G : (int64_t)p.c.B * p.c.HK * p.nq_tiles * kChunkRows;
+      const int64_t at = kShared ? (int64_t)h * p.c.total_q * G + (int64_t)q_begin * G + mw + c : ((int64_t)b * p.c.HK + h) * p.nq_tiles * kChunkRows + mw + c;
+      float* const parts = kShared ? p.pre : p.part;
       float* const op = parts + (int64_t)split * all * (D + 3) + at * D;
       if (hf == 0) {
         float* const ml = parts + (int64_t)split * all * (D + 3) + all * D + at * 3;
@@ -471,7 +467,7 @@ int join_lanes(int n_splits) {
   return lanes;
 }
 // The splits' partial results joined.
-template <typename T, int D, bool kPrefix>
+template <typename T, int D>
 FA_DEVICE void paged_chunk_join(const PagedFwdParams p, int lanes) {
   constexpr int kCols = kJoinCols<D>;
   __shared__ f32x4 os[256];
@@ -489,10 +485,6 @@ FA_DEVICE void paged_chunk_join(const PagedFwdParams p, int lanes) {
   const bool on = s >= 0 && e > s && e <= p.c.total_q && r < (e - s < p.c.max_sq ? e - s : p.c.max_sq) * p.c.G;
   const float cs = p.scale_log2;
   JoinedRow x;
-  if constexpr (kPrefix) {
-    if (on && shared_keys(p.c.prefix[b], p.c.max_prefix, p.c.max_keys, p.c.page_log2) > 0)
-      add_prefix<D>(p, &x, h, (int64_t)s * p.c.G + r, col * 4, cs, 1.f, lane, lanes);
-  }
   if (on) {
 #pragma unroll 4
     for (int i = lane; i < p.n_splits; i += lanes) {

@@ -18,7 +18,8 @@ constexpr int decode_bound(int head_dim, int waves) { return head_dim == 128 ? 1
 
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, decode_bound(D, NW)) fa_paged_decode_kernel(const PagedFwdParams p) {
-  paged_decode<T, D, NW, false, false>(p);
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[DecodeCfg<D, NW, false>::kLds];
+  paged_decode<T, D, NW, false, false>(p, blockIdx.x, lds_raw);
 }
 
 namespace {

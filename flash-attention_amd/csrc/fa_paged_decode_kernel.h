@@ -14,7 +14,7 @@
 
 namespace fa {
 
-template <int D, int NW_, bool k8, bool kPrefix>
+template <int D, int NW_, bool k8>
 struct DecodeCfg {
   static constexpr int NW = NW_;
   static constexpr int BN = 32;
@@ -27,13 +27,12 @@ struct DecodeCfg {
   static constexpr int XS = DV + 4;                       // merge: floats per (wave, row)
   static constexpr int kMerge = NW * 32 * XS * 4 + 3 * NW * 32 * 4;
   static constexpr int kTiles = NW * kWave + kSlack;
-  static constexpr int kEnd = kMerge + (kPrefix ? 64 * NW * 28 : 0);  // (behind a prefix: the threads' joins of its parts)
-  static constexpr int kLds = kTiles > kEnd ? kTiles : kEnd;
+  static constexpr int kLds = kTiles > kMerge ? kTiles : kMerge;
 };
 
 template <typename T, int D, int NW_, bool k8, bool kPrefix>
-FA_DEVICE void paged_decode(const PagedFwdParams p) {
-  using C = DecodeCfg<D, NW_, k8, kPrefix>;
+FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char* const lds_raw) {
+  using C = DecodeCfg<D, NW_, k8>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
   constexpr int NW = C::NW, BN = C::BN, DV = C::DV;
@@ -44,7 +43,6 @@ FA_DEVICE void paged_decode(const PagedFwdParams p) {
   // Numerator and denominator share the rounding of the probabilities - but not in fp16 over pages in 8 bits: a probability times its value's 2^e may be far
   // below fp16's normal numbers while the probability itself is not, and its rounding would be the sum's.
   constexpr bool kSharesRounding = !k8 || std::is_same_v<T, __bf16>;
-  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[C::kLds];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -80,13 +78,13 @@ FA_DEVICE void paged_decode(const PagedFwdParams p) {
     const int sums0 = unit_sums<kPrefix>(p.c, 0);
     const int64_t units = all_units<kPrefix>(p.c, sums0);
     const int n = sharers(p, units);
-    if ((int)blockIdx.x >= n || units == 0) return;
-    u = share_begin(units, blockIdx.x, n);
-    u_end = share_begin(units, blockIdx.x + 1, n);
+    if (wg >= n || units == 0) return;
+    u = share_begin(units, wg, n);
+    u_end = share_begin(units, wg + 1, n);
     at = spot_of<kPrefix>(p.c, u, sums0);
   } else {  // one pair
-    const int b = blockIdx.x / p.c.HK, keys = paged_len(p.c, b) - first_own<kPrefix>(p.c, b);
-    at = Spot{b, (int)blockIdx.x - b * p.c.HK, 0, keys <= kDecodeUnit ? 1 : (keys + kDecodeUnit - 1) / kDecodeUnit};
+    const int b = wg / p.c.HK, keys = paged_len(p.c, b) - first_own<kPrefix>(p.c, b);
+    at = Spot{b, wg - b * p.c.HK, 0, keys <= kDecodeUnit ? 1 : (keys + kDecodeUnit - 1) / kDecodeUnit};
     u = 0;
     u_end = at.units;
   }
@@ -294,61 +292,35 @@ FA_DEVICE void paged_decode(const PagedFwdParams p) {
         }
     }
     __syncthreads();
-    const bool whole = unit0 == 0 && unit1 == pair_units;
-    float* const part_o = whole ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * (kPartRows * (D + 3));
-    const auto merge_waves = [&](int r, int d0) {  // what the workgroup's waves have of row r
+    // (behind a prefix a whole pair's results are a part, too: the join adds the prefix's)
+    constexpr int kEach = kPartRows * (D + 3);
+    const bool alone = unit0 == 0 && unit1 == pair_units, whole = alone && !kPrefix;
+    float* const part_o = whole ? nullptr : kPrefix && alone ? p.whole_part + ((int64_t)b * p.c.HK + h) * kEach : p.part + ((int64_t)wg * 2 + (first ? 0 : 1)) * kEach;
+    for (int idx = tid; idx < rows * (D / 4); idx += 64 * NW) {
+      const int r = idx / (D / 4), d0 = idx % (D / 4) * 4;
       float m = Xm[r];
 #pragma unroll
       for (int w = 1; w < NW; w++) m = fmaxf(m, Xm[w * 32 + r]);
       const float mu = m == -INFINITY ? 0.f : m;
-      JoinedRow x;
-      x.a = PartRow{m, 0.f, 0.f};
+      float l = 0.f, us = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; w++) {
         const float f = fast_exp2((Xm[w * 32 + r] - mu) * mcs);  // 0 for a wave without keys
-        x.a.l = __builtin_fmaf(Xl[w * 32 + r], f, x.a.l);
-        x.a.u = __builtin_fmaf(Xu[w * 32 + r], f, x.a.u);
-        x.o = x.o + *reinterpret_cast<const f32x4*>(X + (w * 32 + r) * C::XS + d0) * f;
+        l = __builtin_fmaf(Xl[w * 32 + r], f, l);
+        us = __builtin_fmaf(Xu[w * 32 + r], f, us);
+        o = o + *reinterpret_cast<const f32x4*>(X + (w * 32 + r) * C::XS + d0) * f;
       }
-      return x;
-    };
-    const auto store = [&](const JoinedRow& x, int r, int d0) {
-      store_row_piece<T>(p, q_begin, h, r, d0, x.o * (x.a.l > 0.f ? fast_rcp(x.a.l) : 1.f));
-      if (d0 == 0) store_lse(p, b, h, r, lse_of(x.a.m, x.a.u, mcs));
-    };
-    if (kPrefix && whole && first_key > 0) {
-      // the parts of the prefix: as many threads to a row's piece as there are, joined through LDS (32 splits, 4 rows, d = 128: one thread a piece reads
-      // 32 parts one after the other)
-      constexpr int kCols = D / 4, kBeside = 64 * NW / kCols;
-      int lanes = 1;
-      while (lanes * 2 * rows <= kBeside && lanes * 2 <= p.pre_splits) lanes *= 2;
-      f32x4* const os = reinterpret_cast<f32x4*>(lds_raw + C::kMerge);
-      PartRow* const ms = reinterpret_cast<PartRow*>(os + 64 * NW);
-      const int at = tid / kCols, d0 = tid % kCols * 4, lane = at & (lanes - 1);
-      for (int r0 = 0; r0 < rows; r0 += kBeside / lanes) {
-        const int r = r0 + at / lanes;
-        JoinedRow x;
-        if (r < rows) {
-          if (lane == 0) x = merge_waves(r, d0);
-          add_prefix<D>(p, &x, h, (int64_t)q_begin * G + r, d0, mcs, k8 ? cs : 1.f, lane, lanes);
-        }
-        x.across<kCols>(lane, lanes, mcs, os, ms);
-        if (lane == 0 && r < rows) store(x, r, d0);
-      }
-    } else {
-      for (int idx = tid; idx < rows * (D / 4); idx += 64 * NW) {
-        const int r = idx / (D / 4), d0 = idx % (D / 4) * 4;
-        const JoinedRow x = merge_waves(r, d0);
-        if (whole) {
-          store(x, r, d0);
-        } else {
-          *reinterpret_cast<f32x4*>(part_o + r * D + d0) = x.o;
-          if (d0 == 0) {
-            float* const ml = part_o + kPartRows * D + r;
-            ml[0] = x.a.m;
-            ml[kPartRows] = x.a.l;
-            ml[2 * kPartRows] = x.a.u;
-          }
+      if (whole) {
+        store_row_piece<T>(p, q_begin, h, r, d0, o * (l > 0.f ? fast_rcp(l) : 1.f));
+        if (d0 == 0) store_lse(p, b, h, r, lse_of(m, us, mcs));
+      } else {
+        *reinterpret_cast<f32x4*>(part_o + r * D + d0) = o;
+        if (d0 == 0) {
+          float* const ml = part_o + kPartRows * D + r;
+          ml[0] = m;
+          ml[kPartRows] = l;
+          ml[2 * kPartRows] = us;
         }
       }
     }
@@ -386,28 +358,29 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
   const int n = sharers(p, units);
   const auto share_of = [&](int64_t u) { return (int)(((u + 1) * n - 1) / units); };  // (the last w with units * w / n <= u)
   const int w0 = share_of(begin), w1 = share_of(begin + pair_units - 1);
-  if (w0 == w1) return;  // whole
+  const bool alone = w0 == w1;
+  if (alone && !kPrefix) return;
   const float cs = k8 ? 1.f : p.scale_log2;
   constexpr int kEach = kPartRows * (D + 3);
   // the pair is the last of share w0, and its first, too, if the share begins with it; it is the first of the others'
   const int first_slot = share_begin(units, w0, n) == begin ? 0 : 1;
+  const bool shares = kPrefix && first_own<kPrefix>(p.c, b) > 0;
+  const int parts = w1 - w0 + 1 + (shares ? p.pre_splits : 0);
   int lanes = 2;
-  while (lanes < kLanes && lanes < w1 - w0 + 1) lanes *= 2;
+  while (lanes < kLanes && lanes < parts) lanes *= 2;
   const int col = threadIdx.x % kCols, at = threadIdx.x / kCols, lane = at & (lanes - 1), side = at / lanes, beside = kLanes / lanes;
   const int rows = Lq * p.c.G;
   for (int r0 = blockIdx.y * beside; r0 < rows; r0 += gridDim.y * beside) {
     const int r = r0 + side;
     JoinedRow x;
-    if constexpr (kPrefix) {
-      if (r < rows && first_own<true>(p.c, b) > 0)
-        add_prefix<D>(p, &x, h, (int64_t)q_begin * p.c.G + r, col * 4, cs, k8 ? p.scale_log2 : 1.f, lane, lanes);
-    }
-    if (r < rows)
+    if (r < rows) {
+      if (shares) add_prefix<D>(p, &x, h, (int64_t)q_begin * p.c.G + r, col * 4, cs, k8 ? p.scale_log2 : 1.f, lane, lanes);
       for (int i = w0 + lane; i <= w1; i += lanes) {
-        const float* const s = p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
+        const float* const s = kPrefix && alone ? p.whole_part + ((int64_t)b * p.c.HK + h) * kEach : p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
         const float* const ml = s + kPartRows * D + r;
         x.add(PartRow{ml[0], ml[kPartRows], ml[2 * kPartRows]}, *reinterpret_cast<const f32x4*>(s + r * D + col * 4), cs);
       }
+    }
     x.across<kCols>(lane, lanes, cs, os, ms);
     if (lane == 0 && r < rows) {
       store_row_piece<T>(p, q_begin, h, r, col * 4, x.o * (x.a.l > 0.f ? fast_rcp(x.a.l) : 1.f));

@@ -6,9 +6,9 @@
 // under the causal mask (aligned at the end), Lk else; a limit of 0 or less: nothing, o = 0 and lse = -inf.
 //
 // Shared prefixes.  The sequences of a group list the same pages for their first prefix[b] keys (whole pages), which all their new tokens see.  To those keys the
-// group's rows are one product, G times the tokens of all its sequences: the chunk kernel reads them once per 128 rows, as if the group were one sequence without a
-// mask (fa_paged_chunk_kernel.h, kShared), and leaves partial results; the sequences' own keys, from `first` on, are attended as ever, and whatever writes a row's
-// result adds the prefix's parts to its own.
+// group's rows are one product, G times the tokens of all its sequences, so that the keys are read once per 128 of them, as if the group were one sequence without a
+// mask; the sequences' own keys are attended as ever; both leave partial results, which a second kernel joins (fa_paged_prefix_kernel.h).  At most 32 rows a pair: with
+// more of them products bound both ways, and reading a key once more costs nothing.
 #pragma once
 
 #include "fa_paged.h"
@@ -33,6 +33,7 @@ struct PagedFwdParams {
   const int32_t* cu_groups;
   int n_groups, pre_splits, pre_tiles;
   float* pre;
+  float* whole_part;  // decode: the part of a pair that one workgroup has whole, for each pair
 };
 
 // Partial results of a row: its output before the division, the maximum m of its scores (before scaling), the sum l of the probabilities as they are
@@ -82,7 +83,7 @@ FA_DEVICE int own_len(const PagedCache& c, int b) {
 template <int D>
 FA_DEVICE void add_prefix(const PagedFwdParams& p, JoinedRow* x, int h, int64_t row, int d0, float cs, float unit, int lane = 0, int lanes = 1) {
   const int64_t rows = (int64_t)p.c.total_q * p.c.G, all = (int64_t)p.c.HK * rows, at = (int64_t)h * rows + row;
-#pragma unroll 8
+#pragma unroll 4
   for (int i = lane; i < p.pre_splits; i += lanes) {
     const float* const from = p.pre + (int64_t)i * all * (D + 3);
     const float* const ml = from + all * D + at * 3;
@@ -131,6 +132,8 @@ constexpr int kDecodeWide(int head_dim) { return head_dim == 128 ? 4 : 8; }
 // ... over pages in 8 bits, whose tiles take half the LDS, and of one that has its share of the line
 constexpr int kDecodeWide8 = 8;
 constexpr int kDecodeWaves8 = 4;
+// ... beside the workgroups of a shared prefix, which have four: two at d = 128 in 16 bits, the other two end at once, so that two workgroups' tiles fit a compute unit
+constexpr int kDecodeBeside(int head_dim, bool k8) { return !k8 && head_dim == 128 ? 2 : 4; }
 
 // floats of a workgroup's two partial results: [2][32][D] outputs, [2][3][32] m, l, u
 inline size_t decode_part_floats(int D) { return 2 * (size_t)kPartRows * (D + 3); }
@@ -140,11 +143,7 @@ hipError_t launch_paged_chunk(const PagedFwdParams& p, int dtype, int head_dim, 
 // of a cache in 8 bits
 hipError_t launch_paged_decode_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 hipError_t launch_paged_chunk_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
-// behind a shared prefix, and over it
-hipError_t launch_paged_decode_own(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
-hipError_t launch_paged_decode_own_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
-hipError_t launch_paged_chunk_own(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
-hipError_t launch_paged_chunk_own_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+// of sequences that share a prefix
 hipError_t launch_paged_prefix(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 hipError_t launch_paged_prefix_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 constexpr int kChunkRows = 128;  // rows of a workgroup of the chunk kernel

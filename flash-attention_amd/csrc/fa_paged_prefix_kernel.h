@@ -1,0 +1,63 @@
+// Attention of sequences that share a prefix, a few rows a key head: one launch has two kinds of workgroups.  The first ones attend with a group's rows to the keys that the
+// group shares (fa_paged_chunk_kernel.h, kShared), the others have the line of the sequences' own keys (fa_paged_decode_kernel.h); all leave partial results, which a second kernel
+// joins.  The first are bound by products and the exponentials, the others by memory: side by side on a compute unit they take little more than the longer of the two.
+#pragma once
+
+#include "fa_paged_chunk_kernel.h"
+#include "fa_paged_decode_kernel.h"
+
+namespace fa {
+
+// Keys of a tile of the prefix: the LDS that the others' tiles take holds 64 at d = 128, too.
+constexpr int kPrefixKeys = 64;
+// Waves a SIMD that registers are to allow.
+constexpr int prefix_bound(int head_dim) { return head_dim == 128 ? 2 : 3; }
+
+template <typename T, int D, bool kLse, bool k8>
+__global__ void __launch_bounds__(256, prefix_bound(D)) fa_paged_prefix_kernel(const PagedFwdParams p) {
+  constexpr int NW = kDecodeBeside(D, k8);
+  constexpr int kDecodeLds = DecodeCfg<D, NW, k8>::kLds, kChunkLds = ChunkCfg<D, kPrefixKeys>::kLds;
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[kDecodeLds > kChunkLds ? kDecodeLds : kChunkLds];
+  const int items = (p.c.HK * p.pre_tiles + 7) / 8 * 8;
+  // (the prefix's first: each of them takes longer.  Both kinds in turn: 61 to 62 us where this takes 61.5, 64 sequences behind 16384 keys)
+  const int shared = items * p.pre_splits, id = blockIdx.x;
+  if (id < shared) {
+    paged_chunk<T, D, kLse, k8, true, kPrefixKeys>(p, id % items, id / items, lds_raw);
+  } else {
+    if (NW < 4 && threadIdx.x >= 64 * NW) return;
+    paged_decode<T, D, NW, k8, true>(p, id - shared, lds_raw);
+  }
+}
+template <typename T, int D, bool k8>
+__global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedFwdParams p) {
+  paged_decode_join<T, D, k8, true>(p);
+}
+
+template <typename T, int D, bool k8>
+hipError_t launch_prefix_d(const PagedFwdParams& p, hipStream_t stream) {
+  const unsigned items = (unsigned)((p.c.HK * p.pre_tiles + 7) / 8 * 8), pairs = (unsigned)(p.c.B * p.c.HK);
+  const dim3 grid(items * (unsigned)p.pre_splits + (unsigned)p.groups);
+  if (p.lse) hipLaunchKernelGGL((fa_paged_prefix_kernel<T, D, true, k8>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((fa_paged_prefix_kernel<T, D, false, k8>), grid, dim3(256), 0, stream, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const unsigned rows = (unsigned)(p.c.max_sq * p.c.G), side = pairs < 1024 ? 1024 / pairs : 1;  // (workgroups beside each other for a pair's rows)
+  hipLaunchKernelGGL((paged_prefix_join_kernel<T, D, k8>), dim3(pairs, rows < side ? rows : side), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+template <bool k8, typename T>
+hipError_t launch_prefix_t(const PagedFwdParams& p, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 16: return launch_prefix_d<T, 16, k8>(p, stream);
+    case 32: return launch_prefix_d<T, 32, k8>(p, stream);
+    case 64: return launch_prefix_d<T, 64, k8>(p, stream);
+    case 128: return launch_prefix_d<T, 128, k8>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+template <bool k8>
+hipError_t launch_prefix_of(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream) {
+  return dtype == 0 ? launch_prefix_t<k8, _Float16>(p, head_dim, stream) : launch_prefix_t<k8, __bf16>(p, head_dim, stream);
+}
+
+}  // namespace fa

@@ -169,7 +169,7 @@ class PagedScales(ctypes.Structure):
 
 class PagedPrefix(ctypes.Structure):
     """struct fa_paged_prefix, field for field."""
-    _fields_ = [("struct_bytes", ctypes.c_uint32), ("n_groups", ctypes.c_int32), ("max_prefix_len", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+    _fields_ = [("struct_bytes", ctypes.c_uint32), ("n_groups", ctypes.c_int32), ("max_prefix_len", ctypes.c_int32), ("always", ctypes.c_int32),
                 ("cu_groups", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p)]
 
 
@@ -1285,9 +1285,9 @@ def paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k,
 
 
 def paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, return_lse=False, out=None,
-              k_scales=None, v_scales=None, cu_groups=None, prefix_lens=None, max_prefix_len=0):
+              k_scales=None, v_scales=None, cu_groups=None, prefix_lens=None, max_prefix_len=0, always=False):
     """Attention of the new tokens' q (total, heads, head_dim) over a paged cache: [o] or [o, softmax_lse] (fa_paged_fwd_with).  cu_groups, prefix_lens: of groups of
-    sequences that begin with the same keys."""
+    sequences that begin with the same keys, which are read once for all where that pays, or (always) wherever it is possible."""
     lib = load_library()
     a = PagedFwdArgs()
     a.struct_bytes = ctypes.sizeof(a)
@@ -1301,7 +1301,7 @@ def paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seql
         _check_seqlens("prefix_lens", prefix_lens, a.cache.batch, k_cache.device)
         _check(cu_groups.device == k_cache.device and cu_groups.dtype == torch.int32 and cu_groups.dim() == 1 and 2 <= cu_groups.numel() <= a.cache.batch + 1 and
                cu_groups.is_contiguous(), "cu_groups must be a contiguous int32 tensor on the cache's device: where each group's sequences begin, and the batch's end")
-        prefix = PagedPrefix(ctypes.sizeof(PagedPrefix), cu_groups.numel() - 1, _int32("max_prefix_len", max_prefix_len), 0, cu_groups.data_ptr(), prefix_lens.data_ptr())
+        prefix = PagedPrefix(ctypes.sizeof(PagedPrefix), cu_groups.numel() - 1, _int32("max_prefix_len", max_prefix_len), int(bool(always)), cu_groups.data_ptr(), prefix_lens.data_ptr())
     more = [None if x is None else ctypes.byref(x) for x in (scales, prefix)]
     with _OnDevice(dev):
         if out is None:

@@ -444,7 +444,7 @@ typedef struct fa_paged_scales {
 typedef struct fa_paged_prefix {
   uint32_t struct_bytes;
   int32_t n_groups, max_prefix_len;
-  int32_t reserved0; /* 0 */
+  int32_t always; /* 0: prefixes are read once where that pays; 1: wherever it is possible (at most 32 new tokens times query heads of a key head a sequence) */
   const int32_t* cu_groups;
   const int32_t* prefix_lens;
 } fa_paged_prefix;

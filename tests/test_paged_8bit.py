@@ -292,12 +292,35 @@ PREFIX = [  # lens, new, groups, prefix, H, HK, D, PS, causal
 @pytest.mark.parametrize("lens, new, groups, prefix, H, HK, D, PS, causal", PREFIX)
 @pytest.mark.parametrize("eight, want_lse", [(False, True), (True, False), (True, True)])
 def test_shared_prefix(lib, lens, new, groups, prefix, H, HK, D, PS, causal, dtype, eight, want_lse):
+    from flash_attn import flash_attn_gfx950 as be
     from flash_attn import flash_attn_paged_interface as p
     c = share((Cache8 if eight else Cache)(lens, HK, D, PS, dtype, 3, head_major=D != 32), groups, prefix).gpu()
     q = randn(sum(new) + 3, H, D, dtype=dtype, seed=5)
     cu, cg = cumulative(new).cuda(), cumulative(groups).cuda()
     pl = torch.tensor(prefix, dtype=torch.int32).repeat_interleave(torch.tensor(groups)).cuda()
-    r = p.flash_attn_paged_prefix_func(q.cuda(), c.dk, c.dv, c.dtable, cu, c.dlens, max(max(new), 1), max(lens), cg, pl, max(prefix), causal=causal,
-                                       return_softmax_lse=want_lse, **(c.scales if eight else {}))
-    out, lse = r if want_lse else (r, None)
-    check_attention(q[:sum(new)], c, new, causal, out[:sum(new)], lse)
+    where = (q.cuda(), c.dk, c.dv, c.dtable, cu, c.dlens, max(max(new), 1), max(lens))
+    scales = c.scales if eight else {}
+    # prefixes read once wherever that is possible, and as the rule has it (these are too small for it)
+    for r in (be.paged_fwd(*where, D ** -0.5, causal, want_lse, cu_groups=cg, prefix_lens=pl, max_prefix_len=max(prefix), always=True, **scales),
+              p.flash_attn_paged_prefix_func(*where, cg, pl, max(prefix), causal=causal, return_softmax_lse=want_lse, **scales)):
+        out, lse = r if want_lse else (r if isinstance(r, torch.Tensor) else r[0], None)
+        check_attention(q[:sum(new)], c, new, causal, out[:sum(new)], lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight, new", [(False, 1), (True, 1), (True, 3)])
+def test_shared_prefix_of_a_serving_batch(lib, eight, new):
+    """sizes at which prefixes are read once by the rule: the same as when every sequence reads its own"""
+    from flash_attn import flash_attn_paged_interface as p
+    lens, groups, prefix = [2500 + 13 * i for i in range(21)] + [1500 + 7 * i for i in range(11)], [21, 11], [2304, 1408]
+    c = share((Cache8 if eight else Cache)(lens, 4, 128, 128, torch.bfloat16, 3), groups, prefix).gpu()
+    scales = c.scales if eight else {}
+    q, cu = randn(32 * new, 16, 128, dtype=torch.bfloat16, seed=5).cuda(), cumulative([new] * 32).cuda()
+    pl = torch.tensor(prefix, dtype=torch.int32).repeat_interleave(torch.tensor(groups)).cuda()
+    where = (q, c.dk, c.dv, c.dtable, cu, c.dlens, new, max(lens))
+    a, la = p.flash_attn_paged_prefix_func(*where, cumulative(groups).cuda(), pl, max(prefix), return_softmax_lse=True, **scales)
+    b, lb = p.flash_attn_paged_func(*where, return_softmax_lse=True, **scales)
+    # each is within 2 u of the largest value (probabilities), u of the result and the scores' errors, a few fp32 roundings of sums of 128 products
+    vmax, u = c.v.float().nan_to_num(0).abs().max().item(), half_step(torch.bfloat16)
+    assert ((a.float() - b.float()).abs() <= (4 * u + 1e-3) * vmax + 2 * u * b.float().abs()).all() and not torch.equal(a, b)
+    assert ((la - lb)[:, :, :new].abs() <= 1e-3).all()
