@@ -148,31 +148,52 @@ class PagedKVCache:
         q = step.append(layer, q, k, v, ...)                       # packed (total, heads, headdim) tensors of the new tokens
         out = step.attend(layer, q)
         cache.evict([a, b], budget, recent)                        # if made with key_weights=True
+        c = cache.fork(b, 512)                                     # begins with b's first 512 tokens
+        k, v, cu_seqlens = cache.read(layer, [b, c])               # what the cache holds of them, packed
         cache.remove(a)
+
+    dtype: the model's.  store_dtype=torch.float8_e4m3fn: pages in 8 bits, half the memory and half the time of a decode step that is bound by reading them (not with
+    key_weights).  A fork shares the whole pages of what it begins with; the steps of sequences that share them, named one after the other, read them once for all
+    where that pays (flash_attn_paged_prefix_func).
 
     A page holds a head's tokens one after the other.  Everything is enqueued on the current stream in the order of the calls; a removed sequence's pages may be
     given to another at once, so steps of one cache belong on one stream."""
 
-    def __init__(self, layers, pages, page_size, nheads_k, headdim, dtype=torch.float16, device=None, key_weights=False):
+    def __init__(self, layers, pages, page_size, nheads_k, headdim, dtype=torch.float16, device=None, key_weights=False, store_dtype=None):
         if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
             raise RuntimeError("page_size must be a power of two from 16 to 1024, got %d" % page_size)
         if layers < 1 or pages < 1 or nheads_k < 1 or headdim not in (16, 32, 64, 128) or dtype not in (torch.float16, torch.bfloat16):
             raise RuntimeError("layers, pages and nheads_k must be positive, headdim 16, 32, 64 or 128, dtype fp16 or bf16")
-        self.page_size = page_size
+        if store_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise RuntimeError("store_dtype must be the dtype or float8_e4m3fn")
+        eight = store_dtype == torch.float8_e4m3fn
+        if eight and key_weights:
+            raise RuntimeError("key_weights, and the eviction that goes by them, are those of a cache in 16 bits")
+        self.page_size, self.dtype = page_size, dtype
         shape = (layers, pages, nheads_k, page_size, headdim)
         device = torch.device("cuda" if device is None else device)
         # (zeros: entries of a page table that are no pages are read as the first or last one)
-        self._k, self._v = (torch.zeros(shape, dtype=dtype, device=device).transpose(2, 3) for _ in range(2))
+        self._k, self._v = (torch.zeros(shape, dtype=torch.uint8 if eight else dtype, device=device).transpose(2, 3) for _ in range(2))
+        self._scales = None
+        if eight:
+            self._k, self._v = (t.view(torch.float8_e4m3fn) for t in (self._k, self._v))
+            self._scales = [torch.zeros(shape[:4], dtype=torch.uint8, device=device) for _ in range(2)]
         self.key_weights = torch.zeros(shape[:4], dtype=torch.float32, device=device) if key_weights else None
         self.key_positions = torch.zeros(shape[:4], dtype=torch.int32, device=device) if key_weights else None
         self.device = self._k.device
         self._free = list(range(pages - 1, -1, -1))
         self._pages, self._len, self._seen = {}, {}, {}
+        self._shared = {}  # sequence: its leading pages that others may list, too
+        self._users = {}   # page: how many sequences list it, if more than one has
         self._next_id = 0
 
     def layer(self, i):
         """(k_cache, v_cache) of layer i: (pages, page size, nheads_k, headdim)"""
         return self._k[i], self._v[i]
+
+    def scales(self, i):
+        """k_scales and v_scales of layer i, as the functions' keywords; {} for a cache in 16 bits"""
+        return {} if self._scales is None else dict(k_scales=self._scales[0][i], v_scales=self._scales[1][i])
 
     def add(self):
         """A new, empty sequence."""
@@ -180,9 +201,80 @@ class PagedKVCache:
         self._pages[seq], self._len[seq], self._seen[seq] = array("i"), 0, 0
         return seq
 
+    def fork(self, seq, tokens=None):
+        """A new sequence that begins with the first `tokens` tokens of seq (all of them).  It lists the same pages for them; a last page that they do not fill is
+        copied, in every layer."""
+        self._not_under_capture("a fork")
+        self._book([seq])
+        if self.key_weights is not None:
+            raise RuntimeError("a cache with key_weights counts what a sequence's keys receive: its pages are not shared")
+        tokens = self._len[seq] if tokens is None else int(tokens)
+        if tokens < 0 or tokens > self._len[seq]:
+            raise RuntimeError("the sequence has %d tokens, not %d" % (self._len[seq], tokens))
+        whole, rest = divmod(tokens, self.page_size)
+        if rest and not self._free:
+            raise RuntimeError("the cache has no free page for the tokens behind the shared ones")
+        new = self.add()
+        pages = self._pages[new]
+        pages.extend(self._pages[seq][:whole])
+        for page in pages:
+            self._users[page] = self._users.get(page, 1) + 1
+        for s in (seq, new) if whole else ():
+            self._shared[s] = max(self._shared.get(s, 0), whole)
+        if rest:
+            page, old = self._free.pop(), self._pages[seq][whole]
+            for t in (self._k.view(torch.uint8), self._v.view(torch.uint8), *self._scales) if self._scales else (self._k, self._v):
+                t[:, page].copy_(t[:, old])
+            pages.append(page)
+        self._len[new] = self._seen[new] = tokens
+        return new
+
+    def read(self, layer, seqs):
+        """(k, v, cu_seqlens): what the cache holds of the sequences in a layer, packed (total, nheads_k, headdim) one sequence after the other"""
+        self._not_under_capture("reading whole sequences")
+        seqs = list(seqs)
+        self._book(seqs)
+        ends = [0]
+        for s in seqs:
+            ends.append(ends[-1] + self._len[s])
+        table, lens, _, cu = self._tables(seqs, ends)
+        with torch.no_grad():
+            return (*paged_read_func(*self.layer(layer), table, cu, lens, ends[-1], dtype=self.dtype, **self.scales(layer)), cu)
+
     def remove(self, seq):
-        self._free.extend(reversed(self._pages.pop(seq)))
+        pages, shared = self._pages.pop(seq), self._shared.pop(seq, 0)
+        for page in reversed(pages):
+            if shared and page in self._users:
+                self._users[page] -= 1
+                if self._users[page] == 1:
+                    del self._users[page]
+            else:
+                self._free.append(page)
         del self._len[seq], self._seen[seq]
+
+    def _groups(self, seqs):
+        """Runs of sequences that begin with the same pages: (where each begins and the end, the tokens shared by each sequence's run); None if there is none"""
+        cu, lens = [0], []
+        for i, s in enumerate(seqs):
+            common = 0
+            if i and self._shared.get(s) and self._shared.get(seqs[i - 1]):
+                a, b = self._pages[s], self._pages[seqs[i - 1]]
+                lo, hi = 0, min(self._shared[s], self._shared[seqs[i - 1]])
+                if a[:hi] == b[:hi]:
+                    lo = hi
+                while lo < hi:  # (the longest equal beginning)
+                    mid = (lo + hi + 1) // 2
+                    lo, hi = (mid, hi) if a[:mid] == b[:mid] else (lo, mid - 1)
+                common = lo
+            run = i - cu[-1]
+            common = common if run == 1 else min(common, lens[-1]) if lens else 0
+            if common and run * common >= (run - 1) * lens[-1]:  # (as many pages saved as by the shorter run, at least)
+                lens[cu[-1]:] = [common] * (run + 1)
+            else:
+                if i:
+                    cu.append(i)
+                lens.append(0)
+        return (cu + [len(seqs)], [n * self.page_size for n in lens]) if any(lens) else None
 
     def length(self, seq):
         """Tokens of the sequence that the cache holds"""
@@ -273,10 +365,14 @@ class PagedStep:
         for n in new:
             at += n
             ends.append(at)
-        self.page_table, self.seqlens_k, _, self.cu_seqlens, self.positions = cache._tables(seqs, ends, positions)
+        groups = cache._groups(seqs) if cache._users else None
+        self.page_table, self.seqlens_k, _, self.cu_seqlens, self.positions, *rest = cache._tables(seqs, ends, positions, *(groups or ()))
         self.total, self.max_seqlen_q = at, max(new)
         self.max_seqlen_k = max(cache._len[s] for s in seqs)
         self.max_position = max(cache._seen[s] for s, n in zip(seqs, new) if n > 0)  # table rows that the new tokens' positions reach
+        self.prefix = ()  # of runs of sequences that begin with the same pages: cu_groups, prefix_lens, max_prefix_len
+        if groups is not None:
+            self.prefix = (*rest, max(groups[1]))
 
     def _own(self, t):
         if t.shape[0] != self.total:
@@ -293,16 +389,19 @@ class PagedStep:
             raise RuntimeError("the tables have %d rows, the step's tokens positions up to %d" % (cos.shape[0], self.max_position - 1))
         return paged_append_func(q, k, v, *c.layer(layer), self.page_table, self.cu_seqlens, self.seqlens_k,
                                  positions=self.positions, key_weights=weights[0], key_positions=weights[1],
-                                 **norm_and_rotary)
+                                 **c.scales(layer), **norm_and_rotary)
 
     def attend(self, layer, q, softmax_scale=None):
-        """flash_attn_paged_func over the layer's pages, causal; a cache with key_weights counts what its keys receive"""
+        """flash_attn_paged_func over the layer's pages, causal (flash_attn_paged_prefix_func where sequences share pages); a cache with key_weights counts what
+        its keys receive"""
         self._own(q)
         c = self.cache
         k, v = c.layer(layer)
         where = (self.page_table, self.cu_seqlens, self.seqlens_k, self.max_seqlen_q, self.max_seqlen_k, softmax_scale)
+        if self.prefix:
+            return flash_attn_paged_prefix_func(q, k, v, *where[:-1], *self.prefix, softmax_scale, **c.scales(layer))
         if c.key_weights is None:
-            return flash_attn_paged_func(q, k, v, *where)
+            return flash_attn_paged_func(q, k, v, *where, **c.scales(layer))
         out, lse = flash_attn_paged_func(q, k, v, *where, return_softmax_lse=True)
         paged_key_weights_func(q, lse, k, c.key_weights[layer], *where)
         return out

@@ -106,6 +106,164 @@ def test_the_reference_format_is_what_it_says():
         assert same(ref_quantise(y, dtype)[0], y)  # stored again, nothing changes
 
 
+# ---- what the entry points refuse (CPU: nothing is enqueued)
+
+def _scales(be, **kw):
+    s = be.PagedScales(ctypes.sizeof(be.PagedScales), 0, 1 << 20, 1 << 20)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+def _prefix(be, **kw):
+    x = be.PagedPrefix(ctypes.sizeof(be.PagedPrefix), 1, 32, 0, 1 << 20, 1 << 20)
+    for k, v in kw.items():
+        setattr(x, k, v)
+    return x
+
+
+def _set(a, change):
+    for k, v in change.items():
+        at, *rest = k.split(".")
+        setattr(getattr(a, at) if rest else a, rest[0] if rest else at, v)
+    return a
+
+
+@pytest.mark.parametrize("scales, change, says", [
+    (dict(struct_bytes=8), {}, "struct size"), (dict(k_scales=None), {}, "k_scales"), (dict(v_scales=None), {}, "v_scales"), (dict(k_scales=(1 << 20) + 8), {}, "16-byte"),
+    ({}, {"cache.k_slot_stride": 72}, "multiples of 16"), ({}, {"cache.v_head_stride": 1032}, "multiples of 16"), ({}, {"cache.k_page_stride": 2056}, "multiples of 16"),
+    ({}, {"cache.head_dim": 48}, "head_dim"), ({}, {"dtype": 2}, "dtype")])
+def test_a_cache_in_8_bits_is_refused(lib, scales, change, says):
+    from flash_attn import flash_attn_gfx950 as be
+    s = _scales(be, **scales)
+    for kind, call in (("append", lambda a: lib.fa_paged_append_with(ctypes.byref(a), ctypes.byref(s))),
+                       ("fwd", lambda a: lib.fa_paged_fwd_with(ctypes.byref(a), ctypes.byref(s), None))):
+        assert call(_set(paged_args(be, kind), change)) == -1 and says in lib.fa_last_error().decode(), kind
+    r = be.PagedReadArgs()
+    r.struct_bytes = ctypes.sizeof(r)
+    r.cache = paged_args(be, "fwd").cache
+    assert lib.fa_paged_read(ctypes.byref(_set(r, change)), ctypes.byref(s)) == -1 and says in lib.fa_last_error().decode()
+
+
+@pytest.mark.parametrize("change, says", [
+    (dict(struct_bytes=8), "struct size"), (dict(n_groups=0), "group"), (dict(n_groups=3), "group"), (dict(max_prefix_len=-1), "max_prefix_len"), (dict(cu_groups=None), "cu_groups"),
+    (dict(prefix_lens=None), "prefix_lens"), (dict(cu_groups=(1 << 20) + 2), "4-byte")])
+def test_a_prefix_is_refused(lib, change, says):
+    from flash_attn import flash_attn_gfx950 as be
+    a, x = paged_args(be, "fwd"), _prefix(be, **change)
+    assert lib.fa_paged_fwd_with(ctypes.byref(a), None, ctypes.byref(x)) == -1 and says in lib.fa_last_error().decode()
+    assert lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), None, ctypes.byref(x)) == 0
+
+
+def test_calls_without_rows_pass_and_ask_for_nothing_more(lib):
+    from flash_attn import flash_attn_gfx950 as be
+    s, x = _scales(be), _prefix(be)
+    assert lib.fa_paged_append_with(ctypes.byref(paged_args(be, "append")), ctypes.byref(s)) == 0
+    assert lib.fa_paged_fwd_with(ctypes.byref(paged_args(be, "fwd")), ctypes.byref(s), ctypes.byref(x)) == 0
+    r = be.PagedReadArgs()
+    r.struct_bytes = ctypes.sizeof(r)
+    r.cache = paged_args(be, "fwd").cache
+    assert lib.fa_paged_read(ctypes.byref(r), ctypes.byref(s)) == 0
+    r.cache.total_q = 3
+    assert lib.fa_paged_read(ctypes.byref(r), ctypes.byref(s)) == -1 and b"k_out" in lib.fa_last_error()
+    # the struct alone decides about the scratch, and a call without it is refused before anything is enqueued
+    a = paged_args(be, "fwd")
+    a.q = a.o = 1 << 20
+    a.q_row_stride = a.o_row_stride = 256
+    a.q_head_stride = a.o_head_stride = 64
+    a.cache.total_q, a.cache.max_seqlen_q, a.cache.max_seqlen_k, a.cache.table_cols, a.cache.table_row_stride = 2, 1, 4096, 300, 300
+    x.always, x.max_prefix_len = 1, 2048
+    need = lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), None, ctypes.byref(x))
+    assert need > 0 and need != lib.fa_paged_fwd_workspace_bytes(ctypes.byref(a))
+    assert lib.fa_paged_fwd_with(ctypes.byref(a), None, ctypes.byref(x)) == -2 and str(need) in lib.fa_last_error().decode()
+
+
+def test_prefixes_are_shared_where_it_pays(lib):
+    """on both sides of the rule, by the scratch that a call asks for: 8 x 4 heads, d = 128, pages of 64"""
+    from flash_attn import flash_attn_gfx950 as be
+
+    def shares(batch, prefix, new=1, groups=1):
+        a = paged_args(be, "fwd")
+        c = a.cache
+        c.head_dim, c.nheads_k, c.nheads_q, c.page_size, c.batch, c.total_q, c.max_seqlen_q, c.max_seqlen_k = 128, 8, 32, 64, batch, batch * new, new, prefix + 300
+        c.table_cols = c.table_row_stride = 1000
+        x = _prefix(be, n_groups=groups, max_prefix_len=prefix)
+        return lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), None, ctypes.byref(x)) != lib.fa_paged_fwd_workspace_bytes(ctypes.byref(a))
+
+    assert shares(4, 2048) and shares(2, 8192) and shares(48, 1024) and shares(16, 8192, 8) and shares(16, 8192, groups=3)
+    assert not shares(2, 2048) and not shares(48, 512) and not shares(48, 1023) and not shares(1, 100000) and not shares(16, 8192, 9) and not shares(16, 8192, groups=16)
+
+
+def test_index_arithmetic_of_prefixes(tmp_path):
+    import os
+    import subprocess
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(r"""
+#include <cassert>
+#include <climits>
+#include <initializer_list>
+#include "fa_paged_index.h"
+using namespace fa;
+int main() {
+  const int v[] = {INT_MIN, -1, 0, 1, 15, 16, 17, 1000, 1 << 20, INT_MAX};
+  for (int a : v)
+    for (int m : {0, 1, 16, 40, 1 << 30, INT_MAX})
+      for (int n : {1, 16, 100, 1 << 30})
+        for (int g = 4; g <= 10; g++) {
+          const int k = shared_keys(a, m, n, g);
+          assert(k >= 0 && k <= n && k <= m && k % (1 << g) == 0);
+          if (a >= 0) assert(k <= a && (k + (1 << g) > a || k + (1 << g) > m || k + (1 << g) > n));
+        }
+}
+""")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", os.path.join(root, "flash-attention_amd", "csrc"), str(src), "-o", str(exe)], check=True)
+    subprocess.run([str(exe)], check=True)
+
+
+def test_the_book_of_forks():
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    c = PagedKVCache(2, 40, 16, 2, 32, dtype=torch.bfloat16, device="cpu", store_dtype=torch.float8_e4m3fn)
+    a = c.add()
+    assert c.step([a], [100]).prefix == () and c.free_pages() == 33
+    c._k.view(torch.uint8)[1, 6] = 5  # (a page's bytes, in the last layer)
+    c._scales[1][1, 6] = 9
+    b, d = c.fork(a), c.fork(a, 64)
+    e = c.fork(b, 33)
+    assert [c.length(s) for s in (a, b, d, e)] == [100, 100, 64, 33] and c.free_pages() == 31  # two part pages were copied
+    page = c._pages[b][6]
+    assert page != c._pages[a][6] and (c._k.view(torch.uint8)[1, page] == 5).all() and (c._scales[1][1, page] == 9).all() and (c._k.view(torch.uint8)[0, page] == 0).all()
+    st = c.step([a, b, d, e], [1, 2, 3, 4])
+    assert [x if isinstance(x, int) else x.tolist() for x in st.prefix] == [[0, 3, 4], [64, 64, 64, 0], 64]  # (with e three would save 32 each)
+    assert c.step([d, a], [1, 1]).prefix[1].tolist() == [64, 64]
+    assert c.step([d, c.add(), a, b], [1, 1, 1, 1]).prefix[0].tolist() == [0, 1, 2, 4]
+    assert c.step([e], [1]).prefix == ()
+    f = c.fork(c.fork(a, 16), 5)  # a fork of a fork, and one that shares no whole page
+    assert c._pages[f][0] not in c._pages[a] and c.step([f, a], [1, 1]).prefix == ()
+    for s in list(c._pages):
+        c.remove(s)
+    assert sorted(c._free) == list(range(40)) and not c._users and not c._shared
+    g = c.add()
+    c.step([g], [39 * 16])
+    with pytest.raises(RuntimeError, match="tokens"):
+        c.fork(g, 39 * 16 + 1)
+    with pytest.raises(RuntimeError, match="tokens"):
+        c.fork(g, -1)
+    h = c.fork(g, 17)  # the last free page
+    with pytest.raises(RuntimeError, match="free page"):
+        c.fork(g, 17)
+    assert c.length(c.fork(g, 32)) == 32 and c.length(h) == 17
+    with pytest.raises(RuntimeError, match="different sequences"):
+        c.fork(77)
+    with pytest.raises(RuntimeError, match="16 bits"):
+        PagedKVCache(1, 4, 16, 2, 32, device="cpu", store_dtype=torch.float8_e4m3fn, key_weights=True)
+    with pytest.raises(RuntimeError, match="store_dtype"):
+        PagedKVCache(1, 4, 16, 2, 32, device="cpu", store_dtype=torch.float8_e5m2)
+    w = PagedKVCache(1, 4, 16, 2, 32, device="cpu", key_weights=True)
+    with pytest.raises(RuntimeError, match="not shared"):
+        w.fork(w.add())
+
+
 # ---- GPU: attention
 
 def check_attention(q, c, new, causal, got, lse=None, scale=None):
@@ -324,3 +482,313 @@ def test_shared_prefix_of_a_serving_batch(lib, eight, new):
     vmax, u = c.v.float().nan_to_num(0).abs().max().item(), half_step(torch.bfloat16)
     assert ((a.float() - b.float()).abs() <= (4 * u + 1e-3) * vmax + 2 * u * b.float().abs()).all() and not torch.equal(a, b)
     assert ((la - lb)[:, :, :new].abs() <= 1e-3).all()
+
+
+# ---- GPU: refusals, bad tables, streams, graphs, large pools
+
+@pytest.mark.gpu
+def test_python_refusals(lib):
+    from flash_attn import flash_attn_paged_interface as p
+    c, c16 = Cache8([40, 20], 2, 64, 16, torch.float16, 1).gpu(), Cache([40, 20], 2, 64, 16, torch.float16, 1).gpu()
+    q, cu, cg = randn(2, 4, 64).cuda(), cumulative([1, 1]).cuda(), cumulative([2]).cuda()
+    pl = torch.full((2,), 16, dtype=torch.int32, device="cuda")
+    k = randn(2, 2, 64).cuda()
+
+    def attend(q=q, k=c.dk, v=c.dv, ks=c.dks, vs=c.dvs):
+        p.flash_attn_paged_func(q, k, v, c.dtable, cu, c.dlens, 1, 40, k_scales=ks, v_scales=vs)
+
+    def shared(cg=cg, pl=pl, most=16):
+        p.flash_attn_paged_prefix_func(q, c.dk, c.dv, c.dtable, cu, c.dlens, 1, 40, cg, pl, most, **c.scales)
+
+    def store(k=k, v=k, **more):
+        p.paged_append_func(None, k, v, c.dk, c.dv, c.dtable, cu, c.dlens, **{**c.scales, **more})
+
+    def read(total=2, dtype=torch.float16, kc=c.dk, vc=c.dv, **more):
+        p.paged_read_func(kc, vc, c.dtable, cu, c.dlens, total, dtype=dtype, **{**c.scales, **more})
+
+    bad = [
+        (attend, dict(ks=None)), (attend, dict(ks=None, vs=None)), (attend, dict(k=c16.dk, v=c16.dv)), (attend, dict(v=c16.dv)), (attend, dict(q=q.float())), (attend, dict(q=q[:, :3])),
+        (attend, dict(ks=c.dks.int())), (attend, dict(ks=c.dks[:-1])), (attend, dict(ks=c.dks.transpose(1, 2))), (attend, dict(vs=c.dvs.cpu())), (attend, dict(k=c.dk.view(torch.float8_e5m2), v=c.dv.view(torch.float8_e5m2))),
+        (shared, dict(cg=None)), (shared, dict(pl=None)), (shared, dict(cg=None, pl=None)), (shared, dict(cg=cg.long())), (shared, dict(cg=cg[:1])), (shared, dict(cg=torch.zeros(4, dtype=torch.int32, device="cuda"))),
+        (shared, dict(pl=pl[:1])), (shared, dict(pl=pl.cpu())), (shared, dict(most=-1)), (shared, dict(most=2 ** 40)),
+        (store, dict(k=k.to(torch.float8_e4m3fn))), (store, dict(k=k.float())), (store, dict(v=k.bfloat16())), (store, dict(k_scales=None)), (store, dict(k_scales=None, v_scales=None)),
+        (store, dict(key_weights=c.dks)), (read, dict(total=-1)), (read, dict(dtype=None)), (read, dict(dtype=torch.float32)), (read, dict(v_scales=None)),
+        (read, dict(kc=c16.dk, vc=c16.dv)), (read, dict(kc=c16.dk, vc=c16.dv, k_scales=None, v_scales=None, dtype=torch.bfloat16)), (read, dict(vc=None)), (read, dict(total=2 ** 40)),
+    ]
+    for i, (call, change) in enumerate(bad):
+        print(i, sorted(change))  # (shown with a failure)
+        with pytest.raises(RuntimeError):
+            call(**change)
+    for call in (lambda: p.paged_key_weights_func(q, torch.zeros(2, 4, 16, device="cuda"), c.dk, torch.zeros(c.n_pages, 2, 16, device="cuda"), c.dtable, cu, c.dlens, 1, 40),
+                 lambda: p.paged_evict_func(c.dk, c.dv, torch.zeros(c.n_pages, 2, 16, device="cuda"), torch.zeros(c.n_pages, 2, 16, dtype=torch.int32, device="cuda"), c.dtable, c.dlens,
+                                            c.dlens, 8, 2, 40),
+                 lambda: attend(q=q.clone().requires_grad_()), lambda: store(k=k.clone().requires_grad_())):
+        with pytest.raises(RuntimeError):
+            call()
+    with torch.no_grad():
+        attend(), shared(), store(), read()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_tables_lengths_and_prefixes_that_are_none(lib, new):
+    """entries of the tables outside the pool, lengths beyond the table and below zero, prefixes and groups that make no sense: whatever comes out, calls end and sequences whose
+    numbers are right get their results; what cannot be stored is not"""
+    from flash_attn import flash_attn_gfx950 as be
+    from flash_attn import flash_attn_paged_interface as p
+    c = Cache8([200, 90, 130, 77], 2, 64, 16, torch.float16, 5, cols=14).gpu()
+    q, cu = randn(4 * new, 4, 64, seed=1).cuda(), cumulative([new] * 4).cuda()
+    table, lens = c.dtable.clone(), c.dlens.clone()
+    c.dk.view(torch.uint8)[:] = torch.where(c.dk.view(torch.uint8) & 127 == 127, 3, c.dk.view(torch.uint8))  # (no NaN where bad entries may point)
+    c.dv.view(torch.uint8)[:] = torch.where(c.dv.view(torch.uint8) & 127 == 127, 3, c.dv.view(torch.uint8))
+    c.dks.clamp_(max=130)
+    c.dvs.clamp_(max=130)
+    want = p.flash_attn_paged_func(q, c.dk, c.dv, table, cu, lens, new, 224, **c.scales)
+    table[0, :4] = torch.tensor([-5, 2 ** 31 - 1, c.n_pages, -2 ** 31], dtype=torch.int32)
+    lens[1], lens[2] = 2 ** 31 - 1, -7
+    got = p.flash_attn_paged_func(q, c.dk, c.dv, table, cu, lens, new, 224, **c.scales)
+    assert torch.equal(got[3 * new:], want[3 * new:]) and (got[2 * new:3 * new] == 0).all() and got.isfinite().all()
+    for groups, prefix in (([0, 2, 4], [64, 64, 2 ** 31 - 1, -3]), ([0, 9, 4], [-2 ** 31, 16, 32, 48]), ([3, 1, 4], [224, 224, 224, 224]), ([-1, 2, 2 ** 31 - 1], [17, 1, 0, 5])):
+        cg, pl = torch.tensor(groups, dtype=torch.int32).cuda(), torch.tensor(prefix, dtype=torch.int32).cuda()
+        be.paged_fwd(q, c.dk, c.dv, table, cu, lens, new, 224, 0.125, True, True, cu_groups=cg, prefix_lens=pl, max_prefix_len=224, always=True, **c.scales)
+    k, v = p.paged_read_func(c.dk, c.dv, table, cu, lens, 4 * new + 2, dtype=torch.float16, **c.scales)
+    assert (k[2 * new:3 * new] == 0).all() and (v[4 * new:] == 0).all() and k.isfinite().all()
+    before = [t.clone() for t in (c.dk.view(torch.uint8), c.dks)]
+    bad = table.clone()
+    bad[:] = torch.tensor([-1, c.n_pages], dtype=torch.int32).repeat(7)
+    p.paged_append_func(None, q[:, :2], q[:, 2:], c.dk, c.dv, bad, cu, lens, **c.scales)
+    assert torch.equal(c.dk.view(torch.uint8), before[0]) and torch.equal(c.dks, before[1])
+    for cu_bad in ([0, -3, 5, 2 ** 31 - 1, 1], [7, 3, 2, 1, 0], [0, 0, 0, 0, 0]):
+        x = torch.tensor(cu_bad, dtype=torch.int32).cuda()
+        p.paged_append_func(None, q[:, :2], q[:, 2:], c.dk, c.dv, table, x, lens, **c.scales)
+        p.paged_read_func(c.dk, c.dv, table, x, lens, 4 * new, dtype=torch.float16, **c.scales)
+        be.paged_fwd(q, c.dk, c.dv, table, x, lens, new, 224, 0.125, True, True, cu_groups=cumulative([2, 2]).cuda(), prefix_lens=lens, max_prefix_len=64, always=True, **c.scales)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 128])
+def test_values_that_are_no_numbers_and_rows_without_keys(lib, D):
+    """an infinity stored becomes NaN and reaches who sees it, and nobody else's sequence; tokens that see nothing give zeros and -inf"""
+    from flash_attn import flash_attn_gfx950 as be
+    from flash_attn import flash_attn_paged_interface as p
+    c = Cache8([60, 60, 3], 2, D, 16, torch.float16, 2).gpu()
+    k = randn(3, 2, D, seed=3)
+    v = k.clone()
+    v[1, 0, 4] = math.inf
+    cu = cumulative([1, 1, 1]).cuda()
+    p.paged_append_func(None, k.cuda(), v.cuda(), c.dk, c.dv, c.dtable, cu, c.dlens, **c.scales)
+    q = randn(7, 4, D, seed=4).cuda()
+    cu = cumulative([1, 1, 5]).cuda()
+    for always in (False, True):
+        more = dict(cu_groups=cumulative([1, 1, 1]).cuda(), prefix_lens=torch.tensor([16, 16, 0], dtype=torch.int32).cuda(), max_prefix_len=16, always=True) if always else {}
+        out, lse = be.paged_fwd(q, c.dk, c.dv, c.dtable, cu, c.dlens, 5, 60, D ** -0.5, True, True, **more, **c.scales)
+        assert out[0].isfinite().all() and out[1, :2, 4].isnan().all() and out[1, 2:].isfinite().all() and out[3:].isfinite().all()
+        assert (out[2:4] == 0).all() and (lse[2, :, :2] == -math.inf).all() and (out[4:] != 0).any(-1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_captured_step_over_8_bits_and_a_prefix(lib, new):
+    """store, attend, attend behind a prefix and read in one graph: replayed with other tokens, lengths, tables and prefixes in the same tensors, with eager calls in between"""
+    from flash_attn import flash_attn_gfx950 as be
+    from flash_attn import flash_attn_paged_interface as p
+    lens = [[200, 177], [190, 300], [141, 140], [299, 301], [200, 177]]
+    prefix = [96, 128, 0, 240, 96]
+    caches = [share(Cache8(n, 2, 64, 16, torch.float16, i, cols=20, spare=60 - sum(-(-x // 16) for x in n)), [2], [m]).gpu() for i, (n, m) in enumerate(zip(lens, prefix))]
+    qkvs = [randn(2 * new, 8, 64, seed=i).cuda() for i in range(len(lens))]
+    cu, cg = cumulative([new, new]).cuda(), cumulative([2]).cuda()
+    w = torch.ones(64, dtype=torch.float16, device="cuda")
+    cos, sin = (t.cuda() for t in tables(400, 64, torch.float16))
+
+    def step(c, qkv):
+        s = dict(k_scales=c["ks"], v_scales=c["vs"])
+        q = p.paged_append_func(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], c["k"], c["v"], c["table"], cu, c["lens"], q_weight=w, k_weight=w, cos_half=cos, sin_half=sin, **s)
+        a, la = p.flash_attn_paged_func(q, c["k"], c["v"], c["table"], cu, c["lens"], new, 310, return_softmax_lse=True, **s)
+        b, lb = be.paged_fwd(q, c["k"], c["v"], c["table"], cu, c["lens"], new, 310, 0.125, True, True, cu_groups=cg, prefix_lens=c["prefix"], max_prefix_len=256, always=True, **s)
+        return a, la[..., :new], b, lb[..., :new], *p.paged_read_func(c["k"], c["v"], c["table"], cu, c["lens"], 2 * new, dtype=torch.float16, **s)
+
+    def fresh(i):
+        c = caches[i]
+        return dict(k=c.dk.clone(), v=c.dv.clone(), ks=c.dks.clone(), vs=c.dvs.clone(), table=c.dtable.clone(), lens=c.dlens.clone(),
+                    prefix=torch.full((2,), prefix[i], dtype=torch.int32, device="cuda"))
+
+    with torch.no_grad():
+        static, qkv = fresh(0), qkvs[0].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(static, qkv)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(static, qkv)
+        for i in range(len(lens)):
+            eager = fresh(i)
+            want = step(eager, qkvs[i])
+            for k, v in fresh(i).items():
+                static[k].copy_(v)
+            qkv.copy_(qkvs[i])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), i
+            assert all(torch.equal(static[k].view(torch.uint8), eager[k].view(torch.uint8)) for k in ("k", "v", "ks", "vs")), i
+
+
+@pytest.mark.gpu
+def test_two_threads_share_prefixes_on_their_own_streams(lib):
+    import threading
+    from flash_attn import flash_attn_gfx950 as be
+    jobs = []
+    for i, (lens, eight) in enumerate((([3000, 2900, 2100], True), ([1200, 1300], False))):
+        c = share((Cache8 if eight else Cache)(lens, 2, 64, 64, torch.float16, 30 + i), [len(lens)], [1024]).gpu()
+        q, cu, cg = randn(len(lens), 8, 64, seed=i).cuda(), cumulative([1] * len(lens)).cuda(), cumulative([len(lens)]).cuda()
+        pl, scales = torch.full((len(lens),), 1024, dtype=torch.int32, device="cuda"), c.scales if eight else {}
+        jobs.append(lambda q=q, c=c, cu=cu, cg=cg, pl=pl, n=max(lens), s=scales: be.paged_fwd(q, c.dk, c.dv, c.dtable, cu, c.dlens, 1, n, 0.125, True, cu_groups=cg, prefix_lens=pl,
+                                                                                               max_prefix_len=1024, always=True, **s)[0])
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(job, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [job() for _ in range(30)]
+            torch.cuda.current_stream().synchronize()
+        wrong.extend(i for i, x in enumerate(outs) if not torch.equal(x, want))
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(jobs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 50])
+def test_8_bits_beyond_32_bit_offsets(lib, new):
+    """pages whose offsets pass 2^32 give what pages at the front give, and so do pools inside larger ones"""
+    from flash_attn import flash_attn_gfx950 as be
+    from flash_attn import flash_attn_paged_interface as p
+    PS, HK, D, lens = 64, 2, 128, [500, 411]
+    pages = -(-(5 << 30) // (PS * HK * D))
+    small = share(Cache8(lens, HK, D, PS, torch.float16, 5), [2], [256]).gpu()
+    big = [torch.empty(pages, HK, PS, D, dtype=torch.uint8, device="cuda").transpose(1, 2) for _ in range(2)]
+    exps = [torch.empty(pages, HK, PS, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    far = pages - small.n_pages
+    for b, x, e, y in zip(big, (small.dk, small.dv), exps, (small.dks, small.dvs)):
+        b[far:], e[far:] = x.view(torch.uint8), y
+    table = torch.where(small.dtable >= 0, small.dtable + far, -1).to(torch.int32)
+    qkv, cu, cg = randn(2 * new, 8, D, seed=6).cuda(), cumulative([new, new]).cuda(), cumulative([2]).cuda()
+    pl = torch.full((2,), 256, dtype=torch.int32, device="cuda")
+    got = []
+    for k, v, t, ks, vs in ((*(b.view(torch.float8_e4m3fn) for b in big), table, *exps), (small.dk, small.dv, small.dtable, small.dks, small.dvs)):
+        s = dict(k_scales=ks, v_scales=vs)
+        q = p.paged_append_func(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], k, v, t, cu, small.dlens, **s)
+        out = p.flash_attn_paged_func(q, k, v, t, cu, small.dlens, new, 500, **s)
+        two = be.paged_fwd(q, k, v, t, cu, small.dlens, new, 500, 0.1, True, cu_groups=cg, prefix_lens=pl, max_prefix_len=256, always=True, **s)[0]
+        got.append((out, two, *p.paged_read_func(k, v, t, cu, small.dlens, 2 * new, dtype=torch.float16, **s)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_views_of_8_bit_pools(lib, new):
+    from flash_attn import flash_attn_paged_interface as p
+    c = Cache8([130, 90, 61], 2, 64, 32, torch.bfloat16, 8).gpu()
+    qkv, cu = randn(3 * new, 8, 64, seed=2, dtype=torch.bfloat16).cuda(), cumulative([new] * 3).cuda()
+    pools = torch.full((2, c.n_pages + 2, 3, 32, 80), 9, dtype=torch.uint8, device="cuda")
+    for i, x in enumerate((c.dk, c.dv)):
+        pools[i, 1:-1, :2, :, 16:] = x.view(torch.uint8).transpose(1, 2)
+    view = [x[1:-1, :2, :, 16:].transpose(1, 2).view(torch.float8_e4m3fn) for x in pools]
+    wide = torch.full((3, c.dtable.shape[1] + 5), 7, dtype=torch.int32, device="cuda")
+    wide[:, 2:-3] = c.dtable
+    got = []
+    for k, v, table, ks, vs in ((c.dk, c.dv, c.dtable, c.dks.clone(), c.dvs.clone()), (*view, wide[:, 2:-3], c.dks.clone(), c.dvs.clone())):
+        s = dict(k_scales=ks, v_scales=vs)
+        q = p.paged_append_func(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], k, v, table, cu, c.dlens, **s)
+        got.append((q, p.flash_attn_paged_func(q, k, v, table, cu, c.dlens, new, 130, **s), ks, vs, k.contiguous().view(torch.uint8), v.contiguous().view(torch.uint8),
+                    *p.paged_read_func(k, v, table, cu, c.dlens, 3 * new, dtype=torch.bfloat16, **s)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert (pools[:, :, 2] == 9).all() and (pools[:, 0] == 9).all() and (pools[:, -1] == 9).all() and (pools[..., :16] == 9).all()
+
+
+# ---- GPU: serving
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", [None, torch.float8_e4m3fn])
+def test_a_serving_loop_with_forks(lib, store):
+    """a prompt, four forks of it, single tokens of all of them: attention over what the cache says it holds (read), at each step"""
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    H, HK, D, dtype = 8, 2, 64, torch.bfloat16
+    cache = PagedKVCache(2, 200, 32, HK, D, dtype=dtype, store_dtype=store)
+    cos, sin = (t.cuda() for t in tables(2000, D, dtype))
+    w = torch.ones(D, dtype=dtype, device="cuda")
+    seed = 0
+
+    def step(seqs, new):
+        nonlocal seed
+        s = cache.step(seqs, new)
+        for layer in range(2):
+            seed += 1
+            qkv = randn(sum(new), H + 2 * HK, D, dtype=dtype, seed=seed).cuda()
+            q = s.append(layer, qkv[:, :H], qkv[:, H:H + HK], qkv[:, H + HK:], q_weight=w, k_weight=w, cos_half=cos, sin_half=sin)
+            out = s.attend(layer, q)
+            k, v, cu = (t.cpu() for t in cache.read(layer, seqs))
+            c = Cache([cache.length(x) for x in seqs], HK, D, 16, dtype, 0)
+            for b, n in enumerate(c.lens):
+                page, slot = c.where(b, n)
+                c.k[page, slot], c.v[page, slot] = k[cu[b]:cu[b + 1]], v[cu[b]:cu[b + 1]]
+            check_attention(q.cpu(), c, new, True, out)
+        return s
+
+    with torch.no_grad():
+        a = cache.add()
+        step([a], [1500])
+        forks = [cache.fork(a, n) for n in (None, 1490, 1024, 700)]
+        free = cache.free_pages()
+        s = step([a] + forks, [1] * 5)
+        # (700 tokens fill 21 pages of 32: a run of five would save less than the four that share 1024; those filled their pages)
+        assert s.prefix[0].tolist() == [0, 4, 5] and s.prefix[1].tolist() == [1024] * 4 + [0] and cache.free_pages() == free - 1
+        step([a] + forks[:2], [3, 1, 2])
+        cache.remove(a)
+        step(forks, [1, 1, 1, 1])
+    for f in forks:
+        cache.remove(f)
+    assert cache.free_pages() == 200
+
+
+@pytest.mark.gpu
+def test_mha_over_a_cache_in_8_bits(lib):
+    """FlashMHA.forward_cached: the block on a cache in 8 bits is the block with attention over what the cache holds"""
+    from flash_attn.flash_attention import FlashMHA
+    from flash_attn.flash_attn_paged_interface import PagedKVCache
+    torch.manual_seed(1)
+    m = FlashMHA(256, 4, causal=True, use_rotary_emb="1d", qk_norm=True, device="cuda", dtype=torch.float16).eval()
+    x = torch.randn(70, 256, device="cuda", dtype=torch.float16)
+    with torch.no_grad():
+        c8, c16 = PagedKVCache(1, 12, 16, 4, 64, store_dtype=torch.float8_e4m3fn), PagedKVCache(1, 12, 16, 4, 64)
+        a, b = c8.add(), c16.add()
+        for at, n in ((0, 50), (50, 1), (51, 19)):
+            y8 = m.forward_cached(x[at:at + n], c8.step([a], [n]))
+            m.forward_cached(x[at:at + n], c16.step([b], [n]))
+            # the same block on a cache in 16 bits that holds what the other one stands for
+            k, v, _ = c8.read(0, [a])
+            k16, v16 = c16.layer(0)
+            t = torch.arange(at + n, device="cuda")
+            page = torch.tensor(c16._pages[b], device="cuda")[t // 16]
+            k16[page, t % 16], v16[page, t % 16] = k, v
+            from flash_attn.flash_attn_paged_interface import flash_attn_paged_func
+            q, kk, _ = m.Wqkv(x[at:at + n]).reshape(n, 3, 4, 64).unbind(1)
+            from flash_attn.rotary import apply_qk_norm_rotary
+            cos, sin = m.rotary_emb.tables_to(at + n, q)
+            q, _ = apply_qk_norm_rotary(q, kk, m.q_norm_weight, m.k_norm_weight, cos, sin, positions=torch.arange(at, at + n, dtype=torch.int32, device="cuda"))
+            cu, lens = cumulative([n]).cuda(), torch.tensor([at + n], dtype=torch.int32, device="cuda")
+            o = flash_attn_paged_func(q, k16, v16, torch.tensor([list(c16._pages[b])], dtype=torch.int32, device="cuda"), cu, lens, n, at + n)
+            y16 = m.out_proj(o.reshape(n, 256))
+            # probabilities rounded at other places (2 u of the largest value on each side), the result once on each (u of it), through the projection's weights, which rounds
+            # once on each side (u); fp32 sums of 256 products
+            u = half_step(torch.float16)
+            bound = m.out_proj.weight.float().abs().sum(1) * v.float().abs().max() * (6 * u + 1e-4) + 2 * u * y16.float().abs() + 1e-4
+            assert ((y8.float() - y16.float()).abs() <= bound).all(), (at, ((y8.float() - y16.float()).abs() / bound).max())
