@@ -30,16 +30,15 @@ FA_DEVICE float vector_sum(float x) {
   return x;
 }
 
-// ... and the largest of values that are numbers
+// ... and the largest of their integers
 template <int CH>
-FA_DEVICE float vector_max(float x) {
-  const auto other = [](float v, auto ctrl) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
-  };
-  x = fmaxf(x, other(x, std::integral_constant<int, 0xB1>{}));
-  if constexpr (CH >= 4) x = fmaxf(x, other(x, std::integral_constant<int, 0x4E>{}));
-  if constexpr (CH >= 8) x = fmaxf(x, other(x, std::integral_constant<int, 0x141>{}));
-  if constexpr (CH >= 16) x = fmaxf(x, other(x, std::integral_constant<int, 0x140>{}));
+FA_DEVICE uint32_t vector_max(uint32_t x) {
+  const auto other = [](uint32_t v, auto ctrl) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xf, 0xf, true); };
+  const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  x = larger(x, other(x, std::integral_constant<int, 0xB1>{}));
+  if constexpr (CH >= 4) x = larger(x, other(x, std::integral_constant<int, 0x4E>{}));
+  if constexpr (CH >= 8) x = larger(x, other(x, std::integral_constant<int, 0x141>{}));
+  if constexpr (CH >= 16) x = larger(x, other(x, std::integral_constant<int, 0x140>{}));
   return x;
 }
 

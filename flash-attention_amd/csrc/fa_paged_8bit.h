@@ -52,22 +52,28 @@ FA_DEVICE typename Elem<T>::vec8 dequant8(u32x2 w, float scale) {
   return dequant8(w, scale, static_cast<typename Elem<T>::vec8*>(nullptr));
 }
 
-// The largest finite magnitude of eight values.  Infinities are rare: they are looked for once for the wave, NaN are nobody's maximum anyway.
-FA_DEVICE float finite_top(const float (&x)[8]) {
-  float top = 0.f;
+// The largest finite magnitude of eight values, as bits (of numbers that are not negative they are in order).  Infinities and NaN are rare: looked for once for the wave.
+FA_DEVICE uint32_t finite_top(const float (&x)[8]) {
+  constexpr uint32_t kInf = 0x7f800000u;
+  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i++) top = fmaxf(top, __builtin_fabsf(x[i]));
-  if (__builtin_expect(__any(top == INFINITY), 0)) {
-    top = 0.f;
+  for (int i = 0; i < 8; i++) {
+    const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+    top = u > top ? u : top;
+  }
+  if (__builtin_expect(__any(top >= kInf), 0)) {
+    top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = __builtin_fabsf(x[i]) < INFINITY ? fmaxf(top, __builtin_fabsf(x[i])) : top;
+    for (int i = 0; i < 8; i++) {
+      const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+      top = u < kInf && u > top ? u : top;
+    }
   }
   return top;
 }
-// The byte of a row whose largest finite magnitude is `top` (448 = 7/8 * 2^9)
+// The byte of a row whose largest finite magnitude has the bits u (448 = 7/8 * 2^9)
 template <typename T>
-FA_DEVICE int row_exponent(float top) {
-  const uint32_t u = __float_as_uint(top);
+FA_DEVICE int row_exponent(uint32_t u) {
   int e = (int)(u >> 23) - 135 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   e = e < RowExponent<T>::least ? RowExponent<T>::least : e;  // (zeros, too)
   return (e > RowExponent<T>::most ? RowExponent<T>::most : e) + 127;

@@ -103,10 +103,10 @@ FA_DEVICE void paged_append(const AppendParams p) {
         }
         const int64_t m = m0 + ((int64_t)h << p.c.page_log2);
         if constexpr (kQuant) {
-          const int byte = row_exponent<T>(vector_max<CH>(finite_top(x)));
           if (part == 0) {
             st_global16(dst, bitcast<u32x4>(y));
           } else {
+            const int byte = row_exponent<T>(vector_max<CH>(finite_top(x)));
             *reinterpret_cast<u32x2*>(dst) = quant8<T>(x, byte);
             if (ch == 0) (part == 1 ? p.c.k_exps : p.c.v_exps)[m] = (uint8_t)byte;
           }

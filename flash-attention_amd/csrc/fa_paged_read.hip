@@ -74,7 +74,7 @@ hipError_t launch_read_d(ReadParams p, hipStream_t stream) {
   const bool few = (int64_t)p.c.total_q * p.pieces <= 2048;
   const int rows = few ? 1 : kRows;
   p.groups = (p.c.total_q + rows - 1) / rows;
-  if (!few) p.groups = std::min(p.groups, std::max(1, walking_workgroups(p.threads / 64, 20) / p.pieces));
+  if (!few) p.groups = std::min(p.groups, std::max(1, walking_workgroups(p.threads / 64, 28) / p.pieces));
   const dim3 grid((unsigned)(p.groups * p.pieces)), block((unsigned)p.threads);
   if (few) hipLaunchKernelGGL((paged_read_kernel<T, D, 1, k8>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((paged_read_kernel<T, D, kRows, k8>), grid, block, 0, stream, p);
