@@ -75,7 +75,17 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
     // 29 / 30, of 2000 71 / 71 | 54 / 53, 1024 of 1000 100 / 104 | 68 / 78
     const bool small = c.head_dim <= 32;
     if (small && max_keys <= 512) pl.wide = false;
-    const bool whole = pl.wide || max_keys <= (small ? 512 : 128) || (pairs > 256 && max_keys <= (small ? 2048 : c.head_dim == 64 && pairs < 1024 ? 512 : 1024));
+    bool whole = pl.wide || max_keys <= (small ? 512 : 128) || (pairs > 256 && max_keys <= (small ? 2048 : c.head_dim == 64 && pairs < 1024 ? 512 : 1024));
+    // pages in 8 bits, whose tiles take half the LDS and whose line begins with wider workgroups.  us of the line / a workgroup a pair / a wide one, all lengths equal | from a
+    // quarter on: d = 128, 32 pairs of 500 keys 11.3 / 10.4 / 10.2, of 1000 11.3 / 15.7 / 13.7; 128 of 1000 17.6 / 16.4 / 15.1, of 2000 21.1 / 26.7 / 22.2; 256 of 2000 30.6 /
+    // 28.4 / 27.2 | 27.2 / 27.4 / 23.7, of 4000 56 / 51 / 53 | 39.5 / 47.8 / 39.4; 384 of 2000 47.8 / 44.4 / 50.7, of 4000 83 / 83 / 88; d = 64, 96 of 1000 12.2 / 12.7 /
+    // 11.0, of 2000 15.1 / 21.4 / 17.1; 192 of 2000 19.2 / 21.5 / 17.8, of 4000 26.8 / 38.4 / 29.5; 384 of 1000 19.0 / 17.6 / 20.9, of 2000 26.6 / 29.2 / 32.6; d = 32, 64
+    // of 1000 11.1 / 12.2 / 10.3, of 2000 12.8 / 20.4 / 16.1; 384 of 2000 26.5 / 27.7 / 23.9, of 4000 38.7 / 50.4 / 41.0
+    if (k8) {
+      const bool many = pairs > (small ? 512 : 256);
+      pl.wide = !many && max_keys <= (pairs >= 192 ? 2048 : pairs >= 96 ? 1280 : 768);
+      whole = pl.wide || max_keys <= 128 || (many && max_keys <= (c.head_dim == 64 ? 1536 : 2048));
+    }
     if (!whole) {
       const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
       pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim, k8), pairs * units);
