@@ -35,14 +35,14 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
   const int64_t pairs = (int64_t)c.batch * c.nheads_k;
   const int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
   pl.decode = rows <= fa::kDecodeMaxQ;
-  // A shared prefix is read once for all if that saves at least 16 MB of 1024 keys or more: the same pages read again come out of the caches, and splitting and joining
+  // A shared prefix is read once for all if that saves at least 8 MB of 1024 keys or more: the same pages read again come out of the caches, and splitting and joining
   // costs a launch.  us so / as if nothing were shared, one new token, 8 x 4 heads, d = 128: 2 sequences behind 2048 keys 12.7 / 13.2, 4 12.8 / 15.5, 48 26 / 48; behind 8192
   // 2 16.6 / 20.6, 16 22 / 52, 48 35 / 132; behind 512 16 15.2 / 15.7, 48 24.2 / 24.7; in 8 bits 8 behind 2048 13.5 / 17.8, 16 behind 512 13.8 / 12.4, 48 23 / 19; 12
   // heads, d = 64: 4 behind 2048 12.4 / 12.6, 16 18.5 / 15.9, 48 27 / 35, 2 behind 8192 18.1 / 16.3, 4 18.3 / 20.2; 8 heads, d = 32: 8 behind 2048 11.9 / 13.3, 48 behind 512
   // 14.7 / 10.8.  More than 32 rows a pair (8 x 4 heads, 24 tokens): 24 sequences behind 8192 keys 243 / 154.
   const int shared = prefix && pl.decode ? std::min(prefix->max_prefix_len, max_keys) / c.page_size * c.page_size : 0;
   const int64_t saved = (int64_t)(c.batch - (prefix ? prefix->n_groups : 0)) * c.nheads_k * shared * c.head_dim * (k8 ? 2 : 4);
-  pl.share = shared > 0 && (prefix->always || (shared >= 1024 && saved >= ((int64_t)16 << 20)));
+  pl.share = shared > 0 && (prefix->always || (shared >= 1024 && saved >= ((int64_t)8 << 20)));
   if (pl.share) {
     // Row tiles of all groups, and how a prefix's keys are split: many splits are short ones, and leave as many parts to write and to read.  Of n splits the keys
     // take t = shared / n * 1.75 us / 64 (d = 128), the parts n times 8 of their bytes at 5 TB/s, beside a stream that wants them, too; together least at n =

@@ -82,8 +82,9 @@ def flash_attn_paged_prefix_func(q, k_cache, v_cache, page_table, cu_seqlens_q, 
     cu_groups (groups + 1,) int32: group g is the sequences cu_groups[g] .. cu_groups[g + 1] - 1, from 0 to the batch's end.  prefix_lens (batch,) int32: how many
     leading keys the sequences of a group have in the same pages - one number within a group, 0 for nothing, and no more keys than the sequence's first new token sees.
     Whole pages count; what is left of a prefix is read as each sequence's own.  max_prefix_len: at least the longest; prefixes count up to it.  As always each sequence
-    lists all its pages, and its result is that of flash_attn_paged_func, rounded elsewhere; where prefixes are shorter in one sequence of a group than in the next, or the
-    pages are not the same, the first one's keys stand for all."""
+    lists all its pages, and its result is that of flash_attn_paged_func, rounded elsewhere.  (Groups that do not hold all sequences, or whose sequences differ in what they are
+    said to share, get results of no use; nothing outside the tensors is read or written.)  Sharing pays for long prefixes, many sequences and a few new tokens; where it does
+    not, by the sizes that the host knows, every sequence reads its own."""
     done = _backend.passes().paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
                                        return_softmax_lse, k_scales, v_scales, cu_groups, prefix_lens, max_prefix_len)
     if done is not None:
@@ -203,7 +204,7 @@ class PagedKVCache:
 
     def fork(self, seq, tokens=None):
         """A new sequence that begins with the first `tokens` tokens of seq (all of them).  It lists the same pages for them; a last page that they do not fill is
-        copied, in every layer."""
+        copied, in every layer.  Between steps: what the last one made room for has been stored by all layers."""
         self._not_under_capture("a fork")
         self._book([seq])
         if self.key_weights is not None:
@@ -377,6 +378,8 @@ class PagedStep:
     def _own(self, t):
         if t.shape[0] != self.total:
             raise RuntimeError("the step has %d tokens, not %d" % (self.total, t.shape[0]))
+        if t.dtype != self.cache.dtype:  # (what rows in 8 bits stand for is exact in the dtype that they came from)
+            raise RuntimeError("the cache was made for %s, not %s" % (self.cache.dtype, t.dtype))
 
     def append(self, layer, q, k, v, **norm_and_rotary):
         """paged_append_func into the layer's pages (q_weight, k_weight, cos_half, sin_half, eps); tokens are turned by their numbers in their sequences,

@@ -190,8 +190,8 @@ def test_prefixes_are_shared_where_it_pays(lib):
         x = _prefix(be, n_groups=groups, max_prefix_len=prefix)
         return lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), None, ctypes.byref(x)) != lib.fa_paged_fwd_workspace_bytes(ctypes.byref(a))
 
-    assert shares(4, 2048) and shares(2, 8192) and shares(48, 1024) and shares(16, 8192, 8) and shares(16, 8192, groups=3)
-    assert not shares(2, 2048) and not shares(48, 512) and not shares(48, 1023) and not shares(1, 100000) and not shares(16, 8192, 9) and not shares(16, 8192, groups=16)
+    assert shares(4, 2048) and shares(2, 2048) and shares(2, 8192) and shares(48, 1024) and shares(16, 8192, 8) and shares(16, 8192, groups=3)
+    assert not shares(2, 1984) and not shares(48, 512) and not shares(48, 1023) and not shares(1, 100000) and not shares(16, 8192, 9) and not shares(16, 8192, groups=16)
 
 
 def test_index_arithmetic_of_prefixes(tmp_path):
@@ -252,13 +252,20 @@ def test_the_book_of_forks():
     h = c.fork(g, 17)  # the last free page
     with pytest.raises(RuntimeError, match="free page"):
         c.fork(g, 17)
-    assert c.length(c.fork(g, 32)) == 32 and c.length(h) == 17
+    c.remove(h)
+    h = c.fork(g, 32)
+    assert c.length(c.fork(g, 32)) == 32 and c.length(h) == 32
     with pytest.raises(RuntimeError, match="different sequences"):
         c.fork(77)
     with pytest.raises(RuntimeError, match="16 bits"):
         PagedKVCache(1, 4, 16, 2, 32, device="cpu", store_dtype=torch.float8_e4m3fn, key_weights=True)
     with pytest.raises(RuntimeError, match="store_dtype"):
         PagedKVCache(1, 4, 16, 2, 32, device="cpu", store_dtype=torch.float8_e5m2)
+    x = torch.zeros(1, 4, 32, dtype=torch.float16)
+    st = c.step([c.fork(g, 16)], [1])
+    for call in (lambda: st.append(0, x, x[:, :2], x[:, :2]), lambda: st.attend(0, x)):
+        with pytest.raises(RuntimeError, match="made for torch.bfloat16"):
+            call()
     w = PagedKVCache(1, 4, 16, 2, 32, device="cpu", key_weights=True)
     with pytest.raises(RuntimeError, match="not shared"):
         w.fork(w.add())
