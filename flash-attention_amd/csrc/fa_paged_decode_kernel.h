@@ -3,8 +3,11 @@
 //
 // In 8 bits the values are widened between LDS and the matrix cores.  K: a lane multiplies a key's row, so the row's exponent is the scale of the instruction that
 // widens two values, for nothing.  V is read transposed, a lane has one column of eight keys, whose exponents differ: they go into the probabilities instead,
-//   o = sum_j p_j 2^e_j y_j,   p_j 2^e_j = 2^(s_j c + e_j - m'),   m' = max (s_j c + e_j),
-// whose maximum is 1 where the product is largest, so that the product loses nothing to fp16's range; the sums of the p_j take 2^-e_j back in fp32.
+//   o = sum_j (p_j 2^e_j) y_j.
+// bf16 has fp32's range: the probability is rounded, and multiplied by a power of two, which rounds nothing.  In fp16, whose e_j lie in -15 .. 8, the largest product has
+// to be brought to 1, or the product would lose to fp16's range:
+//   p_j 2^e_j = 2^(s_j c + e_j - m'),   m' = max (s_j c + e_j),
+// and the sums of the p_j take 2^-e_j back in fp32.  (Not so in bf16: its e_j are up to 220 apart, and of a p_j 2^(e_j - m') that is 0 in fp32 nothing comes back.)
 #pragma once
 
 #include <type_traits>
@@ -13,6 +16,10 @@
 #include "fa_paged_line.h"
 
 namespace fa {
+
+// Whether maxima are those of s_j c + e_j, in log2 units, and not of the scores before scaling
+template <typename T, bool k8>
+constexpr bool kLog2Maxima = k8 && std::is_same_v<T, _Float16>;
 
 template <int D, int NW_, bool k8>
 struct DecodeCfg {
@@ -40,15 +47,15 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
   using VStager = std::conditional_t<k8, GroupStager8<D, kSwzTr>, GroupStager<D, kSwzTr>>;
   constexpr int NI = 2 * KStager::NI;  // loads of a tile's K, and of its V
   constexpr int NX = k8 ? 1 : 0;       // ... and of its exponents
-  // Numerator and denominator share the rounding of the probabilities - but not in fp16 over pages in 8 bits: a probability times its value's 2^e may be far
-  // below fp16's normal numbers while the probability itself is not, and its rounding would be the sum's.
-  constexpr bool kSharesRounding = !k8 || std::is_same_v<T, __bf16>;
+  // (Numerator and denominator share the rounding of the probabilities - but not then: a probability times its value's 2^e may be far below fp16's normal numbers while
+  // the probability itself is not, and its rounding would be the sum's.)
+  constexpr bool kLog2 = kLog2Maxima<T, k8>;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hf = lane >> 5;
   const float cs = p.scale_log2;
-  const float mcs = k8 ? 1.f : cs;  // what brings a maximum to log2 units
+  const float mcs = kLog2 ? 1.f : cs;  // what brings a maximum to log2 units
 
   KStager ks_;
   VStager vs_;
@@ -177,7 +184,7 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
       f32x16 s;
 #pragma unroll
       for (int r = 0; r < 16; r++) s[r] = 0.f;
-      uint32_t ve[4];  // 8 bits: the exponents of this lane's 16 values
+      uint32_t ve[4] = {};  // 8 bits: the exponents of this lane's 16 values
       if constexpr (k8) {
         const unsigned char* const exps = tile + 2 * C::kTile;
         const float scale = power_of_two(exps[c]);
@@ -193,8 +200,10 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
             s = E::mfma32(dequant8<T>(u32x2{w[2], w[3]}, scale), qreg[2 * j + 1], s);
           }
         }
+        if constexpr (kLog2) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], cs, (float)((ve[r >> 2] >> 8 * (r & 3)) & 255));
+          for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(s[r], cs, (float)((ve[r >> 2] >> 8 * (r & 3)) & 255));
+        }
       } else {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ks++) s = E::mfma32(*reinterpret_cast<const vec8*>(Ks + koff[ks]), qreg[ks], s);
@@ -203,8 +212,11 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
       if (n0 + BN > least_limit) {
         const int dead = limit - n0 - 4 * hf;
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-          if (8 * (r >> 2) + (r & 3) >= dead) s[r] = -INFINITY;
+        for (int r = 0; r < 16; r++) {
+          if (8 * (r >> 2) + (r & 3) < dead) continue;
+          s[r] = -INFINITY;
+          if constexpr (k8 && !kLog2) ve[r >> 2] &= ~(255u << 8 * (r & 3));  // (behind the sequence's end it may be 255, infinity)
+        }
       }
       float mt = s[0];
 #pragma unroll
@@ -224,16 +236,14 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
 #pragma unroll
       for (int tt = 0; tt < 2; tt++) {
         f32x8 pf;
-        if constexpr (k8) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) pf[i] = fast_exp2(s[8 * tt + i] - mc);
-          pb[tt] = cvt8<T>(pf);
+        const auto exponent = [&](int i) { return (ve[2 * tt + (i >> 2)] >> 8 * (i & 3)) & 255; };
+        if constexpr (kLog2) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
-            const float back = power_of_minus((ve[2 * tt + (i >> 2)] >> 8 * (i & 3)) & 255);
-            u_i = __builtin_fmaf(pf[i], back, u_i);
-            if constexpr (kSharesRounding) l_i = __builtin_fmaf((float)pb[tt][i], back, l_i);
+            pf[i] = fast_exp2(s[8 * tt + i] - mc);
+            u_i = __builtin_fmaf(pf[i], power_of_minus(exponent(i)), u_i);
           }
+          pb[tt] = cvt8<T>(pf);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -242,6 +252,11 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
           }
           pb[tt] = cvt8<T>(pf);
           l_i = sum8_acc(pb[tt], l_i);
+          if constexpr (k8) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) pf[i] = (float)pb[tt][i] * power_of_two((int)exponent(i));
+            pb[tt] = cvt8<T>(pf);
+          }
         }
       }
       if (next) wait_vmcnt<2 * NI + NX>();
@@ -273,8 +288,10 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
     float* const Xu = Xl + NW * 32;
     l_i = half_sum(l_i);
     u_i = half_sum(u_i);
-    if constexpr (!kSharesRounding) l_i = u_i;
-    if constexpr (k8) m_i -= 127.f;  // (the exponents' bytes have that much too much: from here on results are of 2^m)
+    if constexpr (kLog2) {
+      l_i = u_i;
+      m_i -= 127.f;  // (the exponents' bytes have that much too much: from here on results are of 2^m)
+    }
     if (c < rows) {
       if (hf == 0) {
         Xm[wave * 32 + c] = m_i;
@@ -360,7 +377,8 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
   const int w0 = share_of(begin), w1 = share_of(begin + pair_units - 1);
   const bool alone = w0 == w1;
   if (alone && !kPrefix) return;
-  const float cs = k8 ? 1.f : p.scale_log2;
+  constexpr bool kLog2 = kLog2Maxima<T, k8>;
+  const float cs = kLog2 ? 1.f : p.scale_log2;
   constexpr int kEach = kPartRows * (D + 3);
   // the pair is the last of share w0, and its first, too, if the share begins with it; it is the first of the others'
   const int first_slot = share_begin(units, w0, n) == begin ? 0 : 1;
@@ -374,7 +392,7 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
     const int r = r0 + side;
     JoinedRow x;
     if (r < rows) {
-      if (shares) add_prefix<D>(p, &x, h, (int64_t)q_begin * p.c.G + r, col * 4, cs, k8 ? p.scale_log2 : 1.f, lane, lanes);
+      if (shares) add_prefix<D>(p, &x, h, (int64_t)q_begin * p.c.G + r, col * 4, cs, kLog2 ? p.scale_log2 : 1.f, lane, lanes);
       for (int i = w0 + lane; i <= w1; i += lanes) {
         const float* const s = kPrefix && alone ? p.whole_part + ((int64_t)b * p.c.HK + h) * kEach : p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
         const float* const ml = s + kPartRows * D + r;

@@ -53,7 +53,7 @@ class Cache8(Cache):
     bytes there are 255, NaN under the largest exponent that a byte can have."""
 
     def __init__(self, *a, **kw):
-        spread = kw.pop("spread", 0.0)
+        spread, v_sizes = kw.pop("spread", 0.0), kw.pop("v_sizes", None)
         super().__init__(*a, **kw)
         g = torch.Generator().manual_seed(7)
         dtype, out = self.k.dtype, []
@@ -61,6 +61,8 @@ class Cache8(Cache):
             x = getattr(self, name).double()
             x = x * torch.exp(spread * torch.randn(x.shape[:-1], generator=g, dtype=torch.float64))[..., None]
             there = ~x.isnan().all(-1)
+            if name == "v" and v_sizes is not None:
+                x = x * torch.tensor(v_sizes, dtype=torch.float64)[torch.randint(len(v_sizes), x.shape[:-1], generator=g)][..., None]
             y, e = ref_quantise(torch.where(there[..., None], x.to(dtype).double(), 0.0), dtype)
             codes = torch.where(there[..., None], (y * (2.0 ** -e.double())[..., None]).float().to(torch.float8_e4m3fn).view(torch.uint8), 255)
             setattr(self, name, torch.where(there[..., None], y, math.nan).to(dtype))
@@ -319,6 +321,31 @@ def test_attention_over_8_bits(lib, lens, new, H, HK, D, PS, causal, dtype, want
     r = p.flash_attn_paged_func(q.cuda(), c.dk, c.dv, c.dtable, cu, c.dlens, max(new), max(max(lens), 1), causal=causal, return_softmax_lse=want_lse, **c.scales)
     out, lse = r if want_lse else (r, None)
     check_attention(q[:sum(new)], c, new, causal, out[:sum(new)], lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 4, 40])
+@pytest.mark.parametrize("D", [16, 128])
+@pytest.mark.parametrize("sizes", [1, 0, -1])
+def test_values_of_all_sizes(lib, D, new, dtype, sizes):
+    """Rows of values as far apart as the format has them, zeros among them: each counts in the denominator for what its key says, whatever its value's size"""
+    from flash_attn import flash_attn_gfx950 as be
+    from flash_attn import flash_attn_paged_interface as p
+    most = 2.0 ** (118 if dtype == torch.bfloat16 else 10)
+    v_sizes = {1: [0.0, 1 / most if dtype == torch.float16 else 2.0 ** -95, 1.0, most], 0: [0.0, most], -1: [0.0, 2.0 ** -100 if dtype == torch.bfloat16 else 2.0 ** -14]}[sizes]
+    lens, groups, prefix = [700, 690, 40, 60], [2, 2], [512, 32]
+    news = [new, 1, 1, new]
+    c = share(Cache8(lens, 2, D, 32, dtype, 3, v_sizes=v_sizes), groups, prefix).gpu()
+    q = randn(sum(news), 4, D, dtype=dtype, seed=5)
+    cu, cg = cumulative(news).cuda(), cumulative(groups).cuda()
+    pl = torch.tensor([512, 512, 32, 32], dtype=torch.int32).cuda()
+    where = (q.cuda(), c.dk, c.dv, c.dtable, cu, c.dlens, new, max(lens))
+    out, lse = p.flash_attn_paged_func(*where, return_softmax_lse=True, **c.scales)
+    check_attention(q, c, news, True, out, lse)
+    for want_lse in (False, True):
+        r = be.paged_fwd(*where, D ** -0.5, True, want_lse, cu_groups=cg, prefix_lens=pl, max_prefix_len=512, always=True, **c.scales)
+        check_attention(q, c, news, True, r[0], r[1] if want_lse else None)
 
 
 # ---- GPU: storing and reading
