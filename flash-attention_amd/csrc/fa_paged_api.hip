@@ -26,7 +26,8 @@ struct Plan {
 };
 
 // Workgroups of the decode kernel that are resident at once: two a compute unit at d = 128 (64 KB of tiles each), four else; over pages in 8 bits, whose workgroups
-// have four waves, three at d = 64 (registers).
+// have four waves, three at d = 64.  (us with three / four there, one new token: 2 x 12 heads of 20000 keys 20.8 / 22.6, 8 x 12 of 8000 25.5 / 26.5, 32 x 12 of 4000 .. 16000
+// 105.0 / 104.2; with two 23.3, 29.2 and 106.6 where three take 22.0, 27.3 and 106.2 (bf16); d = 32 with three / four 19.6 / 21.1, 24.6 / 24.6 and 84.1 / 80.1.)
 int decode_resident(int head_dim, bool k8) { return 256 * (head_dim == 128 ? 2 : k8 && head_dim == 64 ? 3 : 4); }
 
 Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* prefix = nullptr) {

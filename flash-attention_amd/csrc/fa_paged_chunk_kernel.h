@@ -1,6 +1,6 @@
-// Attention of many rows a key head over a paged cache, as a kernel body that fa_paged_chunk.hip, fa_paged_chunk_8bit.hip and fa_paged_prefix_kernel.h make kernels of: over pages in 16
-// bits, whose tiles go from memory to LDS by themselves, and in 8 bits (k8), whose tiles are widened on the way: a thread holds the next tile's chunks (16 values each) in
-// registers while the waves compute, and writes what they stand for, in 16 bits, into the buffer that nobody reads; each value is widened once for the workgroup's 128
+// Attention of many rows a key head over a paged cache, as a kernel body that fa_paged_chunk.hip, fa_paged_chunk_8bit.hip and fa_paged_prefix_kernel.h make kernels of: over
+// pages in 16 bits, whose tiles go from memory to LDS by themselves, and in 8 bits (k8), whose tiles are widened on the way: a thread holds the next tile's chunks (16 values
+// each) in registers while the waves compute, and writes what they stand for, in 16 bits, into the buffer that nobody reads; each value is widened once for the workgroup's 128
 // rows, and the main loop is the same.  kShared: the rows of a group of sequences over the keys that the group shares, without a mask; partial results.
 #pragma once
 

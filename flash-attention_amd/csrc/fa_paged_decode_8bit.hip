@@ -5,7 +5,7 @@ namespace fa {
 
 namespace {
 
-// (two waves a SIMD at d = 128 by LDS, too; at d = 64 a fourth would put 32 registers into scratch)
+// (as many workgroups as decode_resident of fa_paged_api.hip has on a compute unit; at d = 128 two by LDS, too)
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, D == 128 ? 2 : D == 64 ? 3 : 4) fa_paged_decode_8bit_kernel(const PagedFwdParams p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[DecodeCfg<D, NW, true>::kLds];

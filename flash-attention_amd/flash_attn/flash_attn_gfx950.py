@@ -1191,7 +1191,8 @@ def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_w
     _check(min(k_cache.shape) > 0 and n_pages < 2 ** 31, "k_cache must have pages, slots and heads, less than 2^31 pages")
     _check((k_scales is None) == (v_scales is None), "k_scales and v_scales come together")
     if k_scales is None:
-        _check(k_cache.dtype in (torch.float16, torch.bfloat16), "the cache must be fp16 or bf16, or (storing, reading and attention) float8_e4m3fn with k_scales and v_scales")
+        _check(k_cache.dtype in (torch.float16, torch.bfloat16),
+               "the cache must be fp16 or bf16, or (storing, reading and attention) float8_e4m3fn with k_scales and v_scales")
     else:
         _check(k_cache.dtype == torch.float8_e4m3fn, "k_scales and v_scales are those of a float8_e4m3fn cache")
     for name, t in (("k", k_cache), ("v", v_cache)):
@@ -1225,7 +1226,8 @@ def _paged_cache(a, k_cache, v_cache, page_table, seqlens_k, max_seqlen_k, key_w
 
 def _paged_queries(a, q, k_cache, cu_seqlens_q, max_seqlen_q):
     _dtype_code(q)
-    _check(q.is_cuda and q.device == k_cache.device and (q.dtype == k_cache.dtype or k_cache.dtype == torch.float8_e4m3fn) and q.dim() == 3 and q.shape[2] == k_cache.shape[3] and q.stride(2) == 1,
+    _check(q.is_cuda and q.device == k_cache.device and (q.dtype == k_cache.dtype or k_cache.dtype == torch.float8_e4m3fn) and q.dim() == 3 and
+           q.shape[2] == k_cache.shape[3] and q.stride(2) == 1,
            "q must be a (total, heads, head_dim) tensor of the cache's dtype and device, contiguous in the last dimension")
     _check(q.shape[1] > 0 and q.shape[1] % k_cache.shape[2] == 0, "the query heads must be a multiple of the key heads")
     _check_cu("cu_seqlens_q", cu_seqlens_q, a.batch)
@@ -1301,7 +1303,8 @@ def paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens_q, seqlens_k, max_seql
         _check_seqlens("prefix_lens", prefix_lens, a.cache.batch, k_cache.device)
         _check(cu_groups.device == k_cache.device and cu_groups.dtype == torch.int32 and cu_groups.dim() == 1 and 2 <= cu_groups.numel() <= a.cache.batch + 1 and
                cu_groups.is_contiguous(), "cu_groups must be a contiguous int32 tensor on the cache's device: where each group's sequences begin, and the batch's end")
-        prefix = PagedPrefix(ctypes.sizeof(PagedPrefix), cu_groups.numel() - 1, _int32("max_prefix_len", max_prefix_len), int(bool(always)), cu_groups.data_ptr(), prefix_lens.data_ptr())
+        prefix = PagedPrefix(ctypes.sizeof(PagedPrefix), cu_groups.numel() - 1, _int32("max_prefix_len", max_prefix_len), int(bool(always)), cu_groups.data_ptr(),
+                             prefix_lens.data_ptr())
     more = [None if x is None else ctypes.byref(x) for x in (scales, prefix)]
     with _OnDevice(dev):
         if out is None:

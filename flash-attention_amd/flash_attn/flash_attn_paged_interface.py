@@ -47,8 +47,8 @@ def paged_append_func(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens
     apply_qk_norm_rotary) and turned by their positions (cos_half, sin_half) - positions[row], or the slot, clamped to the tables: they are on the device, and what
     the tables have to reach is the caller's to know (PagedStep does).  Returns the new q, or None.
     key_weights, key_positions (pages, nheads_k, page size): set to 0 and the position for the new tokens (for paged_key_weights_func and
-    paged_evict_func).  k_scales, v_scales: of a cache in 8 bits, into which k and v are quantised.  Rows behind the last sequence, and tokens for which the page table has no room, are not stored; their rows of the returned q
-    hold nothing."""
+    paged_evict_func).  k_scales, v_scales: of a cache in 8 bits, into which k and v are quantised.  Rows behind the last sequence, and tokens for which the page
+    table has no room, are not stored; their rows of the returned q hold nothing."""
     done = _backend.passes().paged_append(q, k, v, k_cache, v_cache, page_table, cu_seqlens, seqlens_k, q_weight, k_weight, cos_half, sin_half, positions, eps,
                                           key_weights, key_positions, k_scales, v_scales)
     if done is not None:

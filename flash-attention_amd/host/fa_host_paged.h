@@ -205,7 +205,9 @@ struct Scales {
 bool fill_cache(fa_paged_cache* c, const at::Tensor* k, const at::Tensor* v, bool needs_v, const at::Tensor* table, const at::Tensor* lens, int64_t max_k,
                 const at::Tensor* weights, const at::Tensor* positions, const Scales& scales = Scales()) {
   memset(c, 0, sizeof(*c));
-  if (!g_paged_bound || !on_current_device(k) || (scales.k ? k->scalar_type() != at::kFloat8_e4m3fn : dtype_of(*k) < 0) || !scales.k != !scales.v || k->dim() != 4 || k->stride(3) != 1 || !dim_ok(k->size(3)) || (needs_v && !v)) return false;
+  if (!g_paged_bound || !on_current_device(k) || (scales.k ? k->scalar_type() != at::kFloat8_e4m3fn : dtype_of(*k) < 0) || !scales.k != !scales.v || k->dim() != 4 ||
+      k->stride(3) != 1 || !dim_ok(k->size(3)) || (needs_v && !v))
+    return false;
   if (v && (v->device() != k->device() || v->scalar_type() != k->scalar_type() || v->sizes() != k->sizes() || v->stride(3) != 1)) return false;
   if (!table || table->device() != k->device() || table->scalar_type() != at::kInt || table->dim() != 2 || (table->stride(1) != 1 && table->size(1) != 1)) return false;
   const int64_t batch = table->size(0), cols = table->size(1);
@@ -235,8 +237,8 @@ bool fill_cache(fa_paged_cache* c, const at::Tensor* k, const at::Tensor* v, boo
   return true;
 }
 bool fill_queries(fa_paged_cache* c, const at::Tensor* q, const at::Tensor& k, const at::Tensor* cu, int64_t max_q) {
-  if (!q || !cu || !q->is_cuda() || q->device() != k.device() || dtype_of(*q) < 0 || (k.scalar_type() != at::kFloat8_e4m3fn && q->scalar_type() != k.scalar_type()) || q->dim() != 3 || q->size(2) != k.size(3) || q->stride(2) != 1 ||
-      q->size(1) <= 0 || !small(q->size(1)) || q->size(1) % k.size(2) != 0 || !small(q->size(0)) || max_q <= 0 || !is_cu(cu, k) || cu->size(0) != (int64_t)c->batch + 1)
+  if (!q || !cu || !q->is_cuda() || q->device() != k.device() || dtype_of(*q) < 0 || (k.scalar_type() != at::kFloat8_e4m3fn && q->scalar_type() != k.scalar_type()) ||
+      q->dim() != 3 || q->size(2) != k.size(3) || q->stride(2) != 1 || q->size(1) <= 0 || !small(q->size(1)) || q->size(1) % k.size(2) != 0 || !small(q->size(0)) || max_q <= 0 || !is_cu(cu, k) || cu->size(0) != (int64_t)c->batch + 1)
     return false;
   c->cu_seqlens_q = (const int32_t*)ptr(*cu);
   c->nheads_q = (int32_t)q->size(1);
@@ -322,8 +324,11 @@ PyObject* paged_fwd(PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *groups = tensor(a[13], ok), *lens = tensor(a[14], ok);
     int64_t most;
     const auto ints = [&](const at::Tensor* x) { return x && x->device() == kc->device() && x->scalar_type() == at::kInt && x->dim() == 1 && x->is_contiguous(); };
-    if (!ok || !ints(groups) || !ints(lens) || lens->size(0) != f.cache.batch || groups->size(0) < 2 || groups->size(0) > (int64_t)f.cache.batch + 1 || !as_int(a[15], &most)) Py_RETURN_NONE;
-    prefix = fa_paged_prefix{(uint32_t)sizeof(prefix), (int32_t)(groups->size(0) - 1), (int32_t)most, 0, (const int32_t*)ptr(*groups), (const int32_t*)ptr(*lens)};
+    if (!ok || !ints(groups) || !ints(lens) || lens->size(0) != f.cache.batch || groups->size(0) < 2 ||
+        groups->size(0) > (int64_t)f.cache.batch + 1 || !as_int(a[15], &most))
+      Py_RETURN_NONE;
+    prefix = fa_paged_prefix{(uint32_t)sizeof(prefix), (int32_t)(groups->size(0) - 1), (int32_t)most, 0, (const int32_t*)ptr(*groups),
+                             (const int32_t*)ptr(*lens)};
   }
   if (a[8] == Py_None) scale = 1 / std::sqrt((double)f.cache.head_dim);
   at::Tensor o = at::empty(q->sizes(), plain(*q)), lse, ws;
