@@ -373,7 +373,7 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
   int q_begin = 0, Lq = 0;
   if (pair_units == 0 || !paged_rows(p.c, b, &q_begin, &Lq)) return;
   const int n = sharers(p, units);
-  const auto share_of = [&](int64_t u) { return (int)(((u + 1) * n - 1) / units); };  // (the last w with units * w / n <= u)
+  const auto share_of = [&](int64_t u) { return (int)quotient((u + 1) * n - 1, units); };  // (the last w with units * w / n <= u)
   const int w0 = share_of(begin), w1 = share_of(begin + pair_units - 1);
   const bool alone = w0 == w1;
   if (alone && !kPrefix) return;

@@ -60,7 +60,12 @@ FA_DEVICE Spot spot_of(const PagedCache& c, int64_t u, int sums0) {
 FA_DEVICE int sharers(const PagedFwdParams& p, int64_t units) {
   return units >= p.groups ? p.groups : units > 0 ? (int)units : 1;
 }
-FA_DEVICE int64_t share_begin(int64_t units, int w, int sharers) { return units * w / sharers; }
+// (a quotient of numbers that are not negative: 64 bits of division are some hundred instructions, and these stand in front of everything)
+FA_DEVICE int64_t quotient(int64_t x, int64_t y) {
+  if (__builtin_expect(((x | y) >> 32) == 0, 1)) return (uint32_t)x / (uint32_t)y;
+  return x / y;
+}
+FA_DEVICE int64_t share_begin(int64_t units, int w, int sharers) { return quotient(units * w, sharers); }
 // The first unit of the pair after (b, h): false if there is none
 template <bool kPrefix = false>
 FA_DEVICE bool next_pair(const PagedCache& c, Spot* at) {
