@@ -78,16 +78,40 @@ FA_DEVICE int own_len(const PagedCache& c, int b) {
   const int n = paged_len(c, b) - first_own<kPrefix>(c, b);
   return n > 0 ? n : 0;
 }
-// Adds the prefix's parts lane, lane + lanes, .. of a row (of all the call's rows of key head h) to x.  A part's maximum is one of scores before scaling; `unit`
-// brings it to x's units.
+// Adds the prefix's parts lane, lane + lanes, .. of a row (of all the call's rows of key head h) to x, several at a time, whose loads are on their way together and whose
+// maxima are compared first.  A part's maximum is one of scores before scaling; `unit` brings it to x's units.
 template <int D>
 FA_DEVICE void add_prefix(const PagedFwdParams& p, JoinedRow* x, int h, int64_t row, int d0, float cs, float unit, int lane = 0, int lanes = 1) {
+  constexpr int kBatch = 4;
   const int64_t rows = (int64_t)p.c.total_q * p.c.G, all = (int64_t)p.c.HK * rows, at = (int64_t)h * rows + row;
-#pragma unroll 4
-  for (int i = lane; i < p.pre_splits; i += lanes) {
-    const float* const from = p.pre + (int64_t)i * all * (D + 3);
-    const float* const ml = from + all * D + at * 3;
-    x->add(PartRow{ml[0] * unit, ml[1], ml[2]}, *reinterpret_cast<const f32x4*>(from + at * D + d0), cs);
+  const float* from = p.pre + (int64_t)lane * all * (D + 3);
+  const int64_t step = (int64_t)lanes * all * (D + 3);
+  for (int i = lane; i < p.pre_splits; i += kBatch * lanes) {
+    PartRow m[kBatch];
+    f32x4 o[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) {
+      const float* const ml = from + all * D + at * 3;
+      m[j] = PartRow{ml[0] * unit, ml[1], ml[2]};
+      o[j] = *reinterpret_cast<const f32x4*>(from + at * D + d0);
+      if (i + (j + 1) * lanes < p.pre_splits) from += step;  // (behind the last one: that one again, and not counted)
+    }
+#pragma unroll
+    for (int j = 1; j < kBatch; j++)
+      if (i + j * lanes >= p.pre_splits) m[j] = PartRow{-INFINITY, 0.f, 0.f}, o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float top = x->a.m;
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) top = fmaxf(top, m[j].m);
+    const float ref = top == -INFINITY ? 0.f : top * cs, f = fast_exp2(x->a.m * cs - ref);
+    x->a = PartRow{top, x->a.l * f, x->a.u * f};
+    x->o = x->o * f;
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) {
+      const float w = fast_exp2(m[j].m * cs - ref);
+      x->a.l = __builtin_fmaf(m[j].l, w, x->a.l);
+      x->a.u = __builtin_fmaf(m[j].u, w, x->a.u);
+      x->o = x->o + o[j] * w;
+    }
   }
 }
 
