@@ -306,6 +306,9 @@ ATTEND = [  # lens, new, H, HK, D, PS, causal
     ([515, 90], [70, 60], 6, 2, 16, 16, False),
     ([2000], [40], 8, 1, 128, 16, True),
     ([3, 200], [50, 50], 4, 4, 64, 16, True),
+    ([1500, 33], [1, 1], 32, 1, 128, 1024, True),  # 32 rows a pair
+    ([40] * 70, [1] * 70, 2, 2, 64, 16, True),
+    ([90, 2000], [1, 2], 40, 1, 16, 512, True),
 ]
 
 
@@ -476,6 +479,9 @@ PREFIX = [  # lens, new, groups, prefix, H, HK, D, PS, causal
     ([257, 260], [1, 4], [2], [256], 4, 4, 16, 256, True),                 # nothing but the prefix and the new tokens
     ([400, 410], [150, 140], [2], [240], 4, 2, 64, 16, True),
     ([520] * 70, [1] * 70, [1] * 30 + [40], [496] * 31, 2, 2, 32, 16, True),
+    ([150, 140] * 66, [1, 2] * 66, [2] * 66, [128] * 66, 2, 1, 64, 16, True),  # more groups than lanes
+    ([2100, 3000], [1, 1], [2], [2048], 64, 2, 64, 1024, True),               # 32 rows a pair, pages of 1024
+    ([520, 530, 540], [2, 2, 2], [3], [512], 48, 3, 16, 512, True),
 ]
 
 
@@ -724,6 +730,34 @@ def test_8_bits_beyond_32_bit_offsets(lib, new):
         two = be.paged_fwd(q, k, v, t, cu, small.dlens, new, 500, 0.1, True, cu_groups=cg, prefix_lens=pl, max_prefix_len=256, always=True, **s)[0]
         got.append((out, two, *p.paged_read_func(k, v, t, cu, small.dlens, 2 * new, dtype=torch.float16, **s)))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_queries_that_are_views(lib, new):
+    """q, k and v as parts of a packed projection, tables and integers as parts of larger tensors"""
+    from flash_attn import flash_attn_paged_interface as p
+    c = Cache8([300, 280], 2, 64, 16, torch.bfloat16, 3).gpu()
+    packed = randn(2 * new, 3, 4, 64, dtype=torch.bfloat16, seed=5)
+    d = packed.cuda()
+    cu = torch.cat([cumulative([new, new]).cuda()] * 2)[:3]
+    table = torch.cat([c.dtable, c.dtable], 1)[:, :c.dtable.shape[1]]
+    where = (c.dk, c.dv, table, cu, c.dlens)
+    plain = p.flash_attn_paged_func(d[:, 1].contiguous(), *where, new, 300, **c.scales)
+    out = p.flash_attn_paged_func(d[:, 1], *where, new, 300, **c.scales)
+    assert torch.equal(out, plain)
+    check_attention(packed[:, 1], c, [new, new], True, out)
+    cg, pl = cumulative([2]).cuda(), torch.full((4,), 256, dtype=torch.int32, device="cuda")[1:3]
+    share_table = table.clone()
+    share_table[1, :16] = share_table[0, :16]
+    args = (c.dk, c.dv, share_table, cu, c.dlens, new, 300)
+    assert torch.equal(p.flash_attn_paged_prefix_func(d[:, 1], *args, cg, pl, 256, **c.scales), p.flash_attn_paged_prefix_func(d[:, 1].contiguous(), *args, cg, pl, 256, **c.scales))
+    for k, v in ((d[:, 1, :2], d[:, 2, 2:]), (d[:, 1, :2].contiguous(), d[:, 2, 2:].contiguous())):
+        q = p.paged_append_func(d[:, 0], k, v, *where, **c.scales)
+        assert torch.equal(q, d[:, 0])
+        got = p.paged_read_func(*where[:5], 2 * new, dtype=torch.bfloat16, **c.scales)
+        want = [ref_quantise(t.double().cpu(), torch.bfloat16)[0] for t in (k, v)]
+        assert same(got[0].cpu().double(), want[0]) and same(got[1].cpu().double(), want[1])
 
 
 @pytest.mark.gpu
