@@ -1,5 +1,5 @@
 // fa_paged_append: the new tokens' k and v go into their sequences' pages, k (and q, into q_out) normalised and turned on the way (fa_norm.h).
-// HBM-bound for prompts (each vector read once, written once: 4.5 TB/s, of 5.3 that a copy reaches; without norm and rotation 5.1), whose workgroups
+// HBM-bound for prompts (each vector read once, written once: 4.8 TB/s, of 5.4 that a copy reaches; into 8 bits 4.1), whose workgroups
 // walk over the rows; for a decode step's few rows bound by latency: the row's sequence, its
 // length, its page and the store depend on each other, so the rows are loaded before any of them is asked for, and a wave finds a row's sequence
 // with one load and a ballot for 64 sequences.
@@ -53,7 +53,7 @@ FA_DEVICE void paged_append(const AppendParams p) {
   for (int row0 = group * ROWS; row0 < p.c.total_q; row0 += p.groups * ROWS) {
     vec8 x8[ROWS];
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) x8[i] = bitcast<vec8>(ld_global16(src + (int64_t)(row0 + i < p.c.total_q ? row0 + i : p.c.total_q - 1) * rs));
+    for (int i = 0; i < ROWS; i++) x8[i] = bitcast<vec8>(ld_row16<(ROWS > 1)>(src + (int64_t)(row0 + i < p.c.total_q ? row0 + i : p.c.total_q - 1) * rs));
     RowPlaces<ROWS> at;
     at.find(p.c, p.given_positions, row0);
     // (the rows have come in with what that looked up; said here, since on paths that drop a row its load would count as under way, and the next trip's
