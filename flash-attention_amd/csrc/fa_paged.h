@@ -119,7 +119,7 @@ FA_DEVICE int slot_of_group(const PagedCache& c, int g) { return (g << 4) & ((1 
 
 // Stages 16 consecutive keys (or values) of a tile: such a group lies in one page, so its address is wave-uniform and a group's loads are those
 // of fa_stage.h, from a base of its own.  The tile's rows are unpadded and swizzled as there (the swizzles have a period of 16 rows at most).
-template <int D, int KIND>
+template <int D, int KIND, bool kStream = false>
 struct GroupStager {
   static constexpr int CH = D / 8;
   static constexpr int RPI = 64 / CH < 16 ? 64 / CH : 16;  // rows per direct-to-LDS instruction (d = 16: half a wave's lanes)
@@ -139,12 +139,12 @@ struct GroupStager {
     if (64 / CH > 16 && rl >= 16) return;
     if (__builtin_expect(last >= 15, 1)) {
 #pragma unroll
-      for (int i = 0; i < NI; i++) dma16(base, off[i], dst + i * 1024);
+      for (int i = 0; i < NI; i++) dma16<kStream>(base, off[i], dst + i * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const int r = i * RPI + rl;
-        dma16(base, (uint32_t)((r < last ? r : last) * rsb) + 16u * (uint32_t)(pch ^ tile_swz<D, KIND>(r)), dst + i * 1024);
+        dma16<kStream>(base, (uint32_t)((r < last ? r : last) * rsb) + 16u * (uint32_t)(pch ^ tile_swz<D, KIND>(r)), dst + i * 1024);
       }
     }
   }

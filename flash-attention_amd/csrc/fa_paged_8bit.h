@@ -124,7 +124,7 @@ FA_DEVICE int tile_swz8(int r) {
 }
 
 // Stages 16 consecutive keys (or values), as GroupStager does those of 16 bits.
-template <int D, int KIND>
+template <int D, int KIND, bool kStream = false>
 struct GroupStager8 {
   static constexpr int CH = D / 16;
   static constexpr int RPI = 64 / CH < 16 ? 64 / CH : 16;  // rows per instruction (d < 64: some lanes have none)
@@ -144,12 +144,12 @@ struct GroupStager8 {
     if (64 / CH > 16 && rl >= 16) return;
     if (__builtin_expect(last >= 15, 1)) {
 #pragma unroll
-      for (int i = 0; i < NI; i++) dma16(base, off[i], dst + i * 1024);
+      for (int i = 0; i < NI; i++) dma16<kStream>(base, off[i], dst + i * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const int r = i * RPI + rl;
-        dma16(base, (uint32_t)((r < last ? r : last) * rsb) + 16u * (uint32_t)(pch ^ tile_swz8<D, KIND>(r)), dst + i * 1024);
+        dma16<kStream>(base, (uint32_t)((r < last ? r : last) * rsb) + 16u * (uint32_t)(pch ^ tile_swz8<D, KIND>(r)), dst + i * 1024);
       }
     }
   }

@@ -15,6 +15,7 @@ struct Plan {
   bool decode;
   int groups;              // decode (fa_paged_decode.hip)
   bool wide;               // ... eight (d = 128: four) waves a workgroup
+  bool stream;             // ... that read past the caches
   int nq_tiles, n_splits;  // chunk (fa_paged_chunk.hip)
   bool deal;
   size_t bytes;
@@ -87,6 +88,12 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
       pl.wide = !many && max_keys <= (pairs >= 192 ? 2048 : pairs >= 96 ? 1280 : 768);
       whole = pl.wide || max_keys <= 128 || (many && max_keys <= (c.head_dim == 64 ? 1536 : 2048));
     }
+    // Keys are read once.  Past the caches that is faster where they come from memory, 32 x 8 pairs of 4096 .. 16384 keys, d = 128, 237 -> 212 us, in 8 bits 137 -> 121, 48 of 4000 22.9 -> 21.7;
+    // where the caches have them from the call before it costs a little, more so in one workgroup's chain.  us through / past them, memory | caches: wide, 8 bits, 256 pairs of
+    // 1000, d = 128 19.5 / 18.3 | 17.5 / 17.0, 96 of 700, d = 64 (9 MB) 10.1 / 9.9 | 9.6 / 9.7, 32 of 500 (4 MB) 10.8 / 11.0 | 10.3 / 10.8; 16 bits 256 of 1000, d = 128 29.4 / 26.3 |
+    // 25.8 / 25.2, 96 of 1000, d = 64 12.4 / 11.2 | 11.0 / 11.0, 12 of 500 8.2 / 8.6 | 7.7 / 7.7; the line, 16 bits, 8 of 1000, d = 128 12.7 / 12.7 | 12.2 / 12.5, 12 of 4000, d =
+    // 64 12.8 / 12.9 | 12.2 / 12.4, 8 bits 8 of 2000, d = 128 12.7 / 12.7 | 12.0 / 11.9
+    pl.stream = pairs * max_keys * c.head_dim * (k8 ? 2 : 4) >= ((int64_t)8 << 20);
     if (!whole) {
       const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
       pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim, k8), pairs * units);
@@ -181,7 +188,7 @@ int fa_paged_fwd_with(const fa_paged_fwd_args* a, const fa_paged_scales* scales,
     return fa::fail(FA_ERR_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace", name, bytes);
   fa::PagedFwdParams p = params(a, scales);
   p.groups = pl.groups;
-  p.wide = pl.wide;
+  p.wide = !pl.wide ? 0 : pl.stream ? 2 : 1;
   p.nq_tiles = pl.nq_tiles;
   p.n_splits = pl.n_splits;
   p.deal = pl.deal;

@@ -7,7 +7,8 @@
 // units of kDecodeUnit keys of all pairs are laid out in one line, and each of the resident workgroups takes an equal share of it - the end of one
 // pair, some whole pairs, the beginning of another.  Pairs that more than one workgroup has touched are joined by a second kernel.  Pairs that fill
 // the device by themselves, and short ones, have a workgroup each (the rule, with both sides' times, is fa_paged_api.hip's).
-// 32 x 8 pairs of 4096 .. 16384 keys, d = 128, 1.34 GB: 239 us, 5.6 TB/s; 8 pairs of 16000 23, 12 of 500 keys, d = 64, 7.8: a chain of latencies.
+// Keys are read past the caches (kStream) but by wide workgroups of small launches (the rule is there, too).
+// 32 x 8 pairs of 4096 .. 16384 keys, d = 128, 1.34 GB: 212 us, 6.3 TB/s (239 through the caches); 8 pairs of 16000 23, 12 of 500 keys, d = 64, 7.8: a chain of latencies.
 #include "fa_paged_decode_kernel.h"
 
 namespace fa {
@@ -19,10 +20,16 @@ constexpr int decode_bound(int head_dim, int waves) { return head_dim == 128 ? 1
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, decode_bound(D, NW)) fa_paged_decode_kernel(const PagedFwdParams p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[DecodeCfg<D, NW, false>::kLds];
-  paged_decode<T, D, NW, false, false>(p, blockIdx.x, lds_raw);
+  paged_decode<T, D, NW, false, false, NW != kDecodeWide(D)>(p, blockIdx.x, lds_raw);
 }
 
 namespace {
+
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * kDecodeWide(D), decode_bound(D, kDecodeWide(D))) paged_decode_wide_stream_kernel(const PagedFwdParams p) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[DecodeCfg<D, kDecodeWide(D), false>::kLds];
+  paged_decode<T, D, kDecodeWide(D), false, false, true>(p, blockIdx.x, lds_raw);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_decode_join_kernel(const PagedFwdParams p) {
@@ -33,7 +40,8 @@ template <typename T, int D>
 hipError_t launch_d(const PagedFwdParams& p, hipStream_t stream) {
   const unsigned pairs = (unsigned)(p.c.B * p.c.HK);
   const dim3 grid(p.groups > 0 ? (unsigned)p.groups : pairs);
-  if (p.wide) hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWide(D)>), grid, dim3(64 * kDecodeWide(D)), 0, stream, p);
+  if (p.wide == 2) hipLaunchKernelGGL((paged_decode_wide_stream_kernel<T, D>), grid, dim3(64 * kDecodeWide(D)), 0, stream, p);
+  else if (p.wide) hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWide(D)>), grid, dim3(64 * kDecodeWide(D)), 0, stream, p);
   else hipLaunchKernelGGL((fa_paged_decode_kernel<T, D, kDecodeWaves(D)>), grid, dim3(64 * kDecodeWaves(D)), 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.groups == 0) return e;

@@ -9,7 +9,12 @@ namespace {
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, D == 128 ? 2 : D == 64 ? 3 : 4) fa_paged_decode_8bit_kernel(const PagedFwdParams p) {
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[DecodeCfg<D, NW, true>::kLds];
-  paged_decode<T, D, NW, true, false>(p, blockIdx.x, lds_raw);
+  paged_decode<T, D, NW, true, false, NW != kDecodeWide8>(p, blockIdx.x, lds_raw);
+}
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * kDecodeWide8, D == 128 ? 2 : D == 64 ? 3 : 4) paged_decode_wide_stream_8bit_kernel(const PagedFwdParams p) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[DecodeCfg<D, kDecodeWide8, true>::kLds];
+  paged_decode<T, D, kDecodeWide8, true, false, true>(p, blockIdx.x, lds_raw);
 }
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_decode_join_8bit_kernel(const PagedFwdParams p) {
@@ -20,7 +25,8 @@ template <typename T, int D>
 hipError_t launch_d(const PagedFwdParams& p, hipStream_t stream) {
   const unsigned pairs = (unsigned)(p.c.B * p.c.HK);
   const dim3 grid(p.groups > 0 ? (unsigned)p.groups : pairs);
-  if (p.wide) hipLaunchKernelGGL((fa_paged_decode_8bit_kernel<T, D, kDecodeWide8>), grid, dim3(64 * kDecodeWide8), 0, stream, p);
+  if (p.wide == 2) hipLaunchKernelGGL((paged_decode_wide_stream_8bit_kernel<T, D>), grid, dim3(64 * kDecodeWide8), 0, stream, p);
+  else if (p.wide) hipLaunchKernelGGL((fa_paged_decode_8bit_kernel<T, D, kDecodeWide8>), grid, dim3(64 * kDecodeWide8), 0, stream, p);
   else hipLaunchKernelGGL((fa_paged_decode_8bit_kernel<T, D, kDecodeWaves8>), grid, dim3(64 * kDecodeWaves8), 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.groups == 0) return e;

@@ -37,14 +37,14 @@ struct DecodeCfg {
   static constexpr int kLds = kTiles > kMerge ? kTiles : kMerge;
 };
 
-template <typename T, int D, int NW_, bool k8, bool kPrefix>
+template <typename T, int D, int NW_, bool k8, bool kPrefix, bool kStream>
 FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char* const lds_raw) {
   using C = DecodeCfg<D, NW_, k8>;
   using E = Elem<T>;
   using vec8 = typename E::vec8;
   constexpr int NW = C::NW, BN = C::BN, DV = C::DV;
-  using KStager = std::conditional_t<k8, GroupStager8<D, kSwzRow>, GroupStager<D, kSwzRow>>;
-  using VStager = std::conditional_t<k8, GroupStager8<D, kSwzTr>, GroupStager<D, kSwzTr>>;
+  using KStager = std::conditional_t<k8, GroupStager8<D, kSwzRow, kStream>, GroupStager<D, kSwzRow, kStream>>;
+  using VStager = std::conditional_t<k8, GroupStager8<D, kSwzTr, kStream>, GroupStager<D, kSwzTr, kStream>>;
   constexpr int NI = 2 * KStager::NI;  // loads of a tile's K, and of its V
   constexpr int NX = k8 ? 1 : 0;       // ... and of its exponents
   // (Numerator and denominator share the rounding of the probabilities - but not then: a probability times its value's 2^e may be far below fp16's normal numbers while

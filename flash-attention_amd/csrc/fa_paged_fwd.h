@@ -24,7 +24,7 @@ struct PagedFwdParams {
   int sq_r;
   int causal;
   float scale_log2;
-  // decode: the workgroups that share the line of units (0: a workgroup a pair), and whether they are wide.  chunk: query tiles and key splits
+  // decode: the workgroups that share the line of units (0: a workgroup a pair), and whether they are wide (2: and read past the caches).  chunk: query tiles and key splits
   int groups, wide;
   int nq_tiles, n_splits, deal;
   float* part;  // partial results

@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(256, prefix_bound(D)) fa_paged_prefix_kernel(c
     paged_chunk<T, D, kLse, k8, true, kPrefixKeys>(p, id % items, id / items, lds_raw);
   } else {
     if (NW < 4 && threadIdx.x >= 64 * NW) return;
-    paged_decode<T, D, NW, k8, true>(p, id - shared, lds_raw);
+    paged_decode<T, D, NW, k8, true, true>(p, id - shared, lds_raw);
   }
 }
 template <typename T, int D, bool k8>

@@ -67,12 +67,20 @@ FA_DEVICE int tr_off(int r0, int cp, int lane) {
 // reads themselves, in one of two ways: tiles that several waves fetch by wait_vmem() + workgroup barrier; the tiles of fa_decode_kernel, which
 // belong to one wave each, by counting that wave's outstanding loads (wait_vmcnt: loads complete in order, so every load between
 // a tile's and the wait is in the count) and lgkmcnt(0) before a stage is refilled, without a barrier.  M0 carries the LDS address, as the instruction requires.
+// kStream: of memory that is read once, which is to leave the caches to what is read again.
+template <bool kStream = false>
 FA_DEVICE void dma16(const char* base, uint32_t lane_off, unsigned char* lds_dst) {
   const uint32_t lds_addr = (uint32_t)(uintptr_t)(FA_LDS void*)lds_dst;
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
-               : "v"(lane_off), "s"(base), "s"(lds_addr)
-               : "memory", "m0");
+  if constexpr (kStream)
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(lane_off), "s"(base), "s"(lds_addr)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(lane_off), "s"(base), "s"(lds_addr)
+                 : "memory", "m0");
 }
 
 // The same with 4 bytes a lane: lane l's go to lds_dst + 4 * l.
