@@ -396,6 +396,9 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
     JoinedRow x;
     if (r < rows) {
       if (shares) add_prefix<D>(p, &x, h, (int64_t)q_begin * p.c.G + r, col * 4, cs, kLog2 ? p.scale_log2 : 1.f, lane, lanes);
+      // (several parts' loads on their way together: us, then, else, and with eight: 1 pair of 100000 keys, d = 128 26.6 / 39.7 / 24.8, of 30000 16.7 / 22.6 / 16.7; 8 of 8000
+      // 15.7 / 16.4 / 16.6; 16 of 7000, d = 64 14.9 / 14.7 / 14.7)
+#pragma unroll 4
       for (int i = w0 + lane; i <= w1; i += lanes) {
         const float* const s = kPrefix && alone ? p.whole_part + ((int64_t)b * p.c.HK + h) * kEach : p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * kEach;
         const float* const ml = s + kPartRows * D + r;
