@@ -44,8 +44,12 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
   // 14.7 / 10.8.  More than 32 rows a pair (8 x 4 heads, 24 tokens): 24 sequences behind 8192 keys 243 / 154.
   const int shared = prefix && pl.decode ? std::min(prefix->max_prefix_len, max_keys) / c.page_size * c.page_size : 0;
   const int64_t saved = (int64_t)(c.batch - (prefix ? prefix->n_groups : 0)) * c.nheads_k * shared * c.head_dim * (k8 ? 2 : 4);
-  pl.share = shared > 0 && (prefix->always || (shared >= 1024 && saved >= ((int64_t)8 << 20)));
-  if (pl.share) {
+  // ... and not where the prefix's chain of tiles, long where sequences are few or prefixes long, takes longer than reading it for each of them: a workgroup has a tile of 64 keys
+  // in 1.55 us, in 8 bits 2.1 (d = 128; less of fewer channels), and the same pages read again come at 8.8 TB/s, in 8 bits at 7, and 3 us later.  us so / unshared, one token, d =
+  // 128 where nothing is said, 16 bits and 8: 2 sequences of 1 x 8 heads behind 100000 keys 53 / 28 and 58 / 26; of 8 x 4 77 / 93 and 103 / 76; 16 groups of 2 of 8 x 1 heads behind
+  // 2048 35 / 36 and 39 / 31; 64 of 2 of 12, d = 64, behind 1024 76 / 68 and 63 / 56; 32 of 4 of 8 x 4 behind 4096 122 / 271 and 139 / 166; 16 sequences of 2 x 32 heads
+  // behind 8192 27.8 / 28.5 and 30.5 / 26.7; 2 of 12 heads, d = 64, behind 8192 18.1 / 16.6 and 14.9 / 16.7
+  if (shared > 0 && (prefix->always || (shared >= 1024 && saved >= ((int64_t)8 << 20)))) {
     // Row tiles of all groups, and how a prefix's keys are split: many splits are short ones, and leave as many parts to write and to read.  Of n splits the keys
     // take t = shared / n * 1.75 us / 64 (d = 128), the parts n times 8 of their bytes at 5 TB/s, beside a stream that wants them, too; together least at n =
     // sqrt(shared * 160 d / bytes of a split's parts).  At most half of the resident workgroups, and 128 keys each at least.  us with 8 / 16 / 32 splits: 32
@@ -56,13 +60,19 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
     pl.pre_tiles = (int)((all_rows + fa::kChunkRows - 1) / fa::kChunkRows) + prefix->n_groups - 1;
     const int64_t items = (int64_t)c.nheads_k * pl.pre_tiles, best = (int64_t)std::sqrt((double)shared * 160 * c.head_dim / (double)part);
     pl.pre_splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / 2 / std::max<int64_t>(items, 1), shared / 128, best, 64}));
+    const double rounds = std::max(1.0, (double)items * pl.pre_splits / (resident / 2));
+    const int64_t steps = (shared + 64 * (int64_t)pl.pre_splits - 1) / (64 * (int64_t)pl.pre_splits);
+    const double chain = rounds * steps * (k8 ? 2.1 : 1.55) * (c.head_dim + 64) / 192, again = (double)pairs * shared * c.head_dim * (k8 ? 2 / 7e6 : 4 / 8.8e6);
+    pl.share = prefix->always || chain < again + 3;
     pl.pre_bytes = fa::align16((size_t)pl.pre_splits * part);
     // ... beside the line of what comes behind it, which has the other resident workgroups, and a part for each pair
     const int64_t units = (std::max(max_keys - shared, 1) + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
     pl.groups = (int)std::min<int64_t>(std::max<int64_t>(resident - items * pl.pre_splits, resident / 2), pairs * units);
     pl.whole_at = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
     pl.bytes = pl.whole_at + (size_t)pairs * fa::decode_part_floats(c.head_dim) * 2;
-    return pl;
+    if (pl.share) return pl;
+    pl.pre_bytes = pl.bytes = 0;
+    pl.groups = 0;
   }
   if (pl.decode) {
     // A pair to itself, or shares of the line of all keys and a join behind them: the join is another launch and the line's beginning a chain of loads, 14 us

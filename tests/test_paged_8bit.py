@@ -184,15 +184,19 @@ def test_prefixes_are_shared_where_it_pays(lib):
     """on both sides of the rule, by the scratch that a call asks for: 8 x 4 heads, d = 128, pages of 64"""
     from flash_attn import flash_attn_gfx950 as be
 
-    def shares(batch, prefix, new=1, groups=1):
+    def shares(batch, prefix, new=1, groups=1, eight=False, heads=8):
         a = paged_args(be, "fwd")
         c = a.cache
-        c.head_dim, c.nheads_k, c.nheads_q, c.page_size, c.batch, c.total_q, c.max_seqlen_q, c.max_seqlen_k = 128, 8, 32, 64, batch, batch * new, new, prefix + 300
+        c.head_dim, c.nheads_k, c.nheads_q, c.page_size, c.batch, c.total_q, c.max_seqlen_q, c.max_seqlen_k = 128, heads, 32, 64, batch, batch * new, new, prefix + 300
         c.table_cols = c.table_row_stride = 1000
         x = _prefix(be, n_groups=groups, max_prefix_len=prefix)
-        return lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), None, ctypes.byref(x)) != lib.fa_paged_fwd_workspace_bytes(ctypes.byref(a))
+        scales = ctypes.byref(_scales(be)) if eight else None
+        return lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), scales, ctypes.byref(x)) != lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), scales, None)
 
-    assert shares(4, 2048) and shares(2, 2048) and shares(2, 8192) and shares(48, 1024) and shares(16, 8192, 8) and shares(16, 8192, groups=3)
+    assert shares(4, 2048) and shares(2, 8192) and shares(48, 1024) and shares(16, 8192, 8) and shares(16, 8192, groups=3)
+    # ... and by how long a workgroup is at its part of the prefix
+    assert shares(2, 60000) and not shares(2, 60000, eight=True) and not shares(2, 60000, heads=1) and shares(64, 60000, eight=True, heads=1) and shares(2, 2048)
+    assert shares(128, 4096, groups=32, eight=True) and not shares(32, 2048, groups=16, eight=True)
     assert not shares(2, 1984) and not shares(48, 512) and not shares(48, 1023) and not shares(1, 100000) and not shares(16, 8192, 9) and not shares(16, 8192, groups=16)
 
 
