@@ -56,7 +56,7 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
     // sequences of 8 x 4 heads behind 8192 keys 34.2 / 33.0 / 37.9, 64 behind 16384 in 8 bits 81 / 62 / 75; of 128 / 256 / 512 keys: 3 groups of 4 x 4 heads of 3, d = 64, 3
     // tokens, behind 1667 .. 3333 15.9 / 15.2 / 20.8
     const int resident = 256 * (c.head_dim == 128 || (c.head_dim == 64 && !k8) ? 2 : 3);
-    const int64_t all_rows = (int64_t)c.total_q * (c.nheads_q / c.nheads_k), part = std::max<int64_t>(all_rows, 1) * (c.head_dim + 3) * 4 * c.nheads_k;
+    const int64_t all_rows = (int64_t)c.total_q * (c.nheads_q / c.nheads_k), part = std::max<int64_t>(fa::prefix_part_rows(c.total_q, c.nheads_q / c.nheads_k), 4) * (c.head_dim + 3) * 4 * c.nheads_k;
     pl.pre_tiles = (int)((all_rows + fa::kChunkRows - 1) / fa::kChunkRows) + prefix->n_groups - 1;
     const int64_t items = (int64_t)c.nheads_k * pl.pre_tiles, best = (int64_t)std::sqrt((double)shared * 160 * c.head_dim / (double)part);
     pl.pre_splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / 2 / std::max<int64_t>(items, 1), shared / 128, best, 64}));

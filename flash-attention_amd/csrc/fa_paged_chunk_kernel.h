@@ -404,8 +404,9 @@ FA_DEVICE void paged_chunk(const PagedFwdParams p, const int wg, const int split
   if (kShared || n_splits > 1) {  // partial result of this split, fp32: [split][pair][row of nq_tiles * 128][D], m, l and u behind all of them
     if (mw + c < rows) {
       // (of a prefix: [split][key head][row of the call])
-      const int64_t all = kShared ? (int64_t)p.c.HK * p.c.total_q * G : (int64_t)p.c.B * p.c.HK * p.nq_tiles * kChunkRows;
-      const int64_t at = kShared ? (int64_t)h * p.c.total_q * G + (int64_t)q_begin * G + mw + c : ((int64_t)b * p.c.HK + h) * p.nq_tiles * kChunkRows + mw + c;
+      const int64_t part_rows = kShared ? prefix_part_rows(p.c.total_q, G) : (int64_t)p.nq_tiles * kChunkRows;
+      const int64_t all = (kShared ? p.c.HK : (int64_t)p.c.B * p.c.HK) * part_rows;
+      const int64_t at = kShared ? h * part_rows + (int64_t)q_begin * G + mw + c : ((int64_t)b * p.c.HK + h) * part_rows + mw + c;
       float* const parts = kShared ? p.pre : p.part;
       float* const op = parts + (int64_t)split * all * (D + 3) + at * D;
       if (hf == 0) {

@@ -29,7 +29,7 @@ struct PagedFwdParams {
   int nq_tiles, n_splits, deal;
   float* part;  // partial results
   // shared prefixes: groups of sequences (cu_groups[g] .. cu_groups[g + 1]), the splits of a prefix's keys, the row tiles that there can be, and the parts:
-  // [split][key head][G * total_q rows][D], m, l and u behind all of them
+  // [split][key head][G * total_q rows, up to a multiple of four][D], m, l and u behind all of them
   const int32_t* cu_groups;
   int n_groups, pre_splits, pre_tiles;
   float* pre;
@@ -66,6 +66,8 @@ struct JoinedRow {
   }
 };
 
+// Rows of a key head in a prefix's parts: those of the call, up to a multiple of four, since a split's (D + 3) floats a row are to begin at 16 bytes, too
+__host__ __device__ __forceinline__ int64_t prefix_part_rows(int total_q, int G) { return ((int64_t)total_q * G + 3) / 4 * 4; }
 // The keys of sequence b that its group shares: what comes in front of its own ones
 template <bool kPrefix>
 FA_DEVICE int first_own(const PagedCache& c, int b) {
@@ -83,7 +85,7 @@ FA_DEVICE int own_len(const PagedCache& c, int b) {
 template <int D>
 FA_DEVICE void add_prefix(const PagedFwdParams& p, JoinedRow* x, int h, int64_t row, int d0, float cs, float unit, int lane = 0, int lanes = 1) {
   constexpr int kBatch = 4;
-  const int64_t rows = (int64_t)p.c.total_q * p.c.G, all = (int64_t)p.c.HK * rows, at = (int64_t)h * rows + row;
+  const int64_t rows = prefix_part_rows(p.c.total_q, p.c.G), all = (int64_t)p.c.HK * rows, at = (int64_t)h * rows + row;
   const float* from = p.pre + (int64_t)lane * all * (D + 3);
   const int64_t step = (int64_t)lanes * all * (D + 3);
   for (int i = lane; i < p.pre_splits; i += kBatch * lanes) {

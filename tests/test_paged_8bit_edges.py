@@ -1,13 +1,15 @@
-"""The paged cache in 8 bits and shared prefixes: bits of scores.
+"""The paged cache in 8 bits and shared prefixes: bits of scores, layouts of partial results.
 
 Tolerances are counted, not measured: u half a step of the element type, e = 2^-24 a rounding in fp32 (see test_paged.py)."""
+import ctypes
 import math
 
 import pytest
 import torch
 
-from test_paged import E32, cumulative
-from test_paged_8bit import DTYPES, Cache8, ref_quantise
+from test_paged import E32, Cache, cumulative
+from test_paged import _args as paged_args
+from test_paged_8bit import DTYPES, Cache8, _prefix, check_attention, randn, ref_quantise, share
 
 
 # ---- GPU: bits of scores
@@ -39,3 +41,42 @@ def test_lse_of_one_key_over_8_bits(lib, D, dtype, sizes):
     bound = math.log(2) * E32 * (2 * x + (x + far) + (x + far + 1) + (x + 1) + 2 * far + 2 * x)
     err = (lse[:, :, 0].cpu().double() - s).abs()
     assert (err <= bound).all(), (err / bound).max()
+
+
+# ---- parts of a shared prefix: rows that are no multiple of four
+
+def prefix_call(be, batch, H, HK, D, total, prefix, max_k, groups=1, new=1, always=1):
+    """A call's structs, of which nothing is read but the numbers"""
+    a = paged_args(be, "fwd")
+    c = a.cache
+    c.head_dim, c.nheads_k, c.nheads_q, c.page_size, c.batch, c.total_q, c.max_seqlen_q, c.max_seqlen_k = D, HK, H, 64, batch, total, new, max_k
+    c.table_cols = c.table_row_stride = 4000
+    return a, _prefix(be, n_groups=groups, max_prefix_len=prefix, always=always)
+
+
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_parts_of_a_prefix_begin_at_16_bytes(lib, D):
+    """a row's part is D + 3 floats: a split's rows are counted up to a multiple of four"""
+    from flash_attn import flash_attn_gfx950 as be
+
+    def scratch(total, HK=1):
+        a, x = prefix_call(be, 5, HK, HK, D, total, 1024, 1100, new=4)
+        return lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), None, ctypes.byref(x))
+
+    assert scratch(5) == scratch(6) == scratch(8) and scratch(9) > scratch(8)
+    assert scratch(7, HK=3) == scratch(8, HK=3) and scratch(8) % 16 == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("H, HK, D, new", [(1, 1, 128, [1, 1, 1, 1, 1]), (3, 3, 64, [1, 2, 1, 1]), (6, 2, 16, [1, 1, 1]), (5, 5, 32, [2, 1, 0, 2]), (1, 1, 64, [3, 4])])
+def test_parts_of_a_prefix_of_odd_numbers_of_rows(lib, H, HK, D, new, eight, dtype):
+    from flash_attn import flash_attn_gfx950 as be
+    B = len(new)
+    c = share((Cache8 if eight else Cache)([1024 + 20 * i + 5 for i in range(B)], HK, D, 64, dtype, 3, **(dict(spread=0.5) if eight else {})), [B], [1024]).gpu()
+    q = randn(sum(new), H, D, dtype=dtype, seed=5)
+    pl = torch.full((B,), 1024, dtype=torch.int32).cuda()
+    out, lse = be.paged_fwd(q.cuda(), c.dk, c.dv, c.dtable, cumulative(new).cuda(), c.dlens, max(new), max(c.lens), D ** -0.5, True, True, cu_groups=cumulative([B]).cuda(),
+                            prefix_lens=pl, max_prefix_len=1024, always=True, **(c.scales if eight else {}))
+    check_attention(q, c, new, True, out, lse)
