@@ -69,7 +69,7 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
     const int64_t units = (std::max(max_keys - shared, 1) + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
     pl.groups = (int)std::min<int64_t>(std::max<int64_t>(resident - items * pl.pre_splits, resident / 2), pairs * units);
     pl.whole_at = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
-    pl.bytes = pl.whole_at + (size_t)pairs * fa::decode_part_floats(c.head_dim) * 2;
+    pl.bytes = pl.whole_at + (size_t)pairs * fa::whole_part_rows(c.max_seqlen_q, c.nheads_q / c.nheads_k) * (c.head_dim + 3) * 4;
     if (pl.share) return pl;
     pl.pre_bytes = pl.bytes = 0;
     pl.groups = 0;

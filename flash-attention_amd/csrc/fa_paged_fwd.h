@@ -153,6 +153,8 @@ FA_DEVICE float lse_of(float m, float u, float cs) { return u > 0.f ? (m * cs + 
 // ---- decode: keys are dealt out in units of kUnit; a pair (sequence, key head) has ceil(keys / kUnit), one at least, so that its rows are written
 constexpr int kDecodeUnit = 128;
 constexpr int kPartRows = 32;
+// Rows of a whole pair's part behind a shared prefix (there is one for every pair, however few rows the call has): at 16 bytes each, as above
+__host__ __device__ __forceinline__ int whole_part_rows(int max_sq, int G) { return (max_sq * G + 3) / 4 * 4; }
 // Waves of a workgroup that has a pair to itself where pairs about fill the device: as many as their tiles' LDS allows.
 constexpr int kDecodeWide(int head_dim) { return head_dim == 128 ? 4 : 8; }
 // ... over pages in 8 bits, whose tiles take half the LDS, and of one that has its share of the line
