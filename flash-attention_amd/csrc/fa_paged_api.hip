@@ -37,43 +37,6 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
   const int64_t pairs = (int64_t)c.batch * c.nheads_k;
   const int max_keys = (int)std::min<int64_t>(c.max_seqlen_k, (int64_t)c.table_cols * c.page_size);
   pl.decode = rows <= fa::kDecodeMaxQ;
-  // A shared prefix is read once for all if that saves at least 8 MB of 1024 keys or more: the same pages read again come out of the caches, and splitting and joining
-  // costs a launch.  us so / as if nothing were shared, one new token, 8 x 4 heads, d = 128: 2 sequences behind 2048 keys 12.7 / 13.2, 4 12.8 / 15.5, 48 26 / 48; behind 8192
-  // 2 16.6 / 20.6, 16 22 / 52, 48 35 / 132; behind 512 16 15.2 / 15.7, 48 24.2 / 24.7; in 8 bits 8 behind 2048 13.5 / 17.8, 16 behind 512 13.8 / 12.4, 48 23 / 19; 12
-  // heads, d = 64: 4 behind 2048 12.4 / 12.6, 16 18.5 / 15.9, 48 27 / 35, 2 behind 8192 18.1 / 16.3, 4 18.3 / 20.2; 8 heads, d = 32: 8 behind 2048 11.9 / 13.3, 48 behind 512
-  // 14.7 / 10.8.  More than 32 rows a pair (8 x 4 heads, 24 tokens): 24 sequences behind 8192 keys 243 / 154.
-  const int shared = prefix && pl.decode ? std::min(prefix->max_prefix_len, max_keys) / c.page_size * c.page_size : 0;
-  const int64_t saved = (int64_t)(c.batch - (prefix ? prefix->n_groups : 0)) * c.nheads_k * shared * c.head_dim * (k8 ? 2 : 4);
-  // ... and not where the prefix's chain of tiles, long where sequences are few or prefixes long, takes longer than reading it for each of them: a workgroup has a tile of 64 keys
-  // in 1.55 us, in 8 bits 2.1 (d = 128; less of fewer channels), and the same pages read again come at 8.8 TB/s, in 8 bits at 7, and 3 us later.  us so / unshared, one token, d =
-  // 128 where nothing is said, 16 bits and 8: 2 sequences of 1 x 8 heads behind 100000 keys 53 / 28 and 58 / 26; of 8 x 4 77 / 93 and 103 / 76; 16 groups of 2 of 8 x 1 heads behind
-  // 2048 35 / 36 and 39 / 31; 64 of 2 of 12, d = 64, behind 1024 76 / 68 and 63 / 56; 32 of 4 of 8 x 4 behind 4096 122 / 271 and 139 / 166; 16 sequences of 2 x 32 heads
-  // behind 8192 27.8 / 28.5 and 30.5 / 26.7; 2 of 12 heads, d = 64, behind 8192 18.1 / 16.6 and 14.9 / 16.7
-  if (shared > 0 && (prefix->always || (shared >= 1024 && saved >= ((int64_t)8 << 20)))) {
-    // Row tiles of all groups, and how a prefix's keys are split: many splits are short ones, and leave as many parts to write and to read.  Of n splits the keys
-    // take t = shared / n * 1.75 us / 64 (d = 128), the parts n times 8 of their bytes at 5 TB/s, beside a stream that wants them, too; together least at n =
-    // sqrt(shared * 160 d / bytes of a split's parts).  At most half of the resident workgroups, and 128 keys each at least.  us with 8 / 16 / 32 splits: 32
-    // sequences of 8 x 4 heads behind 8192 keys 34.2 / 33.0 / 37.9, 64 behind 16384 in 8 bits 81 / 62 / 75; of 128 / 256 / 512 keys: 3 groups of 4 x 4 heads of 3, d = 64, 3
-    // tokens, behind 1667 .. 3333 15.9 / 15.2 / 20.8
-    const int resident = 256 * (c.head_dim == 128 || (c.head_dim == 64 && !k8) ? 2 : 3);
-    const int64_t all_rows = (int64_t)c.total_q * (c.nheads_q / c.nheads_k), part = std::max<int64_t>(fa::prefix_part_rows(c.total_q, c.nheads_q / c.nheads_k), 4) * (c.head_dim + 3) * 4 * c.nheads_k;
-    pl.pre_tiles = (int)((all_rows + fa::kChunkRows - 1) / fa::kChunkRows) + prefix->n_groups - 1;
-    const int64_t items = (int64_t)c.nheads_k * pl.pre_tiles, best = (int64_t)std::sqrt((double)shared * 160 * c.head_dim / (double)part);
-    pl.pre_splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / 2 / std::max<int64_t>(items, 1), shared / 128, best, 64}));
-    const double rounds = std::max(1.0, (double)items * pl.pre_splits / (resident / 2));
-    const int64_t steps = (shared + 64 * (int64_t)pl.pre_splits - 1) / (64 * (int64_t)pl.pre_splits);
-    const double chain = rounds * steps * (k8 ? 2.1 : 1.55) * (c.head_dim + 64) / 192, again = (double)pairs * shared * c.head_dim * (k8 ? 2 / 7e6 : 4 / 8.8e6);
-    pl.share = prefix->always || chain < again + 3;
-    pl.pre_bytes = fa::align16((size_t)pl.pre_splits * part);
-    // ... beside the line of what comes behind it, which has the other resident workgroups, and a part for each pair
-    const int64_t units = (std::max(max_keys - shared, 1) + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
-    pl.groups = (int)std::min<int64_t>(std::max<int64_t>(resident - items * pl.pre_splits, resident / 2), pairs * units);
-    pl.whole_at = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
-    pl.bytes = pl.whole_at + (size_t)pairs * fa::whole_part_rows(c.max_seqlen_q, c.nheads_q / c.nheads_k) * (c.head_dim + 3) * 4;
-    if (pl.share) return pl;
-    pl.pre_bytes = pl.bytes = 0;
-    pl.groups = 0;
-  }
   if (pl.decode) {
     // A pair to itself, or shares of the line of all keys and a join behind them: the join is another launch and the line's beginning a chain of loads, 14 us
     // at the least; a workgroup alone with a pair reads 26 (d = 128) or 34 keys a wave and us, and the longest sequence decides.  us of a workgroup a pair / of
@@ -108,6 +71,52 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
       const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
       pl.groups = (int)std::min<int64_t>(decode_resident(c.head_dim, k8), pairs * units);
       pl.bytes = (size_t)pl.groups * fa::decode_part_floats(c.head_dim) * 4;
+    }
+    // A shared prefix is read once for all where that is quicker.  Of 1024 keys and 8 MB saved at least: the same pages read again come out of the caches, and splitting and joining costs a
+    // launch.  More than 32 rows a pair are not (8 x 4 heads, 24 tokens: 24 sequences behind 8192 keys 243 us so, 154 where each reads its own).
+    const int shared = prefix ? std::min(prefix->max_prefix_len, max_keys) / c.page_size * c.page_size : 0;
+    const int64_t saved = (int64_t)(c.batch - (prefix ? prefix->n_groups : 0)) * c.nheads_k * shared * c.head_dim * (k8 ? 2 : 4);
+    if (shared > 0 && (prefix->always || (shared >= 1024 && saved >= ((int64_t)8 << 20)))) {
+      Plan so = pl;
+      so.wide = so.stream = false;
+      // Row tiles of all groups, and how a prefix's keys are split: many splits are short ones, and leave as many parts to write and to read.  Of n splits the keys
+      // take t = shared / n * 1.75 us / 64 (d = 128), the parts n times 8 of their bytes at 5 TB/s, beside a stream that wants them, too; together least at n =
+      // sqrt(shared * 160 d / bytes of a split's parts).  At most half of the resident workgroups, and 128 keys each at least.  us with 8 / 16 / 32 splits: 32
+      // sequences of 8 x 4 heads behind 8192 keys 34.2 / 33.0 / 37.9, 64 behind 16384 in 8 bits 81 / 62 / 75; of 128 / 256 / 512 keys: 3 groups of 4 x 4 heads of 3, d = 64, 3
+      // tokens, behind 1667 .. 3333 15.9 / 15.2 / 20.8
+      const int resident = 256 * (c.head_dim == 128 || (c.head_dim == 64 && !k8) ? 2 : 3), G = c.nheads_q / c.nheads_k;
+      const int64_t all_rows = (int64_t)c.total_q * G, part = std::max<int64_t>(fa::prefix_part_rows(c.total_q, G), 4) * (c.head_dim + 3) * 4 * c.nheads_k;
+      so.pre_tiles = (int)((all_rows + fa::kChunkRows - 1) / fa::kChunkRows) + prefix->n_groups - 1;
+      const int64_t items = (int64_t)c.nheads_k * so.pre_tiles, best = (int64_t)std::sqrt((double)shared * 160 * c.head_dim / (double)part);
+      so.pre_splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / 2 / std::max<int64_t>(items, 1), shared / 128, best, 64}));
+      so.pre_bytes = fa::align16((size_t)so.pre_splits * part);
+      // ... beside the line of what comes behind it, which has the other resident workgroups, and a part for each pair
+      const int own = std::max(max_keys - shared, 1);
+      const int64_t units = (own + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
+      so.groups = (int)std::min<int64_t>(std::max<int64_t>(resident - items * so.pre_splits, resident / 2), pairs * units);
+      so.whole_at = (size_t)so.groups * fa::decode_part_floats(c.head_dim) * 4;
+      so.bytes = so.whole_at + (size_t)pairs * fa::whole_part_rows(c.max_seqlen_q, G) * (c.head_dim + 3) * 4;
+      // What either takes, us, fitted to 1185 pairs of times: drawn calls, and heads x sequences x prefixes of 1024 .. 100000 keys at every head dim.  The quicker one's time is exceeded by
+      // 0.6 % on the average, 27 % at most, more than 5 % in one of 20; on 670 other draws by 0.7 %, 37 % at most.  (By the chain and the bytes saved alone: 2.4 %, 132 %, one of 8.)
+      // Each reading its own: one launch, in which the longest sequence's workgroup decides, or the line and its join; either as the pairs' keys come in, and the distinct ones from
+      // memory.  Shared: the prefix's chain of tiles beside the line's workgroups, whose every pair is a chain of its own, and splits to join.
+      const double d128 = c.head_dim / 128., key = (k8 ? std::max(21.5, 25.6 * d128) : std::max(18.6, 48. * d128)) * 1e-6;
+      const int waves = k8 ? (pl.wide ? fa::kDecodeWide8 : fa::kDecodeWaves8) : pl.wide ? fa::kDecodeWide(c.head_dim) : fa::kDecodeWaves(c.head_dim);
+      const double keys = (double)pairs * max_keys * key + (double)prefix->n_groups * c.nheads_k * shared * c.head_dim * (k8 ? 2 : 4) * 0.064e-6;
+      const double alone = whole ? 5.3 + std::max(max_keys / (29. * waves), keys) : (c.head_dim == 128 ? 14.8 : 12.2) + keys;
+      const double rounds = std::max(1.0, (double)items * so.pre_splits / (resident / 2)), each = (double)pairs * units / so.groups;
+      const int64_t steps = (shared + 64 * (int64_t)so.pre_splits - 1) / (64 * (int64_t)so.pre_splits);
+      const double visits = each <= 1 ? 1 : 2 + std::floor((each - 1) / units);  // pairs that a workgroup of the line has to do with
+      const double together = 8.1 + std::max(rounds * steps * 1.65 * std::max(0.9, d128), 7.9 * (visits - 1) + (double)pairs * own * key) + 0.133 * so.pre_splits * d128;
+      // us together / alone, one new token, 300 keys of each sequence's own, 16 bits | 8:
+      // 8 x 4 heads, d = 128: 2 sequences behind 2048 keys 12.4 / 14.2, 48 24.7 / 51.2 | 23.8 / 42.6; 2 behind 8192 15.4 / 20.1, 4 15.9 / 25.0 | 17.0 / 22.3, 48 32 / 133 | 32 / 108; 8 groups
+      // of 4 behind 2048 26.4 / 33.8 | 29.0 / 30.8, 16 of 2 35.2 / 37.7 | 42.8 / 32.4; 2 sequences behind 100000 77 / 93 | 103 / 76.  1 x 8 heads: 4 sequences behind
+      // 8192 20.2 / 15.9 | 19.9 / 14.6, 48 21.5 / 33.6 | 23.1 / 30.4, 2 behind 100000 53 / 28 | 58 / 26
+      // 12 heads, d = 64: 4 behind 2048 12.1 / 13.5 | 12.5 / 14.1, 16 19.7 / 17.3 | 16.6 / 20.4, 48 29 / 38 | 26 / 41, 2 behind 8192 17.6 / 17.1 | 14.7 / 17.1, 4 17.8 / 21.6 | 14.9 / 20.8, 16 behind
+      // 1024 18.6 / 12.5 | 13.5 / 13.4; 16 groups of 2 behind 2048 48 / 33 | 33 / 30 (this one told wrongly)
+      // 8 heads, d = 32: 16 behind 2048 11.2 / 13.4 | 11.7 / 17.0, 8 groups of 4 15.3 / 13.7 | 17.0 / 21.9, 16 of 2 19.5 / 13.8, 16 sequences behind 8192 12.3 / 24.1 | 13.9 / 30.8
+      so.share = prefix->always || together < alone;
+      if (so.share) return so;
     }
     return pl;
   }

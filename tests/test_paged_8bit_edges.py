@@ -1,4 +1,4 @@
-"""The paged cache in 8 bits and shared prefixes: bits of scores, layouts of partial results.
+"""The paged cache in 8 bits and shared prefixes: bits of scores, layouts of partial results, where prefixes are shared.
 
 Tolerances are counted, not measured: u half a step of the element type, e = 2^-24 a rounding in fp32 (see test_paged.py)."""
 import ctypes
@@ -9,7 +9,7 @@ import torch
 
 from test_paged import E32, Cache, cumulative
 from test_paged import _args as paged_args
-from test_paged_8bit import DTYPES, Cache8, _prefix, check_attention, randn, ref_quantise, share
+from test_paged_8bit import DTYPES, Cache8, _prefix, _scales, check_attention, randn, ref_quantise, share
 
 
 # ---- GPU: bits of scores
@@ -93,3 +93,42 @@ def test_parts_of_a_prefix_of_odd_numbers_of_rows(lib, H, HK, D, new, eight, dty
     out, lse = be.paged_fwd(q.cuda(), c.dk, c.dv, c.dtable, cumulative(new).cuda(), c.dlens, max(new), max(c.lens), D ** -0.5, True, True, cu_groups=cumulative([B]).cuda(),
                             prefix_lens=pl, max_prefix_len=1024, always=True, **(c.scales if eight else {}))
     check_attention(q, c, new, True, out, lse)
+
+
+# ---- where prefixes are shared
+
+@pytest.mark.parametrize("eight, HK, G, D, batch, groups, prefix, shares", [
+    # each line: what was measured, us shared / alone
+    (False, 12, 1, 64, 16, 1, 2048, False),   # 18.5 / 15.9, 19.7 / 17.3
+    (False, 12, 1, 64, 2, 1, 8192, False),    # 18.1 / 16.3, 17.6 / 17.1
+    (False, 12, 1, 64, 4, 1, 8192, True),     # 17.8 / 21.6
+    (False, 12, 1, 64, 48, 1, 2048, True),    # 29.3 / 38.0
+    (False, 12, 1, 64, 16, 1, 1024, False),   # 18.6 / 12.5
+    (False, 12, 1, 64, 32, 16, 2048, False),  # 48.5 / 32.9
+    (True, 12, 1, 64, 16, 1, 2048, True),     # 16.6 / 20.4
+    (True, 12, 1, 64, 4, 1, 8192, True),      # 14.9 / 20.8
+    (False, 4, 3, 64, 48, 1, 1024, False),    # 15.8 / 12.6
+    (False, 4, 3, 64, 16, 1, 8192, True),     # 16.2 / 22.1
+    (False, 1, 8, 128, 4, 1, 8192, False),    # 20.2 / 15.9
+    (False, 1, 8, 128, 48, 1, 8192, True),    # 21.5 / 33.6
+    (True, 1, 8, 128, 16, 1, 8192, False),    # 22.4 / 17.9
+    (True, 1, 8, 128, 16, 1, 32768, False),   # 37.9 / 31.2
+    (False, 8, 4, 128, 2, 1, 2048, True),     # 12.4 / 14.2
+    (False, 8, 4, 128, 48, 1, 1024, True),    # 24.2 / 36.1
+    (True, 8, 4, 128, 32, 16, 2048, False),   # 42.8 / 32.4
+    (False, 2, 16, 128, 2, 1, 8192, False),   # 20.9 / 17.0
+    (False, 2, 16, 128, 16, 1, 8192, True),   # 22.4 / 26.6
+    (False, 8, 1, 32, 32, 16, 2048, False),   # 19.5 / 13.8
+    (False, 8, 1, 32, 16, 1, 8192, True),     # 12.3 / 24.1
+    (False, 12, 4, 32, 16, 1, 1024, False),   # 13.3 / 9.9
+    (True, 8, 1, 32, 64, 32, 1024, False),    # 26.2 / 18.6
+    (False, 8, 2, 16, 64, 32, 1024, False),   # 20.8 / 15.4
+    (True, 8, 2, 16, 16, 1, 8192, True),      # 14.0 / 31.2
+])
+def test_prefixes_are_shared_where_that_was_measured_to_be_quicker(lib, eight, HK, G, D, batch, groups, prefix, shares):
+    """one new token, 300 keys of each sequence's own"""
+    from flash_attn import flash_attn_gfx950 as be
+    a, x = prefix_call(be, batch, HK * G, HK, D, batch, prefix, prefix + 300, groups=groups, always=0)
+    scales = ctypes.byref(_scales(be)) if eight else None
+    asked = lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), scales, ctypes.byref(x))
+    assert (asked != lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), scales, None)) == shares
