@@ -95,7 +95,7 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
       const int64_t units = (own + fa::kDecodeUnit - 1) / fa::kDecodeUnit;
       so.groups = (int)std::min<int64_t>(std::max<int64_t>(resident - items * so.pre_splits, resident / 2), pairs * units);
       so.whole_at = (size_t)so.groups * fa::decode_part_floats(c.head_dim) * 4;
-      so.bytes = so.whole_at + (size_t)pairs * fa::whole_part_rows(c.max_seqlen_q, G) * (c.head_dim + 3) * 4;
+      so.bytes = so.whole_at + (size_t)pairs * rows * (c.head_dim + 4) * 4;
       // What either takes, us, fitted to 1185 pairs of times: drawn calls, and heads x sequences x prefixes of 1024 .. 100000 keys at every head dim.  The quicker one's time is exceeded by
       // 0.6 % on the average, 27 % at most, more than 5 % in one of 20; on 670 other draws by 0.7 %, 37 % at most.  (By the chain and the bytes saved alone: 2.4 %, 132 %, one of 8.)
       // Each reading its own: one launch, in which the longest sequence's workgroup decides, or the line and its join; either as the pairs' keys come in, and the distinct ones from

@@ -42,6 +42,12 @@ struct DecodeCfg {
   static constexpr int kLds = kTiles > kMerge ? kTiles : kMerge;
 };
 
+// A pair's part behind a shared prefix: there is one for every pair, of the call's rows (2^24 pairs of 32 rows are counted in 32 bits, for two registers less in scratch)
+template <int D>
+FA_DEVICE float* whole_part(const PagedFwdParams& p, int b, int h) {
+  return p.whole_part + (int64_t)((b * p.c.HK + h) * (p.c.max_sq * p.c.G)) * (D + 4);
+}
+
 template <typename T, int D, int NW_, bool k8, bool kPrefix, bool kStream>
 FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char* const lds_raw) {
   using C = DecodeCfg<D, NW_, k8>;
@@ -316,9 +322,7 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
     __syncthreads();
     // (behind a prefix a whole pair's results are a part, too: the join adds the prefix's)
     const bool alone = unit0 == 0 && unit1 == pair_units, whole = alone && !kPrefix;
-    const int part_rows = kPrefix && alone ? whole_part_rows(p.c.max_sq, p.c.G) : kPartRows;
-    float* const part_o = whole ? nullptr : (kPrefix && alone ? p.whole_part + ((int64_t)b * p.c.HK + h) * part_rows * (D + 3)
-                                                              : p.part + ((int64_t)wg * 2 + (first ? 0 : 1)) * (kPartRows * (D + 3)));
+    float* const part = whole ? nullptr : kPrefix && alone ? whole_part<D>(p, b, h) : p.part + ((int64_t)wg * 2 + (first ? 0 : 1)) * (kPartRows * (D + 4));
     for (int idx = tid; idx < rows * (D / 4); idx += 64 * NW) {
       const int r = idx / (D / 4), d0 = idx % (D / 4) * 4;
       float m = Xm[r];
@@ -338,12 +342,12 @@ FA_DEVICE void paged_decode(const PagedFwdParams p, const int wg, unsigned char*
         store_row_piece<T>(p, q_begin, h, r, d0, o * (l > 0.f ? fast_rcp(l) : 1.f));
         if (d0 == 0) store_lse(p, b, h, r, lse_of(m, us, mcs));
       } else {
-        *reinterpret_cast<f32x4*>(part_o + r * D + d0) = o;
+        *reinterpret_cast<f32x4*>(part + r * (D + 4) + d0) = o;
         if (d0 == 0) {
-          float* const ml = part_o + part_rows * D + r;
+          float* const ml = part + r * (D + 4) + D;
           ml[0] = m;
-          ml[part_rows] = l;
-          ml[2 * part_rows] = us;
+          ml[1] = l;
+          ml[2] = us;
         }
       }
     }
@@ -385,7 +389,6 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
   if (alone && !kPrefix) return;
   constexpr bool kLog2 = kLog2Maxima<T, k8>;
   const float cs = kLog2 ? 1.f : p.scale_log2;
-  const int part_rows = kPrefix && alone ? whole_part_rows(p.c.max_sq, p.c.G) : kPartRows;
   // the pair is the last of share w0, and its first, too, if the share begins with it; it is the first of the others'
   const int first_slot = share_begin(units, w0, n) == begin ? 0 : 1;
   const bool shares = kPrefix && first_own<kPrefix>(p.c, b) > 0;
@@ -406,10 +409,8 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
       // 15.7 / 16.4 / 16.6; 16 of 7000, d = 64 14.9 / 14.7 / 14.7)
 #pragma unroll 4
       for (int i = w0 + lane; i <= w1; i += lanes) {
-        const float* const s = kPrefix && alone ? p.whole_part + ((int64_t)b * p.c.HK + h) * part_rows * (D + 3)
-                                                : p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * (kPartRows * (D + 3));
-        const float* const ml = s + part_rows * D + r;
-        x.add(PartRow{ml[0], ml[part_rows], ml[2 * part_rows]}, *reinterpret_cast<const f32x4*>(s + r * D + col * 4), cs);
+        const float* const s = (kPrefix && alone ? whole_part<D>(p, b, h) : p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * (kPartRows * (D + 4))) + r * (D + 4);
+        x.add(PartRow{s[D], s[D + 1], s[D + 2]}, *reinterpret_cast<const f32x4*>(s + col * 4), cs);
       }
     }
     x.across<kCols>(lane, lanes, cs, os, ms);

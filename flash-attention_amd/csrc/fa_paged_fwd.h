@@ -153,8 +153,6 @@ FA_DEVICE float lse_of(float m, float u, float cs) { return u > 0.f ? (m * cs + 
 // ---- decode: keys are dealt out in units of kUnit; a pair (sequence, key head) has ceil(keys / kUnit), one at least, so that its rows are written
 constexpr int kDecodeUnit = 128;
 constexpr int kPartRows = 32;
-// Rows of a whole pair's part behind a shared prefix (there is one for every pair, however few rows the call has): at 16 bytes each, as above
-__host__ __device__ __forceinline__ int whole_part_rows(int max_sq, int G) { return (max_sq * G + 3) / 4 * 4; }
 // Waves of a workgroup that has a pair to itself where pairs about fill the device: as many as their tiles' LDS allows.
 constexpr int kDecodeWide(int head_dim) { return head_dim == 128 ? 4 : 8; }
 // ... over pages in 8 bits, whose tiles take half the LDS, and of one that has its share of the line
@@ -163,8 +161,8 @@ constexpr int kDecodeWaves8 = 4;
 // ... beside the workgroups of a shared prefix, which have four: two at d = 128 in 16 bits, the other two end at once, so that two workgroups' tiles fit a compute unit
 constexpr int kDecodeBeside(int head_dim, bool k8) { return !k8 && head_dim == 128 ? 2 : 4; }
 
-// floats of a workgroup's two partial results: [2][32][D] outputs, [2][3][32] m, l, u
-inline size_t decode_part_floats(int D) { return 2 * (size_t)kPartRows * (D + 3); }
+// A row's part is D elements, m, l and u and one float more, so that rows begin at 16 bytes; floats of a workgroup's two parts
+inline size_t decode_part_floats(int D) { return 2 * (size_t)kPartRows * (D + 4); }
 
 hipError_t launch_paged_decode(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 hipError_t launch_paged_chunk(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);

@@ -68,15 +68,15 @@ def test_parts_of_a_prefix_begin_at_16_bytes(lib, D):
 
 
 def test_parts_of_pairs_behind_a_prefix_have_the_rows_of_the_call(lib):
-    """a part for every pair, of as many rows as a pair has (up to a multiple of four) and not of the 32 that it may have"""
+    """a part for every pair, of as many rows as a pair has and not of the 32 that it may have; a row is D elements, m, l, u and what brings the next one to 16 bytes"""
     from flash_attn import flash_attn_gfx950 as be
 
     def scratch(batch, HK=32, G=1, new=1, D=128):
         a, x = prefix_call(be, batch, HK * G, HK, D, 64, 2048, 2100, new=new)  # (64 rows whatever the batch is: only the pairs' parts grow with it)
         return lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), None, ctypes.byref(x))
 
-    for more, rows in ((dict(), 4), (dict(new=5), 8), (dict(HK=8, G=4), 4), (dict(HK=8, G=4, new=3), 12), (dict(HK=4, G=8, new=4), 32), (dict(D=16, G=3, new=3), 12)):
-        each = more.get("HK", 32) * rows * (more.get("D", 128) + 3) * 4
+    for more, rows in ((dict(), 1), (dict(new=5), 5), (dict(HK=8, G=4), 4), (dict(HK=8, G=4, new=3), 12), (dict(HK=4, G=8, new=4), 32), (dict(D=16, G=3, new=3), 9)):
+        each = more.get("HK", 32) * rows * (more.get("D", 128) + 4) * 4
         assert scratch(1024, **more) - scratch(256, **more) == 768 * each, more
 
 
