@@ -503,4 +503,13 @@ FA_DEVICE void paged_chunk_join(const PagedFwdParams p, int lanes) {
   }
 }
 
+// A chunk kernel's launch, and behind it, where row tiles share their keys, the join
+inline hipError_t launch_chunk(void (*kernel)(PagedFwdParams), const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream) {
+  const int64_t pairs = (int64_t)p.c.B * p.c.HK, items = pairs * p.nq_tiles;
+  const dim3 grid((unsigned)(p.deal ? (pairs + 7) / 8 * 8 * p.nq_tiles : (items + 7) / 8 * 8), (unsigned)p.n_splits);
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || p.n_splits <= 1 ? e : launch_paged_chunk_join(p, dtype, head_dim, stream);
+}
+
 }  // namespace fa

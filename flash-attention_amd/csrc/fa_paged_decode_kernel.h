@@ -421,4 +421,19 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
   }
 }
 
+// A workgroup a pair, and others beside it for its rows
+inline hipError_t launch_decode_join(void (*join)(PagedFwdParams), const PagedFwdParams& p, hipStream_t stream) {
+  const unsigned pairs = (unsigned)(p.c.B * p.c.HK), rows = (unsigned)(p.c.max_sq * p.c.G), side = pairs < 1024 ? 1024 / pairs : 1;
+  hipLaunchKernelGGL(join, dim3(pairs, rows < side ? rows : side), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+// A decode kernel's launch, and behind it, where workgroups share the line, the join
+inline hipError_t launch_decode(void (*kernel)(PagedFwdParams), int waves, void (*join)(PagedFwdParams), const PagedFwdParams& p, hipStream_t stream) {
+  const unsigned pairs = (unsigned)(p.c.B * p.c.HK);
+  hipLaunchKernelGGL(kernel, dim3(p.groups > 0 ? (unsigned)p.groups : pairs), dim3(64 * waves), 0, stream, p);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || p.groups == 0 ? e : launch_decode_join(join, p, stream);
+}
+
 }  // namespace fa

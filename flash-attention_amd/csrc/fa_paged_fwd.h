@@ -11,6 +11,8 @@
 // more of them products bound both ways, and reading a key once more costs nothing.
 #pragma once
 
+#include <type_traits>
+
 #include "fa_paged.h"
 
 namespace fa {
@@ -173,5 +175,26 @@ hipError_t launch_paged_chunk_8bit(const PagedFwdParams& p, int dtype, int head_
 hipError_t launch_paged_prefix(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 hipError_t launch_paged_prefix_8bit(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
 constexpr int kChunkRows = 128;  // rows of a workgroup of the chunk kernel
+// ... whose splits' parts, in fp32 whatever the cache holds, are joined
+hipError_t launch_paged_chunk_join(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream);
+
+// launch(Type<T>{}, std::integral_constant<int, D>{}) with the element type of a dtype's code and the head dim
+template <typename T>
+struct Type {
+  using type = T;
+};
+template <typename F>
+hipError_t launch_for(int dtype, int head_dim, const F& launch) {
+  const auto of_type = [&](auto t) {
+    switch (head_dim) {
+      case 16: return launch(t, std::integral_constant<int, 16>{});
+      case 32: return launch(t, std::integral_constant<int, 32>{});
+      case 64: return launch(t, std::integral_constant<int, 64>{});
+      case 128: return launch(t, std::integral_constant<int, 128>{});
+      default: return hipErrorInvalidValue;
+    }
+  };
+  return dtype == 0 ? of_type(Type<_Float16>{}) : of_type(Type<__bf16>{});
+}
 
 }  // namespace fa

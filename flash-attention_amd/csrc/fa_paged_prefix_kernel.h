@@ -35,31 +35,16 @@ __global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedFwdPa
   paged_decode_join<T, D, k8, true>(p);
 }
 
-template <typename T, int D, bool k8>
-hipError_t launch_prefix_d(const PagedFwdParams& p, hipStream_t stream) {
-  const unsigned items = (unsigned)((p.c.HK * p.pre_tiles + 7) / 8 * 8), pairs = (unsigned)(p.c.B * p.c.HK);
-  const dim3 grid(items * (unsigned)p.pre_splits + (unsigned)p.groups);
-  if (p.lse) hipLaunchKernelGGL((fa_paged_prefix_kernel<T, D, true, k8>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((fa_paged_prefix_kernel<T, D, false, k8>), grid, dim3(256), 0, stream, p);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const unsigned rows = (unsigned)(p.c.max_sq * p.c.G), side = pairs < 1024 ? 1024 / pairs : 1;  // (workgroups beside each other for a pair's rows)
-  hipLaunchKernelGGL((paged_prefix_join_kernel<T, D, k8>), dim3(pairs, rows < side ? rows : side), dim3(256), 0, stream, p);
-  return hipGetLastError();
-}
-template <bool k8, typename T>
-hipError_t launch_prefix_t(const PagedFwdParams& p, int head_dim, hipStream_t stream) {
-  switch (head_dim) {
-    case 16: return launch_prefix_d<T, 16, k8>(p, stream);
-    case 32: return launch_prefix_d<T, 32, k8>(p, stream);
-    case 64: return launch_prefix_d<T, 64, k8>(p, stream);
-    case 128: return launch_prefix_d<T, 128, k8>(p, stream);
-    default: return hipErrorInvalidValue;
-  }
-}
 template <bool k8>
 hipError_t launch_prefix_of(const PagedFwdParams& p, int dtype, int head_dim, hipStream_t stream) {
-  return dtype == 0 ? launch_prefix_t<k8, _Float16>(p, head_dim, stream) : launch_prefix_t<k8, __bf16>(p, head_dim, stream);
+  return launch_for(dtype, head_dim, [&](auto t, auto d) {
+    using T = typename decltype(t)::type;
+    const unsigned items = (unsigned)((p.c.HK * p.pre_tiles + 7) / 8 * 8);
+    hipLaunchKernelGGL((p.lse ? fa_paged_prefix_kernel<T, d, true, k8> : fa_paged_prefix_kernel<T, d, false, k8>), dim3(items * (unsigned)p.pre_splits + (unsigned)p.groups),
+                       dim3(256), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch_decode_join(paged_prefix_join_kernel<T, d, k8>, p, stream);
+  });
 }
 
 }  // namespace fa
