@@ -1,4 +1,4 @@
-"""The paged cache in 8 bits and shared prefixes: bits of scores, layouts of partial results, where prefixes are shared.
+"""The paged cache in 8 bits and shared prefixes: bits of scores, layouts of partial results, where prefixes are shared, every route of a decode step.
 
 Tolerances are counted, not measured: u half a step of the element type, e = 2^-24 a rounding in fp32 (see test_paged.py)."""
 import ctypes
@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_paged import E32, Cache, cumulative
+from test_paged import E32, Cache, cumulative, half_step
 from test_paged import _args as paged_args
 from test_paged_8bit import DTYPES, Cache8, _prefix, _scales, check_attention, randn, ref_quantise, share
 
@@ -132,3 +132,108 @@ def test_prefixes_are_shared_where_that_was_measured_to_be_quicker(lib, eight, H
     scales = ctypes.byref(_scales(be)) if eight else None
     asked = lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), scales, ctypes.byref(x))
     assert (asked != lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), scales, None)) == shares
+
+
+# ---- GPU: every route of a decode step, each element within what its own keys allow
+
+def mark_tiles(c, keys=32):
+    """The upper half of a key's value says which `keys` of its sequence it belongs to: an element there is those keys' weight, so that a lost, doubled or exchanged tile shows"""
+    D = c.v.shape[-1]
+    eight = hasattr(c, "vc")
+    half = D // 2
+    for b, n in enumerate(c.lens):
+        page, slot = c.where(b, n)
+        x = c.v[page, slot].double()
+        x[..., half:] = 2.0 * (torch.arange(half)[None] == (torch.arange(n)[:, None] // keys) % half).double()[:, None]
+        if eight:
+            x, e = ref_quantise(x, c.v.dtype)
+            c.vc[page, slot] = (x * (2.0 ** -e.double())[..., None]).float().to(torch.float8_e4m3fn).view(torch.uint8)
+            c.vs[page, :, slot] = (e + 127).to(torch.uint8)
+        c.v[page, slot] = x.to(c.v.dtype)
+    return c
+
+
+def check_elements(q, c, new, got, lse=None):
+    """causal attention against 64 bits.  A probability is rounded by u of itself, in the numerator and in the denominator, and where it is below the type's normal numbers by
+    2^-25 (fp16) of the largest (times its value's scale): an element is off by 2 u of the sum of the magnitudes that it is made of, and by those."""
+    D, G, u = q.shape[2], q.shape[1] // c.k.shape[2], half_step(q.dtype)
+    at = 0
+    for b, n in enumerate(new):
+        Lk = c.lens[b]
+        page, slot = c.where(b, Lk)
+        for h in range(q.shape[1]):
+            qh, k, v = q[at:at + n, h].double(), c.k[page, slot, h // G].double(), c.v[page, slot, h // G].double()
+            s = qh @ k.t() * D ** -0.5
+            s = s.masked_fill(torch.arange(Lk)[None] >= (Lk - n + 1 + torch.arange(n))[:, None], -math.inf)
+            p = torch.softmax(s, 1)
+            o, parts = p @ v, p @ v.abs()
+            ds = (D + 12) * E32 * (qh.abs() @ k.abs().t()).max() * D ** -0.5
+            small = Lk * 2.0 ** -25 * p.amax(1, keepdim=True) * v.abs().max() * (4 if q.dtype == torch.float16 else 0)  # (a scale is less than 4 / 448 of the largest value)
+            tol = (2 * u + 2 * ds + 2 * (Lk + 8) * E32) * parts + u * o.abs() + small + 2.0 ** -24
+            err = (got[at:at + n, h].cpu().double() - o).abs()
+            assert (err <= tol).all(), (b, h, (err / tol).max(), (err > tol).nonzero()[:5])
+            if lse is not None:
+                t = torch.logsumexp(s, 1)
+                assert ((lse[b, h, :n].cpu().double() - t).abs() <= ds + (Lk + 8) * E32 + 8 * E32 * (1 + t.abs())).all(), (b, h)
+        at += n
+
+
+ROUTES = [  # lens, new, H, HK, D, PS, whether the keys lie on one line for all workgroups (which takes scratch)
+    # wide workgroups, a pair each, past the caches: 8 MB of keys
+    ([200 + 25 * i for i in range(32)], 1, 16, 8, 128, 64, False),
+    ([40 + 26 * i for i in range(25)], 2, 4, 4, 64, 16, False),
+    ([17 + 20 * i for i in range(32)], 1, 8, 8, 32, 32, False),
+    ([65 * i % 1061 + 1 for i in range(31)] + [1100], 1, 16, 8, 16, 128, False),
+    # more pairs than the device holds at once: the usual workgroups, a pair each
+    ([1 + 37 * i % 300 for i in range(70)], 1, 8, 4, 64, 16, False),
+    ([1 + 41 * i % 210 for i in range(70)], 3, 4, 4, 128, 32, False),
+    ([1 + 43 * i % 170 for i in range(130)], 1, 4, 4, 32, 16, False),
+    ([1 + 29 * i % 150 for i in range(130)], 2, 8, 4, 16, 16, False),
+    # few long pairs
+    ([2500, 1030, 1], 1, 4, 2, 16, 16, True),
+    ([1777, 3000], 2, 6, 2, 32, 64, True),
+    ([1500, 2049], 1, 2, 2, 64, 32, True),
+    ([900, 3001], 1, 8, 1, 128, 16, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens, new, H, HK, D, PS, line", ROUTES)
+@pytest.mark.parametrize("eight, want_lse", [(True, False), (True, True), (False, True)])
+def test_every_route_of_a_decode_step(lib, lens, new, H, HK, D, PS, line, dtype, eight, want_lse):
+    from flash_attn import flash_attn_gfx950 as be
+    from flash_attn import flash_attn_paged_interface as p
+    lens = [max(n, new) for n in lens]
+    c = mark_tiles((Cache8 if eight else Cache)(lens, HK, D, PS, dtype, 3)).gpu()
+    if eight:
+        a = be.PagedFwdArgs()
+        a.struct_bytes = ctypes.sizeof(a)
+        a.cache.head_dim, a.cache.nheads_k, a.cache.nheads_q, a.cache.page_size, a.cache.batch, a.cache.n_pages = D, HK, H, PS, len(lens), c.n_pages
+        a.cache.total_q, a.cache.max_seqlen_q, a.cache.max_seqlen_k, a.cache.table_cols = len(lens) * new, new, max(lens), c.table.shape[1]
+        a.cache.page_table = a.cache.seqlens_k = a.cache.cu_seqlens_q = 1 << 20
+        a.cache.table_row_stride = c.table.shape[1]
+        assert (lib.fa_paged_fwd_with_workspace_bytes(ctypes.byref(a), ctypes.byref(_scales(be)), None) > 0) == line
+    q = randn(len(lens) * new, H, D, dtype=dtype, seed=5)
+    r = p.flash_attn_paged_func(q.cuda(), c.dk, c.dv, c.dtable, cumulative([new] * len(lens)).cuda(), c.dlens, new, max(lens), return_softmax_lse=want_lse,
+                                **(c.scales if eight else {}))
+    out, lse = r if want_lse else (r, None)
+    check_elements(q, c, [new] * len(lens), out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("eight, new", [(False, 1), (True, 1), (True, 3), (False, 2)])
+def test_shared_prefixes_by_the_rule_against_64_bits(lib, eight, new, dtype):
+    from flash_attn import flash_attn_paged_interface as p
+    lens, groups, prefix = [2048 + 60 + 31 * i for i in range(7)] + [1408 + 33 + 40 * i for i in range(5)], [7, 5], [2048, 1408]
+    c = mark_tiles(share((Cache8 if eight else Cache)(lens, 4, 128, 128, dtype, 3), groups, prefix)).gpu()
+    scales = c.scales if eight else {}
+    q, cu = randn(12 * new, 16, 128, dtype=dtype, seed=5), cumulative([new] * 12).cuda()
+    pl = torch.tensor(prefix, dtype=torch.int32).repeat_interleave(torch.tensor(groups)).cuda()
+    where = (q.cuda(), c.dk, c.dv, c.dtable, cu, c.dlens, new, max(lens))
+    out, lse = p.flash_attn_paged_prefix_func(*where, cumulative(groups).cuda(), pl, max(prefix), return_softmax_lse=True, **scales)
+    check_elements(q, c, [new] * 12, out, lse)
+    alone, _ = p.flash_attn_paged_func(*where, return_softmax_lse=True, **scales)
+    check_elements(q, c, [new] * 12, alone)
+    assert not torch.equal(out, alone)  # (the rule shares here)
