@@ -64,8 +64,9 @@ Plan plan_of(const fa_paged_cache& c, bool k8 = false, const fa_paged_prefix* pr
     // Keys are read once.  Past the caches that is faster where they come from memory, 32 x 8 pairs of 4096 .. 16384 keys, d = 128, 237 -> 212 us, in 8 bits 137 -> 121, 48 of 4000 22.9 -> 21.7;
     // where the caches have them from the call before it costs a little, more so in one workgroup's chain.  us through / past them, memory | caches: wide, 8 bits, 256 pairs of
     // 1000, d = 128 19.5 / 18.3 | 17.5 / 17.0, 96 of 700, d = 64 (9 MB) 10.1 / 9.9 | 9.6 / 9.7, 32 of 500 (4 MB) 10.8 / 11.0 | 10.3 / 10.8; 16 bits 256 of 1000, d = 128 29.4 / 26.3 |
-    // 25.8 / 25.2, 96 of 1000, d = 64 12.4 / 11.2 | 11.0 / 11.0, 12 of 500 8.2 / 8.6 | 7.7 / 7.7; the line, 16 bits, 8 of 1000, d = 128 12.7 / 12.7 | 12.2 / 12.5, 12 of 4000, d =
-    // 64 12.8 / 12.9 | 12.2 / 12.4, 8 bits 8 of 2000, d = 128 12.7 / 12.7 | 12.0 / 11.9
+    // 25.8 / 25.2, 96 of 1000, d = 64 12.4 / 11.2 | 11.0 / 11.0, 12 of 500 8.2 / 8.6 | 7.7 / 7.7.  The line always reads past them: 16 bits, 8 of 1000, d = 128 11.9 / 11.3 | 10.8 / 10.8,
+    // 12 of 4000, d = 64 13.1 / 11.9 | 10.9 / 11.0, 16 of 7000 16.9 / 15.6 | 13.3 / 13.5, 8 of 6000, d = 32 10.9 / 10.4 | 9.9 / 9.9, 8 bits 8 of 2000, d = 128 11.8 / 11.4 | 10.5 / 10.5, of
+    // 5000, d = 64 12.1 / 11.5 | 11.0 / 11.0
     pl.stream = pairs * max_keys * c.head_dim * (k8 ? 2 : 4) >= ((int64_t)8 << 20);
     if (!whole) {
       const int64_t units = (max_keys + fa::kDecodeUnit - 1) / fa::kDecodeUnit;

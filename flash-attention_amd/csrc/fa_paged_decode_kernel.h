@@ -405,8 +405,8 @@ FA_DEVICE void paged_decode_join(const PagedFwdParams p) {
     JoinedRow x;
     if (r < rows) {
       if (shares) add_prefix<D>(p, &x, h, (int64_t)q_begin * p.c.G + r, col * 4, cs, kLog2 ? p.scale_log2 : 1.f, lane, lanes);
-      // (several parts' loads on their way together: us, then, else, and with eight: 1 pair of 100000 keys, d = 128 26.6 / 39.7 / 24.8, of 30000 16.7 / 22.6 / 16.7; 8 of 8000
-      // 15.7 / 16.4 / 16.6; 16 of 7000, d = 64 14.9 / 14.7 / 14.7)
+      // (several parts' loads on their way together: us, then, and else: 1 pair of 100000 keys, d = 128 24.2 / 35.4, in 8 bits 23.9 / 38.8, of 30000 15.8 / 22.3; 8 of 8000
+      // 14.6 / 15.4; 16 of 7000, d = 64 13.35 / 13.25)
 #pragma unroll 4
       for (int i = w0 + lane; i <= w1; i += lanes) {
         const float* const s = (kPrefix && alone ? whole_part<D>(p, b, h) : p.part + ((int64_t)i * 2 + (i == w0 ? first_slot : 0)) * (kPartRows * (D + 4))) + r * (D + 4);

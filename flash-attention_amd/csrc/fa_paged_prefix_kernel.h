@@ -1,8 +1,8 @@
 // Attention of sequences that share a prefix, a few rows a key head: one launch has two kinds of workgroups.  The first ones attend with a group's rows to the keys that the
 // group shares (fa_paged_chunk_kernel.h, kShared), the others have the line of the sequences' own keys (fa_paged_decode_kernel.h); all leave partial results, which a second
 // kernel joins.  The first are bound by products and the exponentials, the others by memory: side by side on a compute unit they take little more than the longer of the two.
-// 32 sequences of 8 x 4 heads, d = 128, 100 .. 1024 keys of their own behind 8192: 26 to 27 us and 6.4 for the join, 20 for the bytes; 64 of 450 .. 1500 behind 16384 in 8 bits
-// 56 and 7, 31.
+// 32 sequences of 8 x 4 heads, d = 128, 100 .. 1024 keys of their own behind 8192: 26 to 28 us and 6.4 for the join, 20 for the bytes; 64 of 450 .. 1500 behind 16384 in 8 bits
+// 56 to 57 and 7, 31.
 #pragma once
 
 #include "fa_paged_chunk_kernel.h"

@@ -1,5 +1,5 @@
 // fa_paged_read: the new tokens' (or whole sequences') keys and values out of their pages, packed, in 16 bits: the counterpart of fa_paged_append, whose places they
-// lie in.  HBM-bound (4.8 TB/s, two thirds of it writes); what rows in 8 bits stand for is exact in 16, so nothing is rounded.
+// lie in.  HBM-bound (41600 rows of 2 x 8 heads, d = 128, from memory: 8 bits 256 MB in 54 us, 4.8 TB/s, to 58; 16 bits 341 MB in 64.5, 5.3); what rows in 8 bits stand for is exact in 16, so nothing is rounded.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

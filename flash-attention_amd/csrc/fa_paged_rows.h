@@ -7,7 +7,9 @@ namespace fa {
 
 // 16 bytes that a launch reads or writes once.  Many rows (kStream): marked as such, so that they leave the caches to what is read again.  us with / without, 20000 rows of 3 x 16 heads,
 // d = 64, rows read so by the store into 16 bits 52.5 / 57.7, with attention of the chunk behind it 341 / 342, 4800 rows of 32 + 8 + 8 heads, d = 128, likewise 74.5 / 76.5, in 8 bits 82.1 /
-// 83.4; rows written so by reading, 46000 rows of 2 x 8 heads, d = 128 53.4 / 57.2.  (The new q written so: 2 us less to store, and 2 more for the attention that reads it.)
+// 83.4.  (The new q written so: 2 us less to store, and 2 more for the attention that reads it.)  Rows written so by reading, pages in the caches | in memory: 8 x 2500 rows stored and read back
+// 76.7 / 79.6, 77.3 / 82.0 where the states exceed the caches; rows of 2 x 8 heads, d = 128, 8 bits, 6000 8.3 / 9.7 | 9.2 / 11.4, 15000 16.4 / 18.2 | 22.7 / 21.8, 24000 27.1 / 27.0 | 32.7 / 30.4,
+// 41600 42.6 / 50.8 | 53.6 (three states in turn 58.5) / 48.7, 83200 82 / 107 | 101 / 108; 41600 in 16 bits 53.2 / 62.3 | 64.5 / 64.4.
 template <bool kStream>
 FA_DEVICE u32x4 ld_row16(const void* p) {
   if constexpr (kStream) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
